@@ -1,0 +1,59 @@
+/*
+ * kv_params.h -- kernel arguments shared by the cache, attention and log-probability kernels
+ * and the host code that launches them.
+ */
+#ifndef DFQ_KV_PARAMS_H
+#define DFQ_KV_PARAMS_H
+
+#include <stdint.h>
+
+#define DFQ_KV_THREADS 256
+
+/* One quantised array pair of a cache (K or V), [slots][heads][capacity][..]. */
+struct KvArrays {
+    uint32_t* codes;
+    uint16_t* scales;
+    uint16_t* biases;
+};
+
+struct KvAppendParams {
+    KvArrays out[2];         /* K, V                                             */
+    const uint16_t* in[2];   /* rows [batch * rows], row_stride elements apart   */
+    const int32_t* starts;   /* first position of each sequence, added to start  */
+    int64_t row_stride;
+    int start, rows, heads, capacity;
+};
+
+struct KvReadParams {
+    KvArrays in[2];
+    void* out[2];            /* dense [batch][rows][heads][dim], NULL: not wanted */
+    const int32_t* starts;
+    int start, rows, heads, capacity;
+};
+
+struct KvAttnParams {
+    KvArrays prefix[2];      /* K, V of the shared prefix (slot 0)               */
+    KvArrays own[2];         /* K, V of the sequences' own caches                */
+    const uint16_t* q;
+    uint16_t* y;
+    float* lse;              /* [batch][rows][q_heads] or NULL                   */
+    const int32_t* lengths;  /* own tokens of each sequence, the block's included */
+    const uint32_t* tree;    /* [batch][rows] row masks or NULL (a chain)        */
+    int64_t q_stride;
+    int prefix_length, prefix_capacity, own_capacity, max_length;
+    int batch, rows, heads, q_heads;
+    float scale_log2e;       /* softmax scale * log2(e)                          */
+};
+
+struct LogprobParams {
+    const void* logits;
+    const int32_t* tokens;   /* or NULL */
+    float* logprobs;
+    float* entropy;
+    int32_t* top_tokens;
+    float* top_logprobs;
+    int64_t row_stride;
+    int rows, vocab, top;
+};
+
+#endif

@@ -63,6 +63,12 @@ bool make_plan(int M, int N, int K, int bits, int gs, int num_cus, size_t lds_ma
 /* The device address of the fixed scratch array (qmm_scratch.hip) on `device`, which must be
  * current; taken and cleared once per device. */
 dfq_status scratch_setup(int device, void** out);
+/* The kernels of the cache, attention and log-probability calls (verify_ops.cpp), loaded with
+ * a context on its device, which must be current. */
+struct VerifyOps;
+dfq_status verify_ops_load(VerifyOps** out);
+void verify_ops_unload(VerifyOps* ops);
+VerifyOps* ctx_verify_ops(const dfq_ctx* ctx);
 /* A layer whose only copy of the weight is `packed` (the packed layout, in memory the caller
  * keeps alive); d carries its shape, format, dtype and linear bias, and no MLX arrays. */
 dfq_status make_packed_linear(dfq_ctx* ctx, const dfq_linear_desc& d, const void* packed,

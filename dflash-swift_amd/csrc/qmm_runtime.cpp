@@ -151,6 +151,7 @@ struct dfq_ctx {
     hipFunction_t read_stream = nullptr; // the plain streaming read (bandwidth reference)
     hipFunction_t read_units = nullptr;  // the fast kernel's own loads with no compute
     hipFunction_t read_units_packed = nullptr;  // the same over the packed layout
+    dfq::VerifyOps* verify = nullptr;    // cache, attention and log-probability kernels
     void* scratch = nullptr;             // the fixed scratch of dfq_qmm_noalloc (this device)
     std::mutex mu;
     std::unordered_map<PlanKey, dfq::Plan, PlanKeyHash> plans;
@@ -201,6 +202,8 @@ struct DeviceGuard {
 };
 
 int ctx_device(const dfq_ctx* ctx) { return ctx->device; }
+
+VerifyOps* ctx_verify_ops(const dfq_ctx* ctx) { return ctx->verify; }
 
 DeviceScope::DeviceScope(const dfq_ctx* ctx) : dev_(ctx_device(ctx)) {
     if (hipGetDevice(&prev_) != hipSuccess) prev_ = -1;
@@ -718,8 +721,10 @@ dfq_status dfq_init(int device, dfq_ctx** out) {
         return hip_fail(e, "hipModuleGetFunction");
     }
     dfq_status st = load_gemm(ctx);
+    if (st == DFQ_OK) st = verify_ops_load(&ctx->verify);
     if (st == DFQ_OK) st = scratch_setup(device, &ctx->scratch);
     if (st != DFQ_OK) {
+        verify_ops_unload(ctx->verify);
         if (ctx->gemm_module) (void)hipModuleUnload(ctx->gemm_module);
         (void)hipModuleUnload(ctx->module);
         delete ctx;
@@ -733,6 +738,7 @@ dfq_status dfq_destroy(dfq_ctx* ctx) {
     if (!ctx) return DFQ_OK;
     {
         DeviceGuard g(ctx->device);
+        verify_ops_unload(ctx->verify);
         if (ctx->gemm_module) (void)hipModuleUnload(ctx->gemm_module);
         if (ctx->module) (void)hipModuleUnload(ctx->module);
     }

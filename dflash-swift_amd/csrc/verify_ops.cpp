@@ -1,0 +1,375 @@
+/*
+ * verify_ops.cpp -- the C ABI of the quantised key/value cache, its attention and the log
+ * probabilities: argument checks, work splits and launches of kv_cache.hip and logprobs.hip.
+ */
+#include <hip/hip_runtime_api.h>
+
+#include <cmath>
+#include <cstdint>
+#include <cstdio>
+#include <new>
+
+#include "dflash_qmm.h"
+#include "kv_params.h"
+#include "qmm_internal.h"
+
+#if !defined(DFQ_KV_HSACO_PATH) || !defined(DFQ_LOGPROBS_HSACO_PATH)
+#error "DFQ_KV_HSACO_PATH and DFQ_LOGPROBS_HSACO_PATH must name the gfx950 code objects to embed"
+#endif
+
+__asm__(".section .rodata.dfq_verify_hsaco,\"a\",@progbits\n"
+        ".p2align 12\n"
+        ".globl dfq_kv_hsaco_begin\n"
+        ".hidden dfq_kv_hsaco_begin\n"
+        "dfq_kv_hsaco_begin:\n"
+        ".incbin \"" DFQ_KV_HSACO_PATH "\"\n"
+        ".byte 0\n"
+        ".p2align 12\n"
+        ".globl dfq_logprobs_hsaco_begin\n"
+        ".hidden dfq_logprobs_hsaco_begin\n"
+        "dfq_logprobs_hsaco_begin:\n"
+        ".incbin \"" DFQ_LOGPROBS_HSACO_PATH "\"\n"
+        ".byte 0\n"
+        ".previous\n");
+extern "C" const char dfq_kv_hsaco_begin[];
+extern "C" const char dfq_logprobs_hsaco_begin[];
+
+namespace dfq {
+
+/* One format of a cache: [head_dim 64/128/256][bits 4/8][group 32/64/128][bf16/f16]; groups wider
+ * than the head have no kernels. */
+struct CacheKernels {
+    hipFunction_t append = nullptr, read = nullptr, attention = nullptr;
+};
+
+struct VerifyOps {
+    hipModule_t kv = nullptr, logprobs = nullptr;
+    CacheKernels cache[3][2][3][2];
+    hipFunction_t token_logprobs[3] = {};  // [bf16/f16/f32]
+};
+
+static dfq_status hip_error(hipError_t e, const char* what) {
+    return fail(DFQ_ERR_HIP, "%s: %s (%d)", what, hipGetErrorString(e), (int)e);
+}
+
+static dfq_status resolve(VerifyOps* o) {
+    static const char* kDt[3] = {"bf16", "f16", "f32"};
+    hipError_t e;
+    if ((e = hipModuleLoadData(&o->kv, dfq_kv_hsaco_begin)) != hipSuccess)
+        return hip_error(e, "hipModuleLoadData(gfx950 cache object)");
+    if ((e = hipModuleLoadData(&o->logprobs, dfq_logprobs_hsaco_begin)) != hipSuccess)
+        return hip_error(e, "hipModuleLoadData(gfx950 log-probability object)");
+    char name[80];
+    for (int d = 0; d < 3; ++d)
+        for (int b = 0; b < 2; ++b)
+            for (int g = 0; g < 3 && 32 << g <= 64 << d; ++g)
+                for (int t = 0; t < 2; ++t) {
+                    CacheKernels& c = o->cache[d][b][g][t];
+                    const struct { const char* op; hipFunction_t* fn; } parts[] = {
+                        {"append", &c.append}, {"read", &c.read}, {"attention", &c.attention}};
+                    for (const auto& part : parts) {
+                        snprintf(name, sizeof name, "dfq_cache_%s_d%d_b%d_g%d_%s", part.op,
+                                 64 << d, 4 << b, 32 << g, kDt[t]);
+                        if ((e = hipModuleGetFunction(part.fn, o->kv, name)) != hipSuccess)
+                            return hip_error(e, name);
+                    }
+                }
+    for (int t = 0; t < 3; ++t) {
+        snprintf(name, sizeof name, "dfq_token_logprobs_%s", kDt[t]);
+        if ((e = hipModuleGetFunction(&o->token_logprobs[t], o->logprobs, name)) != hipSuccess)
+            return hip_error(e, name);
+    }
+    return DFQ_OK;
+}
+
+dfq_status verify_ops_load(VerifyOps** out) {
+    *out = nullptr;
+    VerifyOps* o = new (std::nothrow) VerifyOps();
+    if (!o) return fail(DFQ_ERR_HIP, "out of host memory");
+    const dfq_status s = resolve(o);
+    if (s) {
+        verify_ops_unload(o);
+        return s;
+    }
+    *out = o;
+    return DFQ_OK;
+}
+
+void verify_ops_unload(VerifyOps* o) {
+    if (!o) return;
+    if (o->kv) (void)hipModuleUnload(o->kv);
+    if (o->logprobs) (void)hipModuleUnload(o->logprobs);
+    delete o;
+}
+
+}  // namespace dfq
+
+using namespace dfq;
+
+namespace {
+
+bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
+
+int dim_index(int dim) { return dim == 64 ? 0 : dim == 128 ? 1 : dim == 256 ? 2 : -1; }
+int group_index(int gs) { return gs == 32 ? 0 : gs == 64 ? 1 : gs == 128 ? 2 : -1; }
+
+/* The launch grid's limits in y and z. */
+constexpr int kMostGrid = 65535;
+
+dfq_status check_format(const dfq_kv_cache* c) {
+    if (c->dtype != DFQ_BF16 && c->dtype != DFQ_F16)
+        return fail(DFQ_ERR_UNSUPPORTED, "a cache's dtype is bf16 or fp16");
+    if (c->bits != 4 && c->bits != 8) return fail(DFQ_ERR_UNSUPPORTED, "bits must be 4 or 8");
+    if (dim_index(c->head_dim) < 0)
+        return fail(DFQ_ERR_UNSUPPORTED, "head_dim must be 64, 128 or 256 (got %d)", c->head_dim);
+    if (group_index(c->group_size) < 0 || c->group_size > c->head_dim)
+        return fail(DFQ_ERR_UNSUPPORTED,
+                    "group size must be 32, 64 or 128 and divide the head (got %d)",
+                    c->group_size);
+    if (c->slots < 1 || c->heads < 1 || c->capacity < 1)
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "slots, heads and capacity must be >= 1");
+    if (c->heads > kMostGrid || c->slots > kMostGrid / 2)
+        return fail(DFQ_ERR_UNSUPPORTED, "at most %d heads and %d slots", kMostGrid,
+                    kMostGrid / 2);
+    /* offsets inside one head of one slot are 32 bits in the kernels */
+    if ((int64_t)c->capacity * c->head_dim * c->bits / 8 > INT32_MAX)
+        return fail(DFQ_ERR_UNSUPPORTED, "one head of one slot must be smaller than 2 GiB");
+    return DFQ_OK;
+}
+
+dfq_status check_cache(const dfq_kv_cache* c) {
+    if (!c) return fail(DFQ_ERR_INVALID_ARGUMENT, "null cache");
+    const dfq_status s = check_format(c);
+    if (s) return s;
+    if (!c->k_codes || !c->k_scales || !c->k_biases || !c->v_codes || !c->v_scales ||
+        !c->v_biases)
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "null cache array");
+    if (!aligned(c->k_codes, 16) || !aligned(c->v_codes, 16))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "cache codes must be 16-byte aligned");
+    if (!aligned(c->k_scales, 2) || !aligned(c->k_biases, 2) || !aligned(c->v_scales, 2) ||
+        !aligned(c->v_biases, 2))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "cache scales and biases must be 2-byte aligned");
+    return DFQ_OK;
+}
+
+dfq_status check_span(const dfq_kv_cache* c, int batch, int rows) {
+    if (batch < 1 || rows < 1) return fail(DFQ_ERR_INVALID_ARGUMENT, "batch and rows must be >= 1");
+    if (batch > c->slots)
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "%d sequences in a cache of %d slots", batch,
+                    c->slots);
+    return DFQ_OK;
+}
+
+const CacheKernels& kernels_of(const dfq_ctx* ctx, const dfq_kv_cache* c) {
+    return ctx_verify_ops(ctx)->cache[dim_index(c->head_dim)][c->bits == 8]
+                                     [group_index(c->group_size)][c->dtype == DFQ_F16];
+}
+
+KvArrays arrays_of(const dfq_kv_cache* c, bool v) {
+    return v ? KvArrays{c->v_codes, (uint16_t*)c->v_scales, (uint16_t*)c->v_biases}
+             : KvArrays{c->k_codes, (uint16_t*)c->k_scales, (uint16_t*)c->k_biases};
+}
+
+/* Workgroups along the rows of an append or read: 8 channels a thread. */
+unsigned row_blocks(const dfq_kv_cache* c, int rows) {
+    const int per = DFQ_KV_THREADS * 8 / c->head_dim;
+    return ((unsigned)rows + per - 1) / per;
+}
+
+/* The sizes of an attention call; *fmt gets the cache that carries the format. */
+dfq_status check_attention(const dfq_kv_cache* prefix, int prefix_length,
+                           const dfq_kv_cache* cache, int max_length, int batch, int rows,
+                           int q_heads, const dfq_kv_cache** fmt) {
+    if (batch < 1 || rows < 1) return fail(DFQ_ERR_INVALID_ARGUMENT, "batch and rows must be >= 1");
+    if (rows > DFQ_MAXIMUM_ROWS)
+        return fail(DFQ_ERR_UNSUPPORTED, "a block has at most %d rows (got %d)", DFQ_MAXIMUM_ROWS,
+                    rows);
+    if (batch > kMostGrid) return fail(DFQ_ERR_UNSUPPORTED, "at most %d sequences", kMostGrid);
+    if (prefix_length < 0 || max_length < 0)
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "negative length");
+    if (!prefix && prefix_length) return fail(DFQ_ERR_INVALID_ARGUMENT, "null prefix");
+    if (!cache && max_length) return fail(DFQ_ERR_INVALID_ARGUMENT, "null cache");
+    if (!prefix && !cache) return fail(DFQ_ERR_INVALID_ARGUMENT, "neither a prefix nor a cache");
+    dfq_status s;
+    if (prefix) {
+        if ((s = check_format(prefix))) return s;
+        if (prefix_length > prefix->capacity)
+            return fail(DFQ_ERR_INVALID_ARGUMENT, "prefix_length %d is past the capacity %d",
+                        prefix_length, prefix->capacity);
+    }
+    if (cache) {
+        if ((s = check_format(cache)) || (s = check_span(cache, batch, rows))) return s;
+        if (max_length > cache->capacity)
+            return fail(DFQ_ERR_INVALID_ARGUMENT, "max_length %d is past the capacity %d",
+                        max_length, cache->capacity);
+    }
+    if (prefix && cache &&
+        (prefix->heads != cache->heads || prefix->head_dim != cache->head_dim ||
+         prefix->bits != cache->bits || prefix->group_size != cache->group_size ||
+         prefix->dtype != cache->dtype))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "the prefix and the cache differ in format");
+    *fmt = cache ? cache : prefix;
+    if (q_heads < 1 || q_heads % (*fmt)->heads || q_heads > kMostGrid)
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "q_heads %d is not a multiple of the %d heads",
+                    q_heads, (*fmt)->heads);
+    return DFQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+dfq_status dfq_cache_append(dfq_ctx* ctx, const dfq_kv_cache* cache, const void* k, const void* v,
+                            int64_t row_stride, int batch, int rows, int start,
+                            const int32_t* starts, void* stream) {
+    if (!ctx) return fail(DFQ_ERR_INVALID_ARGUMENT, "null context");
+    dfq_status s = check_cache(cache);
+    if (s || (s = check_span(cache, batch, rows))) return s;
+    if (!k || !v) return fail(DFQ_ERR_INVALID_ARGUMENT, "null k or v");
+    if (!aligned(k, 2) || !aligned(v, 2) || !aligned(starts, 4))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "misaligned k, v or starts");
+    if (row_stride < (int64_t)cache->heads * cache->head_dim)
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "row_stride is smaller than a row");
+    KvAppendParams p{{arrays_of(cache, false), arrays_of(cache, true)},
+                     {(const uint16_t*)k, (const uint16_t*)v}, starts, row_stride, start, rows,
+                     cache->heads, cache->capacity};
+    DeviceScope scope(ctx);
+    void* args[] = {&p};
+    const hipError_t e = hipModuleLaunchKernel(
+        kernels_of(ctx, cache).append, row_blocks(cache, rows), (unsigned)cache->heads,
+        2u * batch, DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
+    return e == hipSuccess ? DFQ_OK : hip_error(e, "launch dfq_cache_append");
+}
+
+dfq_status dfq_cache_read(dfq_ctx* ctx, const dfq_kv_cache* cache, void* k, void* v,
+                          dfq_dtype dtype, int batch, int rows, int start, const int32_t* starts,
+                          void* stream) {
+    if (!ctx) return fail(DFQ_ERR_INVALID_ARGUMENT, "null context");
+    dfq_status s = check_cache(cache);
+    if (s || (s = check_span(cache, batch, rows))) return s;
+    if (!k && !v) return fail(DFQ_ERR_INVALID_ARGUMENT, "null k and v");
+    if (dtype != cache->dtype && dtype != DFQ_F32)
+        return fail(DFQ_ERR_UNSUPPORTED, "values are read in the cache's dtype or fp32");
+    if (!aligned(k, 16) || !aligned(v, 16) || !aligned(starts, 4))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "misaligned k, v or starts");
+    KvReadParams p{{arrays_of(cache, false), arrays_of(cache, true)}, {k, v}, starts, start, rows,
+                   cache->heads, cache->capacity};
+    int dt = (int)dtype;
+    DeviceScope scope(ctx);
+    void* args[] = {&p, &dt};
+    const hipError_t e = hipModuleLaunchKernel(
+        kernels_of(ctx, cache).read, row_blocks(cache, rows), (unsigned)cache->heads, 2u * batch,
+        DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
+    return e == hipSuccess ? DFQ_OK : hip_error(e, "launch dfq_cache_read");
+}
+
+dfq_status dfq_cache_attention_workspace_bytes(dfq_ctx* ctx, const dfq_kv_cache* prefix,
+                                               int prefix_length, const dfq_kv_cache* cache,
+                                               int max_length, int batch, int rows, int q_heads,
+                                               size_t* bytes) {
+    if (!bytes) return fail(DFQ_ERR_INVALID_ARGUMENT, "null bytes");
+    *bytes = 0;
+    if (!ctx) return fail(DFQ_ERR_INVALID_ARGUMENT, "null context");
+    const dfq_kv_cache* fmt;
+    return check_attention(prefix, prefix_length, cache, max_length, batch, rows, q_heads, &fmt);
+}
+
+dfq_status dfq_cache_attention(dfq_ctx* ctx, const dfq_kv_cache* prefix, int prefix_length,
+                               const dfq_kv_cache* cache, const int32_t* lengths, int max_length,
+                               const uint32_t* tree, const void* q, int64_t q_stride, void* y,
+                               float* lse, int batch, int rows, int q_heads, float scale,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+    if (!ctx) return fail(DFQ_ERR_INVALID_ARGUMENT, "null context");
+    const dfq_kv_cache* fmt;
+    dfq_status s =
+        check_attention(prefix, prefix_length, cache, max_length, batch, rows, q_heads, &fmt);
+    if (s || (prefix && (s = check_cache(prefix))) || (cache && (s = check_cache(cache)))) return s;
+    if (!q || !y) return fail(DFQ_ERR_INVALID_ARGUMENT, "null q or y");
+    if (!cache && (lengths || tree))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "lengths and tree are of a cache, and it is null");
+    if (!aligned(q, 2) || !aligned(y, 16) || !aligned(lse, 4) || !aligned(lengths, 4) ||
+        !aligned(tree, 4))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "misaligned q, y, lse, lengths or tree");
+    if (q_stride < (int64_t)q_heads * fmt->head_dim)
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "q_stride is smaller than a row");
+    if (!(scale > 0.0f) || !std::isfinite(scale))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
+    (void)workspace;
+    (void)workspace_bytes;
+    KvAttnParams p{};
+    if (prefix)
+        for (int i = 0; i < 2; ++i) p.prefix[i] = arrays_of(prefix, i);
+    if (cache)
+        for (int i = 0; i < 2; ++i) p.own[i] = arrays_of(cache, i);
+    p.q = (const uint16_t*)q;
+    p.y = (uint16_t*)y;
+    p.lse = lse;
+    p.lengths = lengths;
+    p.tree = tree;
+    p.q_stride = q_stride;
+    p.prefix_length = prefix_length;
+    p.prefix_capacity = prefix ? prefix->capacity : 0;
+    p.own_capacity = cache ? cache->capacity : 0;
+    p.max_length = max_length;
+    p.batch = batch;
+    p.rows = rows;
+    p.heads = fmt->heads;
+    p.q_heads = q_heads;
+    p.scale_log2e = scale * 1.44269504088896340736f;
+    DeviceScope scope(ctx);
+    void* args[] = {&p};
+    const hipError_t e = hipModuleLaunchKernel(
+        kernels_of(ctx, fmt).attention, (unsigned)q_heads, (unsigned)rows, (unsigned)batch,
+        DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
+    return e == hipSuccess ? DFQ_OK : hip_error(e, "launch dfq_cache_attention");
+}
+
+static dfq_status check_logprobs(int M, int V, int top_k) {
+    if (M < 1 || V < 1) return fail(DFQ_ERR_INVALID_ARGUMENT, "M and V must be positive");
+    if (V > 0x7fffffff / 2) return fail(DFQ_ERR_UNSUPPORTED, "V too large");
+    if (top_k < 0 || top_k > DFQ_TOP_MAX)
+        return fail(DFQ_ERR_UNSUPPORTED, "top_k must be 0..%d (got %d)", DFQ_TOP_MAX, top_k);
+    return DFQ_OK;
+}
+
+dfq_status dfq_token_logprobs_workspace_bytes(dfq_ctx* ctx, int M, int V, int top_k,
+                                              size_t* bytes) {
+    if (!bytes) return fail(DFQ_ERR_INVALID_ARGUMENT, "null bytes");
+    *bytes = 0;
+    if (!ctx) return fail(DFQ_ERR_INVALID_ARGUMENT, "null context");
+    return check_logprobs(M, V, top_k);
+}
+
+dfq_status dfq_token_logprobs(dfq_ctx* ctx, const void* logits, int64_t row_stride, int M, int V,
+                              dfq_dtype dtype, const int32_t* tokens, int top_k, float* logprobs,
+                              float* entropy, int32_t* top_tokens, float* top_logprobs,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+    if (!ctx) return fail(DFQ_ERR_INVALID_ARGUMENT, "null context");
+    if (!logits) return fail(DFQ_ERR_INVALID_ARGUMENT, "null logits");
+    dfq_status s = check_logprobs(M, V, top_k);
+    if (s) return s;
+    if (dtype != DFQ_BF16 && dtype != DFQ_F16 && dtype != DFQ_F32)
+        return fail(DFQ_ERR_UNSUPPORTED, "logits are bf16, fp16 or fp32");
+    if (row_stride < V) return fail(DFQ_ERR_INVALID_ARGUMENT, "row_stride is smaller than a row");
+    if (tokens && !logprobs) return fail(DFQ_ERR_INVALID_ARGUMENT, "null logprobs");
+    if (top_k && (!top_tokens || !top_logprobs))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "null top_tokens or top_logprobs");
+    if (!tokens && !entropy && !top_k)
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "nothing is asked for");
+    if (!aligned(logits, dtype == DFQ_F32 ? 4 : 2) || !aligned(tokens, 4) ||
+        !aligned(logprobs, 4) || !aligned(entropy, 4) || !aligned(top_tokens, 4) ||
+        !aligned(top_logprobs, 4))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "misaligned buffer");
+    (void)workspace;
+    (void)workspace_bytes;
+    LogprobParams p{logits, tokens, logprobs, entropy, top_tokens, top_logprobs, row_stride, M, V,
+                    top_k};
+    DeviceScope scope(ctx);
+    void* args[] = {&p};
+    const hipError_t e = hipModuleLaunchKernel(
+        ctx_verify_ops(ctx)->token_logprobs[(int)dtype], (unsigned)M, 1, 1, DFQ_KV_THREADS, 1, 1,
+        0, (hipStream_t)stream, args, nullptr);
+    return e == hipSuccess ? DFQ_OK : hip_error(e, "launch dfq_token_logprobs");
+}
+
+}  // extern "C"

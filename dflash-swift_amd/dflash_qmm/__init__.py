@@ -23,7 +23,8 @@ import ctypes
 import os
 
 __all__ = [
-    "BF16", "F16", "F32", "DfqError", "Context", "PackedWeight", "SmallMQuantizedMatmul",
+    "BF16", "F16", "F32", "DfqError", "Context", "KVCache", "PackedWeight",
+    "SmallMQuantizedMatmul",
     "QuantizedLinear",
     "SmallMQuantizedLinear", "Model", "enable_small_m_quantized_matmul", "library_path",
     "load_library",
@@ -53,6 +54,17 @@ class _LinearDesc(ctypes.Structure):
         ("bias", ctypes.c_void_p), ("out_features", ctypes.c_int),
         ("in_features", ctypes.c_int), ("bits", ctypes.c_int), ("group_size", ctypes.c_int),
         ("mode_affine", ctypes.c_int), ("dtype", ctypes.c_int),
+    ]
+
+
+class _KVCacheDesc(ctypes.Structure):
+    _fields_ = [
+        ("k_codes", ctypes.c_void_p), ("k_scales", ctypes.c_void_p),
+        ("k_biases", ctypes.c_void_p), ("v_codes", ctypes.c_void_p),
+        ("v_scales", ctypes.c_void_p), ("v_biases", ctypes.c_void_p),
+        ("slots", ctypes.c_int), ("heads", ctypes.c_int), ("capacity", ctypes.c_int),
+        ("head_dim", ctypes.c_int), ("bits", ctypes.c_int), ("group_size", ctypes.c_int),
+        ("dtype", ctypes.c_int),
     ]
 
 
@@ -93,7 +105,7 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         raise ImportError(f"{p} is not built: run `make -C dflash-swift_amd` (no CPU fallback)")
     lib = ctypes.CDLL(p)
     P, I, S, Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.POINTER(ctypes.c_size_t)
-    PP = ctypes.POINTER(ctypes.c_void_p)
+    PP, L = ctypes.POINTER(ctypes.c_void_p), ctypes.c_int64
     sig = {
         "dfq_init": ([I, PP], I), "dfq_destroy": ([P], I), "dfq_last_error": ([], ctypes.c_char_p),
         "dfq_status_string": ([I], ctypes.c_char_p), "dfq_abi_version": ([], I),
@@ -154,6 +166,13 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         "dfq_small_m_linear_pack": ([P, P], I), "dfq_linear_packed": ([P], P),
         "dfq_qmm_silu_gate_up": ([P, P, P, P, P, P, P, I, I, I, I, I, I, P, S, P], I),
         "dfq_interleave_gate_up": ([P, P, P, P, I, S, P], I),
+        "dfq_cache_append": ([P, P, P, P, L, I, I, I, P, P], I),
+        "dfq_cache_read": ([P, P, P, P, I, I, I, I, P, P], I),
+        "dfq_cache_attention_workspace_bytes": ([P, P, I, P, I, I, I, I, Z], I),
+        "dfq_cache_attention": ([P, P, I, P, P, I, P, P, L, P, P, I, I, I,
+                                 ctypes.c_float, P, S, P], I),
+        "dfq_token_logprobs_workspace_bytes": ([P, I, I, I, Z], I),
+        "dfq_token_logprobs": ([P, P, L, I, I, I, P, I, P, P, P, P, P, S, P], I),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
@@ -214,13 +233,14 @@ class Context:
         # lazily grown workspaces of the convenience calls, one per stream; a grown one
         # replaces the old, which is kept (a graph or another stream may still hold it)
         self._ws = {}
+        self._scratch = {}
         self._retired = []
 
     def close(self):
         if self.handle:
             self.lib.dfq_destroy(self.handle)
             self.handle = None
-        self._ws, self._retired = {}, []
+        self._ws, self._scratch, self._retired = {}, {}, []
 
     def __del__(self):
         try:
@@ -416,6 +436,142 @@ class Context:
                "dfq_argmax_accept")
         return tokens, accepted
 
+    # ---- the quantised key/value cache ---------------------------------------------------
+    def cache_append(self, cache, k, v, start=0, starts=None, stream=None):
+        """Quantise rows k, v [batch, rows, heads*head_dim] (the cache's dtype; rows may be cut
+        from a fused output) into slots 0..batch-1 of `cache` at positions start + starts[b] +
+        0, 1, ... (starts: int32 [batch] on the device)."""
+        if k.shape != v.shape or k.dim() != 3 or k.shape[2] != cache.heads * cache.head_dim:
+            raise ValueError("k and v are [batch, rows, heads*head_dim]")
+        batch, rows, _ = k.shape
+        stride = _row_stride(k)
+        if _row_stride(v) != stride:
+            raise ValueError("k and v must have the same strides")
+        cache.check_dtype(k, v)
+        _check_int32("starts", starts, (batch,))
+        _check(self.lib.dfq_cache_append(self.handle, cache.desc, k.data_ptr(), v.data_ptr(),
+                                         stride, batch, rows, start, _ptr(starts),
+                                         _stream(stream)), "dfq_cache_append")
+
+    def cache_read(self, cache, rows, start=0, starts=None, batch=None, dtype=None, k=None,
+                   v=None, stream=None):
+        """The values (k, v) [batch, rows, heads, head_dim] of a span of `cache`, in its dtype
+        or fp32; batch defaults to that of starts, else to all slots."""
+        import torch
+        if batch is None:
+            batch = cache.slots if starts is None else starts.shape[0]
+        _check_int32("starts", starts, (batch,))
+        dt = cache.dtype if dtype is None else dtype
+        shape = (batch, rows, cache.heads, cache.head_dim)
+        for a in (k, v):
+            if a is not None and (a.shape != shape or a.dtype != dt or not a.is_contiguous()):
+                raise ValueError(f"outputs are contiguous {shape} of {dt}")
+        if k is None:
+            k = torch.empty(shape, dtype=dt, device=cache.device)
+        if v is None:
+            v = torch.empty(shape, dtype=dt, device=cache.device)
+        _check(self.lib.dfq_cache_read(self.handle, cache.desc, k.data_ptr(), v.data_ptr(),
+                                       dtype_code(dt), batch, rows, start, _ptr(starts),
+                                       _stream(stream)), "dfq_cache_read")
+        return k, v
+
+    def cache_attention(self, q, cache=None, lengths=None, max_length=None, prefix=None,
+                        prefix_length=None, tree=None, scale=None, out=None, lse=None, ws=None,
+                        stream=None):
+        """(y, lse) of a block q [batch, rows, q_heads*head_dim] over a shared prefix and the
+        sequences' own caches (dfq_cache_attention): y [batch, rows, q_heads*head_dim] in q's
+        dtype, lse fp32 [batch, rows, q_heads].
+
+        lengths [batch] int32 counts each sequence's own tokens, the block's rows included;
+        max_length bounds them (the capacity when left out).  prefix_length defaults to the
+        prefix's capacity, scale to head_dim ** -0.5.  tree [batch, rows] int32 holds the rows
+        of the block that each row sees (bit j: row j); without it the block is a chain."""
+        import torch
+        fmt = cache if cache is not None else prefix
+        if fmt is None:
+            raise ValueError("cache_attention needs a cache or a prefix")
+        if q.dim() != 3 or q.shape[2] % fmt.head_dim:
+            raise ValueError("q is [batch, rows, q_heads*head_dim]")
+        batch, rows, width = q.shape
+        heads = width // fmt.head_dim
+        fmt.check_dtype(q)
+        _check_int32("lengths", lengths, (batch,))
+        _check_int32("tree", tree, (batch, rows))
+        if max_length is None:
+            max_length = cache.capacity if cache is not None else 0
+        if prefix_length is None:
+            prefix_length = prefix.capacity if prefix is not None else 0
+        if scale is None:
+            scale = fmt.head_dim ** -0.5
+        if out is None:
+            out = torch.empty((batch, rows, width), dtype=q.dtype, device=q.device)
+        elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+            raise ValueError("out is contiguous, of q's shape and dtype")
+        if lse is None:
+            lse = torch.empty((batch, rows, heads), dtype=torch.float32, device=q.device)
+        elif lse.shape != (batch, rows, heads) or lse.dtype != torch.float32 or \
+                not lse.is_contiguous():
+            raise ValueError("lse is contiguous fp32 [batch, rows, q_heads]")
+        pd = prefix.desc if prefix is not None else None
+        cd = cache.desc if cache is not None else None
+        if ws is None:
+            need = ctypes.c_size_t()
+            _check(self.lib.dfq_cache_attention_workspace_bytes(
+                self.handle, pd, prefix_length, cd, max_length, batch, rows, heads,
+                ctypes.byref(need)), "dfq_cache_attention_workspace_bytes")
+            ws = self.workspace_uncleared(need.value, stream)
+        _check(self.lib.dfq_cache_attention(
+            self.handle, pd, prefix_length, cd, _ptr(lengths), max_length, _ptr(tree),
+            q.data_ptr(), _row_stride(q), out.data_ptr(), lse.data_ptr(), batch, rows, heads,
+            scale, _ptr(ws), ws.numel() if ws is not None else 0, _stream(stream)),
+            "dfq_cache_attention")
+        return out, lse
+
+    def token_logprobs(self, logits, tokens=None, top_k=0, ws=None, stream=None):
+        """(logprobs [M], entropy [M], top_tokens [M, top_k], top_logprobs [M, top_k]) of logits
+        [M, V] (rows may be strided) and tokens [M] int32; what is not asked for is None."""
+        import torch
+        if logits.dim() != 2 or logits.stride(1) != 1:
+            raise ValueError("logits are [M, V] with contiguous rows")
+        M, V = logits.shape
+        _check_int32("tokens", tokens, (M,))
+        dev = logits.device
+        lp = torch.empty(M, dtype=torch.float32, device=dev) if tokens is not None else None
+        entropy = torch.empty(M, dtype=torch.float32, device=dev)
+        ids = top = None
+        if top_k > 0:
+            ids = torch.empty((M, top_k), dtype=torch.int32, device=dev)
+            top = torch.empty((M, top_k), dtype=torch.float32, device=dev)
+        if ws is None:
+            need = ctypes.c_size_t()
+            _check(self.lib.dfq_token_logprobs_workspace_bytes(self.handle, M, V, top_k,
+                                                               ctypes.byref(need)),
+                   "dfq_token_logprobs_workspace_bytes")
+            ws = self.workspace_uncleared(need.value, stream)
+        _check(self.lib.dfq_token_logprobs(
+            self.handle, logits.data_ptr(), logits.stride(0) if M > 1 else V, M, V,
+            dtype_code(logits), _ptr(tokens), top_k, _ptr(lp), entropy.data_ptr(), _ptr(ids),
+            _ptr(top), _ptr(ws), ws.numel() if ws is not None else 0, _stream(stream)),
+            "dfq_token_logprobs")
+        return lp, entropy, ids, top
+
+    def workspace_uncleared(self, nbytes: int, stream=None):
+        """Scratch of the calls whose workspace needs no clearing, one per stream, apart from
+        `workspace`'s (which those calls would not leave zero); a grown one replaces the old,
+        which is kept as there."""
+        import torch
+        if nbytes == 0:
+            return None
+        key = _stream(stream)
+        ws = self._scratch.get(key)
+        if ws is None or ws.numel() < nbytes:
+            if ws is not None:
+                self._retired.append(ws)
+            ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8,
+                             device=f"cuda:{self.device}")
+            self._scratch[key] = ws
+        return ws
+
     # ---- the packed layout ---------------------------------------------------------------
     def pack(self, w, scales, biases, bits, gs, stream=None) -> "PackedWeight":
         """The weight, scales and biases of an MLX layer in the packed layout
@@ -529,6 +685,74 @@ class Context:
         _check(self.lib.dfq_graph_compose(self.handle, arr, len(graphs), ctypes.byref(g)),
                "dfq_graph_compose")
         return Graph(self.lib, g)
+
+
+def _row_stride(t) -> int:
+    """Elements between the rows of t [batch, rows, width], the same within and across
+    sequences."""
+    batch, rows, width = t.shape
+    if t.stride(2) != 1 and width > 1:
+        raise ValueError("a row's elements must be contiguous")
+    stride = t.stride(1) if rows > 1 else t.stride(0) if batch > 1 else width
+    if batch > 1 and rows > 1 and t.stride(0) != rows * stride:
+        raise ValueError("rows must be evenly spaced across sequences")
+    return stride
+
+
+def _check_int32(name, t, shape):
+    if t is None:
+        return
+    import torch
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} is a contiguous int32 tensor of shape {shape}")
+
+
+class KVCache:
+    """A quantised key/value cache (dfq_kv_cache): codes int32 [slots, heads, capacity,
+    head_dim*bits/32], scales and biases [slots, heads, capacity, head_dim/group_size].
+
+    `k` and `v` are (codes, scales, biases) torch tensors on one device, kept alive here."""
+
+    def __init__(self, slots, heads, capacity, head_dim, bits=4, group_size=64, dtype=None,
+                 device="cuda"):
+        import torch
+        dtype = torch.bfloat16 if dtype is None else dtype
+
+        def arrays():
+            lead = (slots, heads, capacity)
+            return (torch.zeros(lead + (head_dim * bits // 32,), dtype=torch.int32,
+                                device=device),
+                    torch.zeros(lead + (head_dim // group_size,), dtype=dtype, device=device),
+                    torch.zeros(lead + (head_dim // group_size,), dtype=dtype, device=device))
+        self._set(arrays(), arrays(), bits, group_size)
+
+    @classmethod
+    def from_arrays(cls, k, v, bits, group_size) -> "KVCache":
+        """A cache over existing arrays (codes, scales, biases) for K and V, in place."""
+        self = cls.__new__(cls)
+        self._set(tuple(k), tuple(v), bits, group_size)
+        return self
+
+    def _set(self, k, v, bits, group_size):
+        self.k, self.v, self.bits, self.group_size = k, v, bits, group_size
+        self.slots, self.heads, self.capacity, words = k[0].shape
+        self.head_dim = words * 32 // bits
+        self.dtype, self.device = k[1].dtype, k[0].device
+        lead = (self.slots, self.heads, self.capacity)
+        for codes, scales, biases in (k, v):
+            if codes.shape != lead + (words,) or codes.element_size() != 4 or \
+                    any(a.shape != lead + (self.head_dim // group_size,) or
+                        a.dtype != self.dtype for a in (scales, biases)) or \
+                    not all(a.is_contiguous() for a in (codes, scales, biases)):
+                raise ValueError("the cache's arrays do not agree in shape and dtype")
+        d = _KVCacheDesc(*(a.data_ptr() for a in (*k, *v)), self.slots, self.heads,
+                         self.capacity, self.head_dim, bits, group_size, dtype_code(self.dtype))
+        self._desc, self.desc = d, ctypes.addressof(d)
+
+    def check_dtype(self, *tensors):
+        for t in tensors:
+            if t.dtype != self.dtype:
+                raise ValueError(f"the cache holds {self.dtype}, got {t.dtype}")
 
 
 class PackedWeight:

@@ -299,6 +299,97 @@ dfq_status dfq_qmm_argmax_accept(dfq_ctx* ctx, const void* x, const uint32_t* w,
                                  const int32_t* proposals, int32_t* tokens, int32_t* accepted,
                                  void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- the quantised key/value cache of a verify pass ------------------------------------- */
+/* K and V rows held as the weights are: affine codes of 4 or 8 bits with a scale and a bias per
+ * group of 32, 64 or 128 channels, in the layout of MLX's quantised caches: codes uint32
+ * [slots][heads][capacity][head_dim*bits/32] with element 0 in the low bits, scales and biases
+ * [slots][heads][capacity][head_dim/group_size] in the cache's dtype (bf16 or fp16).  head_dim is
+ * 64, 128 or 256 and group_size divides it.  A slot holds one sequence's tokens by position.  The
+ * arrays are the caller's; codes are 16-byte aligned, the others 2-byte; one slot of one head is
+ * under 2 GiB in each array.  The reference's caches are its target's (a snapshot is taken and
+ * restored whole, Sources/DFlashKit/PrefixCache.swift:86-141); a prompt's tokens that several
+ * sequences share are one cache of one slot here, read in place by all of them. */
+typedef struct dfq_kv_cache {
+    uint32_t* k_codes;
+    void* k_scales;
+    void* k_biases;
+    uint32_t* v_codes;
+    void* v_scales;
+    void* v_biases;
+    int slots, heads, capacity, head_dim, bits, group_size;
+    dfq_dtype dtype;
+} dfq_kv_cache;
+
+/* Quantises `rows` new K and V rows of each of `batch` sequences (slots 0..batch-1) as it writes
+ * them to positions start + starts[b] + 0, 1, ... (starts: device memory, may be NULL for
+ * zeros).  k and v are in the cache's dtype, row m of sequence b at (b*rows + m)*row_stride
+ * elements, heads side by side in it (a slice of a fused q|k|v output is fine: any element
+ * alignment).  Positions outside [0, capacity) are not written.  Per group, in fp32:
+ * bias = the least element, scale = (greatest - least) / (2^bits - 1), both rounded to the dtype;
+ * code = (x - bias) / scale rounded to nearest even and clamped, 0 where the scale is 0.  A group
+ * whose scale or bias is not finite reads back as NaN throughout.  Asynchronous on `stream`. */
+dfq_status dfq_cache_append(dfq_ctx* ctx, const dfq_kv_cache* cache, const void* k, const void* v,
+                            int64_t row_stride, int batch, int rows, int start,
+                            const int32_t* starts, void* stream);
+
+/* The same span back as values scale*code + bias, each rounded once to `dtype` (the cache's or
+ * fp32): k and v dense [batch][rows][heads][head_dim], 16-byte aligned; either may be NULL.
+ * Positions outside [0, capacity) read as 0.  Asynchronous on `stream`. */
+dfq_status dfq_cache_read(dfq_ctx* ctx, const dfq_kv_cache* cache, void* k, void* v,
+                          dfq_dtype dtype, int batch, int rows, int start, const int32_t* starts,
+                          void* stream);
+
+/* Attention of a block of `rows` (1..16, DFQ_MAXIMUM_ROWS) queries of each of `batch` sequences
+ * over the quantised values themselves (not rounded to the dtype in between):
+ *   z[t] = scale * q . k[t],  y = sum softmax(z)[t] v[t],  lse = log sum exp z[t]  (natural)
+ * for query head j with K/V head j / (q_heads / heads).  The tokens of a row are
+ *   - all prefix_length tokens of `prefix` (its slot 0; NULL or 0: none), held once and read for
+ *     all sequences together;
+ *   - of the sequence's own slot, the tokens before its block: positions 0 .. n-rows-1 with
+ *     n = lengths[b] (device memory; NULL: max_length for all), the block's rows included, which
+ *     are the last `rows` (dfq_cache_append them first).  n is clamped to [0, max_length], and
+ *     max_length is at most the capacity; where n < rows the block's first rows are not there;
+ *   - of the block itself, rows 0..m for row m (a draft chain) or, with `tree` [batch][rows]
+ *     (device memory), the rows j whose bit j of tree[b][m] is set (a draft tree,
+ *     Sources/DFlashKit/DFlashDraftTree.swift:54).
+ * `cache` may be NULL with max_length 0 (then rows see the prefix alone).  Tokens that a row does
+ * not see take no part in it, whatever they hold.  A row that sees nothing has y = 0 and
+ * lse = -inf.  q is in the caches' dtype, row m of sequence b at (b*rows + m)*q_stride elements,
+ * heads side by side (any element alignment); y is dense [batch][rows][q_heads*head_dim] in that
+ * dtype; lse fp32 [batch][rows][q_heads] or NULL.  prefix and cache agree in heads, head_dim,
+ * bits, group_size and dtype.  scale is positive and finite.  Scores, softmax sums and outputs
+ * are summed in fp32; the same call gives the same bits every time.  The workspace
+ * (dfq_cache_attention_workspace_bytes for the same sizes, 16-byte aligned) needs no clearing.
+ * Asynchronous on `stream`. */
+dfq_status dfq_cache_attention_workspace_bytes(dfq_ctx* ctx, const dfq_kv_cache* prefix,
+                                               int prefix_length, const dfq_kv_cache* cache,
+                                               int max_length, int batch, int rows, int q_heads,
+                                               size_t* bytes);
+dfq_status dfq_cache_attention(dfq_ctx* ctx, const dfq_kv_cache* prefix, int prefix_length,
+                               const dfq_kv_cache* cache, const int32_t* lengths, int max_length,
+                               const uint32_t* tree, const void* q, int64_t q_stride, void* y,
+                               float* lse, int batch, int rows, int q_heads, float scale,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- log probabilities of a verify pass's logits ----------------------------------------- */
+#define DFQ_TOP_MAX 32 /* most alternatives of a row */
+/* For each of M rows of V logits (bf16, fp16 or fp32, row_stride elements apart), in fp32:
+ *   logprobs[m]            log softmax(logits[m])[tokens[m]] (tokens NULL: not wanted; NaN for a
+ *                          token outside 0..V-1, as dfq_argmax_accept's -1)
+ *   entropy[m]             -sum p log p, natural (may be NULL)
+ *   top_tokens[m][top_k]   the top_k (0..32) tokens by logit, equal ones by index, NaN left out
+ *   top_logprobs[m][top_k] theirs; -1 and NaN where a row has fewer numbers
+ * A logit of -inf has probability 0.  A row with a NaN or +inf, or with nothing above -inf, has
+ * NaN for its probabilities and entropy.  What a sampler's client is told of the tokens that the
+ * greedy accept takes (acceptedPrefix, DFlashSpeculativeGenerator.swift:555-571, keeps the tokens
+ * alone).  The workspace (16-byte aligned) needs no clearing.  Asynchronous on `stream`. */
+dfq_status dfq_token_logprobs_workspace_bytes(dfq_ctx* ctx, int M, int V, int top_k,
+                                              size_t* bytes);
+dfq_status dfq_token_logprobs(dfq_ctx* ctx, const void* logits, int64_t row_stride, int M, int V,
+                              dfq_dtype dtype, const int32_t* tokens, int top_k, float* logprobs,
+                              float* entropy, int32_t* top_tokens, float* top_logprobs,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- the drop-in layer (SmallMQuantizedMatmul.swift:227-317) -------------------------- */
 
 typedef struct dfq_linear dfq_linear;
