@@ -134,81 +134,6 @@ __device__ __forceinline__ void read_rows(const KvReadParams& p, int out_dt) {
     *(u32x4_t*)((uint16_t*)p.out[kv] + at) = v;
 }
 
-/* Attention of one query row and head over the prefix and the sequence's own cache, in fp32: a
- * block of 256 tokens at a time, one token's score a thread, then one channel a thread. */
-template <int DIM, int BITS, int GS, bool F16>
-__device__ __forceinline__ float cache_value(const KvArrays& a, int64_t row, int d) {
-    const uint32_t w = a.codes[row * (DIM * BITS / 32) + d * BITS / 32];
-    const uint32_t c = w >> (d * BITS % 32) & ((1u << BITS) - 1);
-    const int64_t g = row * (DIM / GS) + d / GS;
-    return fmaf(elem_to_f32<F16>(a.scales[g]), (float)c, elem_to_f32<F16>(a.biases[g]));
-}
-
-template <int DIM, int BITS, int GS, bool F16>
-__device__ __forceinline__ void attention(const KvAttnParams& p) {
-    __shared__ float q[DIM];
-    __shared__ float prob[DFQ_KV_THREADS];
-    __shared__ float part[DFQ_KV_THREADS / 64];
-    const int hq = blockIdx.x, m = blockIdx.y, b = blockIdx.z, h = hq / (p.q_heads / p.heads);
-    const int tid = threadIdx.x;
-    const uint16_t* qr = p.q + ((int64_t)b * p.rows + m) * p.q_stride + (int64_t)hq * DIM;
-    if (tid < DIM) q[tid] = elem_to_f32<F16>(qr[tid]);
-    int len = 0;
-    if (p.max_length > 0) {
-        const int most = p.max_length < p.own_capacity ? p.max_length : p.own_capacity;
-        len = p.lengths ? p.lengths[b] : most;
-        len = len < 0 ? 0 : len > most ? most : len;
-    }
-    const int first = len - p.rows;  /* the position of the block's row 0 */
-    const uint32_t mask = p.tree ? p.tree[(int64_t)b * p.rows + m] : (2u << m) - 1;
-    float top = -__builtin_inff(), sum = 0.0f, acc = 0.0f;
-    __syncthreads();
-    for (int part_i = 0; part_i < 2; ++part_i) {
-        const KvArrays& k = part_i ? p.own[0] : p.prefix[0];
-        const KvArrays& v = part_i ? p.own[1] : p.prefix[1];
-        const int n = part_i ? len : p.prefix_length;
-        const int64_t base = part_i ? ((int64_t)b * p.heads + h) * p.own_capacity
-                                    : (int64_t)h * p.prefix_capacity;
-        for (int t0 = 0; t0 < n; t0 += DFQ_KV_THREADS) {
-            const int t = t0 + tid;
-            bool seen = t < n;
-            if (part_i && seen && t >= first) seen = mask >> (t - first) & 1;
-            float s = -__builtin_inff();
-            if (seen) {
-                s = 0.0f;
-                for (int d = 0; d < DIM; ++d)
-                    s = fmaf(q[d], cache_value<DIM, BITS, GS, F16>(k, base + t, d), s);
-                s *= p.scale_log2e;
-            }
-            float best = s;
-            for (int d = 1; d < 64; d *= 2) best = fmaxf(best, __shfl_xor(best, d));
-            if (tid % 64 == 0) part[tid / 64] = best;
-            __syncthreads();
-            for (int w = 0; w < DFQ_KV_THREADS / 64; ++w) best = fmaxf(best, part[w]);
-            const float next = fmaxf(top, best);
-            prob[tid] = seen ? exp2f(s - next) : 0.0f;
-            const float keep = top == next ? 1.0f : exp2f(top - next);
-            top = next;
-            __syncthreads();
-            sum *= keep;
-            acc *= keep;
-            const int most = n - t0 < DFQ_KV_THREADS ? n - t0 : DFQ_KV_THREADS;
-            for (int i = 0; i < most; ++i) {
-                const float w = prob[i];
-                sum += w;
-                /* a hidden token's value takes no part, whatever it is */
-                if (tid < DIM && (w != 0.0f || w != w))
-                    acc = fmaf(w, cache_value<DIM, BITS, GS, F16>(v, base + t0 + i, tid), acc);
-            }
-            __syncthreads();
-        }
-    }
-    const int64_t row = ((int64_t)b * p.rows + m) * p.q_heads + hq;
-    if (tid < DIM) p.y[row * DIM + tid] = f32_to_out<F16>(sum == 0.0f ? 0.0f : acc / sum);
-    if (p.lse && tid == 0)
-        p.lse[row] = sum == 0.0f ? -__builtin_inff() : (top + log2f(sum)) * 0.69314718056f;
-}
-
 }  // namespace
 
 #define DFQ_KV_KERNELS(dim, bits, gs, name, f16)                                               \
@@ -219,10 +144,6 @@ __device__ __forceinline__ void attention(const KvAttnParams& p) {
     extern "C" __global__ __launch_bounds__(DFQ_KV_THREADS) void                               \
         dfq_cache_read_d##dim##_b##bits##_g##gs##_##name(KvReadParams p, int out_dt) {         \
         read_rows<dim, bits, gs, f16>(p, out_dt);                                              \
-    }                                                                                          \
-    extern "C" __global__ __launch_bounds__(DFQ_KV_THREADS) void                               \
-        dfq_cache_attention_d##dim##_b##bits##_g##gs##_##name(KvAttnParams p) {                \
-        attention<dim, bits, gs, f16>(p);                                                      \
     }
 #define DFQ_KV_DTYPES(dim, bits, gs)            \
     DFQ_KV_KERNELS(dim, bits, gs, bf16, false)  \

@@ -39,9 +39,16 @@ struct KvAttnParams {
     float* lse;              /* [batch][rows][q_heads] or NULL                   */
     const int32_t* lengths;  /* own tokens of each sequence, the block's included */
     const uint32_t* tree;    /* [batch][rows] row masks or NULL (a chain)        */
+    /* The parts of a row from each range of tokens: [slot][head][row] pairs (offset, sum) and
+     * [slot][head][row][dim] sums in the kernel's channel order; slots are the prefix's ranges,
+     * then the own caches' ranges. */
+    float* part_ml;
+    float* part_o;
     int64_t q_stride;
     int prefix_length, prefix_capacity, own_capacity, max_length;
-    int batch, rows, heads, q_heads;
+    int batch, rows, heads, group;      /* group: query heads of a K/V head         */
+    int prefix_splits, prefix_blocks;   /* ranges of the prefix; blocks of its rows */
+    int own_splits, own_blocks;         /* the same for one sequence                */
     float scale_log2e;       /* softmax scale * log2(e)                          */
 };
 

@@ -1,9 +1,11 @@
 /*
  * verify_ops.cpp -- the C ABI of the quantised key/value cache, its attention and the log
- * probabilities: argument checks, work splits and launches of kv_cache.hip and logprobs.hip.
+ * probabilities: argument checks, work splits and launches of kv_cache.hip, kv_attention.hip and
+ * logprobs.hip.
  */
 #include <hip/hip_runtime_api.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <cstdio>
@@ -13,37 +15,39 @@
 #include "kv_params.h"
 #include "qmm_internal.h"
 
-#if !defined(DFQ_KV_HSACO_PATH) || !defined(DFQ_LOGPROBS_HSACO_PATH)
-#error "DFQ_KV_HSACO_PATH and DFQ_LOGPROBS_HSACO_PATH must name the gfx950 code objects to embed"
+#if !defined(DFQ_KV_HSACO_PATH) || !defined(DFQ_LOGPROBS_HSACO_PATH) || \
+    !defined(DFQ_ATTN64_HSACO_PATH) || !defined(DFQ_ATTN128_HSACO_PATH) || \
+    !defined(DFQ_ATTN256_HSACO_PATH)
+#error "DFQ_*_HSACO_PATH must name the gfx950 code objects to embed"
 #endif
 
-__asm__(".section .rodata.dfq_verify_hsaco,\"a\",@progbits\n"
-        ".p2align 12\n"
-        ".globl dfq_kv_hsaco_begin\n"
-        ".hidden dfq_kv_hsaco_begin\n"
-        "dfq_kv_hsaco_begin:\n"
-        ".incbin \"" DFQ_KV_HSACO_PATH "\"\n"
-        ".byte 0\n"
-        ".p2align 12\n"
-        ".globl dfq_logprobs_hsaco_begin\n"
-        ".hidden dfq_logprobs_hsaco_begin\n"
-        "dfq_logprobs_hsaco_begin:\n"
-        ".incbin \"" DFQ_LOGPROBS_HSACO_PATH "\"\n"
-        ".byte 0\n"
-        ".previous\n");
-extern "C" const char dfq_kv_hsaco_begin[];
-extern "C" const char dfq_logprobs_hsaco_begin[];
+#define DFQ_EMBED(name, path)                      \
+    __asm__(".section .rodata.dfq_verify_hsaco,\"a\",@progbits\n" \
+            ".p2align 12\n"                        \
+            ".globl " #name "\n"                   \
+            ".hidden " #name "\n"                  \
+            #name ":\n"                            \
+            ".incbin \"" path "\"\n"              \
+            ".byte 0\n"                            \
+            ".previous\n");                        \
+    extern "C" const char name[];
+DFQ_EMBED(dfq_kv_hsaco, DFQ_KV_HSACO_PATH)
+DFQ_EMBED(dfq_logprobs_hsaco, DFQ_LOGPROBS_HSACO_PATH)
+DFQ_EMBED(dfq_attn64_hsaco, DFQ_ATTN64_HSACO_PATH)
+DFQ_EMBED(dfq_attn128_hsaco, DFQ_ATTN128_HSACO_PATH)
+DFQ_EMBED(dfq_attn256_hsaco, DFQ_ATTN256_HSACO_PATH)
 
 namespace dfq {
 
 /* One format of a cache: [head_dim 64/128/256][bits 4/8][group 32/64/128][bf16/f16]; groups wider
  * than the head have no kernels. */
 struct CacheKernels {
-    hipFunction_t append = nullptr, read = nullptr, attention = nullptr;
+    hipFunction_t append = nullptr, read = nullptr, join = nullptr;
+    hipFunction_t attention[3] = {};  // 1, 2 and 4 row tiles, as many as attention_tiles gives
 };
 
 struct VerifyOps {
-    hipModule_t kv = nullptr, logprobs = nullptr;
+    hipModule_t kv = nullptr, logprobs = nullptr, attention[3] = {};
     CacheKernels cache[3][2][3][2];
     hipFunction_t token_logprobs[3] = {};  // [bf16/f16/f32]
 };
@@ -52,27 +56,48 @@ static dfq_status hip_error(hipError_t e, const char* what) {
     return fail(DFQ_ERR_HIP, "%s: %s (%d)", what, hipGetErrorString(e), (int)e);
 }
 
+/* The most tiles of 16 rows that a format's attention kernels take in one pass: what the
+ * registers hold (outputs, and the sums of every group). */
+static int attention_tiles(int dim, int gs) {
+    if (dim == 256) return gs == 128 ? 2 : 1;
+    return dim == 128 && gs == 32 ? 2 : 4;
+}
+
 static dfq_status resolve(VerifyOps* o) {
     static const char* kDt[3] = {"bf16", "f16", "f32"};
     hipError_t e;
-    if ((e = hipModuleLoadData(&o->kv, dfq_kv_hsaco_begin)) != hipSuccess)
+    if ((e = hipModuleLoadData(&o->kv, dfq_kv_hsaco)) != hipSuccess)
         return hip_error(e, "hipModuleLoadData(gfx950 cache object)");
-    if ((e = hipModuleLoadData(&o->logprobs, dfq_logprobs_hsaco_begin)) != hipSuccess)
+    if ((e = hipModuleLoadData(&o->logprobs, dfq_logprobs_hsaco)) != hipSuccess)
         return hip_error(e, "hipModuleLoadData(gfx950 log-probability object)");
     char name[80];
+    static const char* kAttn[3] = {dfq_attn64_hsaco, dfq_attn128_hsaco, dfq_attn256_hsaco};
+    for (int d = 0; d < 3; ++d)
+        if ((e = hipModuleLoadData(&o->attention[d], kAttn[d])) != hipSuccess)
+            return hip_error(e, "hipModuleLoadData(gfx950 attention object)");
     for (int d = 0; d < 3; ++d)
         for (int b = 0; b < 2; ++b)
             for (int g = 0; g < 3 && 32 << g <= 64 << d; ++g)
                 for (int t = 0; t < 2; ++t) {
                     CacheKernels& c = o->cache[d][b][g][t];
                     const struct { const char* op; hipFunction_t* fn; } parts[] = {
-                        {"append", &c.append}, {"read", &c.read}, {"attention", &c.attention}};
+                        {"append", &c.append}, {"read", &c.read}};
                     for (const auto& part : parts) {
                         snprintf(name, sizeof name, "dfq_cache_%s_d%d_b%d_g%d_%s", part.op,
                                  64 << d, 4 << b, 32 << g, kDt[t]);
                         if ((e = hipModuleGetFunction(part.fn, o->kv, name)) != hipSuccess)
                             return hip_error(e, name);
                     }
+                    for (int r = 0; 1 << r <= attention_tiles(64 << d, 32 << g); ++r) {
+                        snprintf(name, sizeof name, "dfq_cache_attention_b%d_g%d_%s_r%d", 4 << b,
+                                 32 << g, kDt[t], 1 << r);
+                        if ((e = hipModuleGetFunction(&c.attention[r], o->attention[d], name)) !=
+                            hipSuccess)
+                            return hip_error(e, name);
+                    }
+                    snprintf(name, sizeof name, "dfq_cache_attention_join_g%d_%s", 32 << g, kDt[t]);
+                    if ((e = hipModuleGetFunction(&c.join, o->attention[d], name)) != hipSuccess)
+                        return hip_error(e, name);
                 }
     for (int t = 0; t < 3; ++t) {
         snprintf(name, sizeof name, "dfq_token_logprobs_%s", kDt[t]);
@@ -99,6 +124,8 @@ void verify_ops_unload(VerifyOps* o) {
     if (!o) return;
     if (o->kv) (void)hipModuleUnload(o->kv);
     if (o->logprobs) (void)hipModuleUnload(o->logprobs);
+    for (hipModule_t m : o->attention)
+        if (m) (void)hipModuleUnload(m);
     delete o;
 }
 
@@ -215,6 +242,50 @@ dfq_status check_attention(const dfq_kv_cache* prefix, int prefix_length,
     return DFQ_OK;
 }
 
+/* How an attention call is cut: row blocks of tiles * 16 rows, and ranges of tokens. */
+struct AttentionPlan {
+    int tiles_log2 = 0;
+    int prefix_splits = 0, prefix_blocks = 0, own_splits = 0, own_blocks = 0;
+    int64_t rows = 0;   /* part rows of a slot: heads * batch * rows * group */
+    size_t ml_bytes = 0, bytes = 0;
+    int64_t groups(int heads, int batch) const {
+        return (int64_t)heads * ((int64_t)prefix_splits * prefix_blocks +
+                                 (int64_t)batch * own_splits * own_blocks);
+    }
+};
+
+/* Tokens that a workgroup takes in one round, 32 a wave. */
+constexpr int kRoundTokens = DFQ_KV_THREADS / 2;
+
+AttentionPlan plan_attention(int num_cus, const dfq_kv_cache* fmt, int prefix_length,
+                             int max_length, int batch, int rows, int q_heads) {
+    AttentionPlan a;
+    const int group = q_heads / fmt->heads;
+    const int64_t own_rows = (int64_t)rows * group, all_rows = own_rows * batch;
+    const int most = attention_tiles(fmt->head_dim, fmt->group_size);
+    /* no more row tiles than the larger row block has */
+    const int64_t need = prefix_length ? all_rows : own_rows;
+    while ((1 << a.tiles_log2) < most && (int64_t)16 << a.tiles_log2 < need) ++a.tiles_log2;
+    const int block = 16 << a.tiles_log2;
+    a.rows = fmt->heads * all_rows;
+    a.prefix_blocks = (int)((all_rows + block - 1) / block);
+    a.own_blocks = (int)((own_rows + block - 1) / block);
+    /* the shortest ranges that keep every workgroup resident at once */
+    const int resident = num_cus * (a.tiles_log2 == 0 ? 3 : a.tiles_log2 == 1 ? 2 : 1);
+    const int prefix_rounds = (prefix_length + kRoundTokens - 1) / kRoundTokens;
+    const int own_rounds = (max_length + kRoundTokens - 1) / kRoundTokens;
+    const int longest = std::max(prefix_rounds, own_rounds);
+    for (int each = 1; each <= longest; each = each < 16 ? each + 1 : each + each / 16) {
+        a.prefix_splits = (prefix_rounds + each - 1) / each;
+        a.own_splits = (own_rounds + each - 1) / each;
+        if (a.groups(fmt->heads, batch) <= resident) break;
+    }
+    const size_t slots = (size_t)a.prefix_splits + a.own_splits;
+    a.ml_bytes = (slots * a.rows * 8 + 255) & ~(size_t)255;
+    a.bytes = a.ml_bytes + slots * a.rows * fmt->head_dim * 4;
+    return a;
+}
+
 }  // namespace
 
 extern "C" {
@@ -271,7 +342,12 @@ dfq_status dfq_cache_attention_workspace_bytes(dfq_ctx* ctx, const dfq_kv_cache*
     *bytes = 0;
     if (!ctx) return fail(DFQ_ERR_INVALID_ARGUMENT, "null context");
     const dfq_kv_cache* fmt;
-    return check_attention(prefix, prefix_length, cache, max_length, batch, rows, q_heads, &fmt);
+    dfq_status s =
+        check_attention(prefix, prefix_length, cache, max_length, batch, rows, q_heads, &fmt);
+    if (s) return s;
+    *bytes = plan_attention(dfq_num_cus(ctx), fmt, prefix_length, max_length, batch, rows, q_heads)
+                 .bytes;
+    return DFQ_OK;
 }
 
 dfq_status dfq_cache_attention(dfq_ctx* ctx, const dfq_kv_cache* prefix, int prefix_length,
@@ -294,8 +370,17 @@ dfq_status dfq_cache_attention(dfq_ctx* ctx, const dfq_kv_cache* prefix, int pre
         return fail(DFQ_ERR_INVALID_ARGUMENT, "q_stride is smaller than a row");
     if (!(scale > 0.0f) || !std::isfinite(scale))
         return fail(DFQ_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
-    (void)workspace;
-    (void)workspace_bytes;
+    const AttentionPlan a =
+        plan_attention(dfq_num_cus(ctx), fmt, prefix_length, max_length, batch, rows, q_heads);
+    const int64_t groups = a.groups(fmt->heads, batch);
+    const int group = q_heads / fmt->heads;
+    if (groups > INT32_MAX || (int64_t)batch * rows * group > INT32_MAX)
+        return fail(DFQ_ERR_UNSUPPORTED, "grid too large");
+    if (a.bytes && (!workspace || workspace_bytes < a.bytes))
+        return fail(DFQ_ERR_WORKSPACE, "workspace of %zu bytes needed (got %zu)", a.bytes,
+                    workspace ? workspace_bytes : (size_t)0);
+    if (!aligned(workspace, 16))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
     KvAttnParams p{};
     if (prefix)
         for (int i = 0; i < 2; ++i) p.prefix[i] = arrays_of(prefix, i);
@@ -306,6 +391,8 @@ dfq_status dfq_cache_attention(dfq_ctx* ctx, const dfq_kv_cache* prefix, int pre
     p.lse = lse;
     p.lengths = lengths;
     p.tree = tree;
+    p.part_ml = (float*)workspace;
+    p.part_o = (float*)((char*)workspace + a.ml_bytes);
     p.q_stride = q_stride;
     p.prefix_length = prefix_length;
     p.prefix_capacity = prefix ? prefix->capacity : 0;
@@ -314,13 +401,23 @@ dfq_status dfq_cache_attention(dfq_ctx* ctx, const dfq_kv_cache* prefix, int pre
     p.batch = batch;
     p.rows = rows;
     p.heads = fmt->heads;
-    p.q_heads = q_heads;
+    p.group = group;
+    p.prefix_splits = a.prefix_splits;
+    p.prefix_blocks = a.prefix_blocks;
+    p.own_splits = a.own_splits;
+    p.own_blocks = a.own_blocks;
     p.scale_log2e = scale * 1.44269504088896340736f;
+    const CacheKernels& fn = kernels_of(ctx, fmt);
     DeviceScope scope(ctx);
     void* args[] = {&p};
-    const hipError_t e = hipModuleLaunchKernel(
-        kernels_of(ctx, fmt).attention, (unsigned)q_heads, (unsigned)rows, (unsigned)batch,
-        DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
+    hipError_t e = hipSuccess;
+    if (groups)
+        e = hipModuleLaunchKernel(fn.attention[a.tiles_log2], (unsigned)groups, 1, 1,
+                                  DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
+    if (e == hipSuccess)
+        e = hipModuleLaunchKernel(fn.join, (unsigned)(batch * rows * group),
+                                  (unsigned)fmt->heads, 1, DFQ_KV_THREADS, 1, 1, 0,
+                                  (hipStream_t)stream, args, nullptr);
     return e == hipSuccess ? DFQ_OK : hip_error(e, "launch dfq_cache_attention");
 }
 
