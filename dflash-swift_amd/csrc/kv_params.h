@@ -59,8 +59,11 @@ struct LogprobParams {
     float* entropy;
     int32_t* top_tokens;
     float* top_logprobs;
+    uint64_t* part_keys;     /* [row][part][top]: its best order keys, 0 where it has fewer */
+    float* part_sums;        /* [row][part][4]: maximum, sum, entropy sum                   */
     int64_t row_stride;
     int rows, vocab, top;
+    int splits;              /* workgroups a row; parts = splits * waves                    */
 };
 
 #endif

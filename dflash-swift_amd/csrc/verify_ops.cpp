@@ -49,7 +49,7 @@ struct CacheKernels {
 struct VerifyOps {
     hipModule_t kv = nullptr, logprobs = nullptr, attention[3] = {};
     CacheKernels cache[3][2][3][2];
-    hipFunction_t token_logprobs[3] = {};  // [bf16/f16/f32]
+    hipFunction_t logprobs_part[3] = {}, logprobs_join[3] = {};  // [bf16/f16/f32]
 };
 
 static dfq_status hip_error(hipError_t e, const char* what) {
@@ -101,7 +101,10 @@ static dfq_status resolve(VerifyOps* o) {
                 }
     for (int t = 0; t < 3; ++t) {
         snprintf(name, sizeof name, "dfq_token_logprobs_%s", kDt[t]);
-        if ((e = hipModuleGetFunction(&o->token_logprobs[t], o->logprobs, name)) != hipSuccess)
+        if ((e = hipModuleGetFunction(&o->logprobs_part[t], o->logprobs, name)) != hipSuccess)
+            return hip_error(e, name);
+        snprintf(name, sizeof name, "dfq_token_logprobs_join_%s", kDt[t]);
+        if ((e = hipModuleGetFunction(&o->logprobs_join[t], o->logprobs, name)) != hipSuccess)
             return hip_error(e, name);
     }
     return DFQ_OK;
@@ -429,12 +432,29 @@ static dfq_status check_logprobs(int M, int V, int top_k) {
     return DFQ_OK;
 }
 
+/* Workgroups a row: ranges of 1024 logits a wave or more, for about eight workgroups a CU. */
+static int logprob_splits(int num_cus, int M, int V) {
+    const int most = std::max(1, 8 * num_cus / M);
+    return std::min({most, (int)(((int64_t)V + 4095) / 4096), 64});
+}
+
+/* The keys of a row's parts, then their sums; 4 waves a workgroup. */
+static size_t logprob_keys_bytes(int M, int splits, int top_k) {
+    return ((size_t)M * splits * (DFQ_KV_THREADS / 64) * top_k * 8 + 15) & ~(size_t)15;
+}
+static size_t logprob_bytes(int M, int splits, int top_k) {
+    return logprob_keys_bytes(M, splits, top_k) + (size_t)M * splits * (DFQ_KV_THREADS / 64) * 16;
+}
+
 dfq_status dfq_token_logprobs_workspace_bytes(dfq_ctx* ctx, int M, int V, int top_k,
                                               size_t* bytes) {
     if (!bytes) return fail(DFQ_ERR_INVALID_ARGUMENT, "null bytes");
     *bytes = 0;
     if (!ctx) return fail(DFQ_ERR_INVALID_ARGUMENT, "null context");
-    return check_logprobs(M, V, top_k);
+    const dfq_status s = check_logprobs(M, V, top_k);
+    if (s) return s;
+    *bytes = logprob_bytes(M, logprob_splits(dfq_num_cus(ctx), M, V), top_k);
+    return DFQ_OK;
 }
 
 dfq_status dfq_token_logprobs(dfq_ctx* ctx, const void* logits, int64_t row_stride, int M, int V,
@@ -457,15 +477,27 @@ dfq_status dfq_token_logprobs(dfq_ctx* ctx, const void* logits, int64_t row_stri
         !aligned(logprobs, 4) || !aligned(entropy, 4) || !aligned(top_tokens, 4) ||
         !aligned(top_logprobs, 4))
         return fail(DFQ_ERR_INVALID_ARGUMENT, "misaligned buffer");
-    (void)workspace;
-    (void)workspace_bytes;
-    LogprobParams p{logits, tokens, logprobs, entropy, top_tokens, top_logprobs, row_stride, M, V,
-                    top_k};
+    const int splits = logprob_splits(dfq_num_cus(ctx), M, V);
+    const size_t need = logprob_bytes(M, splits, top_k);
+    if (!workspace || workspace_bytes < need)
+        return fail(DFQ_ERR_WORKSPACE, "workspace of %zu bytes needed (got %zu)", need,
+                    workspace ? workspace_bytes : (size_t)0);
+    if (!aligned(workspace, 16))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
+    if ((int64_t)M * splits > INT32_MAX) return fail(DFQ_ERR_UNSUPPORTED, "grid too large");
+    LogprobParams p{logits, tokens, logprobs, entropy, top_tokens, top_logprobs,
+                    (uint64_t*)workspace,
+                    (float*)((char*)workspace + logprob_keys_bytes(M, splits, top_k)), row_stride,
+                    M, V, top_k, splits};
+    const VerifyOps* ops = ctx_verify_ops(ctx);
     DeviceScope scope(ctx);
     void* args[] = {&p};
-    const hipError_t e = hipModuleLaunchKernel(
-        ctx_verify_ops(ctx)->token_logprobs[(int)dtype], (unsigned)M, 1, 1, DFQ_KV_THREADS, 1, 1,
-        0, (hipStream_t)stream, args, nullptr);
+    hipError_t e = hipModuleLaunchKernel(ops->logprobs_part[(int)dtype], (unsigned)M * splits, 1,
+                                         1, DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args,
+                                         nullptr);
+    if (e == hipSuccess)
+        e = hipModuleLaunchKernel(ops->logprobs_join[(int)dtype], (unsigned)M, 1, 1, 64, 1, 1, 0,
+                                  (hipStream_t)stream, args, nullptr);
     return e == hipSuccess ? DFQ_OK : hip_error(e, "launch dfq_token_logprobs");
 }
 
