@@ -214,6 +214,13 @@ def _stream(stream) -> int | None:
     return stream.cuda_stream or None
 
 
+def _current_stream(device: int) -> int:
+    """Handle of torch's current stream on a device."""
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
+
+
 def dtype_code(t) -> int:
     """dfq dtype code of a torch dtype (or tensor)."""
     import torch
@@ -234,6 +241,7 @@ class Context:
         # replaces the old, which is kept (a graph or another stream may still hold it)
         self._ws = {}
         self._scratch = {}
+        self._need = ctypes.c_size_t()
         self._retired = []
 
     def close(self):
@@ -441,17 +449,19 @@ class Context:
         """Quantise rows k, v [batch, rows, heads*head_dim] (the cache's dtype; rows may be cut
         from a fused output) into slots 0..batch-1 of `cache` at positions start + starts[b] +
         0, 1, ... (starts: int32 [batch] on the device)."""
-        if k.shape != v.shape or k.dim() != 3 or k.shape[2] != cache.heads * cache.head_dim:
+        shape = k.shape
+        if len(shape) != 3 or v.shape != shape or shape[2] != cache.heads * cache.head_dim:
             raise ValueError("k and v are [batch, rows, heads*head_dim]")
-        batch, rows, _ = k.shape
         stride = _row_stride(k)
         if _row_stride(v) != stride:
             raise ValueError("k and v must have the same strides")
-        cache.check_dtype(k, v)
-        _check_int32("starts", starts, (batch,))
-        _check(self.lib.dfq_cache_append(self.handle, cache.desc, k.data_ptr(), v.data_ptr(),
-                                         stride, batch, rows, start, _ptr(starts),
-                                         _stream(stream)), "dfq_cache_append")
+        if k.dtype != cache.dtype or v.dtype != cache.dtype:
+            raise ValueError(f"the cache holds {cache.dtype}")
+        st = self.lib.dfq_cache_append(
+            self.handle, cache.desc, k.data_ptr(), v.data_ptr(), stride, shape[0], shape[1], start,
+            _check_int32("starts", starts, shape[:1]), self._stream_of(stream))
+        if st:
+            _check(st, "dfq_cache_append")
 
     def cache_read(self, cache, rows, start=0, starts=None, batch=None, dtype=None, k=None,
                    v=None, stream=None):
@@ -460,7 +470,6 @@ class Context:
         import torch
         if batch is None:
             batch = cache.slots if starts is None else starts.shape[0]
-        _check_int32("starts", starts, (batch,))
         dt = cache.dtype if dtype is None else dtype
         shape = (batch, rows, cache.heads, cache.head_dim)
         for a in (k, v):
@@ -470,9 +479,11 @@ class Context:
             k = torch.empty(shape, dtype=dt, device=cache.device)
         if v is None:
             v = torch.empty(shape, dtype=dt, device=cache.device)
-        _check(self.lib.dfq_cache_read(self.handle, cache.desc, k.data_ptr(), v.data_ptr(),
-                                       dtype_code(dt), batch, rows, start, _ptr(starts),
-                                       _stream(stream)), "dfq_cache_read")
+        st = self.lib.dfq_cache_read(
+            self.handle, cache.desc, k.data_ptr(), v.data_ptr(), dtype_code(dt), batch, rows,
+            start, _check_int32("starts", starts, (batch,)), self._stream_of(stream))
+        if st:
+            _check(st, "dfq_cache_read")
         return k, v
 
     def cache_attention(self, q, cache=None, lengths=None, max_length=None, prefix=None,
@@ -490,13 +501,15 @@ class Context:
         fmt = cache if cache is not None else prefix
         if fmt is None:
             raise ValueError("cache_attention needs a cache or a prefix")
-        if q.dim() != 3 or q.shape[2] % fmt.head_dim:
+        shape = q.shape
+        if len(shape) != 3 or shape[2] % fmt.head_dim:
             raise ValueError("q is [batch, rows, q_heads*head_dim]")
-        batch, rows, width = q.shape
+        batch, rows, width = shape
         heads = width // fmt.head_dim
-        fmt.check_dtype(q)
-        _check_int32("lengths", lengths, (batch,))
-        _check_int32("tree", tree, (batch, rows))
+        if q.dtype != fmt.dtype:
+            raise ValueError(f"the cache holds {fmt.dtype}, got {q.dtype}")
+        d_lengths = _check_int32("lengths", lengths, (batch,))
+        d_tree = _check_int32("tree", tree, (batch, rows))
         if max_length is None:
             max_length = cache.capacity if cache is not None else 0
         if prefix_length is None:
@@ -504,8 +517,8 @@ class Context:
         if scale is None:
             scale = fmt.head_dim ** -0.5
         if out is None:
-            out = torch.empty((batch, rows, width), dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+            out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        elif out.shape != shape or out.dtype != q.dtype or not out.is_contiguous():
             raise ValueError("out is contiguous, of q's shape and dtype")
         if lse is None:
             lse = torch.empty((batch, rows, heads), dtype=torch.float32, device=q.device)
@@ -514,17 +527,20 @@ class Context:
             raise ValueError("lse is contiguous fp32 [batch, rows, q_heads]")
         pd = prefix.desc if prefix is not None else None
         cd = cache.desc if cache is not None else None
+        stream = self._stream_of(stream)
         if ws is None:
-            need = ctypes.c_size_t()
-            _check(self.lib.dfq_cache_attention_workspace_bytes(
-                self.handle, pd, prefix_length, cd, max_length, batch, rows, heads,
-                ctypes.byref(need)), "dfq_cache_attention_workspace_bytes")
-            ws = self.workspace_uncleared(need.value, stream)
-        _check(self.lib.dfq_cache_attention(
-            self.handle, pd, prefix_length, cd, _ptr(lengths), max_length, _ptr(tree),
-            q.data_ptr(), _row_stride(q), out.data_ptr(), lse.data_ptr(), batch, rows, heads,
-            scale, _ptr(ws), ws.numel() if ws is not None else 0, _stream(stream)),
-            "dfq_cache_attention")
+            st = self.lib.dfq_cache_attention_workspace_bytes(
+                self.handle, pd, prefix_length, cd, max_length, batch, rows, heads, self._need)
+            if st:
+                _check(st, "dfq_cache_attention_workspace_bytes")
+            ws = self.workspace_uncleared(self._need.value, stream)
+        ws_ptr, ws_bytes = (ws.data_ptr(), ws.numel()) if ws is not None else (None, 0)
+        st = self.lib.dfq_cache_attention(
+            self.handle, pd, prefix_length, cd, d_lengths, max_length, d_tree, q.data_ptr(),
+            _row_stride(q), out.data_ptr(), lse.data_ptr(), batch, rows, heads, scale, ws_ptr,
+            ws_bytes, stream)
+        if st:
+            _check(st, "dfq_cache_attention")
         return out, lse
 
     def token_logprobs(self, logits, tokens=None, top_k=0, ws=None, stream=None):
@@ -534,42 +550,52 @@ class Context:
         if logits.dim() != 2 or logits.stride(1) != 1:
             raise ValueError("logits are [M, V] with contiguous rows")
         M, V = logits.shape
-        _check_int32("tokens", tokens, (M,))
-        dev = logits.device
-        lp = torch.empty(M, dtype=torch.float32, device=dev) if tokens is not None else None
-        entropy = torch.empty(M, dtype=torch.float32, device=dev)
+        d_tokens = _check_int32("tokens", tokens, (M,))
+        # the fp32 outputs of one allocation, as wide as they are asked for
+        more = top_k if top_k > 0 else 0
+        f = torch.empty(M * (2 + more), dtype=torch.float32, device=logits.device)
+        entropy = f[:M]
+        lp = f[M:2 * M] if tokens is not None else None
+        p = f.data_ptr()
         ids = top = None
-        if top_k > 0:
-            ids = torch.empty((M, top_k), dtype=torch.int32, device=dev)
-            top = torch.empty((M, top_k), dtype=torch.float32, device=dev)
+        if more:
+            ids = torch.empty((M, more), dtype=torch.int32, device=logits.device)
+            top = f[2 * M:].view(M, more)
+        stream = self._stream_of(stream)
         if ws is None:
-            need = ctypes.c_size_t()
-            _check(self.lib.dfq_token_logprobs_workspace_bytes(self.handle, M, V, top_k,
-                                                               ctypes.byref(need)),
-                   "dfq_token_logprobs_workspace_bytes")
-            ws = self.workspace_uncleared(need.value, stream)
-        _check(self.lib.dfq_token_logprobs(
+            st = self.lib.dfq_token_logprobs_workspace_bytes(self.handle, M, V, top_k, self._need)
+            if st:
+                _check(st, "dfq_token_logprobs_workspace_bytes")
+            ws = self.workspace_uncleared(self._need.value, stream)
+        st = self.lib.dfq_token_logprobs(
             self.handle, logits.data_ptr(), logits.stride(0) if M > 1 else V, M, V,
-            dtype_code(logits), _ptr(tokens), top_k, _ptr(lp), entropy.data_ptr(), _ptr(ids),
-            _ptr(top), _ptr(ws), ws.numel() if ws is not None else 0, _stream(stream)),
-            "dfq_token_logprobs")
+            dtype_code(logits), d_tokens, top_k, p + 4 * M if tokens is not None else None, p,
+            ids.data_ptr() if more else None, p + 8 * M if more else None,
+            ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, stream)
+        if st:
+            _check(st, "dfq_token_logprobs")
         return lp, entropy, ids, top
 
+    def _stream_of(self, stream):
+        """A stream's handle: the one given, or torch's current one on this context's device."""
+        if stream is None:
+            return _current_stream(self.device) or None
+        return _stream(stream)
+
     def workspace_uncleared(self, nbytes: int, stream=None):
-        """Scratch of the calls whose workspace needs no clearing, one per stream, apart from
-        `workspace`'s (which those calls would not leave zero); a grown one replaces the old,
-        which is kept as there."""
-        import torch
-        if nbytes == 0:
-            return None
-        key = _stream(stream)
-        ws = self._scratch.get(key)
+        """Scratch of the calls whose workspace needs no clearing, one per stream (a handle or
+        None for the default stream), apart from `workspace`'s (which those calls would not
+        leave zero); a grown one replaces the old, which is kept as there."""
+        ws = self._scratch.get(stream)
         if ws is None or ws.numel() < nbytes:
+            import torch
+            if nbytes == 0:
+                return None
             if ws is not None:
                 self._retired.append(ws)
             ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8,
                              device=f"cuda:{self.device}")
-            self._scratch[key] = ws
+            self._scratch[stream] = ws
         return ws
 
     # ---- the packed layout ---------------------------------------------------------------
@@ -691,20 +717,22 @@ def _row_stride(t) -> int:
     """Elements between the rows of t [batch, rows, width], the same within and across
     sequences."""
     batch, rows, width = t.shape
-    if t.stride(2) != 1 and width > 1:
+    outer, inner, one = t.stride()
+    if one != 1 and width > 1:
         raise ValueError("a row's elements must be contiguous")
-    stride = t.stride(1) if rows > 1 else t.stride(0) if batch > 1 else width
-    if batch > 1 and rows > 1 and t.stride(0) != rows * stride:
+    stride = inner if rows > 1 else outer if batch > 1 else width
+    if batch > 1 and rows > 1 and outer != rows * stride:
         raise ValueError("rows must be evenly spaced across sequences")
     return stride
 
 
 def _check_int32(name, t, shape):
     if t is None:
-        return
+        return None
     import torch
     if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} is a contiguous int32 tensor of shape {shape}")
+    return t.data_ptr()
 
 
 class KVCache:
@@ -748,11 +776,6 @@ class KVCache:
         d = _KVCacheDesc(*(a.data_ptr() for a in (*k, *v)), self.slots, self.heads,
                          self.capacity, self.head_dim, bits, group_size, dtype_code(self.dtype))
         self._desc, self.desc = d, ctypes.addressof(d)
-
-    def check_dtype(self, *tensors):
-        for t in tensors:
-            if t.dtype != self.dtype:
-                raise ValueError(f"the cache holds {self.dtype}, got {t.dtype}")
 
 
 class PackedWeight:
