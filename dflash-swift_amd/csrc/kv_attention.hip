@@ -20,14 +20,16 @@ constexpr int kDim = DFQ_HEAD_DIM;
 constexpr int kWaves = DFQ_KV_THREADS / 64;
 constexpr float kNever = -1e30f;      /* the offset of a row that has seen nothing */
 
-typedef uint32_t u32_any __attribute__((aligned(2)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
-typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
 /* fp16 operands hold codes as the denormal numbers c 2^-24 (or 16 c 2^-24 where a code stays in
  * the upper nibble of a byte), which the matrix cores multiply exactly: a code costs a mask, and
  * no conversion.  The sums are scaled back by 2^24. */
 constexpr float kUnit = 16777216.0f;
+/* Scores are kept 2^-8 of what the scaled queries give, so that a query's sums fit fp16. */
+constexpr float kScaleUnit = kUnit / 256.0f;
+constexpr float kMost = 3.38e38f;     /* finite numbers below it stay so in bf16 */
 
 template <bool F16>
 __device__ __forceinline__ float half_of(uint32_t word, bool high) {
@@ -46,10 +48,28 @@ __device__ __forceinline__ f32x4_t mfma(f16x8_t a, f16x8_t b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+__device__ __forceinline__ f32x4_t mfma(bf16x8_t a, bf16x8_t b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+/* A pointer that is the same in every lane, in scalar registers. */
+__device__ __forceinline__ const char* uniform(const void* p) {
+    const uint64_t a = (uint64_t)(uintptr_t)p;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a);
+    const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+    return (const char*)(uintptr_t)((uint64_t)hi << 32 | lo);
+}
+
+/* Orders a wave's own LDS writes and reads. */
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 /* Everything of one (head, row block, token range) of a launch. */
 struct Job {
     const char *k, *v;          /* codes of the slot-and-head's first token        */
-    const uint16_t* scale;      /* this lane's array of scales or biases from there */
+    const uint16_t *scale, *bias;   /* this lane's (K's or V's) from there         */
     int64_t slot;       /* part slot of the range                                 */
     int row0, nrows;    /* rows of this block, among the head's batch*rows*group   */
     int t0, t1;         /* the range                                              */
@@ -61,76 +81,80 @@ template <int BITS, int GS, bool F16, int RT>
 struct Attention {
     static constexpr int kGroups = kDim / GS;
     static constexpr int kSteps = GS / 32;               /* matrix steps of a group    */
+    static constexpr int kChunk = kSteps < 2 ? 1 : 2;    /* steps read from LDS at once */
+    static constexpr int kChunks = kGroups * kSteps / kChunk;
+    static constexpr int kWords = kChunk * BITS / 4;     /* a lane's words of them     */
     static constexpr int kRowBytes = kDim * BITS / 8;
-    static constexpr int kKWords = GS * BITS / 128;      /* a lane's words of a group  */
     static constexpr int kTiles = GS / 16;               /* V column tiles of a group  */
     static constexpr int kVBytes = GS * BITS / 128;      /* a lane's bytes of a group  */
-    static constexpr int kVWords = kVBytes < 4 ? 4 : 8 * kVBytes / 4;
+    static constexpr int kTileBytes = 32 * kRowBytes;    /* codes of 32 tokens         */
+    static constexpr int kLoads = kTileBytes / 1024;     /* wave loads of them         */
+    /* K and V tiles in LDS: two of each, or one where two would leave a CU one workgroup. */
+    static constexpr int kBufs = kRowBytes <= 64 ? 2 : 1;
     static constexpr float kCentre = BITS == 4 ? 8.0f : 128.0f;
     static constexpr int kRows = 16 * RT;
+    /* column tiles that the waves exchange at a time when they join */
+    static constexpr int kMergeTiles = kDim / 16 < 4 ? kDim / 16 : 4;
+    using half8_t = std::conditional_t<F16, f16x8_t, bf16x8_t>;
 
-    struct KTile {
-        uint32_t code[2][kGroups][kKWords];
-        uint32_t scale[kGroups];   /* this lane's part of the tile's scales and biases */
-    };
-    struct VTile {
-        uint32_t code[kGroups][kVWords];
-    };
-    /* A wave's tile of scales and biases in fp32, by token: K's, V's; size: a token's largest
-     * finite V scale. */
+    /* A wave's tile of scales and biases, by token.  K's biases stay as they are stored: they
+     * meet the queries' sums in one matrix product.  So do, with bf16, V's and the weights. */
     struct Scales {
-        float s[4][kGroups][32];   /* K scales, K biases, V scales, V biases */
-        float size[32];
+        float k[kGroups][32];                  /* K scales * kScaleUnit                     */
+        float v[kGroups][32];                  /* V scales                                  */
+        float size[32];                        /* a token's largest V scale                 */
+        uint16_t kb[32 * kGroups];             /* K biases                                  */
+        union {
+            uint16_t parts[2 * kGroups][32];   /* bf16: V's b + centre s in two bf16 parts  */
+            float vb[kGroups][32];             /* fp16: the same in fp32                    */
+        };
     };
 
-    /* Lane l loads array l / 16 (K scales, K biases, V scales, V biases), tokens t + 2 (l % 16)
-     * and the next: 2 kGroups neighbouring 16-bit numbers. */
-    template <bool TAIL>
+    /* Lanes 0..31 load K's scale and bias of token t + lane, lanes 32..63 V's of t + lane - 32. */
+    struct TokenScales {
+        uint16_t s[kGroups], b[kGroups];
+    };
     static __device__ __forceinline__ void load_scales(const Job& job, int t, int lane,
-                                                       uint32_t (&out)[kGroups]) {
-        const int tok = t + 2 * (lane & 15);
-        if constexpr (!TAIL) {
-            const uint16_t* p = job.scale + (int64_t)tok * kGroups;
-#pragma unroll
-            for (int g = 0; g < kGroups; ++g) out[g] = *(const u32_any*)(p + 2 * g);
-        } else {
-            uint32_t h[2 * kGroups];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int64_t at = tok + r < job.n ? tok + r : job.n - 1;
-#pragma unroll
-                for (int g = 0; g < kGroups; ++g) h[r * kGroups + g] = job.scale[at * kGroups + g];
-            }
-#pragma unroll
-            for (int g = 0; g < kGroups; ++g) out[g] = h[2 * g] | h[2 * g + 1] << 16;
-        }
+                                                       TokenScales& out) {
+        int tok = t + (lane & 31);
+        if (tok >= job.n) tok = job.n - 1;
+        __builtin_memcpy(out.s, job.scale + (int64_t)tok * kGroups, 2 * kGroups);
+        __builtin_memcpy(out.b, job.bias + (int64_t)tok * kGroups, 2 * kGroups);
     }
 
-    /* Orders a wave's LDS writes and reads of its own tile of scales. */
-    static __device__ __forceinline__ void wave_fence() {
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-    }
-
-    static __device__ __forceinline__ void stage_scales(const uint32_t (&in)[kGroups], int lane,
+    /* A V group whose scale or bias is not finite (or the middle of its range past bf16) counts as a NaN scale and no bias: the rows
+     * that see it get NaN, and the others, whose weight is 0, nothing. */
+    static __device__ __forceinline__ void stage_scales(const TokenScales& in, int lane,
                                                         Scales& sc) {
-        const int arr = lane >> 4, tok = 2 * (lane & 15);
-        float size[2] = {0.0f, 0.0f};
-        wave_fence();
+        const int tok = lane & 31;
+        wave_order();
+        if (lane < 32) {
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-            float f[2];
+            for (int g = 0; g < kGroups; ++g) sc.k[g][tok] = elem_to_f32<F16>(in.s[g]) * kScaleUnit;
+            __builtin_memcpy(__builtin_assume_aligned(sc.kb + tok * kGroups, 2 * kGroups), in.b,
+                             2 * kGroups);
+        } else {
+            float size = 0.0f;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int i = r * kGroups + g;
-                f[r] = half_of<F16>(in[i >> 1], i & 1);
-                const float a = fabsf(f[r]);
-                size[r] = fmaxf(size[r], a < __builtin_inff() ? a : 0.0f);
+            for (int g = 0; g < kGroups; ++g) {
+                const float s = elem_to_f32<F16>(in.s[g]);
+                const float mid = fmaf(kCentre, s, elem_to_f32<F16>(in.b[g]));
+                const bool fine = fabsf(s) < __builtin_inff() && fabsf(mid) < kMost;
+                const float m = fine ? mid : 0.0f;
+                size = fmaxf(size, fine ? fabsf(s) : 0.0f);
+                sc.v[g][tok] = fine ? s : __builtin_nanf("");
+                if constexpr (F16) {
+                    sc.vb[g][tok] = m;
+                } else {
+                    const __bf16 hi = (__bf16)m;
+                    sc.parts[2 * g][tok] = __builtin_bit_cast(uint16_t, hi);
+                    sc.parts[2 * g + 1][tok] =
+                        __builtin_bit_cast(uint16_t, (__bf16)(m - (float)hi));
+                }
             }
-            *(f32x2_t*)&sc.s[arr][g][tok] = f32x2_t{f[0], f[1]};
+            sc.size[tok] = size;
         }
-        if (arr == 2) *(f32x2_t*)&sc.size[tok] = f32x2_t{size[0], size[1]};
-        wave_fence();
+        wave_order();
     }
 
     /* A lane's 8 tokens of one array and group: 4 c + 0..3 of each half of the tile. */
@@ -143,64 +167,50 @@ struct Attention {
         }
     }
 
-    /* K rows t .. t+31 (and all the tile's scales) as the row operand: lane l holds token l % 16 of each half and, of every
-     * group, the kSteps 8-channel pieces that its quarter l / 16 multiplies. */
-    template <bool TAIL>
-    static __device__ __forceinline__ void load_k(const Job& job, int t, int lane, KTile& k) {
-        const int row = lane & 15, c = lane >> 4;
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
-            int tok = t + 16 * tt + row;
-            if (TAIL && tok >= job.n) tok = job.n - 1;
-            const uint32_t at = (uint32_t)tok * kRowBytes + c * kKWords * 4;
-#pragma unroll
-            for (int g = 0; g < kGroups; ++g)
-                __builtin_memcpy(k.code[tt][g],
-                                 __builtin_assume_aligned(job.k + (at + g * (GS * BITS / 8)),
-                                                          kKWords < 4 ? kKWords * 4 : 16),
-                                 kKWords * 4);
-        }
-        load_scales<TAIL>(job, t, lane, k.scale);
+    /* Codes of tokens t .. t+31 straight into LDS, a row after the other as in memory, each row's
+     * 16-byte pieces exchanged by turn(): rows that one read instruction takes together then lie
+     * in different banks.  The instruction takes its LDS address from M0 and puts lane l's 16
+     * bytes 16 l behind it, so the exchange is made in the address that a lane loads from; the
+     * compiler does not see the loads, and loaded() waits for them.  Tokens past the last are the
+     * last. */
+    static constexpr int kPieces = kRowBytes / 16;
+    static __device__ __forceinline__ int turn(int row) {
+        if constexpr (kPieces <= 4) return row / (8 / kPieces) % kPieces * 16;
+        else return row % 8 * 16;
     }
-
-    /* V rows as the column operand: lane l holds, of every group, channels (GS / 16) (l % 16) ..
-     * of the 8 tokens whose scores it also holds: t + 4 c + r and t + 16 + 4 c + r, c = l / 16. */
-    template <bool TAIL>
-    static __device__ __forceinline__ void load_v(const Job& job, int t, int lane, VTile& v) {
-        const int col = lane & 15, c = lane >> 4;
+    static __device__ __forceinline__ void load_codes(const char* base, int n, int t, int lane,
+                                                      char* to) {
+        const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)to;
+        const int row = lane / kPieces, piece = lane % kPieces * 16;
+        const bool whole = t + 32 <= n;
+        uint32_t at = (uint32_t)(t + row) * kRowBytes + (piece ^ turn(row));
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-            uint32_t at[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                int tok = t + 16 * (j >> 2) + 4 * c + (j & 3) + i;
-                if (TAIL && tok >= job.n) tok = job.n - 1;
-                at[i] = (uint32_t)tok * kRowBytes + col * kVBytes;
+        for (int i = 0; i < kLoads; ++i) {
+            constexpr int kEach = 64 / kPieces;   /* rows a load */
+            uint32_t a = (kEach % 8 ? at ^ (uint32_t)(i * kEach % 8 * 16) : at) + i * 1024;
+            if (!whole) {
+                const int tok = t + i * kEach + row;
+                a -= (uint32_t)(tok < n ? 0 : tok - n + 1) * kRowBytes;
             }
-#pragma unroll
-            for (int g = 0; g < kGroups; ++g) {
-                constexpr int kStep = GS * BITS / 8;
-                if constexpr (kVBytes >= 4) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        __builtin_memcpy(&v.code[g][(j + i) * (kVBytes / 4)],
-                                         __builtin_assume_aligned(job.v + (at[i] + g * kStep),
-                                                                  kVBytes), kVBytes);
-                } else {
-                    /* two tokens' halves of one register, which loads fill one by one */
-                    using Piece = std::conditional_t<kVBytes == 2, uint16_t, uint8_t>;
-                    u16x2_t x;
-                    x[0] = *(const Piece*)(job.v + (at[0] + g * kStep));
-                    x[1] = *(const Piece*)(job.v + (at[1] + g * kStep));
-                    v.code[g][j >> 1] = __builtin_bit_cast(uint32_t, x);
-                }
-            }
+            __asm__ volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                             :: "v"(a), "s"(base),
+                                "s"(__builtin_amdgcn_readfirstlane(lds + i * 1024)) : "memory");
         }
     }
 
-    /* 8 codes of step st of a group.  4 bits: the word's nibbles in the order 0 4 1 5 2 6 3 7,
+    /* Waits until no more than LEFT of the wave's loads are under way. */
+    template <int LEFT>
+    static __device__ __forceinline__ void loaded() {
+        __asm__ volatile("s_waitcnt vmcnt(%0)" :: "n"(LEFT) : "memory");
+    }
+    /* Waits for the wave's LDS reads: what they read may be written over. */
+    static __device__ __forceinline__ void read_done() {
+        __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+
+    /* 8 codes of step st of a chunk.  4 bits: the word's nibbles in the order 0 4 1 5 2 6 3 7,
      * the odd ones times 16; 8 bits: in order.  The queries are laid out to match. */
-    static __device__ __forceinline__ f16x8_t k_operand(const uint32_t (&w)[kKWords], int st) {
+    static __device__ __forceinline__ f16x8_t k_operand(const uint32_t (&w)[kWords], int st) {
         if constexpr (BITS == 4) {
             const uint32_t a = w[st], b = a >> 8;
             return as_f16x8(a & 0x000f000fu, a & 0x00f000f0u, b & 0x000f000fu, b & 0x00f000f0u);
@@ -216,80 +226,146 @@ struct Attention {
     /* Whether column tile i holds its codes times 16. */
     static constexpr __device__ bool odd_tile(int i) { return BITS == 4 && (i & 1); }
 
-    /* The 8 tokens' codes of channel i of a lane's group channels. */
-    static __device__ __forceinline__ f16x8_t v_operand(const uint32_t (&w)[kVWords], int i) {
-        uint32_t o[4];
+    /* What a lane reads for one chunk of steps: its quarter's 8-channel pieces of tokens l % 16
+     * and l % 16 + 16, and the queries'. */
+    struct Chunk {
+        uint32_t w[2][kWords];
+        f16x8_t q[RT][kChunk];
+    };
+    static __device__ __forceinline__ void read_chunk(const char* tile, const f16x8_t* qlds, int ch,
+                                                      int lane, Chunk& out) {
+        constexpr int kPer = kSteps / kChunk;   /* chunks of a group */
+        const int g = ch / kPer, part = ch % kPer, row = lane & 15;
+        const int at = ((lane >> 4) * kPer + part) * kWords * 4;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+            const char* p = tile + ((row + 16 * tt) * kRowBytes + (at ^ turn(row) ^ (g * (GS * BITS / 8))));
+            __builtin_memcpy(out.w[tt], __builtin_assume_aligned(p, kWords * 4), kWords * 4);
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int s = 0; s < kChunk; ++s)
+                out.q[rt][s] = qlds[(rt * (kDim / 32) + ch * kChunk + s) * 64 + lane];
+    }
+
+    /* What a lane reads for the values of group g: channels (GS / 16) (l % 16) .. of the 8 tokens
+     * whose scores it also holds, 4 c + r and 16 + 4 c + r, and the tokens' scales. */
+    struct Values {
+        uint32_t w[8][kVBytes < 4 ? 1 : kVBytes / 4];
+        float s[8];
+    };
+    static __device__ __forceinline__ void read_values(const char* tile, const Scales& sc, int g,
+                                                       int lane, Values& out) {
+        const int c = lane >> 4, at = (lane & 15) * kVBytes ^ (g * (GS * BITS / 8));
+        tokens_of(sc.v[g], c, out.s);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int row = 4 * c + (j & 3);
+            const char* p = tile + (row * kRowBytes + (at ^ turn(row))) + (j >> 2) * 16 * kRowBytes;
+            if constexpr (kVBytes == 1) out.w[j][0] = *(const uint8_t*)p;
+            else if constexpr (kVBytes == 2) out.w[j][0] = *(const uint16_t*)p;
+            else __builtin_memcpy(out.w[j], __builtin_assume_aligned(p, kVBytes), kVBytes);
+        }
+    }
+    static __device__ __forceinline__ void v_operands(const Values& v, f16x8_t (&out)[kTiles]) {
+        uint32_t o[kTiles][4];
 #pragma unroll
         for (int jp = 0; jp < 4; ++jp) {
-            if constexpr (BITS == 4) {
-                uint32_t pair;  /* tokens 2 jp and 2 jp + 1: 16 bits of codes each */
-                if constexpr (kVBytes == 4)
-                    pair = __builtin_amdgcn_perm(w[2 * jp + 1], w[2 * jp],
-                                                 i < 4 ? 0x05040100u : 0x07060302u);
-                else
-                    pair = w[jp];
-                const int n = i & 3;
-                const uint32_t x = n < 2 ? pair : pair >> 8;
-                o[jp] = x & (n & 1 ? 0x00f000f0u : 0x000f000fu);
+            const auto &a = v.w[2 * jp], &b = v.w[2 * jp + 1];
+            if constexpr (BITS == 8 && kVBytes >= 4) {
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i)
+                    o[i][jp] = __builtin_amdgcn_perm(b[i / 4], a[i / 4],
+                                                     0x0c000c00u | (4 + (i & 3)) << 16 | (i & 3));
             } else {
-                if constexpr (kVBytes == 2) {
-                    o[jp] = (i ? w[jp] >> 8 : w[jp]) & 0x00ff00ffu;
-                } else {
-                    constexpr int kW = kVBytes / 4;
-                    const uint32_t a = w[2 * jp * kW + i / 4], b = w[(2 * jp + 1) * kW + i / 4];
-                    const uint32_t n = i & 3;
-                    o[jp] = __builtin_amdgcn_perm(b, a, 0x0c000c00u | (4 + n) << 16 | n);
+                uint32_t pair[2];   /* two tokens' next 16 bits of codes */
+                pair[0] = __builtin_amdgcn_perm(b[0], a[0], 0x05040100u);
+                pair[1] = kVBytes == 4 ? __builtin_amdgcn_perm(b[0], a[0], 0x07060302u) : 0;
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) {
+                    if constexpr (BITS == 8) {
+                        o[i][jp] = pair[0] >> 8 * i & 0x00ff00ffu;
+                    } else {
+                        const uint32_t x = pair[i >> 2] >> (i & 2 ? 8 : 0);
+                        o[i][jp] = x & (i & 1 ? 0x00f000f0u : 0x000f000fu);
+                    }
                 }
             }
         }
-        return as_f16x8(o[0], o[1], o[2], o[3]);
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) out[i] = as_f16x8(o[i][0], o[i][1], o[i][2], o[i][3]);
     }
 
     struct Rows {
         f32x4_t o[RT][kDim / 16];      /* rows 4 c + r of a tile, one column a lane        */
         float off[RT], sum[RT];        /* a row's offset M; its lane's part of sum p       */
         float code_sum[RT][kGroups];   /* its part of sum of the rounded p s               */
-        float bias_sum[RT][kGroups];   /* its part of sum p (b + centre s)                 */
+        float bias_sum[F16 ? RT : 1][kGroups];  /* fp16: its part of sum p (b + centre s)  */
+        f32x4_t bias[F16 ? 1 : RT];    /* bf16: the same as a matrix product, column 2 g + part */
         float unit[RT];                /* score units to log2                              */
-        float qsum[RT][kGroups];
         uint32_t mask[RT];             /* block rows that the row sees                     */
     };
 
     /* One tile of 32 tokens: scores from k, then the next tile's K, then the values. */
     template <bool MASKED>
-    static __device__ __forceinline__ void scores(const Job& job, int t, int lane, int tiles,
-                                                  const KTile& k, const Scales& sc,
-                                                  const f16x8_t* qlds, const Rows& st,
-                                                  float (&z)[RT][8]) {
+    static __device__ __forceinline__ void scores(const Job& job, int t, int lane,
+                                                  const char* k, const Scales& sc,
+                                                  const f16x8_t* qlds, const half8_t* qsums,
+                                                  const Rows& st, float (&z)[RT][8]) {
         const int c = lane >> 4;
+        /* what is read from LDS is read one chunk ahead of its use */
+        uint32_t kb[2][4] = {};
+        half8_t qs[RT];
+        Chunk in;
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-            f32x4_t acc[RT][2];
+        for (int tt = 0; tt < 2; ++tt)
+            __builtin_memcpy(kb[tt], __builtin_assume_aligned(
+                sc.kb + ((lane & 15) + 16 * tt) * kGroups, 2 * kGroups), 2 * kGroups);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-                for (int tt = 0; tt < 2; ++tt) acc[rt][tt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int rt = 0; rt < RT; ++rt) qs[rt] = qsums[rt * 64 + lane];
+        read_chunk(k, qlds, 0, lane, in);
+        __builtin_amdgcn_sched_barrier(0);
+        /* sum_g b_g sum(q_g): the sums come in three 16-bit parts, one a quarter of the lanes */
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                const f16x8_t a0 = k_operand(k.code[0][g], s), a1 = k_operand(k.code[1][g], s);
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) {
+                const u32x4_t v = {kb[tt][0], kb[tt][1], kb[tt][2], kb[tt][3]};
+                const f32x4_t b = mfma(__builtin_bit_cast(half8_t, v), qs[rt],
+                                       f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                for (int r = 0; r < 4; ++r) z[rt][4 * tt + r] = b[r];
+            }
+        f32x4_t acc[RT][2];
+#pragma unroll
+        for (int ch = 0; ch < kChunks; ++ch) {
+            constexpr int kPer = kSteps / kChunk;
+            if (ch % kPer == 0)
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+                    for (int tt = 0; tt < 2; ++tt) acc[rt][tt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int st = 0; st < kChunk; ++st) {
+                const f16x8_t a0 = k_operand(in.w[0], st), a1 = k_operand(in.w[1], st);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
-                    if (rt >= tiles) break;
-                    const f16x8_t q = qlds[(rt * (kDim / 32) + g * kSteps + s) * 64 + lane];
-                    acc[rt][0] = mfma(a0, q, acc[rt][0]);
-                    acc[rt][1] = mfma(a1, q, acc[rt][1]);
+                    acc[rt][0] = mfma(a0, in.q[rt][st], acc[rt][0]);
+                    acc[rt][1] = mfma(a1, in.q[rt][st], acc[rt][1]);
                 }
             }
-            float s[8], b[8];
-            tokens_of(sc.s[0][g], c, s);
-            tokens_of(sc.s[1][g], c, b);
+            const int g = ch / kPer;
+            const bool last = ch % kPer == kPer - 1;
+            float s[8];
+            if (last) tokens_of(sc.k[g], c, s);
+            if (ch + 1 < kChunks) read_chunk(k, qlds, ch + 1, lane, in);
+            __builtin_amdgcn_sched_barrier(0);
+            if (last)
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+                for (int j = 0; j < 8; ++j)
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    const float v = g ? fmaf(b[j], st.qsum[rt][g], z[rt][j]) : b[j] * st.qsum[rt][g];
-                    z[rt][j] = fmaf(s[j], acc[rt][j >> 2][j & 3], v);
-                }
-            if constexpr (kGroups >= 4) __builtin_amdgcn_sched_barrier(0);
+                    for (int rt = 0; rt < RT; ++rt)
+                        z[rt][j] = fmaf(s[j], acc[rt][j >> 2][j & 3], z[rt][j]);
         }
         if constexpr (MASKED) {
 #pragma unroll
@@ -311,18 +387,28 @@ struct Attention {
      * least normal number then lies 2^-29 under it.  M rises only when a tile would pass 2^15,
      * to where its largest is 2^11. */
     template <bool MASKED>
-    static __device__ __forceinline__ void weigh(const Job& job, int t, int lane, int tiles,
-                                                 const VTile& v, const Scales& sc, Rows& st,
+    static __device__ __forceinline__ void weigh(const Job& job, int t, int lane,
+                                                 const char* v, const Scales& sc, Rows& st,
                                                  float (&z)[RT][8]) {
         const int c = lane >> 4;
-        float size[8];
+        Values in;
+        float size[8], vb[8];
+        uint32_t mid[4];
         tokens_of(sc.size, c, size);
+        if constexpr (!F16) {
+            const uint16_t* p = sc.parts[lane & 15 & (2 * kGroups - 1)] + 4 * c;
+            __builtin_memcpy(mid, __builtin_assume_aligned(p, 8), 8);
+            __builtin_memcpy(mid + 2, __builtin_assume_aligned(p + 16, 8), 8);
+        } else {
+            tokens_of(sc.vb[0], c, vb);
+        }
+        read_values(v, sc, 0, lane, in);
+        __builtin_amdgcn_sched_barrier(0);
         float most = size[0];
 #pragma unroll
         for (int j = 1; j < 8; ++j) most = fmaxf(most, size[j]);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            if (rt >= tiles) break;
             float top = z[rt][0];
 #pragma unroll
             for (int j = 1; j < 8; ++j) top = fmaxf(top, z[rt][j]);
@@ -350,11 +436,12 @@ struct Attention {
 #pragma unroll
                 for (int g = 0; g < kGroups; ++g) {
                     st.code_sum[rt][g] *= keep;
-                    st.bias_sum[rt][g] *= keep;
+                    if constexpr (F16) st.bias_sum[rt][g] *= keep;
                 }
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const float f = __shfl(keep, 4 * c + r);
+                    if constexpr (!F16) st.bias[rt][r] *= f;
 #pragma unroll
                     for (int i = 0; i < kDim / 16; ++i) st.o[rt][i][r] *= f;
                 }
@@ -365,31 +452,54 @@ struct Attention {
                 st.sum[rt] += z[rt][j];
             }
         }
+        if constexpr (!F16) {
+            /* sum p (b + centre s) of all groups at once.  p is rounded to bf16 here, so this
+             * term, and no other, is off by 2^-9 a token: less than the output's own rounding. */
+            const u32x4_t b = {mid[0], mid[1], mid[2], mid[3]};
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                u32x4_t a;
+#pragma unroll
+                for (int jp = 0; jp < 4; ++jp) {
+                    const f32x2_t x = {z[rt][2 * jp], z[rt][2 * jp + 1]};
+                    a[jp] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2_t));
+                }
+                st.bias[rt] = mfma(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
+                                   st.bias[rt]);
+            }
+        }
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
             f16x8_t w[kTiles];
-#pragma unroll
-            for (int i = 0; i < kTiles; ++i) w[i] = v_operand(v.code[g], i);
+            v_operands(in, w);
             float s[8], b[8];
-            tokens_of(sc.s[2][g], c, s);
-            tokens_of(sc.s[3][g], c, b);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) b[j] = fmaf(kCentre, s[j], b[j]);
+            for (int j = 0; j < 8; ++j) {
+                s[j] = in.s[j];
+                if constexpr (F16) b[j] = vb[j];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (g + 1 < kGroups) {
+                read_values(v, sc, g + 1, lane, in);
+                if constexpr (F16) tokens_of(sc.vb[g + 1], c, vb);
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                if (rt >= tiles) break;
                 uint32_t ps[4];
 #pragma unroll
                 for (int jp = 0; jp < 4; ++jp) {
                     f32x2_t x = {z[rt][2 * jp] * s[2 * jp], z[rt][2 * jp + 1] * s[2 * jp + 1]};
-                    float y0 = z[rt][2 * jp] * b[2 * jp], y1 = z[rt][2 * jp + 1] * b[2 * jp + 1];
                     if constexpr (MASKED) {
                         const int tok = t + 16 * (jp >> 1) + 4 * c + 2 * (jp & 1);
-                        if (!sees(job, st.mask[rt], tok)) x[0] = y0 = 0.0f;
-                        if (!sees(job, st.mask[rt], tok + 1)) x[1] = y1 = 0.0f;
+                        if (!sees(job, st.mask[rt], tok)) x[0] = 0.0f;
+                        if (!sees(job, st.mask[rt], tok + 1)) x[1] = 0.0f;
                     }
-                    st.bias_sum[rt][g] += y0;
-                    st.bias_sum[rt][g] += y1;
+                    if constexpr (F16) {
+                        st.bias_sum[rt][g] = fmaf(z[rt][2 * jp], b[2 * jp], st.bias_sum[rt][g]);
+                        st.bias_sum[rt][g] =
+                            fmaf(z[rt][2 * jp + 1], b[2 * jp + 1], st.bias_sum[rt][g]);
+                    }
                     const f16x2_t h = __builtin_convertvector(x, f16x2_t);
                     ps[jp] = __builtin_bit_cast(uint32_t, h);
                     const f16x2_t one = {(_Float16)1.0f, (_Float16)1.0f};
@@ -400,117 +510,109 @@ struct Attention {
                 for (int i = 0; i < kTiles; ++i)
                     st.o[rt][g * kTiles + i] = mfma(a, w[i], st.o[rt][g * kTiles + i]);
             }
-            if constexpr (kGroups >= 4) __builtin_amdgcn_sched_barrier(0);
         }
     }
+
+    /* LDS of a workgroup.  The waves' results meet in it when the loop is over. */
+    struct Lds {
+        union {
+            struct {
+                __attribute__((aligned(16))) char pool[kRows * kDim * 2];   /* queries */
+                char k[kWaves][kBufs][kTileBytes], v[kWaves][kBufs][kTileBytes];
+            };
+            f32x4_t merge[kWaves][RT][kMergeTiles][64];
+        };
+        Scales scales[kWaves];
+        __attribute__((aligned(16))) uint16_t qsums[kRows * 4 * 8];
+        uint32_t masks[kRows];
+        float units[kRows];
+        float offs[kWaves][kRows], sums[kWaves][kRows];
+        float fix[kWaves][kRows][kGroups];
+        float bias[F16 ? 1 : kWaves][F16 ? 1 : kRows][2 * kGroups];
+    };
 
     /* The block's queries into LDS, in the order of the K operands and scaled by a power of two
      * so that a row's largest element lies in [2^14, 2^15): fp16 then holds them as exactly as
      * bf16 or fp16 did, down to 2^-29 of the largest.  unit: what takes a sum over codes times
      * 2^-24 to scores in log2; qsum: the sums of a row's groups in those units. */
     static __device__ __forceinline__ void stage_queries(const KvAttnParams& p, const Job& job,
-                                                         int h, uint16_t* qlds, float* unit,
-                                                         float* qsum) {
-        constexpr int kLanes = kDim / 8;
+                                                         int h, Lds& lds) {
+        constexpr int kLanes = kDim / 8, kPass = DFQ_KV_THREADS / kLanes;
+        constexpr int kPasses = (kRows + kPass - 1) / kPass;
         const int piece = threadIdx.x % kLanes, q_heads = p.heads * p.group;
-        for (int r = threadIdx.x / kLanes; r < kRows; r += DFQ_KV_THREADS / kLanes) {
-            float f[8] = {};
+        u32x4_t raw[kPasses];
+        uint32_t mask[kPasses];
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            const int r = threadIdx.x / kLanes + i * kPass;
+            raw[i] = u32x4_t{0, 0, 0, 0};
+            mask[i] = 0;
             if (r < job.nrows) {
                 const int row = job.row0 + r, bm = row / p.group;
-                const uint16_t* q = p.q + bm * p.q_stride +
-                                    (int64_t)(h * p.group + row - bm * p.group) * kDim + piece * 8;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) f[i] = elem_to_f32<F16>(q[i]);
+                raw[i] = *(const u32x4_any*)(p.q + bm * p.q_stride +
+                                             (int64_t)(h * p.group + row - bm * p.group) * kDim +
+                                             piece * 8);
+                mask[i] = p.tree ? p.tree[bm] : (2u << (bm % p.rows)) - 1;
             }
-            float top = 0.0f;
+        }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(f[i]));
+        for (int i = 0; i < kPasses; ++i) {
+            const int r = threadIdx.x / kLanes + i * kPass;
+            if (r >= kRows) break;
+            float f[8], top = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                f[j] = elem_to_f32<F16>(j & 1 ? raw[i][j / 2] >> 16 : raw[i][j / 2] & 0xffffu);
+                top = fmaxf(top, fabsf(f[j]));
+            }
             for (int d = 1; d < kLanes; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
             int e = (int)(__float_as_uint(top) >> 23) - 127;
             if (e < -100 || e > 127) e = e > 127 ? 127 : -100; /* a tiny or an infinite row */
             float total = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                f[i] = ldexpf(f[i], 14 - e);
-                total += f[i];
+            for (int j = 0; j < 8; ++j) {
+                f[j] = ldexpf(f[j], 14 - e);
+                total += f[j];
             }
             for (int d = 1; d < GS / 8; d *= 2) total += __shfl_xor(total, d);
             const int g = piece / (GS / 8), u = piece % (GS / 8), c = u / kSteps, st = u % kSteps;
-            if (u == 0) qsum[r * kGroups + g] = total / kUnit;
-            if (piece == 0) unit[r] = ldexpf(p.scale_log2e, 24 + e - 14);
-            uint16_t* o = qlds + (((r / 16) * (kDim / 32) + g * kSteps + st) * 64 + c * 16 + r % 16) * 8;
+            if (u < 4) {
+                /* 2^-8 of the group's sum in three parts of 16 bits, part i for quarter i of the
+                 * lanes; quarter 3 and the elements past the groups are 0 */
+                float rest = total / 256.0f;
+                uint16_t part = f32_to_out<F16>(rest);
+                for (int k = 0; k < u; ++k) {
+                    rest -= elem_to_f32<F16>(part);
+                    part = f32_to_out<F16>(rest);
+                }
+                uint16_t* to = lds.qsums + ((r / 16) * 64 + u * 16 + r % 16) * 8;
+                to[g] = u < 3 ? part : 0;
+                if (g == 0)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                /* nibble order of k_operand: operand element i is channel i/2 + 4 (i%2) */
-                const int src = BITS == 4 ? i / 2 + 4 * (i % 2) : i;
-                const float x = BITS == 4 && (i / 2) % 2 ? f[src] * 0.0625f : f[src];
-                o[i] = f32_to_out<true>(x);
+                    for (int j = kGroups; j < 8; ++j) to[j] = 0;
             }
+            if (piece == 0) {
+                lds.units[r] = ldexpf(p.scale_log2e, 8 + e - 14);
+                lds.masks[r] = mask[i];
+            }
+            /* nibble order of k_operand: operand element j is channel j/2 + 4 (j%2) */
+            u32x4_t o;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int a = BITS == 4 ? j : 2 * j, b = BITS == 4 ? j + 4 : 2 * j + 1;
+                const float by = BITS == 4 && j % 2 ? 0.0625f : 1.0f;
+                const f32x2_t x = {f[a] * by, f[b] * by};
+                o[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2_t));
+            }
+            *(u32x4_t*)(lds.pool + (((r / 16) * (kDim / 32) + g * kSteps + st) * 64 + c * 16 + r % 16) * 16) = o;
         }
     }
 
-    static __device__ __forceinline__ void run(const KvAttnParams& p) {
-        constexpr int kQBytes = kRows * kDim * 2, kMerge = kWaves * kRows * 16 * 4;
-        __shared__ __attribute__((aligned(16))) char pool[kQBytes > kMerge ? kQBytes : kMerge];
-        __shared__ __attribute__((aligned(16))) Scales scales[kWaves];
-        __shared__ float units[kRows], qsums[kRows * kGroups];
-        __shared__ float offs[kWaves][kRows], sums[kWaves][kRows];
-        __shared__ float fix[kWaves][kRows][kGroups];
+    static __device__ __forceinline__ void run(const KvAttnParams& p, const Job& job, int h,
+                                               char* room) {
+        Lds& lds = *(Lds*)room;
         const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-
-        /* the job: heads go fastest, so that with 8 of them an XCD's L2 serves one */
-        Job job;
-        int i = blockIdx.x;
-        const int h = i % p.heads;
-        i /= p.heads;
-        const int seq_rows = p.rows * p.group;
-        int range, ranges;
-        int64_t token0;   /* index of the slot-and-head's first token in the arrays */
-        KvArrays jk, jv;
-        const int prefix_jobs = p.prefix_splits * p.prefix_blocks;
-        if (i < prefix_jobs) {
-            range = i / p.prefix_blocks;
-            ranges = p.prefix_splits;
-            jk = p.prefix[0];
-            jv = p.prefix[1];
-            token0 = (int64_t)h * p.prefix_capacity;
-            job.slot = range;
-            job.row0 = (i % p.prefix_blocks) * kRows;
-            job.nrows = p.batch * seq_rows - job.row0;
-            job.n = job.clear = job.first = p.prefix_length;
-        } else {
-            i -= prefix_jobs;
-            const int b = i / (p.own_splits * p.own_blocks);
-            i %= p.own_splits * p.own_blocks;
-            range = i / p.own_blocks;
-            ranges = p.own_splits;
-            jk = p.own[0];
-            jv = p.own[1];
-            token0 = ((int64_t)b * p.heads + h) * p.own_capacity;
-            job.slot = p.prefix_splits + range;
-            const int r0 = (i % p.own_blocks) * kRows;
-            job.row0 = b * seq_rows + r0;
-            job.nrows = seq_rows - r0;
-            int n = p.lengths ? p.lengths[b] : p.max_length;
-            n = n < 0 ? 0 : n > p.max_length ? p.max_length : n;
-            job.n = n;
-            job.first = n - p.rows;
-            job.clear = job.first < 0 ? 0 : job.first;
-        }
-        if (job.nrows > kRows) job.nrows = kRows;
-        job.k = (const char*)jk.codes + token0 * kRowBytes;
-        job.v = (const char*)jv.codes + token0 * kRowBytes;
-        const uint16_t* ks = lane & 16 ? jk.biases : jk.scales;
-        const uint16_t* vs = lane & 16 ? jv.biases : jv.scales;
-        job.scale = (lane < 32 ? ks : vs) + token0 * kGroups;
-        /* ranges of whole rounds of 32 tokens a wave */
-        const int rounds = (job.n + 32 * kWaves - 1) / (32 * kWaves);
-        const int each = (rounds + ranges - 1) / ranges * 32 * kWaves;
-        job.t0 = range * each < job.n ? range * each : job.n;
-        job.t1 = job.t0 + each < job.n ? job.t0 + each : job.n;
-        const int tiles = (job.nrows + 15) / 16;
-
-        stage_queries(p, job, h, (uint16_t*)pool, units, qsums);
+        stage_queries(p, job, h, lds);
         __syncthreads();
 
         Rows st;
@@ -519,141 +621,259 @@ struct Attention {
             const int r = rt * 16 + (lane & 15);
             st.off[rt] = kNever;
             st.sum[rt] = 0.0f;
-            st.unit[rt] = units[r];
+            st.unit[rt] = lds.units[r];
+            st.mask[rt] = lds.masks[r];
 #pragma unroll
             for (int g = 0; g < kGroups; ++g) {
-                st.code_sum[rt][g] = st.bias_sum[rt][g] = 0.0f;
-                st.qsum[rt][g] = qsums[r * kGroups + g];
+                st.code_sum[rt][g] = 0.0f;
+                if constexpr (F16) st.bias_sum[rt][g] = 0.0f;
             }
+            if constexpr (!F16) st.bias[rt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int d = 0; d < kDim / 16; ++d) st.o[rt][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            st.mask[rt] = 0;
-            if (r < job.nrows) {
-                const int bm = (job.row0 + r) / p.group;
-                st.mask[rt] = p.tree ? p.tree[bm] : (2u << (bm % p.rows)) - 1;
-            }
         }
 
         int t = job.t0 + 32 * wave;
-        KTile k;
-        VTile v;
+        TokenScales scale;
         float z[RT][8];
-        const f16x8_t* q = (const f16x8_t*)pool;
+        const f16x8_t* q = (const f16x8_t*)lds.pool;
+        Scales& sc = lds.scales[wave];
+        char (&k)[kBufs][kTileBytes] = lds.k[wave], (&v)[kBufs][kTileBytes] = lds.v[wave];
+        int buf = 0;
         if (t < job.t1) {
-            if (t + 32 <= job.n) load_k<false>(job, t, lane, k);
-            else load_k<true>(job, t, lane, k);
+            load_scales(job, t, lane, scale);
+            load_codes(job.k, job.n, t, lane, k[0]);
+            if (kBufs == 2) load_codes(job.v, job.n, t, lane, v[0]);
         }
         while (t < job.t1) {
-            const int next = t + 32 * kWaves;
-            stage_scales(k.scale, lane, scales[wave]);
-            if (t + 32 <= job.clear) {
-                load_v<false>(job, t, lane, v);
-                scores<false>(job, t, lane, tiles, k, scales[wave], q, st, z);
+            const int next = t + 32 * kWaves, other = kBufs == 2 ? buf ^ 1 : 0;
+            loaded<0>();
+            stage_scales(scale, lane, sc);
+            if (next < job.t1) load_scales(job, next, lane, scale);
+            if constexpr (kBufs == 2) {
                 if (next < job.t1) {
-                    if (next + 32 <= job.n) load_k<false>(job, next, lane, k);
-                    else load_k<true>(job, next, lane, k);
+                    load_codes(job.k, job.n, next, lane, k[other]);
+                    load_codes(job.v, job.n, next, lane, v[other]);
                 }
-                weigh<false>(job, t, lane, tiles, v, scales[wave], st, z);
             } else {
-                load_v<true>(job, t, lane, v);
-                scores<true>(job, t, lane, tiles, k, scales[wave], q, st, z);
-                if (next < job.t1) load_k<true>(job, next, lane, k);
-                weigh<true>(job, t, lane, tiles, v, scales[wave], st, z);
+                load_codes(job.v, job.n, t, lane, v[0]);
             }
+            const bool masked = t + 32 > job.clear;
+            if (masked) scores<true>(job, t, lane, k[buf], sc, q, (const half8_t*)lds.qsums, st, z);
+            else scores<false>(job, t, lane, k[buf], sc, q, (const half8_t*)lds.qsums, st, z);
+            if constexpr (kBufs == 1) {
+                read_done();
+                if (next < job.t1) {
+                    load_codes(job.k, job.n, next, lane, k[0]);
+                    loaded<kLoads>();
+                } else {
+                    loaded<0>();
+                }
+            }
+            if (masked) weigh<true>(job, t, lane, v[buf], sc, st, z);
+            else weigh<false>(job, t, lane, v[buf], sc, st, z);
+            read_done();
+            buf = other;
             t = next;
         }
 
-        /* the waves' rows together: offsets and sums first, then 16 columns at a time */
+        /* The waves' rows together: offsets, sums and what the codes' centre and the biases add,
+         * then four column tiles at a time, of which each wave adds up one of every row tile. */
+        __syncthreads();
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            const int r = rt * 16 + (lane & 15);
+            const int r = rt * 16 + (lane & 15), row = rt * 16 + 4 * (lane >> 4);
             float sum = st.sum[rt];
             sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);
+            if (lane < 16) {
+                lds.offs[wave][r] = st.off[rt];
+                lds.sums[wave][r] = sum;
+            }
 #pragma unroll
             for (int g = 0; g < kGroups; ++g) {
-                float f = fmaf(-kCentre, st.code_sum[rt][g], st.bias_sum[rt][g]);
+                float f = -kCentre * st.code_sum[rt][g];
+                if constexpr (F16) f += st.bias_sum[rt][g];
                 f += __shfl_xor(f, 16);
                 f += __shfl_xor(f, 32);
-                if (lane < 16) fix[wave][r][g] = f;
+                if (lane < 16) lds.fix[wave][r][g] = f;
             }
-            if (lane < 16) {
-                offs[wave][r] = st.off[rt];
-                sums[wave][r] = sum;
-            }
+            if constexpr (!F16)
+                if ((lane & 15) < 2 * kGroups)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) lds.bias[wave][row + i][lane & 15] = st.bias[rt][i];
         }
         __syncthreads();
-        const int64_t nrows = (int64_t)p.batch * seq_rows;
+        const int64_t nrows = (int64_t)p.batch * p.rows * p.group;
         const int64_t out = (job.slot * p.heads + h) * nrows + job.row0;
-        if ((int)threadIdx.x < job.nrows) {
+        if ((int)threadIdx.x < kRows) {
             const int r = threadIdx.x;
-            float top = offs[0][r], sum = 0.0f;
-            for (int w = 1; w < kWaves; ++w) top = fmaxf(top, offs[w][r]);
-            for (int w = 0; w < kWaves; ++w) {
-                const float f = offs[w][r] == top ? 1.0f : exp2f(offs[w][r] - top);
-                sum = fmaf(sums[w][r], f, sum);
-                offs[w][r] = f;   /* from here on the wave's weight */
-            }
-            p.part_ml[(out + r) * 2] = top;
-            p.part_ml[(out + r) * 2 + 1] = sum;
-        }
-        float* merge = (float*)pool;
+            float off[kWaves], top = kNever, sum = 0.0f;
 #pragma unroll
-        for (int d = 0; d < kDim / 16; ++d) {
+            for (int w = 0; w < kWaves; ++w) {
+                off[w] = lds.offs[w][r];
+                top = fmaxf(top, off[w]);
+            }
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const float f = off[w] == top ? 1.0f : exp2f(off[w] - top);
+                sum = fmaf(lds.sums[w][r], f, sum);
+                lds.offs[w][r] = f;   /* from here on the wave's weight */
+                for (int g = 0; g < kGroups; ++g) {
+                    float x = lds.fix[w][r][g];
+                    if constexpr (!F16) x += lds.bias[w][r][2 * g] + lds.bias[w][r][2 * g + 1];
+                    lds.fix[w][r][g] = x * f;
+                }
+            }
+            if (r < job.nrows) *(f32x2_t*)(p.part_ml + (out + r) * 2) = f32x2_t{top, sum};
+        }
+#pragma unroll
+        for (int d0 = 0; d0 < kDim / 16; d0 += kMergeTiles) {
             __syncthreads();
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    merge[(wave * kRows + rt * 16 + 4 * (lane >> 4) + r) * 16 + (lane & 15)] =
-                        st.o[rt][d][r];
+                for (int d = 0; d < kMergeTiles; ++d)
+                    lds.merge[wave][rt][d][lane] = st.o[rt][d0 + d];
             __syncthreads();
-            const float back = odd_tile(d % kTiles) ? kUnit / 16.0f : kUnit;
-            for (int e = threadIdx.x; e < job.nrows * 16; e += DFQ_KV_THREADS) {
-                const int r = e / 16;
-                float sum = 0.0f;
+            for (int d = wave; d < kMergeTiles; d += kWaves) {
+                const int g = (d0 + d) / kTiles;
+                const float back = odd_tile((d0 + d) % kTiles) ? kUnit / 16.0f : kUnit;
 #pragma unroll
-                for (int w = 0; w < kWaves; ++w)
-                    sum = fmaf(fmaf(merge[w * kRows * 16 + e], back, fix[w][r][d / kTiles]),
-                               offs[w][r], sum);
-                p.part_o[(out + r) * kDim + d * 16 + e % 16] = sum;
+                for (int rt = 0; rt < RT; ++rt) {
+                    f32x4_t x[kWaves];
+#pragma unroll
+                    for (int w = 0; w < kWaves; ++w) x[w] = lds.merge[w][rt][d][lane];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = rt * 16 + 4 * (lane >> 4) + i;
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int w = 0; w < kWaves; ++w)
+                            sum = fmaf(x[w][i] * back, lds.offs[w][r], sum + lds.fix[w][r][g]);
+                        if (r < job.nrows)
+                            p.part_o[(out + r) * kDim + (d0 + d) * 16 + (lane & 15)] = sum;
+                    }
+                }
             }
         }
     }
 };
 
+/* A workgroup of a launch whose row blocks have up to RT tiles: its job, and the code for the
+ * tiles that the job has. */
+template <int BITS, int GS, bool F16, int RT>
+__device__ __forceinline__ void attention(const KvAttnParams& p) {
+    using Most = Attention<BITS, GS, F16, RT>;
+    constexpr int kRows = Most::kRows, kRowBytes = Most::kRowBytes, kGroups = Most::kGroups;
+    __shared__ __attribute__((aligned(16))) char lds[sizeof(typename Most::Lds)];
+    const int lane = threadIdx.x % 64;
+
+    /* the job: heads go fastest, so that with 8 of them an XCD's L2 serves one */
+    Job job;
+    int i = blockIdx.x;
+    const int h = i % p.heads;
+    i /= p.heads;
+    const int seq_rows = p.rows * p.group;
+    int range, ranges;
+    int64_t token0;   /* index of the slot-and-head's first token in the arrays */
+    KvArrays jk, jv;
+    const int prefix_jobs = p.prefix_splits * p.prefix_blocks;
+    if (i < prefix_jobs) {
+        range = i / p.prefix_blocks;
+        ranges = p.prefix_splits;
+        jk = p.prefix[0];
+        jv = p.prefix[1];
+        token0 = (int64_t)h * p.prefix_capacity;
+        job.slot = range;
+        job.row0 = (i % p.prefix_blocks) * kRows;
+        job.nrows = p.batch * seq_rows - job.row0;
+        job.n = job.clear = job.first = p.prefix_length;
+    } else {
+        i -= prefix_jobs;
+        const int b = i / (p.own_splits * p.own_blocks);
+        i %= p.own_splits * p.own_blocks;
+        range = i / p.own_blocks;
+        ranges = p.own_splits;
+        jk = p.own[0];
+        jv = p.own[1];
+        token0 = ((int64_t)b * p.heads + h) * p.own_capacity;
+        job.slot = p.prefix_splits + range;
+        const int r0 = (i % p.own_blocks) * kRows;
+        job.row0 = b * seq_rows + r0;
+        job.nrows = seq_rows - r0;
+        int n = p.lengths ? p.lengths[b] : p.max_length;
+        n = n < 0 ? 0 : n > p.max_length ? p.max_length : n;
+        job.n = n;
+        job.first = n - p.rows;
+        job.clear = job.first < 0 ? 0 : job.first;
+    }
+    if (job.nrows > kRows) job.nrows = kRows;
+    job.k = uniform((const char*)jk.codes + token0 * kRowBytes);
+    job.v = uniform((const char*)jv.codes + token0 * kRowBytes);
+    job.scale = (lane < 32 ? jk.scales : jv.scales) + token0 * kGroups;
+    job.bias = (lane < 32 ? jk.biases : jv.biases) + token0 * kGroups;
+    /* ranges of whole rounds of 32 tokens a wave */
+    const int rounds = (job.n + 32 * kWaves - 1) / (32 * kWaves);
+    const int each = (rounds + ranges - 1) / ranges * 32 * kWaves;
+    job.t0 = range * each < job.n ? range * each : job.n;
+    job.t1 = job.t0 + each < job.n ? job.t0 + each : job.n;
+
+    const int tiles = (job.nrows + 15) / 16;
+    if constexpr (RT > 1)
+        if (tiles == 1) return Attention<BITS, GS, F16, 1>::run(p, job, h, lds);
+    if constexpr (RT > 2)
+        if (tiles == 2) return Attention<BITS, GS, F16, 2>::run(p, job, h, lds);
+    if constexpr (RT > 3)
+        if (tiles == 3) return Attention<BITS, GS, F16, 3>::run(p, job, h, lds);
+    Most::run(p, job, h, lds);
+}
+
 /* The parts of a row from all ranges, in the order of their slots: y = sum 2^(M - top) o / sum
- * 2^(M - top) l.  One workgroup a row: its waves take every fourth slot, a lane kDim / 64
- * channels. */
+ * 2^(M - top) l.  One workgroup a row: a wave takes every fourth slot, a lane kDim / 64 channels;
+ * the slots' offsets and sums come in one load a lane (64 slots at a time), and eight slots' parts
+ * are under way together, since the row waits for memory and for nothing else. */
 template <int GS, bool F16>
 __device__ __forceinline__ void join(const KvAttnParams& p) {
-    __shared__ float acc[kWaves][kDim], tops[kWaves], sums[kWaves];
+    constexpr int kEach = kDim / 64, kAhead = 8;
+    typedef float part_t __attribute__((ext_vector_type(kEach)));
+    __shared__ float acc[kWaves][kDim];
+    __shared__ float weight[kWaves][64];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int64_t nrows = (int64_t)p.batch * p.rows * p.group;
     const int h = blockIdx.y, slots = p.prefix_splits + p.own_splits;
     const int64_t row = blockIdx.x, stride = nrows * p.heads, at = h * nrows + row;
+    const f32x2_t* ml = (const f32x2_t*)p.part_ml + at;
     float top = kNever;
-    for (int s = wave; s < slots; s += kWaves) top = fmaxf(top, p.part_ml[(s * stride + at) * 2]);
-    if (lane == 0) tops[wave] = top;
-    __syncthreads();
+    for (int s = lane; s < slots; s += 64) top = fmaxf(top, ml[s * stride][0]);
+    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    float sum = 0.0f;
+    part_t o = {};
+    for (int s0 = 0; s0 < slots; s0 += 64) {
+        const f32x2_t v = s0 + lane < slots ? ml[(s0 + lane) * stride] : f32x2_t{kNever, 0.0f};
+        const float f = v[0] == top ? 1.0f : exp2f(v[0] - top);
+        sum = fmaf(v[1], f, sum);
+        weight[wave][lane] = f;
+        wave_order();
+        const int n = slots - s0 < 64 ? slots - s0 : 64;
+        for (int s = wave; s < n; s += kAhead * kWaves) {
+            part_t x[kAhead];
+            float w[kAhead];
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, tops[w]);
-    float sum = 0.0f, o[kDim / 64] = {};
-    for (int s = wave; s < slots; s += kWaves) {
-        const float off = p.part_ml[(s * stride + at) * 2], l = p.part_ml[(s * stride + at) * 2 + 1];
-        const float f = off == top ? 1.0f : exp2f(off - top);
-        sum = fmaf(l, f, sum);
-        const float* part = p.part_o + (s * stride + at) * kDim;
+            for (int i = 0; i < kAhead; ++i) {
+                const int k = s + i * kWaves < n ? s + i * kWaves : s;
+                x[i] = *(const part_t*)(p.part_o + ((s0 + k) * stride + at) * kDim + lane * kEach);
+                w[i] = s + i * kWaves < n ? weight[wave][k] : 0.0f;
+            }
 #pragma unroll
-        for (int i = 0; i < kDim / 64; ++i) o[i] = fmaf(part[i * 64 + lane], f, o[i]);
+            for (int i = 0; i < kAhead; ++i)
+                if (s + i * kWaves < n) o += x[i] * w[i];
+        }
+        wave_order();
     }
-#pragma unroll
-    for (int i = 0; i < kDim / 64; ++i) acc[wave][i * 64 + lane] = o[i];
-    if (lane == 0) sums[wave] = sum;
+    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+    *(part_t*)&acc[wave][lane * kEach] = o;
     __syncthreads();
-    sum = sums[0];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) sum += sums[w];
     const int64_t bm = row / p.group, q_heads = p.heads * p.group;
     const int64_t head = h * p.group + row % p.group;
     for (int d = threadIdx.x; d < kDim; d += DFQ_KV_THREADS) {
@@ -677,7 +897,7 @@ __device__ __forceinline__ void join(const KvAttnParams& p) {
 #define DFQ_ATTN(bits, gs, name, f16, rt, per_simd)                                            \
     extern "C" __global__ __launch_bounds__(DFQ_KV_THREADS, per_simd) void                     \
         dfq_cache_attention_b##bits##_g##gs##_##name##_r##rt(KvAttnParams p) {                 \
-        Attention<bits, gs, f16, rt>::run(p);                                                  \
+        attention<bits, gs, f16, rt>(p);                                                       \
     }
 #define DFQ_JOIN(gs, name, f16)                                                                \
     extern "C" __global__ __launch_bounds__(DFQ_KV_THREADS) void                               \
@@ -694,24 +914,21 @@ DFQ_JOINS(64)
 #if DFQ_HEAD_DIM == 64
 DFQ_FORMATS(DFQ_ATTN, 32, 1, 3)
 DFQ_FORMATS(DFQ_ATTN, 32, 2, 2)
-DFQ_FORMATS(DFQ_ATTN, 32, 4, 1)
-DFQ_FORMATS(DFQ_ATTN, 64, 1, 4)
+DFQ_FORMATS(DFQ_ATTN, 64, 1, 3)
 DFQ_FORMATS(DFQ_ATTN, 64, 2, 3)
-DFQ_FORMATS(DFQ_ATTN, 64, 4, 1)
 #elif DFQ_HEAD_DIM == 128
 DFQ_JOINS(128)
-DFQ_FORMATS(DFQ_ATTN, 32, 1, 2)
-DFQ_FORMATS(DFQ_ATTN, 32, 2, 1)
+DFQ_FORMATS(DFQ_ATTN, 32, 1, 3)
+DFQ_FORMATS(DFQ_ATTN, 32, 2, 2)
 DFQ_FORMATS(DFQ_ATTN, 64, 1, 3)
 DFQ_FORMATS(DFQ_ATTN, 64, 2, 2)
-DFQ_FORMATS(DFQ_ATTN, 64, 4, 1)
-DFQ_FORMATS(DFQ_ATTN, 128, 1, 2)
+DFQ_FORMATS(DFQ_ATTN, 128, 1, 3)
 DFQ_FORMATS(DFQ_ATTN, 128, 2, 2)
-DFQ_FORMATS(DFQ_ATTN, 128, 4, 1)
 #elif DFQ_HEAD_DIM == 256
 DFQ_JOINS(128)
 DFQ_FORMATS(DFQ_ATTN, 32, 1, 1)
-DFQ_FORMATS(DFQ_ATTN, 64, 1, 1)
+DFQ_FORMATS(DFQ_ATTN, 64, 1, 2)
+DFQ_FORMATS(DFQ_ATTN, 64, 2, 1)
 DFQ_FORMATS(DFQ_ATTN, 128, 1, 2)
 DFQ_FORMATS(DFQ_ATTN, 128, 2, 1)
 #else

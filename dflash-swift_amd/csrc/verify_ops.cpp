@@ -43,7 +43,7 @@ namespace dfq {
  * than the head have no kernels. */
 struct CacheKernels {
     hipFunction_t append = nullptr, read = nullptr, join = nullptr;
-    hipFunction_t attention[3] = {};  // 1, 2 and 4 row tiles, as many as attention_tiles gives
+    hipFunction_t attention[2] = {};  // up to 1 and 2 row tiles (see attention_tiles)
 };
 
 struct VerifyOps {
@@ -58,10 +58,7 @@ static dfq_status hip_error(hipError_t e, const char* what) {
 
 /* The most tiles of 16 rows that a format's attention kernels take in one pass: what the
  * registers hold (outputs, and the sums of every group). */
-static int attention_tiles(int dim, int gs) {
-    if (dim == 256) return gs == 128 ? 2 : 1;
-    return dim == 128 && gs == 32 ? 2 : 4;
-}
+static int attention_tiles(int dim, int gs) { return dim == 256 && gs == 32 ? 1 : 2; }
 
 static dfq_status resolve(VerifyOps* o) {
     static const char* kDt[3] = {"bf16", "f16", "f32"};
@@ -88,9 +85,9 @@ static dfq_status resolve(VerifyOps* o) {
                         if ((e = hipModuleGetFunction(part.fn, o->kv, name)) != hipSuccess)
                             return hip_error(e, name);
                     }
-                    for (int r = 0; 1 << r <= attention_tiles(64 << d, 32 << g); ++r) {
+                    for (int r = 0; r < attention_tiles(64 << d, 32 << g); ++r) {
                         snprintf(name, sizeof name, "dfq_cache_attention_b%d_g%d_%s_r%d", 4 << b,
-                                 32 << g, kDt[t], 1 << r);
+                                 32 << g, kDt[t], r + 1);
                         if ((e = hipModuleGetFunction(&c.attention[r], o->attention[d], name)) !=
                             hipSuccess)
                             return hip_error(e, name);
@@ -247,7 +244,7 @@ dfq_status check_attention(const dfq_kv_cache* prefix, int prefix_length,
 
 /* How an attention call is cut: row blocks of tiles * 16 rows, and ranges of tokens. */
 struct AttentionPlan {
-    int tiles_log2 = 0;
+    int tiles = 1;      /* most row tiles of a block */
     int prefix_splits = 0, prefix_blocks = 0, own_splits = 0, own_blocks = 0;
     int64_t rows = 0;   /* part rows of a slot: heads * batch * rows * group */
     size_t ml_bytes = 0, bytes = 0;
@@ -257,8 +254,10 @@ struct AttentionPlan {
     }
 };
 
-/* Tokens that a workgroup takes in one round, 32 a wave. */
+/* Tokens that a workgroup takes in one round, 32 a wave; what a workgroup costs besides its
+ * rounds; what the join costs for one more range. */
 constexpr int kRoundTokens = DFQ_KV_THREADS / 2;
+constexpr double kFixedRounds = 2.0, kPartRounds = 0.1;
 
 AttentionPlan plan_attention(int num_cus, const dfq_kv_cache* fmt, int prefix_length,
                              int max_length, int batch, int rows, int q_heads) {
@@ -266,22 +265,37 @@ AttentionPlan plan_attention(int num_cus, const dfq_kv_cache* fmt, int prefix_le
     const int group = q_heads / fmt->heads;
     const int64_t own_rows = (int64_t)rows * group, all_rows = own_rows * batch;
     const int most = attention_tiles(fmt->head_dim, fmt->group_size);
-    /* no more row tiles than the larger row block has */
-    const int64_t need = prefix_length ? all_rows : own_rows;
-    while ((1 << a.tiles_log2) < most && (int64_t)16 << a.tiles_log2 < need) ++a.tiles_log2;
-    const int block = 16 << a.tiles_log2;
+    /* row blocks of whole tiles, as even as they come */
+    const int64_t need = ((prefix_length ? all_rows : own_rows) + 15) / 16;
+    const int64_t blocks = (need + most - 1) / most;
+    a.tiles = (int)((need + blocks - 1) / blocks);
+    const int block = 16 * a.tiles;
     a.rows = fmt->heads * all_rows;
     a.prefix_blocks = (int)((all_rows + block - 1) / block);
     a.own_blocks = (int)((own_rows + block - 1) / block);
-    /* the shortest ranges that keep every workgroup resident at once */
-    const int resident = num_cus * (a.tiles_log2 == 0 ? 3 : a.tiles_log2 == 1 ? 2 : 1);
+    /* The ranges' length that ends first, by rounds: workgroups take what they have in order, the
+     * prefix's first, on the slots that the chip has, each with a fixed cost (staging the queries,
+     * joining the waves) of about two rounds. */
+    const double resident = num_cus * (a.tiles == 1 ? 3 : 2);
     const int prefix_rounds = (prefix_length + kRoundTokens - 1) / kRoundTokens;
     const int own_rounds = (max_length + kRoundTokens - 1) / kRoundTokens;
     const int longest = std::max(prefix_rounds, own_rounds);
+    double best = 0;
     for (int each = 1; each <= longest; each = each < 16 ? each + 1 : each + each / 16) {
-        a.prefix_splits = (prefix_rounds + each - 1) / each;
-        a.own_splits = (own_rounds + each - 1) / each;
-        if (a.groups(fmt->heads, batch) <= resident) break;
+        const int ps = (prefix_rounds + each - 1) / each, os = (own_rounds + each - 1) / each;
+        const double pn = (double)fmt->heads * a.prefix_blocks * ps;
+        const double on = (double)fmt->heads * batch * a.own_blocks * os;
+        const double pl = ps ? (prefix_rounds + ps - 1) / ps + kFixedRounds : 0;
+        const double ol = os ? (own_rounds + os - 1) / os + kFixedRounds : 0;
+        const double longer = std::max(pl, ol);
+        const double t = std::max(std::ceil(pn / resident) * pl,
+                                  std::ceil((pn * pl + on * ol) / resident / longer) * longer) +
+                         kPartRounds * (ps + os);
+        if (best == 0 || t < best) {
+            best = t;
+            a.prefix_splits = ps;
+            a.own_splits = os;
+        }
     }
     const size_t slots = (size_t)a.prefix_splits + a.own_splits;
     a.ml_bytes = (slots * a.rows * 8 + 255) & ~(size_t)255;
@@ -415,7 +429,7 @@ dfq_status dfq_cache_attention(dfq_ctx* ctx, const dfq_kv_cache* prefix, int pre
     void* args[] = {&p};
     hipError_t e = hipSuccess;
     if (groups)
-        e = hipModuleLaunchKernel(fn.attention[a.tiles_log2], (unsigned)groups, 1, 1,
+        e = hipModuleLaunchKernel(fn.attention[a.tiles - 1], (unsigned)groups, 1, 1,
                                   DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
     if (e == hipSuccess)
         e = hipModuleLaunchKernel(fn.join, (unsigned)(batch * rows * group),
