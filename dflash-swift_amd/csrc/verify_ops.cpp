@@ -179,11 +179,19 @@ dfq_status check_cache(const dfq_kv_cache* c) {
     return DFQ_OK;
 }
 
+/* Workgroups of an append or read of one sequence: 8 channels a thread, the heads of the same rows
+ * side by side, so that they touch the dense side's rows together. */
+int64_t row_blocks(const dfq_kv_cache* c, int rows) {
+    const int64_t per = DFQ_KV_THREADS * 8 / c->head_dim;
+    return (rows + per - 1) / per * c->heads;
+}
+
 dfq_status check_span(const dfq_kv_cache* c, int batch, int rows) {
     if (batch < 1 || rows < 1) return fail(DFQ_ERR_INVALID_ARGUMENT, "batch and rows must be >= 1");
     if (batch > c->slots)
         return fail(DFQ_ERR_INVALID_ARGUMENT, "%d sequences in a cache of %d slots", batch,
                     c->slots);
+    if (row_blocks(c, rows) > INT32_MAX) return fail(DFQ_ERR_UNSUPPORTED, "grid too large");
     return DFQ_OK;
 }
 
@@ -195,12 +203,6 @@ const CacheKernels& kernels_of(const dfq_ctx* ctx, const dfq_kv_cache* c) {
 KvArrays arrays_of(const dfq_kv_cache* c, bool v) {
     return v ? KvArrays{c->v_codes, (uint16_t*)c->v_scales, (uint16_t*)c->v_biases}
              : KvArrays{c->k_codes, (uint16_t*)c->k_scales, (uint16_t*)c->k_biases};
-}
-
-/* Workgroups along the rows of an append or read: 8 channels a thread. */
-unsigned row_blocks(const dfq_kv_cache* c, int rows) {
-    const int per = DFQ_KV_THREADS * 8 / c->head_dim;
-    return ((unsigned)rows + per - 1) / per;
 }
 
 /* The sizes of an attention call; *fmt gets the cache that carries the format. */
@@ -324,8 +326,7 @@ dfq_status dfq_cache_append(dfq_ctx* ctx, const dfq_kv_cache* cache, const void*
     DeviceScope scope(ctx);
     void* args[] = {&p};
     const hipError_t e = hipModuleLaunchKernel(
-        kernels_of(ctx, cache).append, row_blocks(cache, rows), (unsigned)cache->heads,
-        2u * batch, DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
+        kernels_of(ctx, cache).append, (unsigned)row_blocks(cache, rows), 1, (unsigned)batch, DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
     return e == hipSuccess ? DFQ_OK : hip_error(e, "launch dfq_cache_append");
 }
 
@@ -346,8 +347,7 @@ dfq_status dfq_cache_read(dfq_ctx* ctx, const dfq_kv_cache* cache, void* k, void
     DeviceScope scope(ctx);
     void* args[] = {&p, &dt};
     const hipError_t e = hipModuleLaunchKernel(
-        kernels_of(ctx, cache).read, row_blocks(cache, rows), (unsigned)cache->heads, 2u * batch,
-        DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
+        kernels_of(ctx, cache).read, (unsigned)row_blocks(cache, rows), 1, 2u * batch, DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
     return e == hipSuccess ? DFQ_OK : hip_error(e, "launch dfq_cache_read");
 }
 
