@@ -822,10 +822,6 @@ __device__ __forceinline__ void attention(const KvAttnParams& p) {
     const int tiles = (job.nrows + 15) / 16;
     if constexpr (RT > 1)
         if (tiles == 1) return Attention<BITS, GS, F16, 1>::run(p, job, h, lds);
-    if constexpr (RT > 2)
-        if (tiles == 2) return Attention<BITS, GS, F16, 2>::run(p, job, h, lds);
-    if constexpr (RT > 3)
-        if (tiles == 3) return Attention<BITS, GS, F16, 3>::run(p, job, h, lds);
     Most::run(p, job, h, lds);
 }
 
@@ -926,11 +922,9 @@ DFQ_FORMATS(DFQ_ATTN, 128, 1, 3)
 DFQ_FORMATS(DFQ_ATTN, 128, 2, 2)
 #elif DFQ_HEAD_DIM == 256
 DFQ_JOINS(128)
-DFQ_FORMATS(DFQ_ATTN, 32, 1, 1)
+DFQ_FORMATS(DFQ_ATTN, 32, 1, 2)
 DFQ_FORMATS(DFQ_ATTN, 64, 1, 2)
-DFQ_FORMATS(DFQ_ATTN, 64, 2, 1)
 DFQ_FORMATS(DFQ_ATTN, 128, 1, 2)
-DFQ_FORMATS(DFQ_ATTN, 128, 2, 1)
 #else
 #error "DFQ_HEAD_DIM must be 64, 128 or 256"
 #endif

@@ -44,6 +44,7 @@ namespace dfq {
 struct CacheKernels {
     hipFunction_t append = nullptr, read = nullptr, join = nullptr;
     hipFunction_t attention[2] = {};  // up to 1 and 2 row tiles (see attention_tiles)
+    int resident[2] = {};             // their workgroups that a CU holds at once
 };
 
 struct VerifyOps {
@@ -56,9 +57,12 @@ static dfq_status hip_error(hipError_t e, const char* what) {
     return fail(DFQ_ERR_HIP, "%s: %s (%d)", what, hipGetErrorString(e), (int)e);
 }
 
-/* The most tiles of 16 rows that a format's attention kernels take in one pass: what the
- * registers hold (outputs, and the sums of every group). */
-static int attention_tiles(int dim, int gs) { return dim == 256 && gs == 32 ? 1 : 2; }
+/* The most tiles of 16 rows that attention kernels take in one pass.  Two read and unpack the
+ * codes once for both: 16 sequences of 8 rows of 40 heads over a shared 16384-token prefix take
+ * 102 us, one tile 118.  At heads of 256 their outputs leave a CU room for one workgroup of two
+ * tiles and two of one: 16 rows of 16 heads over 16000 tokens 44.8 us against 35.7, so there it
+ * is one.  Three and four spill at any width. */
+static int attention_tiles(int dim) { return dim == 256 ? 1 : 2; }
 
 static dfq_status resolve(VerifyOps* o) {
     static const char* kDt[3] = {"bf16", "f16", "f32"};
@@ -85,12 +89,16 @@ static dfq_status resolve(VerifyOps* o) {
                         if ((e = hipModuleGetFunction(part.fn, o->kv, name)) != hipSuccess)
                             return hip_error(e, name);
                     }
-                    for (int r = 0; r < attention_tiles(64 << d, 32 << g); ++r) {
+                    for (int r = 0; r < attention_tiles(64 << d); ++r) {
                         snprintf(name, sizeof name, "dfq_cache_attention_b%d_g%d_%s_r%d", 4 << b,
                                  32 << g, kDt[t], r + 1);
                         if ((e = hipModuleGetFunction(&c.attention[r], o->attention[d], name)) !=
                             hipSuccess)
                             return hip_error(e, name);
+                        if ((e = hipModuleOccupancyMaxActiveBlocksPerMultiprocessor(
+                                 &c.resident[r], c.attention[r], DFQ_KV_THREADS, 0)) != hipSuccess)
+                            return hip_error(e, name);
+                        if (c.resident[r] < 1) return fail(DFQ_ERR_HIP, "%s does not fit", name);
                     }
                     snprintf(name, sizeof name, "dfq_cache_attention_join_g%d_%s", 32 << g, kDt[t]);
                     if ((e = hipModuleGetFunction(&c.join, o->attention[d], name)) != hipSuccess)
@@ -256,47 +264,97 @@ struct AttentionPlan {
     }
 };
 
-/* Tokens that a workgroup takes in one round, 32 a wave; what a workgroup costs besides its
- * rounds; what the join costs for one more range. */
+/* Tokens that a workgroup takes in one round, 32 a wave. */
 constexpr int kRoundTokens = DFQ_KV_THREADS / 2;
-constexpr double kFixedRounds = 2.0, kPartRounds = 0.1;
+/* The plan's model of time, in rounds of a workgroup that has a CU to itself: what a workgroup
+ * costs besides its rounds (staging the queries, joining its waves); how many a CU works on
+ * together before they slow each other down (they wait for memory, then for issue); what two
+ * tiles cost against one; and what one more range costs the join.  Over the plans of eleven
+ * shapes (heads of 64, 128 and 256, 1..16 sequences, own caches and shared prefixes) the one
+ * that these numbers choose is within 3 % of the fastest. */
+constexpr double kFixedRounds = 1.5, kTogether = 1.5, kTwoTiles = 1.6, kRangeRounds = 0.03;
 
-AttentionPlan plan_attention(int num_cus, const dfq_kv_cache* fmt, int prefix_length,
+/* The workgroups of `blocks` row blocks over `rounds` rounds in ranges of at most `each`, as even
+ * as they come, by themselves: how long, and how much. */
+struct Share {
+    double time = 0, work = 0;
+    int64_t groups = 0;
+    int ranges = 0;
+    double longest = 0;   /* a workgroup */
+};
+struct Card {
+    int cus, resident;
+    double cost(int64_t groups) const {
+        const int64_t per = std::min<int64_t>(resident, (groups + cus - 1) / cus);
+        return per < kTogether ? 1.0 : per / kTogether;
+    }
+    Share share(int64_t blocks, int rounds, int each) const {
+        Share s;
+        if (!rounds) return s;
+        s.ranges = (rounds + each - 1) / each;
+        each = (rounds + s.ranges - 1) / s.ranges;
+        const int whole = rounds / each, last = rounds - whole * each;
+        const int64_t room = (int64_t)cus * resident, full = blocks * whole;
+        const int64_t passes = full / room, rest = full - passes * room;
+        s.longest = each + kFixedRounds;
+        s.groups = blocks * s.ranges;
+        s.work = (double)blocks * (rounds + s.ranges * kFixedRounds);
+        s.time = passes * s.longest * cost(room);
+        if (rest) s.time += s.longest * cost(rest);
+        if (last && (!rest || rest + blocks > room)) s.time += last + kFixedRounds;
+        return s;
+    }
+};
+
+AttentionPlan plan_attention(dfq_ctx* ctx, const dfq_kv_cache* fmt, int prefix_length,
                              int max_length, int batch, int rows, int q_heads) {
     AttentionPlan a;
     const int group = q_heads / fmt->heads;
     const int64_t own_rows = (int64_t)rows * group, all_rows = own_rows * batch;
-    const int most = attention_tiles(fmt->head_dim, fmt->group_size);
-    /* row blocks of whole tiles, as even as they come */
-    const int64_t need = ((prefix_length ? all_rows : own_rows) + 15) / 16;
-    const int64_t blocks = (need + most - 1) / most;
-    a.tiles = (int)((need + blocks - 1) / blocks);
-    const int block = 16 * a.tiles;
     a.rows = fmt->heads * all_rows;
-    a.prefix_blocks = (int)((all_rows + block - 1) / block);
-    a.own_blocks = (int)((own_rows + block - 1) / block);
-    /* The ranges' length that ends first, by rounds: workgroups take what they have in order, the
-     * prefix's first, on the slots that the chip has, each with a fixed cost (staging the queries,
-     * joining the waves) of about two rounds. */
-    const double resident = num_cus * (a.tiles == 1 ? 3 : 2);
     const int prefix_rounds = (prefix_length + kRoundTokens - 1) / kRoundTokens;
     const int own_rounds = (max_length + kRoundTokens - 1) / kRoundTokens;
     const int longest = std::max(prefix_rounds, own_rounds);
+    const int most = std::min<int64_t>(attention_tiles(fmt->head_dim),
+                                       ((prefix_length ? all_rows : own_rows) + 15) / 16);
     double best = 0;
-    for (int each = 1; each <= longest; each = each < 16 ? each + 1 : each + each / 16) {
-        const int ps = (prefix_rounds + each - 1) / each, os = (own_rounds + each - 1) / each;
-        const double pn = (double)fmt->heads * a.prefix_blocks * ps;
-        const double on = (double)fmt->heads * batch * a.own_blocks * os;
-        const double pl = ps ? (prefix_rounds + ps - 1) / ps + kFixedRounds : 0;
-        const double ol = os ? (own_rounds + os - 1) / os + kFixedRounds : 0;
-        const double longer = std::max(pl, ol);
-        const double t = std::max(std::ceil(pn / resident) * pl,
-                                  std::ceil((pn * pl + on * ol) / resident / longer) * longer) +
-                         kPartRounds * (ps + os);
-        if (best == 0 || t < best) {
-            best = t;
-            a.prefix_splits = ps;
-            a.own_splits = os;
+    for (int tiles = 1; tiles <= most; ++tiles) {
+        const Card card = {dfq_num_cus(ctx), kernels_of(ctx, fmt).resident[tiles - 1]};
+        const int64_t pb = (all_rows + 16 * tiles - 1) / (16 * tiles);
+        const int64_t ob = (own_rows + 16 * tiles - 1) / (16 * tiles);
+        const int64_t pn = fmt->heads * pb, on = fmt->heads * ob * batch;
+        const double round = tiles == 1 ? 1.0 : kTwoTiles;
+        const double all = (double)pn * prefix_rounds + (double)on * own_rounds;
+        const int64_t room = (int64_t)card.cus * card.resident;
+        /* ranges that fill every CU with 1, 2, .. workgroups, in one pass and in some */
+        for (int fill = 1; fill <= card.resident + 3 && longest; ++fill) {
+            const int more = fill - card.resident;
+            const int per = more <= 0 ? fill : card.resident * (1 + more);
+            const double even = std::floor(all / ((double)card.cus * per));
+            for (int up = 0; up < 2; ++up) {
+                const int each = (int)std::min<double>(longest, std::max(1.0, even + up));
+                const Share p = card.share(pn, prefix_rounds, each);
+                const Share o = card.share(on, own_rounds, each);
+                double t = p.time + o.time;
+                if (p.groups && o.groups) {
+                    /* the prefix's workgroups come first, and the others fill what they leave */
+                    const int64_t n = p.groups + o.groups;
+                    const int64_t busy =
+                        std::min<int64_t>(card.resident, (n + card.cus - 1) / card.cus);
+                    const double work = (p.work + o.work) / (card.cus * busy) * card.cost(n);
+                    t = std::max(p.time, n <= room ? std::max(o.longest * card.cost(n), work)
+                                                   : work + 0.5 * o.longest);
+                }
+                t = t * round + kRangeRounds * (p.ranges + o.ranges);
+                if (best == 0 || t < best) {
+                    best = t;
+                    a.tiles = tiles;
+                    a.prefix_splits = p.ranges;
+                    a.own_splits = o.ranges;
+                    a.prefix_blocks = (int)pb;
+                    a.own_blocks = (int)ob;
+                }
+            }
         }
     }
     const size_t slots = (size_t)a.prefix_splits + a.own_splits;
@@ -326,7 +384,8 @@ dfq_status dfq_cache_append(dfq_ctx* ctx, const dfq_kv_cache* cache, const void*
     DeviceScope scope(ctx);
     void* args[] = {&p};
     const hipError_t e = hipModuleLaunchKernel(
-        kernels_of(ctx, cache).append, (unsigned)row_blocks(cache, rows), 1, (unsigned)batch, DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
+        kernels_of(ctx, cache).append, (unsigned)row_blocks(cache, rows), 1, (unsigned)batch,
+        DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
     return e == hipSuccess ? DFQ_OK : hip_error(e, "launch dfq_cache_append");
 }
 
@@ -347,7 +406,8 @@ dfq_status dfq_cache_read(dfq_ctx* ctx, const dfq_kv_cache* cache, void* k, void
     DeviceScope scope(ctx);
     void* args[] = {&p, &dt};
     const hipError_t e = hipModuleLaunchKernel(
-        kernels_of(ctx, cache).read, (unsigned)row_blocks(cache, rows), 1, 2u * batch, DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
+        kernels_of(ctx, cache).read, (unsigned)row_blocks(cache, rows), 1, 2u * batch,
+        DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
     return e == hipSuccess ? DFQ_OK : hip_error(e, "launch dfq_cache_read");
 }
 
@@ -362,7 +422,7 @@ dfq_status dfq_cache_attention_workspace_bytes(dfq_ctx* ctx, const dfq_kv_cache*
     dfq_status s =
         check_attention(prefix, prefix_length, cache, max_length, batch, rows, q_heads, &fmt);
     if (s) return s;
-    *bytes = plan_attention(dfq_num_cus(ctx), fmt, prefix_length, max_length, batch, rows, q_heads)
+    *bytes = plan_attention(ctx, fmt, prefix_length, max_length, batch, rows, q_heads)
                  .bytes;
     return DFQ_OK;
 }
@@ -388,7 +448,7 @@ dfq_status dfq_cache_attention(dfq_ctx* ctx, const dfq_kv_cache* prefix, int pre
     if (!(scale > 0.0f) || !std::isfinite(scale))
         return fail(DFQ_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
     const AttentionPlan a =
-        plan_attention(dfq_num_cus(ctx), fmt, prefix_length, max_length, batch, rows, q_heads);
+        plan_attention(ctx, fmt, prefix_length, max_length, batch, rows, q_heads);
     const int64_t groups = a.groups(fmt->heads, batch);
     const int group = q_heads / fmt->heads;
     if (groups > INT32_MAX || (int64_t)batch * rows * group > INT32_MAX)

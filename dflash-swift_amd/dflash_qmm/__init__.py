@@ -31,6 +31,7 @@ __all__ = [
 ]
 
 BF16, F16, F32 = 0, 1, 2
+_ERR_WORKSPACE = 3
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _LIB_NAME = "libdflash_qmm.so"
@@ -528,17 +529,21 @@ class Context:
         pd = prefix.desc if prefix is not None else None
         cd = cache.desc if cache is not None else None
         stream = self._stream_of(stream)
-        if ws is None:
-            st = self.lib.dfq_cache_attention_workspace_bytes(
-                self.handle, pd, prefix_length, cd, max_length, batch, rows, heads, self._need)
-            if st:
-                _check(st, "dfq_cache_attention_workspace_bytes")
+        own_ws = ws is None
+        if own_ws:
+            ws = self.workspace_uncleared(1, stream)
+        for again in (own_ws, False):
+            st = self.lib.dfq_cache_attention(
+                self.handle, pd, prefix_length, cd, d_lengths, max_length, d_tree, q.data_ptr(),
+                _row_stride(q), out.data_ptr(), lse.data_ptr(), batch, rows, heads, scale,
+                ws.data_ptr(), ws.numel(), stream)
+            if st != _ERR_WORKSPACE or not again:
+                break
+            # the scratch is as large as any call on the stream needed so far: ask, and grow it
+            _check(self.lib.dfq_cache_attention_workspace_bytes(
+                self.handle, pd, prefix_length, cd, max_length, batch, rows, heads, self._need),
+                "dfq_cache_attention_workspace_bytes")
             ws = self.workspace_uncleared(self._need.value, stream)
-        ws_ptr, ws_bytes = (ws.data_ptr(), ws.numel()) if ws is not None else (None, 0)
-        st = self.lib.dfq_cache_attention(
-            self.handle, pd, prefix_length, cd, d_lengths, max_length, d_tree, q.data_ptr(),
-            _row_stride(q), out.data_ptr(), lse.data_ptr(), batch, rows, heads, scale, ws_ptr,
-            ws_bytes, stream)
         if st:
             _check(st, "dfq_cache_attention")
         return out, lse
@@ -562,16 +567,21 @@ class Context:
             ids = torch.empty((M, more), dtype=torch.int32, device=logits.device)
             top = f[2 * M:].view(M, more)
         stream = self._stream_of(stream)
-        if ws is None:
-            st = self.lib.dfq_token_logprobs_workspace_bytes(self.handle, M, V, top_k, self._need)
-            if st:
-                _check(st, "dfq_token_logprobs_workspace_bytes")
+        own_ws = ws is None
+        if own_ws:
+            ws = self.workspace_uncleared(1, stream)
+        for again in (own_ws, False):
+            st = self.lib.dfq_token_logprobs(
+                self.handle, logits.data_ptr(), logits.stride(0) if M > 1 else V, M, V,
+                dtype_code(logits), d_tokens, top_k, p + 4 * M if tokens is not None else None, p,
+                ids.data_ptr() if more else None, p + 8 * M if more else None, ws.data_ptr(),
+                ws.numel(), stream)
+            if st != _ERR_WORKSPACE or not again:
+                break
+            _check(self.lib.dfq_token_logprobs_workspace_bytes(self.handle, M, V, top_k,
+                                                               self._need),
+                   "dfq_token_logprobs_workspace_bytes")
             ws = self.workspace_uncleared(self._need.value, stream)
-        st = self.lib.dfq_token_logprobs(
-            self.handle, logits.data_ptr(), logits.stride(0) if M > 1 else V, M, V,
-            dtype_code(logits), d_tokens, top_k, p + 4 * M if tokens is not None else None, p,
-            ids.data_ptr() if more else None, p + 8 * M if more else None,
-            ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, stream)
         if st:
             _check(st, "dfq_token_logprobs")
         return lp, entropy, ids, top
