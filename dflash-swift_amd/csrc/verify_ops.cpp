@@ -517,6 +517,7 @@ static size_t logprob_keys_bytes(int M, int splits, int top_k) {
     return ((size_t)M * splits * (DFQ_KV_THREADS / 64) * top_k * 8 + 15) & ~(size_t)15;
 }
 static size_t logprob_bytes(int M, int splits, int top_k) {
+    if (splits == 1) return 0;
     return logprob_keys_bytes(M, splits, top_k) + (size_t)M * splits * (DFQ_KV_THREADS / 64) * 16;
 }
 
@@ -553,7 +554,7 @@ dfq_status dfq_token_logprobs(dfq_ctx* ctx, const void* logits, int64_t row_stri
         return fail(DFQ_ERR_INVALID_ARGUMENT, "misaligned buffer");
     const int splits = logprob_splits(dfq_num_cus(ctx), M, V);
     const size_t need = logprob_bytes(M, splits, top_k);
-    if (!workspace || workspace_bytes < need)
+    if (need && (!workspace || workspace_bytes < need))
         return fail(DFQ_ERR_WORKSPACE, "workspace of %zu bytes needed (got %zu)", need,
                     workspace ? workspace_bytes : (size_t)0);
     if (!aligned(workspace, 16))
@@ -569,7 +570,7 @@ dfq_status dfq_token_logprobs(dfq_ctx* ctx, const void* logits, int64_t row_stri
     hipError_t e = hipModuleLaunchKernel(ops->logprobs_part[(int)dtype], (unsigned)M * splits, 1,
                                          1, DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args,
                                          nullptr);
-    if (e == hipSuccess)
+    if (e == hipSuccess && splits > 1)
         e = hipModuleLaunchKernel(ops->logprobs_join[(int)dtype], (unsigned)M, 1, 1, 64, 1, 1, 0,
                                   (hipStream_t)stream, args, nullptr);
     return e == hipSuccess ? DFQ_OK : hip_error(e, "launch dfq_token_logprobs");

@@ -559,13 +559,16 @@ class Context:
         # the fp32 outputs of one allocation, as wide as they are asked for
         more = top_k if top_k > 0 else 0
         f = torch.empty(M * (2 + more), dtype=torch.float32, device=logits.device)
-        entropy = f[:M]
-        lp = f[M:2 * M] if tokens is not None else None
+        entropy, lp, top = f.split((M, M, M * more))
+        if tokens is None:
+            lp = None
         p = f.data_ptr()
-        ids = top = None
+        ids = None
         if more:
             ids = torch.empty((M, more), dtype=torch.int32, device=logits.device)
-            top = f[2 * M:].view(M, more)
+            top = top.view(M, more)
+        else:
+            top = None
         stream = self._stream_of(stream)
         own_ws = ws is None
         if own_ws:
