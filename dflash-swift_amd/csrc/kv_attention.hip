@@ -888,8 +888,8 @@ __device__ __forceinline__ void join(const KvAttnParams& p) {
 
 }  // namespace
 
-/* Built for as many row tiles as the registers hold without spilling; per_simd is the waves a
- * SIMD then has room for.  attention_tiles (verify_ops.cpp) knows which exist. */
+/* Built for the row tiles that attention_tiles (verify_ops.cpp) asks for; per_4 and per_8 are the
+ * waves that a SIMD has registers and LDS for with 4 and 8 bits. */
 #define DFQ_ATTN(bits, gs, name, f16, rt, per_simd)                                            \
     extern "C" __global__ __launch_bounds__(DFQ_KV_THREADS, per_simd) void                     \
         dfq_cache_attention_b##bits##_g##gs##_##name##_r##rt(KvAttnParams p) {                 \
@@ -900,31 +900,31 @@ __device__ __forceinline__ void join(const KvAttnParams& p) {
         dfq_cache_attention_join_g##gs##_##name(KvAttnParams p) {                              \
         join<gs, f16>(p);                                                                      \
     }
-#define DFQ_FORMATS(M, gs, rt, per_simd)                                  \
-    M(4, gs, bf16, false, rt, per_simd) M(8, gs, bf16, false, rt, per_simd) \
-    M(4, gs, f16, true, rt, per_simd) M(8, gs, f16, true, rt, per_simd)
+#define DFQ_FORMATS(M, gs, rt, per_4, per_8)                          \
+    M(4, gs, bf16, false, rt, per_4) M(8, gs, bf16, false, rt, per_8) \
+    M(4, gs, f16, true, rt, per_4) M(8, gs, f16, true, rt, per_8)
 #define DFQ_JOINS(gs) DFQ_JOIN(gs, bf16, false) DFQ_JOIN(gs, f16, true)
 
 DFQ_JOINS(32)
 DFQ_JOINS(64)
 #if DFQ_HEAD_DIM == 64
-DFQ_FORMATS(DFQ_ATTN, 32, 1, 3)
-DFQ_FORMATS(DFQ_ATTN, 32, 2, 2)
-DFQ_FORMATS(DFQ_ATTN, 64, 1, 3)
-DFQ_FORMATS(DFQ_ATTN, 64, 2, 3)
+DFQ_FORMATS(DFQ_ATTN, 32, 1, 3, 3)
+DFQ_FORMATS(DFQ_ATTN, 32, 2, 2, 2)
+DFQ_FORMATS(DFQ_ATTN, 64, 1, 3, 3)
+DFQ_FORMATS(DFQ_ATTN, 64, 2, 3, 3)
 #elif DFQ_HEAD_DIM == 128
 DFQ_JOINS(128)
-DFQ_FORMATS(DFQ_ATTN, 32, 1, 3)
-DFQ_FORMATS(DFQ_ATTN, 32, 2, 2)
-DFQ_FORMATS(DFQ_ATTN, 64, 1, 3)
-DFQ_FORMATS(DFQ_ATTN, 64, 2, 2)
-DFQ_FORMATS(DFQ_ATTN, 128, 1, 3)
-DFQ_FORMATS(DFQ_ATTN, 128, 2, 2)
+DFQ_FORMATS(DFQ_ATTN, 32, 1, 3, 3)
+DFQ_FORMATS(DFQ_ATTN, 32, 2, 2, 2)
+DFQ_FORMATS(DFQ_ATTN, 64, 1, 3, 3)
+DFQ_FORMATS(DFQ_ATTN, 64, 2, 2, 2)
+DFQ_FORMATS(DFQ_ATTN, 128, 1, 3, 3)
+DFQ_FORMATS(DFQ_ATTN, 128, 2, 2, 2)
 #elif DFQ_HEAD_DIM == 256
 DFQ_JOINS(128)
-DFQ_FORMATS(DFQ_ATTN, 32, 1, 2)
-DFQ_FORMATS(DFQ_ATTN, 64, 1, 2)
-DFQ_FORMATS(DFQ_ATTN, 128, 1, 2)
+DFQ_FORMATS(DFQ_ATTN, 32, 1, 2, 1)
+DFQ_FORMATS(DFQ_ATTN, 64, 1, 2, 1)
+DFQ_FORMATS(DFQ_ATTN, 128, 1, 2, 2)
 #else
 #error "DFQ_HEAD_DIM must be 64, 128 or 256"
 #endif

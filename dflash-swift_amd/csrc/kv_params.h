@@ -63,7 +63,7 @@ struct LogprobParams {
     float* part_sums;        /* [row][part][4]: maximum, sum, entropy sum                   */
     int64_t row_stride;
     int rows, vocab, top;
-    int splits;              /* workgroups a row; parts = splits * waves                    */
+    int splits;              /* workgroups, and parts, a row                                */
 };
 
 #endif

@@ -245,8 +245,7 @@ struct Pieces {
     }
 
     static __device__ __forceinline__ void part(const LogprobParams& p) {
-        __shared__ __attribute__((aligned(16))) uint64_t room[kWaves][kRoom];
-        static_assert(kWaves * 32 <= 64 * kPiece && kRoom % 2 == 0, "a row's keys in one piece");
+        __shared__ uint64_t room[kWaves][kRoom];
         const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
         const int r = blockIdx.x / p.splits, parts = p.splits * kWaves;
         const int part = blockIdx.x % p.splits * kWaves + wave;
@@ -302,37 +301,65 @@ struct Pieces {
         }
         for (int d = 1; d < 64; d *= 2)
             s.join(__shfl_xor(s.m, d), __shfl_xor(s.l, d), __shfl_xor(s.e, d));
-        if (p.top) b.sort<kLow>(lane);
-        const f32x4_t sum = {s.m, s.l, s.e, 0.0f};
-        const uint64_t key = lane < p.top && lane < b.count ? b.keys[lane] : 0;
-        if (p.splits == 1) {
-            /* the whole row is here: its keys go to the first wave's room, which takes them into
-             * registers before it uses the room again, and its sums to the second's */
-            f32x4_t* sums = (f32x4_t*)room[1];
-            __syncthreads();
-            if (lane == 0) sums[wave] = sum;
-            if (lane < p.top) room[0][wave * p.top + lane] = key;
-            __syncthreads();
-            if (wave == 0) join(p, r, lane, kWaves, sums, room[0], room[0]);
-            return;
+        /* the waves' sums and candidates together, by the first wave */
+        __shared__ f32x4_t sums[kWaves];
+        __shared__ int counts[kWaves];
+        if (lane == 0) {
+            sums[wave] = f32x4_t{s.m, s.l, s.e, 0.0f};
+            counts[wave] = b.count;
         }
-        const int64_t slot = (int64_t)r * parts + part;
-        if (lane == 0) *(f32x4_t*)(p.part_sums + slot * 4) = sum;
-        if (lane < p.top) p.part_keys[slot * p.top + lane] = key;
+        __syncthreads();
+        if (wave != 0) return;
+        for (int w = 1; w < kWaves; ++w) {
+            s.join(sums[w][0], sums[w][1], sums[w][2]);
+            if (p.top == 0) continue;
+            const int n = __builtin_amdgcn_readfirstlane(counts[w]);   /* at most kKept */
+            b.push(lane < n ? room[w][lane] : 0, lane);
+            if (b.count > kKept) b.sort<kLow>(lane);
+        }
+        if (p.top) b.sort<kLow>(lane);
+        if (p.splits == 1) return finish(p, r, lane, s, b);
+        if (lane == 0) *(f32x4_t*)(p.part_sums + (int64_t)blockIdx.x * 4) = f32x4_t{s.m, s.l, s.e, 0.0f};
+        if (lane < p.top)
+            p.part_keys[(int64_t)blockIdx.x * p.top + lane] = lane < b.count ? b.keys[lane] : 0;
     }
 
     /* A row's parts together, by one wave. */
-    static __device__ __forceinline__ void join(const LogprobParams& p, int r, int lane, int parts,
-                                                const f32x4_t* sums, const uint64_t* keys,
-                                                uint64_t* room) {
+    static __device__ __forceinline__ void join(const LogprobParams& p) {
+        __shared__ uint64_t room[kRoom];
+        const int lane = threadIdx.x, r = blockIdx.x;
+        const f32x4_t* sums = (const f32x4_t*)p.part_sums + (int64_t)r * p.splits;
         Sums s;
         s.start();
-        for (int i = lane; i < parts; i += 64) {
+        for (int i = lane; i < p.splits; i += 64) {
             const f32x4_t v = sums[i];
             s.join(v[0], v[1], v[2]);
         }
         for (int d = 1; d < 64; d *= 2)
             s.join(__shfl_xor(s.m, d), __shfl_xor(s.l, d), __shfl_xor(s.e, d));
+        Best b;
+        b.start(room, p.top);
+        const int n = p.splits * p.top;
+        const uint64_t* keys = p.part_keys + (int64_t)r * n;
+        for (int at = 0; at < n; at += 64 * kPiece) {
+            uint64_t k[kPiece];
+#pragma unroll
+            for (int j = 0; j < kPiece; ++j) {
+                const int i = at + j * 64 + lane;
+                k[j] = i < n ? keys[i] : 0;
+            }
+#pragma unroll
+            for (int j = 0; j < kPiece; ++j)
+                if (at + j * 64 < n) b.push(k[j], lane);
+            if (b.count > kKept) b.sort<kLow>(lane);
+        }
+        if (p.top) b.sort<kLow>(lane);
+        finish(p, r, lane, s, b);
+    }
+
+    /* A row's outputs from its sums and its best, sorted. */
+    static __device__ __forceinline__ void finish(const LogprobParams& p, int r, int lane,
+                                                  const Sums& s, const Best& b) {
         /* no number above -inf: no distribution */
         const float log_l = s.l > 0.0f ? logf(s.l) : __builtin_nanf("");
         if (lane == 0) {
@@ -344,22 +371,6 @@ struct Pieces {
                                                       : __builtin_nanf("");
             }
         }
-        if (!p.top) return;
-        Best b;
-        b.start(room, p.top);
-        const int n = parts * p.top;
-        for (int at = 0; at < n; at += 64 * kPiece) {
-            uint64_t k[kPiece];
-#pragma unroll
-            for (int j = 0; j < kPiece; ++j) {
-                const int i = at + j * 64 + lane;
-                k[j] = i < n ? keys[i] : 0;
-            }
-#pragma unroll
-            for (int j = 0; j < kPiece; ++j) b.push(k[j], lane);
-            if (b.count > kKept) b.sort<kLow>(lane);
-        }
-        b.sort<kLow>(lane);
         if (lane < p.top) {
             const bool has = lane < b.count;
             const uint64_t k = b.keys[lane];
@@ -379,11 +390,7 @@ struct Pieces {
     }                                                                            \
     extern "C" __global__ __launch_bounds__(64) void                             \
         dfq_token_logprobs_join_##name(LogprobParams p) {                        \
-        __shared__ uint64_t room[kRoom];                                         \
-        const int r = blockIdx.x, parts = p.splits * kWaves;                     \
-        Pieces<dt>::join(p, r, threadIdx.x, parts,                               \
-                         (const f32x4_t*)p.part_sums + (int64_t)r * parts,       \
-                         p.part_keys + (int64_t)r * parts * p.top, room);        \
+        Pieces<dt>::join(p);                                                     \
     }
 DFQ_LOGPROB_KERNELS(bf16, 0)
 DFQ_LOGPROB_KERNELS(f16, 1)

@@ -512,13 +512,13 @@ static int logprob_splits(int num_cus, int M, int V) {
     return std::min({most, (int)(((int64_t)V + 4095) / 4096), 64});
 }
 
-/* The keys of a row's parts, then their sums; 4 waves a workgroup. */
+/* The keys of the rows' parts, then their sums. */
 static size_t logprob_keys_bytes(int M, int splits, int top_k) {
-    return ((size_t)M * splits * (DFQ_KV_THREADS / 64) * top_k * 8 + 15) & ~(size_t)15;
+    return ((size_t)M * splits * top_k * 8 + 15) & ~(size_t)15;
 }
 static size_t logprob_bytes(int M, int splits, int top_k) {
     if (splits == 1) return 0;
-    return logprob_keys_bytes(M, splits, top_k) + (size_t)M * splits * (DFQ_KV_THREADS / 64) * 16;
+    return logprob_keys_bytes(M, splits, top_k) + (size_t)M * splits * 16;
 }
 
 dfq_status dfq_token_logprobs_workspace_bytes(dfq_ctx* ctx, int M, int V, int top_k,
