@@ -66,6 +66,35 @@ __device__ __forceinline__ void wave_order() {
     __builtin_amdgcn_wave_barrier();
 }
 
+/* n / by and n - n / by * by. */
+__device__ __forceinline__ int divided(int n, const Divisor& d) {
+    return (int)((__umulhi((uint32_t)n, d.mul) + (uint32_t)n) >> d.shift);
+}
+
+/* The largest and the sum of the L neighbouring lanes around each (4, 8, 16 or 32). */
+template <int L>
+__device__ __forceinline__ float largest_of(float v) {
+    v = __uint_as_float(group_of<L < 16 ? L : 16>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }));
+    return L == 32 ? fmaxf(v, __shfl_xor(v, 16)) : v;
+}
+template <int L>
+__device__ __forceinline__ float sum_of(float v) {
+    return __uint_as_float(group_of<L>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+    }));
+}
+
+/* The sum of a lane's value and of those 16, 32 and 48 lanes on, by exchanging halves of rows. */
+__device__ __forceinline__ float quarters_sum(float v) {
+    uint32_t u = __float_as_uint(v);
+    auto x = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    u = __float_as_uint(__uint_as_float(x[0]) + __uint_as_float(x[1]));
+    x = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+}
+
 /* Everything of one (head, row block, token range) of a launch. */
 struct Job {
     const char *k, *v;          /* codes of the slot-and-head's first token        */
@@ -93,8 +122,6 @@ struct Attention {
     static constexpr int kBufs = kRowBytes <= 64 ? 2 : 1;
     static constexpr float kCentre = BITS == 4 ? 8.0f : 128.0f;
     static constexpr int kRows = 16 * RT;
-    /* column tiles that the waves exchange at a time when they join */
-    static constexpr int kMergeTiles = kDim / 16 < 4 ? kDim / 16 : 4;
     using half8_t = std::conditional_t<F16, f16x8_t, bf16x8_t>;
 
     /* A wave's tile of scales and biases, by token.  K's biases stay as they are stored: they
@@ -519,42 +546,58 @@ struct Attention {
             struct {
                 __attribute__((aligned(16))) char pool[kRows * kDim * 2];   /* queries */
                 char k[kWaves][kBufs][kTileBytes], v[kWaves][kBufs][kTileBytes];
+                Scales scales[kWaves];
+                __attribute__((aligned(16))) uint16_t qsums[kRows * 4 * 8];
+                uint32_t masks[kRows];
+                float units[kRows];
             };
-            f32x4_t merge[kWaves][RT][kMergeTiles][64];
+            struct {
+                f32x4_t merge[kWaves][kDim / 16][RT][64];
+                /* by row: offset, sum; what the centre and (fp16) the biases add to a group's
+                 * channels; with bf16 the biases' two parts */
+                float offs[kWaves][kRows], sums[kWaves][kRows];
+                float fix[kWaves][kGroups][kRows];
+                float bias[F16 ? 0 : kWaves][2 * kGroups][kRows];
+            };
         };
-        Scales scales[kWaves];
-        __attribute__((aligned(16))) uint16_t qsums[kRows * 4 * 8];
-        uint32_t masks[kRows];
-        float units[kRows];
-        float offs[kWaves][kRows], sums[kWaves][kRows];
-        float fix[kWaves][kRows][kGroups];
-        float bias[F16 ? 1 : kWaves][F16 ? 1 : kRows][2 * kGroups];
     };
 
     /* The block's queries into LDS, in the order of the K operands and scaled by a power of two
      * so that a row's largest element lies in [2^14, 2^15): fp16 then holds them as exactly as
      * bf16 or fp16 did, down to 2^-29 of the largest.  unit: what takes a sum over codes times
      * 2^-24 to scores in log2; qsum: the sums of a row's groups in those units. */
-    static __device__ __forceinline__ void stage_queries(const KvAttnParams& p, const Job& job,
-                                                         int h, Lds& lds) {
-        constexpr int kLanes = kDim / 8, kPass = DFQ_KV_THREADS / kLanes;
-        constexpr int kPasses = (kRows + kPass - 1) / kPass;
-        const int piece = threadIdx.x % kLanes, q_heads = p.heads * p.group;
+    static constexpr int kLanes = kDim / 8, kPass = DFQ_KV_THREADS / kLanes;
+    static constexpr int kPasses = (kRows + kPass - 1) / kPass;
+    struct Queries {
         u32x4_t raw[kPasses];
         uint32_t mask[kPasses];
+    };
+    static __device__ __forceinline__ void load_queries(const KvAttnParams& p, const Job& job,
+                                                        int h, Queries& in) {
+        const int piece = threadIdx.x % kLanes, group = (int)p.group.by;
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) {
             const int r = threadIdx.x / kLanes + i * kPass;
-            raw[i] = u32x4_t{0, 0, 0, 0};
-            mask[i] = 0;
+            in.raw[i] = u32x4_t{0, 0, 0, 0};
+            in.mask[i] = 0;
             if (r < job.nrows) {
-                const int row = job.row0 + r, bm = row / p.group;
-                raw[i] = *(const u32x4_any*)(p.q + bm * p.q_stride +
-                                             (int64_t)(h * p.group + row - bm * p.group) * kDim +
-                                             piece * 8);
-                mask[i] = p.tree ? p.tree[bm] : (2u << (bm % p.rows)) - 1;
+                const int row = job.row0 + r, bm = divided(row, p.group);
+                in.raw[i] = *(const u32x4_any*)(p.q + bm * p.q_stride +
+                                                (int64_t)(h * group + row - bm * group) * kDim +
+                                                piece * 8);
+                in.mask[i] = p.tree ? p.tree[bm]
+                                    : (2u << (bm - divided(bm, p.rows) * (int)p.rows.by)) - 1;
             }
         }
+        /* all there, before loads that the compiler does not see are under way: it would wait
+         * for those too */
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i)
+            __asm__ volatile("" :: "v"(in.raw[i]), "v"(in.mask[i]) : "memory");
+    }
+    static __device__ __forceinline__ void stage_queries(const KvAttnParams& p, const Queries& in,
+                                                         Lds& lds) {
+        const int piece = threadIdx.x % kLanes;
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) {
             const int r = threadIdx.x / kLanes + i * kPass;
@@ -562,10 +605,10 @@ struct Attention {
             float f[8], top = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                f[j] = elem_to_f32<F16>(j & 1 ? raw[i][j / 2] >> 16 : raw[i][j / 2] & 0xffffu);
+                f[j] = elem_to_f32<F16>(j & 1 ? in.raw[i][j / 2] >> 16 : in.raw[i][j / 2] & 0xffffu);
                 top = fmaxf(top, fabsf(f[j]));
             }
-            for (int d = 1; d < kLanes; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+            top = largest_of<kLanes>(top);
             int e = (int)(__float_as_uint(top) >> 23) - 127;
             if (e < -100 || e > 127) e = e > 127 ? 127 : -100; /* a tiny or an infinite row */
             float total = 0.0f;
@@ -574,7 +617,7 @@ struct Attention {
                 f[j] = ldexpf(f[j], 14 - e);
                 total += f[j];
             }
-            for (int d = 1; d < GS / 8; d *= 2) total += __shfl_xor(total, d);
+            total = sum_of<GS / 8>(total);
             const int g = piece / (GS / 8), u = piece % (GS / 8), c = u / kSteps, st = u % kSteps;
             if (u < 4) {
                 /* 2^-8 of the group's sum in three parts of 16 bits, part i for quarter i of the
@@ -593,7 +636,7 @@ struct Attention {
             }
             if (piece == 0) {
                 lds.units[r] = ldexpf(p.scale_log2e, 8 + e - 14);
-                lds.masks[r] = mask[i];
+                lds.masks[r] = in.mask[i];
             }
             /* nibble order of k_operand: operand element j is channel j/2 + 4 (j%2) */
             u32x4_t o;
@@ -612,7 +655,17 @@ struct Attention {
                                                char* room) {
         Lds& lds = *(Lds*)room;
         const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-        stage_queries(p, job, h, lds);
+        Queries queries;
+        load_queries(p, job, h, queries);
+        int t = job.t0 + 32 * wave;
+        TokenScales scale;
+        char (&k)[kBufs][kTileBytes] = lds.k[wave], (&v)[kBufs][kTileBytes] = lds.v[wave];
+        if (t < job.t1) {
+            load_codes(job.k, job.n, t, lane, k[0]);
+            if (kBufs == 2) load_codes(job.v, job.n, t, lane, v[0]);
+            load_scales(job, t, lane, scale);
+        }
+        stage_queries(p, queries, lds);
         __syncthreads();
 
         Rows st;
@@ -633,18 +686,10 @@ struct Attention {
             for (int d = 0; d < kDim / 16; ++d) st.o[rt][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
         }
 
-        int t = job.t0 + 32 * wave;
-        TokenScales scale;
         float z[RT][8];
         const f16x8_t* q = (const f16x8_t*)lds.pool;
         Scales& sc = lds.scales[wave];
-        char (&k)[kBufs][kTileBytes] = lds.k[wave], (&v)[kBufs][kTileBytes] = lds.v[wave];
         int buf = 0;
-        if (t < job.t1) {
-            load_scales(job, t, lane, scale);
-            load_codes(job.k, job.n, t, lane, k[0]);
-            if (kBufs == 2) load_codes(job.v, job.n, t, lane, v[0]);
-        }
         while (t < job.t1) {
             const int next = t + 32 * kWaves, other = kBufs == 2 ? buf ^ 1 : 0;
             loaded<0>();
@@ -677,15 +722,18 @@ struct Attention {
             t = next;
         }
 
-        /* The waves' rows together: offsets, sums and what the codes' centre and the biases add,
-         * then four column tiles at a time, of which each wave adds up one of every row tile. */
+        /* The waves' rows together: their outputs, offsets, sums and what the codes' centre and
+         * the biases add meet in LDS.  A wave then adds up every fourth column tile, each of its
+         * lanes with the weights of its four rows. */
         __syncthreads();
+#pragma unroll
+        for (int d = 0; d < kDim / 16; ++d)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) lds.merge[wave][d][rt][lane] = st.o[rt][d];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const int r = rt * 16 + (lane & 15), row = rt * 16 + 4 * (lane >> 4);
-            float sum = st.sum[rt];
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
+            const float sum = quarters_sum(st.sum[rt]);
             if (lane < 16) {
                 lds.offs[wave][r] = st.off[rt];
                 lds.sums[wave][r] = sum;
@@ -694,67 +742,62 @@ struct Attention {
             for (int g = 0; g < kGroups; ++g) {
                 float f = -kCentre * st.code_sum[rt][g];
                 if constexpr (F16) f += st.bias_sum[rt][g];
-                f += __shfl_xor(f, 16);
-                f += __shfl_xor(f, 32);
-                if (lane < 16) lds.fix[wave][r][g] = f;
+                f = quarters_sum(f);
+                if (lane < 16) lds.fix[wave][g][r] = f;
             }
             if constexpr (!F16)
                 if ((lane & 15) < 2 * kGroups)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) lds.bias[wave][row + i][lane & 15] = st.bias[rt][i];
+                    *(f32x4_t*)&lds.bias[wave][lane & 15][row] = st.bias[rt];
         }
         __syncthreads();
-        const int64_t nrows = (int64_t)p.batch * p.rows * p.group;
-        const int64_t out = (job.slot * p.heads + h) * nrows + job.row0;
-        if ((int)threadIdx.x < kRows) {
-            const int r = threadIdx.x;
-            float off[kWaves], top = kNever, sum = 0.0f;
+        const int64_t nrows = (int64_t)p.batch * p.rows.by * p.group.by;
+        const int64_t out = (job.slot * p.heads.by + h) * nrows + job.row0;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                off[w] = lds.offs[w][r];
-                top = fmaxf(top, off[w]);
+        for (int rt = 0; rt < RT; ++rt) {
+            const int row = rt * 16 + 4 * (lane >> 4);
+            f32x4_t weight[kWaves], top, sum = {};
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) weight[w] = *(const f32x4_t*)&lds.offs[w][row];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                top[i] = weight[0][i];
+#pragma unroll
+                for (int w = 1; w < kWaves; ++w) top[i] = fmaxf(top[i], weight[w][i]);
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w)
+                    weight[w][i] = __builtin_amdgcn_exp2f(weight[w][i] - top[i]);
             }
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) {
-                const float f = off[w] == top ? 1.0f : exp2f(off[w] - top);
-                sum = fmaf(lds.sums[w][r], f, sum);
-                lds.offs[w][r] = f;   /* from here on the wave's weight */
-                for (int g = 0; g < kGroups; ++g) {
-                    float x = lds.fix[w][r][g];
-                    if constexpr (!F16) x += lds.bias[w][r][2 * g] + lds.bias[w][r][2 * g + 1];
-                    lds.fix[w][r][g] = x * f;
-                }
+                const f32x4_t l = *(const f32x4_t*)&lds.sums[w][row];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] = fmaf(l[i], weight[w][i], sum[i]);
             }
-            if (r < job.nrows) *(f32x2_t*)(p.part_ml + (out + r) * 2) = f32x2_t{top, sum};
-        }
+            if (wave == 0 && (lane & 15) == 0)
 #pragma unroll
-        for (int d0 = 0; d0 < kDim / 16; d0 += kMergeTiles) {
-            __syncthreads();
+                for (int i = 0; i < 4; ++i)
+                    if (row + i < job.nrows)
+                        *(f32x2_t*)(p.part_ml + (out + row + i) * 2) = f32x2_t{top[i], sum[i]};
+#pragma unroll 1
+            for (int d = wave; d < kDim / 16; d += kWaves) {
+                const int g = d / kTiles;
+                const float back = odd_tile(d % kTiles) ? kUnit / 16.0f : kUnit;
+                f32x4_t y = {};
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
+                for (int w = 0; w < kWaves; ++w) {
+                    const f32x4_t x = lds.merge[w][d][rt][lane];
+                    f32x4_t fix = *(const f32x4_t*)&lds.fix[w][g][row];
+                    if constexpr (!F16)
+                        fix += *(const f32x4_t*)&lds.bias[w][2 * g][row] +
+                               *(const f32x4_t*)&lds.bias[w][2 * g + 1][row];
 #pragma unroll
-                for (int d = 0; d < kMergeTiles; ++d)
-                    lds.merge[wave][rt][d][lane] = st.o[rt][d0 + d];
-            __syncthreads();
-            for (int d = wave; d < kMergeTiles; d += kWaves) {
-                const int g = (d0 + d) / kTiles;
-                const float back = odd_tile((d0 + d) % kTiles) ? kUnit / 16.0f : kUnit;
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    f32x4_t x[kWaves];
-#pragma unroll
-                    for (int w = 0; w < kWaves; ++w) x[w] = lds.merge[w][rt][d][lane];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = rt * 16 + 4 * (lane >> 4) + i;
-                        float sum = 0.0f;
-#pragma unroll
-                        for (int w = 0; w < kWaves; ++w)
-                            sum = fmaf(x[w][i] * back, lds.offs[w][r], sum + lds.fix[w][r][g]);
-                        if (r < job.nrows)
-                            p.part_o[(out + r) * kDim + (d0 + d) * 16 + (lane & 15)] = sum;
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        y[i] = fmaf(fmaf(x[i], back, fix[i]), weight[w][i], y[i]);
                 }
+                float* to = p.part_o + (out + row) * kDim + d * 16 + (lane & 15);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (row + i < job.nrows) to[i * kDim] = y[i];
             }
         }
     }
@@ -771,41 +814,43 @@ __device__ __forceinline__ void attention(const KvAttnParams& p) {
 
     /* the job: heads go fastest, so that with 8 of them an XCD's L2 serves one */
     Job job;
-    int i = blockIdx.x;
-    const int h = i % p.heads;
-    i /= p.heads;
-    const int seq_rows = p.rows * p.group;
-    int range, ranges;
+    int i = divided(blockIdx.x, p.heads);
+    const int h = (int)(blockIdx.x - i * p.heads.by);
+    const int seq_rows = (int)(p.rows.by * p.group.by);
+    int range, block;
+    Divisor ranges;
     int64_t token0;   /* index of the slot-and-head's first token in the arrays */
     KvArrays jk, jv;
-    const int prefix_jobs = p.prefix_splits * p.prefix_blocks;
+    const int prefix_jobs = (int)(p.prefix_splits.by * p.prefix_blocks.by);
     if (i < prefix_jobs) {
-        range = i / p.prefix_blocks;
+        range = divided(i, p.prefix_blocks);
+        block = i - range * (int)p.prefix_blocks.by;
         ranges = p.prefix_splits;
         jk = p.prefix[0];
         jv = p.prefix[1];
         token0 = (int64_t)h * p.prefix_capacity;
         job.slot = range;
-        job.row0 = (i % p.prefix_blocks) * kRows;
+        job.row0 = block * kRows;
         job.nrows = p.batch * seq_rows - job.row0;
         job.n = job.clear = job.first = p.prefix_length;
     } else {
         i -= prefix_jobs;
-        const int b = i / (p.own_splits * p.own_blocks);
-        i %= p.own_splits * p.own_blocks;
-        range = i / p.own_blocks;
+        const int b = divided(i, p.own_jobs);
+        i -= b * (int)p.own_jobs.by;
+        range = divided(i, p.own_blocks);
+        block = i - range * (int)p.own_blocks.by;
         ranges = p.own_splits;
         jk = p.own[0];
         jv = p.own[1];
-        token0 = ((int64_t)b * p.heads + h) * p.own_capacity;
-        job.slot = p.prefix_splits + range;
-        const int r0 = (i % p.own_blocks) * kRows;
+        token0 = ((int64_t)b * p.heads.by + h) * p.own_capacity;
+        job.slot = (int)p.prefix_splits.by + range;
+        const int r0 = block * kRows;
         job.row0 = b * seq_rows + r0;
         job.nrows = seq_rows - r0;
         int n = p.lengths ? p.lengths[b] : p.max_length;
         n = n < 0 ? 0 : n > p.max_length ? p.max_length : n;
         job.n = n;
-        job.first = n - p.rows;
+        job.first = n - (int)p.rows.by;
         job.clear = job.first < 0 ? 0 : job.first;
     }
     if (job.nrows > kRows) job.nrows = kRows;
@@ -815,7 +860,7 @@ __device__ __forceinline__ void attention(const KvAttnParams& p) {
     job.bias = (lane < 32 ? jk.biases : jv.biases) + token0 * kGroups;
     /* ranges of whole rounds of 32 tokens a wave */
     const int rounds = (job.n + 32 * kWaves - 1) / (32 * kWaves);
-    const int each = (rounds + ranges - 1) / ranges * 32 * kWaves;
+    const int each = divided(rounds + (int)ranges.by - 1, ranges) * 32 * kWaves;
     job.t0 = range * each < job.n ? range * each : job.n;
     job.t1 = job.t0 + each < job.n ? job.t0 + each : job.n;
 
@@ -836,9 +881,9 @@ __device__ __forceinline__ void join(const KvAttnParams& p) {
     __shared__ float acc[kWaves][kDim];
     __shared__ float weight[kWaves][64];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const int64_t nrows = (int64_t)p.batch * p.rows * p.group;
-    const int h = blockIdx.y, slots = p.prefix_splits + p.own_splits;
-    const int64_t row = blockIdx.x, stride = nrows * p.heads, at = h * nrows + row;
+    const int64_t nrows = (int64_t)p.batch * p.rows.by * p.group.by;
+    const int h = blockIdx.y, slots = (int)(p.prefix_splits.by + p.own_splits.by);
+    const int64_t row = blockIdx.x, stride = nrows * p.heads.by, at = h * nrows + row;
     const f32x2_t* ml = (const f32x2_t*)p.part_ml + at;
     float top = kNever;
     for (int s = lane; s < slots; s += 64) top = fmaxf(top, ml[s * stride][0]);
@@ -870,8 +915,9 @@ __device__ __forceinline__ void join(const KvAttnParams& p) {
     for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
     *(part_t*)&acc[wave][lane * kEach] = o;
     __syncthreads();
-    const int64_t bm = row / p.group, q_heads = p.heads * p.group;
-    const int64_t head = h * p.group + row % p.group;
+    const int bm = divided((int)row, p.group), group = (int)p.group.by;
+    const int64_t q_heads = (int64_t)p.heads.by * group;
+    const int64_t head = h * group + (int)row - bm * group;
     for (int d = threadIdx.x; d < kDim; d += DFQ_KV_THREADS) {
         /* channel d of group g is column (d % GS) / (GS / 16) of the group's tile d % (GS / 16) */
         constexpr int kTiles = GS / 16;

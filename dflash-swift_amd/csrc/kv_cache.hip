@@ -25,21 +25,6 @@ __device__ __forceinline__ int position(const int32_t* starts, int start, int b,
     return pos >= 0 && pos < capacity ? (int)pos : -1;
 }
 
-/* The combination of the L lanes (4, 8 or 16) of a group, in each of them, by exchanges within a
- * row of 16 lanes: neighbours, pairs, then mirrored quads and halves. */
-template <int CTRL, typename Op>
-__device__ __forceinline__ uint32_t exchange(uint32_t v, Op op) {
-    return op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true));
-}
-template <int L, typename Op>
-__device__ __forceinline__ uint32_t group_of(uint32_t v, Op op) {
-    v = exchange<0xB1>(v, op);
-    v = exchange<0x4E>(v, op);
-    if constexpr (L >= 8) v = exchange<0x141>(v, op);
-    if constexpr (L >= 16) v = exchange<0x140>(v, op);
-    return v;
-}
-
 /* The code of x - bias = d, in the low bits of a float: d / s to nearest even, clamped to 0..TOP,
  * plus 1.5 2^23.  The product with a reciprocal of s is within 3 2^-24 of the quotient, relative, so
  * it rounds to the same whole number unless it lies that near to the middle of two; there the

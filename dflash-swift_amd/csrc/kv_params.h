@@ -16,6 +16,13 @@ struct KvArrays {
     uint16_t* biases;
 };
 
+/* Division of 0 .. 2^31 - 1 by a number that the host knows: with l the number's bits rounded up
+ * and mul = floor(2^32 (2^l - by) / by) + 1, n / by = (n + floor(n mul / 2^32)) >> l. */
+struct Divisor {
+    uint32_t by, mul;
+    int shift;
+};
+
 struct KvAppendParams {
     KvArrays out[2];         /* K, V                                             */
     const uint16_t* in[2];   /* rows [batch * rows], row_stride elements apart   */
@@ -46,9 +53,11 @@ struct KvAttnParams {
     float* part_o;
     int64_t q_stride;
     int prefix_length, prefix_capacity, own_capacity, max_length;
-    int batch, rows, heads, group;      /* group: query heads of a K/V head         */
-    int prefix_splits, prefix_blocks;   /* ranges of the prefix; blocks of its rows */
-    int own_splits, own_blocks;         /* the same for one sequence                */
+    int batch;
+    Divisor rows, heads, group;             /* group: query heads of a K/V head         */
+    Divisor prefix_splits, prefix_blocks;   /* ranges of the prefix; blocks of its rows */
+    Divisor own_splits, own_blocks;         /* the same for one sequence                */
+    Divisor own_jobs;                       /* the product of those two                 */
     float scale_log2e;       /* softmax scale * log2(e)                          */
 };
 

@@ -115,6 +115,21 @@ __device__ __forceinline__ float dpp_f32(float v) {
         __builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
 }
 
+/* The combination of the L lanes (4, 8 or 16) of a group, in each of them, by exchanges within a
+ * row of 16 lanes: neighbours, pairs, then mirrored quads and halves. */
+template <int CTRL, typename Op>
+__device__ __forceinline__ uint32_t exchange(uint32_t v, Op op) {
+    return op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true));
+}
+template <int L, typename Op>
+__device__ __forceinline__ uint32_t group_of(uint32_t v, Op op) {
+    v = exchange<0xB1>(v, op);
+    v = exchange<0x4E>(v, op);
+    if constexpr (L >= 8) v = exchange<0x141>(v, op);
+    if constexpr (L >= 16) v = exchange<0x140>(v, op);
+    return v;
+}
+
 /* (x0..x7) -> (x0,x4, x1,x5, x2,x6, x3,x7): the k order of a nibble operand. */
 __device__ __forceinline__ u32x4_t nibble_permute(u32x4_t v) {
     u32x4_t o;

@@ -264,6 +264,14 @@ struct AttentionPlan {
     }
 };
 
+/* by 0: of a part of the call that is not there, and nothing is divided */
+Divisor divisor(int by) {
+    const uint64_t d = by > 0 ? by : 1;
+    int shift = 0;
+    while ((1ull << shift) < d) ++shift;
+    return {(uint32_t)by, (uint32_t)((((1ull << shift) - d) << 32) / d + 1), shift};
+}
+
 /* Tokens that a workgroup takes in one round, 32 a wave. */
 constexpr int kRoundTokens = DFQ_KV_THREADS / 2;
 /* The plan's model of time, in rounds of a workgroup that has a CU to itself: what a workgroup
@@ -476,13 +484,14 @@ dfq_status dfq_cache_attention(dfq_ctx* ctx, const dfq_kv_cache* prefix, int pre
     p.own_capacity = cache ? cache->capacity : 0;
     p.max_length = max_length;
     p.batch = batch;
-    p.rows = rows;
-    p.heads = fmt->heads;
-    p.group = group;
-    p.prefix_splits = a.prefix_splits;
-    p.prefix_blocks = a.prefix_blocks;
-    p.own_splits = a.own_splits;
-    p.own_blocks = a.own_blocks;
+    p.rows = divisor(rows);
+    p.heads = divisor(fmt->heads);
+    p.group = divisor(group);
+    p.prefix_splits = divisor(a.prefix_splits);
+    p.prefix_blocks = divisor(a.prefix_blocks);
+    p.own_splits = divisor(a.own_splits);
+    p.own_blocks = divisor(a.own_blocks);
+    p.own_jobs = divisor(a.own_splits * a.own_blocks);
     p.scale_log2e = scale * 1.44269504088896340736f;
     const CacheKernels& fn = kernels_of(ctx, fmt);
     DeviceScope scope(ctx);
