@@ -86,13 +86,22 @@ __device__ __forceinline__ float sum_of(float v) {
     }));
 }
 
-/* The sum of a lane's value and of those 16, 32 and 48 lanes on, by exchanging halves of rows. */
+/* The sum and the largest of a lane's value and of those 16, 32 and 48 lanes on, by exchanging
+ * rows of 16 lanes, then halves. */
 __device__ __forceinline__ float quarters_sum(float v) {
     uint32_t u = __float_as_uint(v);
     auto x = __builtin_amdgcn_permlane16_swap(u, u, false, false);
     u = __float_as_uint(__uint_as_float(x[0]) + __uint_as_float(x[1]));
     x = __builtin_amdgcn_permlane32_swap(u, u, false, false);
     return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+}
+
+__device__ __forceinline__ float quarters_largest(float v) {
+    uint32_t u = __float_as_uint(v);
+    auto x = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    u = __float_as_uint(fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])));
+    x = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
 }
 
 /* Everything of one (head, row block, token range) of a launch. */
@@ -871,63 +880,67 @@ __device__ __forceinline__ void attention(const KvAttnParams& p) {
 }
 
 /* The parts of a row from all ranges, in the order of their slots: y = sum 2^(M - top) o / sum
- * 2^(M - top) l.  One workgroup a row: a wave takes every fourth slot, a lane kDim / 64 channels;
- * the slots' offsets and sums come in one load a lane (64 slots at a time), and eight slots' parts
- * are under way together, since the row waits for memory and for nothing else. */
-template <int GS, bool F16>
+ * 2^(M - top) l.  WAVES waves take a row's slots in turn, a lane kDim / 64 channels; the slots'
+ * offsets and sums come in one load a lane (64 slots at a time), and eight slots' parts are under
+ * way together, since the row waits for memory and for nothing else.  With few slots a wave has a
+ * row to itself, and a workgroup four rows. */
+template <int GS, bool F16, int WAVES>
 __device__ __forceinline__ void join(const KvAttnParams& p) {
     constexpr int kEach = kDim / 64, kAhead = 8;
     typedef float part_t __attribute__((ext_vector_type(kEach)));
     __shared__ float acc[kWaves][kDim];
     __shared__ float weight[kWaves][64];
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, first = wave % WAVES;
     const int64_t nrows = (int64_t)p.batch * p.rows.by * p.group.by;
     const int h = blockIdx.y, slots = (int)(p.prefix_splits.by + p.own_splits.by);
-    const int64_t row = blockIdx.x, stride = nrows * p.heads.by, at = h * nrows + row;
+    const int64_t row = (int64_t)blockIdx.x * (kWaves / WAVES) + wave / WAVES;
+    if (WAVES == 1 && row >= nrows) return;
+    const int64_t stride = nrows * p.heads.by, at = h * nrows + row;
     const f32x2_t* ml = (const f32x2_t*)p.part_ml + at;
     float top = kNever;
     for (int s = lane; s < slots; s += 64) top = fmaxf(top, ml[s * stride][0]);
-    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    top = quarters_largest(largest_of<16>(top));
     float sum = 0.0f;
     part_t o = {};
     for (int s0 = 0; s0 < slots; s0 += 64) {
         const f32x2_t v = s0 + lane < slots ? ml[(s0 + lane) * stride] : f32x2_t{kNever, 0.0f};
-        const float f = v[0] == top ? 1.0f : exp2f(v[0] - top);
+        const float f = __builtin_amdgcn_exp2f(v[0] - top);
         sum = fmaf(v[1], f, sum);
         weight[wave][lane] = f;
         wave_order();
         const int n = slots - s0 < 64 ? slots - s0 : 64;
-        for (int s = wave; s < n; s += kAhead * kWaves) {
+        for (int s = first; s < n; s += kAhead * WAVES) {
             part_t x[kAhead];
             float w[kAhead];
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
-                const int k = s + i * kWaves < n ? s + i * kWaves : s;
+                const int k = s + i * WAVES < n ? s + i * WAVES : s;
                 x[i] = *(const part_t*)(p.part_o + ((s0 + k) * stride + at) * kDim + lane * kEach);
-                w[i] = s + i * kWaves < n ? weight[wave][k] : 0.0f;
+                w[i] = weight[wave][k];
             }
 #pragma unroll
             for (int i = 0; i < kAhead; ++i)
-                if (s + i * kWaves < n) o += x[i] * w[i];
+                if (s + i * WAVES < n) o += x[i] * w[i];
         }
         wave_order();
     }
-    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+    sum = quarters_sum(sum_of<16>(sum));
     *(part_t*)&acc[wave][lane * kEach] = o;
-    __syncthreads();
+    if (WAVES > 1) __syncthreads();
+    else wave_order();
     const int bm = divided((int)row, p.group), group = (int)p.group.by;
     const int64_t q_heads = (int64_t)p.heads.by * group;
     const int64_t head = h * group + (int)row - bm * group;
-    for (int d = threadIdx.x; d < kDim; d += DFQ_KV_THREADS) {
+    for (int d = WAVES > 1 ? threadIdx.x : lane; d < kDim; d += 64 * WAVES) {
         /* channel d of group g is column (d % GS) / (GS / 16) of the group's tile d % (GS / 16) */
         constexpr int kTiles = GS / 16;
         const int e = (d / GS * kTiles + d % kTiles) * 16 + d % GS / kTiles;
-        float v = 0.0f;
+        float v = acc[WAVES > 1 ? 0 : wave][e];
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) v += acc[w][e];
+        for (int w = 1; w < WAVES; ++w) v += acc[w][e];
         p.y[(bm * q_heads + head) * kDim + d] = f32_to_out<F16>(sum == 0.0f ? 0.0f : v / sum);
     }
-    if (p.lse && threadIdx.x == 0)
+    if (p.lse && first == 0 && lane == 0)
         p.lse[bm * q_heads + head] =
             sum == 0.0f ? -__builtin_inff() : (top + log2f(sum)) * 0.693147180559945309f;
 }
@@ -944,7 +957,8 @@ __device__ __forceinline__ void join(const KvAttnParams& p) {
 #define DFQ_JOIN(gs, name, f16)                                                                \
     extern "C" __global__ __launch_bounds__(DFQ_KV_THREADS) void                               \
         dfq_cache_attention_join_g##gs##_##name(KvAttnParams p) {                              \
-        join<gs, f16>(p);                                                                      \
+        if (p.join_rows == 1) join<gs, f16, kWaves>(p);                                        \
+        else join<gs, f16, 1>(p);                                                              \
     }
 #define DFQ_FORMATS(M, gs, rt, per_4, per_8)                          \
     M(4, gs, bf16, false, rt, per_4) M(8, gs, bf16, false, rt, per_8) \

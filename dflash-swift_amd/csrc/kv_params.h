@@ -58,6 +58,7 @@ struct KvAttnParams {
     Divisor prefix_splits, prefix_blocks;   /* ranges of the prefix; blocks of its rows */
     Divisor own_splits, own_blocks;         /* the same for one sequence                */
     Divisor own_jobs;                       /* the product of those two                 */
+    int join_rows;           /* rows that a workgroup joins: 1 or (a wave a row) 4 */
     float scale_log2e;       /* softmax scale * log2(e)                          */
 };
 

@@ -492,6 +492,9 @@ dfq_status dfq_cache_attention(dfq_ctx* ctx, const dfq_kv_cache* prefix, int pre
     p.own_splits = divisor(a.own_splits);
     p.own_blocks = divisor(a.own_blocks);
     p.own_jobs = divisor(a.own_splits * a.own_blocks);
+    /* a wave joins up to eight slots with all loads under way; 5120 rows of 4 slots took 11 us with
+     * a workgroup each */
+    p.join_rows = a.prefix_splits + a.own_splits <= 8 ? DFQ_KV_THREADS / 64 : 1;
     p.scale_log2e = scale * 1.44269504088896340736f;
     const CacheKernels& fn = kernels_of(ctx, fmt);
     DeviceScope scope(ctx);
@@ -501,7 +504,8 @@ dfq_status dfq_cache_attention(dfq_ctx* ctx, const dfq_kv_cache* prefix, int pre
         e = hipModuleLaunchKernel(fn.attention[a.tiles - 1], (unsigned)groups, 1, 1,
                                   DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
     if (e == hipSuccess)
-        e = hipModuleLaunchKernel(fn.join, (unsigned)(batch * rows * group),
+        e = hipModuleLaunchKernel(fn.join,
+                                  (unsigned)((batch * rows * group + p.join_rows - 1) / p.join_rows),
                                   (unsigned)fmt->heads, 1, DFQ_KV_THREADS, 1, 1, 0,
                                   (hipStream_t)stream, args, nullptr);
     return e == hipSuccess ? DFQ_OK : hip_error(e, "launch dfq_cache_attention");
