@@ -86,22 +86,21 @@ __device__ __forceinline__ float sum_of(float v) {
     }));
 }
 
-/* The sum and the largest of a lane's value and of those 16, 32 and 48 lanes on, by exchanging
- * rows of 16 lanes, then halves. */
-__device__ __forceinline__ float quarters_sum(float v) {
-    uint32_t u = __float_as_uint(v);
-    auto x = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    u = __float_as_uint(__uint_as_float(x[0]) + __uint_as_float(x[1]));
-    x = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+/* v combined with the lanes 16, 32 and 48 on, in each: rows of 16 lanes, then halves of the wave are
+ * exchanged between two copies.  The swaps carry their own wait states on both sides. */
+template <typename Op>
+__device__ __forceinline__ float quarters(float v, Op op) {
+    float a = v, b = v;
+    __asm__ volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 4" : "+v"(a), "+v"(b));
+    a = b = op(a, b);
+    __asm__ volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 4" : "+v"(a), "+v"(b));
+    return op(a, b);
 }
-
+__device__ __forceinline__ float quarters_sum(float v) {
+    return quarters(v, [](float a, float b) { return a + b; });
+}
 __device__ __forceinline__ float quarters_largest(float v) {
-    uint32_t u = __float_as_uint(v);
-    auto x = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    u = __float_as_uint(fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])));
-    x = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+    return quarters(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
 /* Everything of one (head, row block, token range) of a launch. */
@@ -166,7 +165,8 @@ struct Attention {
         wave_order();
         if (lane < 32) {
 #pragma unroll
-            for (int g = 0; g < kGroups; ++g) sc.k[g][tok] = elem_to_f32<F16>(in.s[g]) * kScaleUnit;
+            for (int g = 0; g < kGroups; ++g)
+                sc.k[g][tok] = elem_to_f32<F16>(in.s[g]) * (BITS == 4 ? kScaleUnit / 16.0f : kScaleUnit);
             __builtin_memcpy(__builtin_assume_aligned(sc.kb + tok * kGroups, 2 * kGroups), in.b,
                              2 * kGroups);
         } else {
@@ -244,12 +244,16 @@ struct Attention {
         __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 
-    /* 8 codes of step st of a chunk.  4 bits: the word's nibbles in the order 0 4 1 5 2 6 3 7,
-     * the odd ones times 16; 8 bits: in order.  The queries are laid out to match. */
+    /* 8 codes of step st of a chunk.  4 bits: the word's nibbles in the order 0 4 1 5 2 6 3 7, all
+     * times 16; 8 bits: in order.  The queries are laid out to match.  The matrix cores line up the
+     * products of a sum by their operands' exponents, which for denormal codes say nothing of
+     * their size: with nibbles left in the low four bits, where they cost no shift, sums kept
+     * some 2^-20 of their size, and a log-sum of 18 tokens was 1.2e-6 off. */
     static __device__ __forceinline__ f16x8_t k_operand(const uint32_t (&w)[kWords], int st) {
         if constexpr (BITS == 4) {
-            const uint32_t a = w[st], b = a >> 8;
-            return as_f16x8(a & 0x000f000fu, a & 0x00f000f0u, b & 0x000f000fu, b & 0x00f000f0u);
+            constexpr uint32_t kMid = 0x00f000f0u;
+            const uint32_t a = w[st];
+            return as_f16x8(a << 4 & kMid, a & kMid, a >> 4 & kMid, a >> 8 & kMid);
         } else {
             const uint32_t a = w[2 * st], b = w[2 * st + 1];
             return as_f16x8(__builtin_amdgcn_perm(0u, a, 0x0c010c00u),
@@ -652,8 +656,7 @@ struct Attention {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int a = BITS == 4 ? j : 2 * j, b = BITS == 4 ? j + 4 : 2 * j + 1;
-                const float by = BITS == 4 && j % 2 ? 0.0625f : 1.0f;
-                const f32x2_t x = {f[a] * by, f[b] * by};
+                const f32x2_t x = {f[a], f[b]};
                 o[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2_t));
             }
             *(u32x4_t*)(lds.pool + (((r / 16) * (kDim / 32) + g * kSteps + st) * 64 + c * 16 + r % 16) * 16) = o;
