@@ -341,3 +341,21 @@ def test_refusals(ctx):
         c.run(ctx, tree=torch.zeros(2, 4, dtype=torch.int32, device="cuda"))
     with pytest.raises(ValueError):
         ctx.cache_attention(c.d_q)
+
+
+@pytest.mark.parametrize("dim,bits,gs,dt", FORMATS)
+def test_large_scores_keep_fp32(ctx, dim, bits, gs, dt):
+    """With one token a row's lse is its score z.  Its products have random signs, so that the
+    partial sums are some Z / sqrt(dim) (Z their sizes' sum) and each of the dim / 32 + 2 dim / gs
+    additions of a matrix step or a group rounds by 2^-25 of that at most: 2^-25 Z for the errors'
+    root mean square.  Eight roundings of z follow (to log2 and back, the offset off and on), and
+    one of a logarithm below 2^4 (2^-21).  Large queries leave that last one small beside sums of
+    fewer than 24 bits."""
+    c = Case(37, dim, bits, gs, dt, batch=16, rows=1, heads=4, group=4, capacity=1,
+             q_spread=64.0).device()
+    announce(f"large scores dim={dim} bits={bits} gs={gs} {dt}")
+    _, lse = c.run(ctx)
+    _, want, worst = c.expected()
+    off = (lse.double().cpu() - want).square().mean().sqrt()
+    size = c.scale * worst[..., 1].mean() + 8 * want.square().mean().sqrt()
+    assert off <= 2.0 ** -25 * size + 2.0 ** -21
