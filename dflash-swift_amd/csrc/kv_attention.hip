@@ -8,6 +8,23 @@
  *   y   = sum_t p_t [ s_tg c_t + b_tg ] / sum_t p_t,   p_t = 2^(z_t log2 e - M)
  * so that both products run on the codes themselves, and scales and biases meet the scores in
  * fp32: no value of the cache is rounded on the way.
+ *
+ * A workgroup takes a block of 16 or 32 rows of one head (a verify block's rows and the query heads
+ * of a K/V head together; over a shared prefix, those of all sequences) and a range of tokens, 32
+ * a wave at a time: the scores of a tile of 32 tokens leave the matrix cores in the layout in which
+ * the weights go back into them, so that a wave needs no other wave until its range is over.  The
+ * codes go from memory straight into LDS.  The ranges' parts meet in a second kernel (join).
+ *
+ * What bounds it.  Long caches and shared prefixes: issue of vector instructions.  A tile of 32
+ * rows and 32 tokens with heads of 128 is some 430 of them at 4.3 cycles and 38 matrix steps at 16
+ * on each SIMD; it takes 2650 cycles.  16 sequences of 8 rows of 40 heads over 16384 shared tokens
+ * (44 GFLOP) 99 us, 440 TFLOP/s; 8 rows over 32776 tokens of their own 27.8 us, 38 MB at 1.4 TB/s.
+ * Few tokens: two launches and code that each CU runs once (up to 128 tokens 8.5 us with heads of
+ * 64, 10 of 128, 13 of 256).
+ *
+ * Measured and not taken: unpacking codes once a workgroup into fp16 tiles in LDS for up to 64 rows
+ * (half the vector instructions, but a barrier a round and two waves a SIMD: 112 us where this took
+ * 111); three and four row tiles (registers spill).
  */
 #include <type_traits>
 
@@ -29,6 +46,9 @@ typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 constexpr float kUnit = 16777216.0f;
 /* Scores are kept 2^-8 of what the scaled queries give, so that a query's sums fit fp16. */
 constexpr float kScaleUnit = kUnit / 256.0f;
+/* K's scales carry it; 4-bit codes stand in the operands sixteenfold. */
+template <int BITS>
+constexpr float kKScaleOf = BITS == 4 ? kScaleUnit / 16.0f : kScaleUnit;
 constexpr float kMost = 3.38e38f;     /* finite numbers below it stay so in bf16 */
 
 template <bool F16>
@@ -126,7 +146,9 @@ struct Attention {
     static constexpr int kVBytes = GS * BITS / 128;      /* a lane's bytes of a group  */
     static constexpr int kTileBytes = 32 * kRowBytes;    /* codes of 32 tokens         */
     static constexpr int kLoads = kTileBytes / 1024;     /* wave loads of them         */
-    /* K and V tiles in LDS: two of each, or one where two would leave a CU one workgroup. */
+    /* K and V tiles in LDS: two of each, or one where two would leave a CU fewer workgroups.  One
+     * row a sequence of 16 over 8192 tokens 36.4 us with one, 35.5 with two; at rows of 128 bytes,
+     * 16 rows of 4 heads over 16000 tokens 37.7 with one, 47.9 with two. */
     static constexpr int kBufs = kRowBytes <= 64 ? 2 : 1;
     static constexpr float kCentre = BITS == 4 ? 8.0f : 128.0f;
     static constexpr int kRows = 16 * RT;
@@ -157,8 +179,10 @@ struct Attention {
         __builtin_memcpy(out.b, job.bias + (int64_t)tok * kGroups, 2 * kGroups);
     }
 
-    /* A V group whose scale or bias is not finite (or the middle of its range past bf16) counts as a NaN scale and no bias: the rows
-     * that see it get NaN, and the others, whose weight is 0, nothing. */
+    /* A V group whose scale or bias is not finite (or the middle of its range past bf16) counts as
+     * a NaN scale and no bias: the rows that see it get NaN, and the others, whose weight is 0,
+     * nothing.  With bf16 the middle meets the weights in two bf16 parts (16 bits of it, 2^-17 of
+     * the middle off at most, far under the outputs' own rounding). */
     static __device__ __forceinline__ void stage_scales(const TokenScales& in, int lane,
                                                         Scales& sc) {
         const int tok = lane & 31;
@@ -166,7 +190,7 @@ struct Attention {
         if (lane < 32) {
 #pragma unroll
             for (int g = 0; g < kGroups; ++g)
-                sc.k[g][tok] = elem_to_f32<F16>(in.s[g]) * (BITS == 4 ? kScaleUnit / 16.0f : kScaleUnit);
+                sc.k[g][tok] = elem_to_f32<F16>(in.s[g]) * kKScaleOf<BITS>;
             __builtin_memcpy(__builtin_assume_aligned(sc.kb + tok * kGroups, 2 * kGroups), in.b,
                              2 * kGroups);
         } else {
@@ -263,7 +287,8 @@ struct Attention {
         }
     }
 
-    /* Whether column tile i holds its codes times 16. */
+    /* Whether column tile i holds its codes times 16.  (V's may stay in the low nibble: 2^-20 of a
+     * sum is far under the outputs' own rounding.) */
     static constexpr __device__ bool odd_tile(int i) { return BITS == 4 && (i & 1); }
 
     /* What a lane reads for one chunk of steps: its quarter's 8-channel pieces of tokens l % 16
@@ -279,7 +304,8 @@ struct Attention {
         const int at = ((lane >> 4) * kPer + part) * kWords * 4;
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
-            const char* p = tile + ((row + 16 * tt) * kRowBytes + (at ^ turn(row) ^ (g * (GS * BITS / 8))));
+            const char* p = tile + ((row + 16 * tt) * kRowBytes +
+                                    (at ^ turn(row) ^ (g * (GS * BITS / 8))));
             __builtin_memcpy(out.w[tt], __builtin_assume_aligned(p, kWords * 4), kWords * 4);
         }
 #pragma unroll
@@ -659,7 +685,8 @@ struct Attention {
                 const f32x2_t x = {f[a], f[b]};
                 o[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2_t));
             }
-            *(u32x4_t*)(lds.pool + (((r / 16) * (kDim / 32) + g * kSteps + st) * 64 + c * 16 + r % 16) * 16) = o;
+            const int step = (r / 16) * (kDim / 32) + g * kSteps + st;
+            *(u32x4_t*)(lds.pool + (step * 64 + c * 16 + r % 16) * 16) = o;
         }
     }
 
@@ -886,7 +913,7 @@ __device__ __forceinline__ void attention(const KvAttnParams& p) {
  * 2^(M - top) l.  WAVES waves take a row's slots in turn, a lane kDim / 64 channels; the slots'
  * offsets and sums come in one load a lane (64 slots at a time), and eight slots' parts are under
  * way together, since the row waits for memory and for nothing else.  With few slots a wave has a
- * row to itself, and a workgroup four rows. */
+ * row to itself, and a workgroup four rows (40 rows of 17 slots 2.6 us, 5120 rows of 4 5.3). */
 template <int GS, bool F16, int WAVES>
 __device__ __forceinline__ void join(const KvAttnParams& p) {
     constexpr int kEach = kDim / 64, kAhead = 8;

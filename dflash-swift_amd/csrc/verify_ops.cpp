@@ -492,8 +492,9 @@ dfq_status dfq_cache_attention(dfq_ctx* ctx, const dfq_kv_cache* prefix, int pre
     p.own_splits = divisor(a.own_splits);
     p.own_blocks = divisor(a.own_blocks);
     p.own_jobs = divisor(a.own_splits * a.own_blocks);
-    /* a wave joins up to eight slots with all loads under way; 5120 rows of 4 slots took 11 us with
-     * a workgroup each */
+    /* a wave joins up to eight slots with all loads under way: 5120 rows of 4 slots 5.3 us, with a
+     * workgroup each 11; past eight the other way about (a call of 40 rows of 17 slots 11.1 us, with
+     * a wave each 12.5) */
     p.join_rows = a.prefix_splits + a.own_splits <= 8 ? DFQ_KV_THREADS / 64 : 1;
     p.scale_log2e = scale * 1.44269504088896340736f;
     const CacheKernels& fn = kernels_of(ctx, fmt);
@@ -505,7 +506,8 @@ dfq_status dfq_cache_attention(dfq_ctx* ctx, const dfq_kv_cache* prefix, int pre
                                   DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
     if (e == hipSuccess)
         e = hipModuleLaunchKernel(fn.join,
-                                  (unsigned)((batch * rows * group + p.join_rows - 1) / p.join_rows),
+                                  (unsigned)(((int64_t)batch * rows * group + p.join_rows - 1) /
+                                             p.join_rows),
                                   (unsigned)fmt->heads, 1, DFQ_KV_THREADS, 1, 1, 0,
                                   (hipStream_t)stream, args, nullptr);
     return e == hipSuccess ? DFQ_OK : hip_error(e, "launch dfq_cache_attention");

@@ -382,7 +382,8 @@ dfq_status dfq_cache_attention(dfq_ctx* ctx, const dfq_kv_cache* prefix, int pre
  * A logit of -inf has probability 0.  A row with a NaN or +inf, or with nothing above -inf, has
  * NaN for its probabilities and entropy.  What a sampler's client is told of the tokens that the
  * greedy accept takes (acceptedPrefix, DFlashSpeculativeGenerator.swift:555-571, keeps the tokens
- * alone).  The workspace (16-byte aligned) needs no clearing.  Asynchronous on `stream`. */
+ * alone).  The workspace (16-byte aligned; none where its size is 0) needs no clearing.
+ * Asynchronous on `stream`. */
 dfq_status dfq_token_logprobs_workspace_bytes(dfq_ctx* ctx, int M, int V, int top_k,
                                               size_t* bytes);
 dfq_status dfq_token_logprobs(dfq_ctx* ctx, const void* logits, int64_t row_stride, int M, int V,
