@@ -13,7 +13,8 @@
  * of a K/V head together; over a shared prefix, those of all sequences) and a range of tokens, 32
  * a wave at a time: the scores of a tile of 32 tokens leave the matrix cores in the layout in which
  * the weights go back into them, so that a wave needs no other wave until its range is over.  The
- * codes go from memory straight into LDS.  The ranges' parts meet in a second kernel (join).
+ * codes go from memory straight into LDS.  The ranges' parts meet in a second kernel (join), where
+ * there is more than one.
  *
  * What bounds it.  Long caches and shared prefixes: issue of vector instructions.  A tile of 32
  * rows and 32 tokens with heads of 128 is some 430 of them at 4.3 cycles and 38 matrix steps at 16
@@ -86,7 +87,12 @@ __device__ __forceinline__ void wave_order() {
     __builtin_amdgcn_wave_barrier();
 }
 
-/* n / by and n - n / by * by. */
+/* log of 2^top sum. */
+__device__ __forceinline__ float log_sum(float top, float sum) {
+    return sum == 0.0f ? -__builtin_inff() : (top + log2f(sum)) * 0.693147180559945309f;
+}
+
+/* n / by. */
 __device__ __forceinline__ int divided(int n, const Divisor& d) {
     return (int)((__umulhi((uint32_t)n, d.mul) + (uint32_t)n) >> d.shift);
 }
@@ -791,6 +797,8 @@ struct Attention {
         __syncthreads();
         const int64_t nrows = (int64_t)p.batch * p.rows.by * p.group.by;
         const int64_t out = (job.slot * p.heads.by + h) * nrows + job.row0;
+        /* one range is the whole answer */
+        const bool alone = p.prefix_splits.by + p.own_splits.by == 1;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const int row = rt * 16 + 4 * (lane >> 4);
@@ -812,11 +820,24 @@ struct Attention {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sum[i] = fmaf(l[i], weight[w][i], sum[i]);
             }
+            int64_t whole[4];   /* where the row's outputs go */
+            if (alone) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int at = job.row0 + row + i, bm = divided(at, p.group);
+                    whole[i] = (int64_t)bm * p.heads.by * p.group.by + h * p.group.by +
+                               (at - bm * (int)p.group.by);
+                }
+            }
             if (wave == 0 && (lane & 15) == 0)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (row + i < job.nrows)
+                for (int i = 0; i < 4; ++i) {
+                    if (row + i >= job.nrows) continue;
+                    if (!alone)
                         *(f32x2_t*)(p.part_ml + (out + row + i) * 2) = f32x2_t{top[i], sum[i]};
+                    else if (p.lse)
+                        p.lse[whole[i]] = log_sum(top[i], sum[i]);
+                }
 #pragma unroll 1
             for (int d = wave; d < kDim / 16; d += kWaves) {
                 const int g = d / kTiles;
@@ -832,6 +853,15 @@ struct Attention {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         y[i] = fmaf(fmaf(x[i], back, fix[i]), weight[w][i], y[i]);
+                }
+                if (alone) {
+                    const int channel = g * GS + (lane & 15) * kTiles + d % kTiles;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (row + i < job.nrows)
+                            p.y[whole[i] * kDim + channel] =
+                                f32_to_out<F16>(sum[i] == 0.0f ? 0.0f : y[i] / sum[i]);
+                    continue;
                 }
                 float* to = p.part_o + (out + row) * kDim + d * 16 + (lane & 15);
 #pragma unroll
@@ -971,8 +1001,7 @@ __device__ __forceinline__ void join(const KvAttnParams& p) {
         p.y[(bm * q_heads + head) * kDim + d] = f32_to_out<F16>(sum == 0.0f ? 0.0f : v / sum);
     }
     if (p.lse && first == 0 && lane == 0)
-        p.lse[bm * q_heads + head] =
-            sum == 0.0f ? -__builtin_inff() : (top + log2f(sum)) * 0.693147180559945309f;
+        p.lse[bm * q_heads + head] = log_sum(top, sum);
 }
 
 }  // namespace

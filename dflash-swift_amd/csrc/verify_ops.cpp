@@ -281,6 +281,12 @@ constexpr int kRoundTokens = DFQ_KV_THREADS / 2;
  * shapes (heads of 64, 128 and 256, 1..16 sequences, own caches and shared prefixes) the one
  * that these numbers choose is within 3 % of the fastest. */
 constexpr double kFixedRounds = 1.5, kTogether = 1.5, kTwoTiles = 1.6, kRangeRounds = 0.03;
+/* And the join itself, a launch that a single range does without; a round of heads of 256 is twice
+ * one of 128.  Device time of 8 rows of 4 sequences (a caller that launches one call after the other
+ * saves 2.5 us of its own besides), one range / 128 tokens a range:
+ *   heads of 128: 128 tokens 7.5 / 9.9 us, 512 10.7 / 9.9;  64: 6.4 / 8.4, 8.6 / 8.5;
+ *   heads of 256: 10.6 / 13.0, 16.1 / 13.0. */
+double join_rounds(int dim) { return dim > 128 ? 1.5 : 3.0; }
 
 /* The workgroups of `blocks` row blocks over `rounds` rounds in ranges of at most `each`, as even
  * as they come, by themselves: how long, and how much. */
@@ -334,11 +340,13 @@ AttentionPlan plan_attention(dfq_ctx* ctx, const dfq_kv_cache* fmt, int prefix_l
         const double round = tiles == 1 ? 1.0 : kTwoTiles;
         const double all = (double)pn * prefix_rounds + (double)on * own_rounds;
         const int64_t room = (int64_t)card.cus * card.resident;
-        /* ranges that fill every CU with 1, 2, .. workgroups, in one pass and in some */
-        for (int fill = 1; fill <= card.resident + 3 && longest; ++fill) {
+        /* one range, and ranges that fill every CU with 1, 2, .. workgroups, in one pass and in
+         * some */
+        for (int fill = 0; fill <= card.resident + 3 && longest; ++fill) {
             const int more = fill - card.resident;
             const int per = more <= 0 ? fill : card.resident * (1 + more);
-            const double even = std::floor(all / ((double)card.cus * per));
+            const double even =
+                fill ? std::floor(all / ((double)card.cus * per)) : (double)longest;
             for (int up = 0; up < 2; ++up) {
                 const int each = (int)std::min<double>(longest, std::max(1.0, even + up));
                 const Share p = card.share(pn, prefix_rounds, each);
@@ -354,6 +362,7 @@ AttentionPlan plan_attention(dfq_ctx* ctx, const dfq_kv_cache* fmt, int prefix_l
                                                    : work + 0.5 * o.longest);
                 }
                 t = t * round + kRangeRounds * (p.ranges + o.ranges);
+                if (p.ranges + o.ranges > 1) t += join_rounds(fmt->head_dim);
                 if (best == 0 || t < best) {
                     best = t;
                     a.tiles = tiles;
@@ -366,6 +375,7 @@ AttentionPlan plan_attention(dfq_ctx* ctx, const dfq_kv_cache* fmt, int prefix_l
         }
     }
     const size_t slots = (size_t)a.prefix_splits + a.own_splits;
+    if (slots == 1) return a;
     a.ml_bytes = (slots * a.rows * 8 + 255) & ~(size_t)255;
     a.bytes = a.ml_bytes + slots * a.rows * fmt->head_dim * 4;
     return a;
@@ -504,7 +514,7 @@ dfq_status dfq_cache_attention(dfq_ctx* ctx, const dfq_kv_cache* prefix, int pre
     if (groups)
         e = hipModuleLaunchKernel(fn.attention[a.tiles - 1], (unsigned)groups, 1, 1,
                                   DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
-    if (e == hipSuccess)
+    if (e == hipSuccess && a.prefix_splits + a.own_splits != 1)
         e = hipModuleLaunchKernel(fn.join,
                                   (unsigned)(((int64_t)batch * rows * group + p.join_rows - 1) /
                                              p.join_rows),

@@ -222,11 +222,15 @@ def _current_stream(device: int) -> int:
     return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
 
 
+_dtype_codes = {}
+
+
 def dtype_code(t) -> int:
     """dfq dtype code of a torch dtype (or tensor)."""
-    import torch
-    dt = t.dtype if hasattr(t, "dtype") else t
-    return {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}[dt]
+    if not _dtype_codes:
+        import torch
+        _dtype_codes.update({torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32})
+    return _dtype_codes[getattr(t, "dtype", t)]
 
 
 class Context:
