@@ -20,8 +20,8 @@
  * rows and 32 tokens with heads of 128 is some 430 of them at 4.3 cycles and 38 matrix steps at 16
  * on each SIMD; it takes 2650 cycles.  16 sequences of 8 rows of 40 heads over 16384 shared tokens
  * (44 GFLOP) 99 us, 440 TFLOP/s; 8 rows over 32776 tokens of their own 27.8 us, 38 MB at 1.4 TB/s.
- * Few tokens: two launches and code that each CU runs once (up to 128 tokens 8.5 us with heads of
- * 64, 10 of 128, 13 of 256).
+ * Few tokens: a launch and code that each CU runs once (up to 128 tokens 6.4 us with heads of 64,
+ * 7.5 of 128, 10.7 of 256; where a join follows, 8.4, 9.9 and 13).
  *
  * Measured and not taken: unpacking codes once a workgroup into fp16 tiles in LDS for up to 64 rows
  * (half the vector instructions, but a barrier a round and two waves a SIMD: 112 us where this took

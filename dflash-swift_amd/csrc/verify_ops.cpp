@@ -275,12 +275,12 @@ Divisor divisor(int by) {
 /* Tokens that a workgroup takes in one round, 32 a wave. */
 constexpr int kRoundTokens = DFQ_KV_THREADS / 2;
 /* The plan's model of time, in rounds of a workgroup that has a CU to itself: what a workgroup
- * costs besides its rounds (staging the queries, joining its waves); how many a CU works on
- * together before they slow each other down (they wait for memory, then for issue); what two
- * tiles cost against one; and what one more range costs the join.  Over the plans of eleven
- * shapes (heads of 64, 128 and 256, 1..16 sequences, own caches and shared prefixes) the one
- * that these numbers choose is within 3 % of the fastest. */
-constexpr double kFixedRounds = 1.5, kTogether = 1.5, kTwoTiles = 1.6, kRangeRounds = 0.03;
+ * costs besides its rounds (staging the queries, joining its waves); what each workgroup more on
+ * a CU adds to a round of all (they wait for memory, then for issue); what two tiles cost against
+ * one; and what one more range costs the join.  Over the plans of sixteen shapes (heads of 64, 128
+ * and 256, 1..32 sequences, own caches and shared prefixes) the one that these numbers choose is
+ * within 7 % of the fastest, mostly the fastest itself. */
+constexpr double kFixedRounds = 1.5, kAnother = 0.45, kTwoTiles = 1.7, kRangeRounds = 0.02;
 /* And the join itself, a launch that a single range does without; a round of heads of 256 is twice
  * one of 128.  Device time of 8 rows of 4 sequences (a caller that launches one call after the other
  * saves 2.5 us of its own besides), one range / 128 tokens a range:
@@ -300,7 +300,7 @@ struct Card {
     int cus, resident;
     double cost(int64_t groups) const {
         const int64_t per = std::min<int64_t>(resident, (groups + cus - 1) / cus);
-        return per < kTogether ? 1.0 : per / kTogether;
+        return 1.0 + kAnother * (per - 1);
     }
     Share share(int64_t blocks, int rounds, int each) const {
         Share s;
@@ -314,8 +314,12 @@ struct Card {
         s.groups = blocks * s.ranges;
         s.work = (double)blocks * (rounds + s.ranges * kFixedRounds);
         s.time = passes * s.longest * cost(room);
-        if (rest) s.time += s.longest * cost(rest);
-        if (last && (!rest || rest + blocks > room)) s.time += last + kFixedRounds;
+        if (rest && last && rest + blocks <= room)   /* the short ones beside the others */
+            s.time += (last + kFixedRounds) * cost(rest + blocks) + (each - last) * cost(rest);
+        else if (rest)
+            s.time += s.longest * cost(rest);
+        if (last && (!rest || rest + blocks > room))   /* behind the first that end */
+            s.time += 0.5 * (last + kFixedRounds);
         return s;
     }
 };
@@ -347,10 +351,11 @@ AttentionPlan plan_attention(dfq_ctx* ctx, const dfq_kv_cache* fmt, int prefix_l
             const int per = more <= 0 ? fill : card.resident * (1 + more);
             const double even =
                 fill ? std::floor(all / ((double)card.cus * per)) : (double)longest;
-            for (int up = 0; up < 2; ++up) {
-                const int each = (int)std::min<double>(longest, std::max(1.0, even + up));
+            /* rounded down and up; own ranges of the prefix's length, and of half of it */
+            for (int way = 0; way < (prefix_rounds && own_rounds ? 4 : 2); ++way) {
+                const int each = (int)std::min<double>(longest, std::max(1.0, even + way % 2));
                 const Share p = card.share(pn, prefix_rounds, each);
-                const Share o = card.share(on, own_rounds, each);
+                const Share o = card.share(on, own_rounds, way < 2 ? each : (each + 1) / 2);
                 double t = p.time + o.time;
                 if (p.groups && o.groups) {
                     /* the prefix's workgroups come first, and the others fill what they leave */
@@ -359,7 +364,7 @@ AttentionPlan plan_attention(dfq_ctx* ctx, const dfq_kv_cache* fmt, int prefix_l
                         std::min<int64_t>(card.resident, (n + card.cus - 1) / card.cus);
                     const double work = (p.work + o.work) / (card.cus * busy) * card.cost(n);
                     t = std::max(p.time, n <= room ? std::max(o.longest * card.cost(n), work)
-                                                   : work + 0.5 * o.longest);
+                                                   : work + 0.3 * o.longest);
                 }
                 t = t * round + kRangeRounds * (p.ranges + o.ranges);
                 if (p.ranges + o.ranges > 1) t += join_rounds(fmt->head_dim);
