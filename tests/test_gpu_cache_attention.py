@@ -359,3 +359,11 @@ def test_large_scores_keep_fp32(ctx, dim, bits, gs, dt):
     off = (lse.double().cpu() - want).square().mean().sqrt()
     size = c.scale * worst[..., 1].mean() + 8 * want.square().mean().sqrt()
     assert off <= 2.0 ** -25 * size + 2.0 ** -21
+
+
+@pytest.mark.parametrize("dim,bits,gs,dt", FORMATS)
+@pytest.mark.parametrize("capacity", [83, 1571])
+def test_own_caches_in_every_format(ctx, capacity, dim, bits, gs, dt):
+    """Few tokens (one range, whose workgroups write the outputs) and many (several, joined)."""
+    run_case(ctx, f"own{capacity}_{dim}_{bits}_{gs}_{dt}", dim=dim, bits=bits, gs=gs, dt=dt,
+             batch=2, rows=5, heads=2, group=4, capacity=capacity, lengths=[capacity, 38])

@@ -185,3 +185,18 @@ def test_refusals(ctx):
 def dflash_qmm_error():
     import dflash_qmm
     return dflash_qmm.DfqError
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("M,V,top", [(700, 9001, 20), (1300, 2503, 32), (6, 100003, 32)])
+def test_many_rows_and_long_joins(ctx, M, V, top, dt):
+    """More rows than workgroups are there at once (each row one workgroup's), and few long rows
+    with more alternatives in their parts than one piece of the join holds."""
+    gen = torch.Generator().manual_seed(M + V)
+    few = (3 * torch.randn(2, V, generator=gen)).to(DT[dt])
+    tokens = torch.randint(0, V, (2,), generator=gen).to(torch.int32)
+    announce(f"logprobs M={M} V={V} top={top} {dt}")
+    got = ctx.token_logprobs(few.repeat(M // 2, 1).cuda(), tokens.repeat(M // 2).cuda(), top_k=top)
+    torch.cuda.synchronize()
+    want = [w.repeat(M // 2, *[1] * (w.dim() - 1)) for w in logprobs(few, tokens, top)]
+    check(got, want, top)
