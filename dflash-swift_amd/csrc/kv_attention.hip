@@ -5,9 +5,10 @@
  * With token t's K and V values s c + b (c the code, s and b its group's scale and bias) and a
  * row's query q:
  *   z_t = scale sum_g [ s_tg (q_g . c_tg) + b_tg sum(q_g) ]
- *   y   = sum_t p_t [ s_tg c_t + b_tg ] / sum_t p_t,   p_t = 2^(z_t log2 e - M)
- * so that both products run on the codes themselves, and scales and biases meet the scores in
- * fp32: no value of the cache is rounded on the way.
+ *   y   = sum_t h_tg [ c_t + b_tg / s_tg ] / sum_t p_t,   h_tg = p_t s_tg,
+ *   p_t = 2^(z_t log2 e - M)
+ * so that both products run on the codes themselves.  K's scales and biases meet the sums in fp32;
+ * the weights h are rounded to fp16, and V's ratios b / s to 22 bits (see stage_scales).
  *
  * A workgroup takes a block of 16 or 32 rows of one head (a verify block's rows and the query heads
  * of a K/V head together; over a shared prefix, those of all sequences) and a range of tokens, 32
@@ -161,16 +162,16 @@ struct Attention {
     using half8_t = std::conditional_t<F16, f16x8_t, bf16x8_t>;
 
     /* A wave's tile of scales and biases, by token.  K's biases stay as they are stored: they
-     * meet the queries' sums in one matrix product.  So do, with bf16, V's and the weights. */
+     * meet the queries' sums in one matrix product. */
     struct Scales {
-        float k[kGroups][32];                  /* K scales * kScaleUnit                     */
+        union {
+            float k[kGroups][32];              /* K scales * kScaleUnit                     */
+            uint16_t far[2 * kGroups][32];     /* later: V's far middles in two bf16 parts  */
+        };
         float v[kGroups][32];                  /* V scales                                  */
         float size[32];                        /* a token's largest V scale                 */
         uint16_t kb[32 * kGroups];             /* K biases                                  */
-        union {
-            uint16_t parts[2 * kGroups][32];   /* bf16: V's b + centre s in two bf16 parts  */
-            float vb[kGroups][32];             /* fp16: the same in fp32                    */
-        };
+        uint16_t ratio[2 * kGroups][32];       /* what is added to V's codes, in two fp16 parts */
     };
 
     /* Lanes 0..31 load K's scale and bias of token t + lane, lanes 32..63 V's of t + lane - 32. */
@@ -185,13 +186,33 @@ struct Attention {
         __builtin_memcpy(out.b, job.bias + (int64_t)tok * kGroups, 2 * kGroups);
     }
 
-    /* A V group whose scale or bias is not finite (or the middle of its range past bf16) counts as
+    /* What V's biases add.  The matrix cores take a token's weight and scale as h = p s rounded to
+     * fp16, and h meets the codes and, in the same form, the ratio r = b / s: h (c + r) is off by
+     * what h is, 2^-12 of the value itself.  With the bias met by p instead, codes and bias cancel
+     * with different roundings where a group's values lie far from its middle (a channel that
+     * stands apart from its group's others): 64 tokens with one of 64 channels off by 16 of their
+     * 0.3, the others' errors were 9 (8 bits, 25) times the output's own rounding, and with p in
+     * 16 bits still 2.  r comes in two fp16 parts, 22 bits.
+     * Where the middle b + centre s is more than twice the codes' half range (or s is 0), h would
+     * carry most of the value in a number that may be small beside the other groups'.  There r is
+     * -centre, codes count from the middle, which is no larger than the value, and the far middle
+     * meets p itself, both in two bf16 parts (16 bits).
+     * A V group whose scale or bias is not finite (or the middle of its range past bf16) counts as
      * a NaN scale and no bias: the rows that see it get NaN, and the others, whose weight is 0,
-     * nothing.  With bf16 the middle meets the weights in two bf16 parts (16 bits of it, 2^-17 of
-     * the middle off at most, far under the outputs' own rounding). */
+     * nothing. */
+    struct Far {
+        uint32_t m[kGroups];   /* lanes 32..63: a token's far middles, high part below, or 0 */
+        bool any, nan;         /* whether the tile has such a middle, a NaN scale */
+    };
+    static __device__ __forceinline__ void put_ratio(Scales& sc, int g, int tok, float r) {
+        const _Float16 hi = (_Float16)r, lo = (_Float16)(r - (float)hi);
+        sc.ratio[2 * g][tok] = __builtin_bit_cast(uint16_t, hi);
+        sc.ratio[2 * g + 1][tok] = __builtin_bit_cast(uint16_t, lo);
+    }
     static __device__ __forceinline__ void stage_scales(const TokenScales& in, int lane,
-                                                        Scales& sc) {
+                                                        Scales& sc, Far& far) {
         const int tok = lane & 31;
+        bool all_near = true;
         wave_order();
         if (lane < 32) {
 #pragma unroll
@@ -203,24 +224,50 @@ struct Attention {
             float size = 0.0f;
 #pragma unroll
             for (int g = 0; g < kGroups; ++g) {
-                const float s = elem_to_f32<F16>(in.s[g]);
-                const float mid = fmaf(kCentre, s, elem_to_f32<F16>(in.b[g]));
-                const bool fine = fabsf(s) < __builtin_inff() && fabsf(mid) < kMost;
-                const float m = fine ? mid : 0.0f;
-                size = fmaxf(size, fine ? fabsf(s) : 0.0f);
-                sc.v[g][tok] = fine ? s : __builtin_nanf("");
-                if constexpr (F16) {
-                    sc.vb[g][tok] = m;
-                } else {
-                    const __bf16 hi = (__bf16)m;
-                    sc.parts[2 * g][tok] = __builtin_bit_cast(uint16_t, hi);
-                    sc.parts[2 * g + 1][tok] =
-                        __builtin_bit_cast(uint16_t, (__bf16)(m - (float)hi));
-                }
+                const float s = elem_to_f32<F16>(in.s[g]), b = elem_to_f32<F16>(in.b[g]);
+                all_near &= is_near(s, b);
+                size = fmaxf(size, fabsf(s));
+                sc.v[g][tok] = s;
+                put_ratio(sc, g, tok, b * __builtin_amdgcn_rcpf(s));
             }
             sc.size[tok] = size;
         }
+        far.any = far.nan = false;
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) far.m[g] = 0;
+        if (!__all(all_near)) {
+            bool nan = false;
+            uint32_t seen = 0;
+            if (lane >= 32) {
+                float size = 0.0f;
+#pragma unroll
+                for (int g = 0; g < kGroups; ++g) {
+                    const float s = elem_to_f32<F16>(in.s[g]), b = elem_to_f32<F16>(in.b[g]);
+                    const float mid = fmaf(kCentre, s, b);
+                    const bool fine = fabsf(s) < __builtin_inff() && fabsf(mid) < kMost;
+                    if (fine) size = fmaxf(size, fabsf(s));
+                    else sc.v[g][tok] = __builtin_nanf("");
+                    if (!is_near(s, b)) {
+                        put_ratio(sc, g, tok, -kCentre);
+                        const float m = fine ? mid : 0.0f;
+                        const __bf16 top = (__bf16)m, rest = (__bf16)(m - (float)top);
+                        far.m[g] = __builtin_bit_cast(uint16_t, top) |
+                                   (uint32_t)__builtin_bit_cast(uint16_t, rest) << 16;
+                    }
+                    seen |= far.m[g];
+                    nan |= !fine;
+                }
+                sc.size[tok] = size;
+            }
+            far.any = __any(seen != 0);
+            far.nan = __any(nan);
+        }
         wave_order();
+    }
+    /* Whether a group's middle is within twice its codes' half range: false where the scale is 0
+     * (or under 2^-100, whose reciprocal may not be finite), infinite or NaN. */
+    static __device__ __forceinline__ bool is_near(float s, float b) {
+        return fabsf(fmaf(kCentre, s, b)) < fmaf(2.0f * kCentre, fabsf(s), -0x1p-100f);
     }
 
     /* A lane's 8 tokens of one array and group: 4 c + 0..3 of each half of the tile. */
@@ -231,6 +278,14 @@ struct Attention {
 #pragma unroll
             for (int r = 0; r < 4; ++r) out[4 * tt + r] = v[r];
         }
+    }
+
+    /* The same of what a lane's column (2 g + part) of a product with the biases takes. */
+    static __device__ __forceinline__ void parts_of(const uint16_t (*a)[32], int lane,
+                                                    uint32_t (&out)[4]) {
+        const uint16_t* p = a[lane & 15 & (2 * kGroups - 1)] + 4 * (lane >> 4);
+        __builtin_memcpy(out, __builtin_assume_aligned(p, 8), 8);
+        __builtin_memcpy(out + 2, __builtin_assume_aligned(p + 16, 8), 8);
     }
 
     /* Codes of tokens t .. t+31 straight into LDS, a row after the other as in memory, each row's
@@ -372,9 +427,7 @@ struct Attention {
     struct Rows {
         f32x4_t o[RT][kDim / 16];      /* rows 4 c + r of a tile, one column a lane        */
         float off[RT], sum[RT];        /* a row's offset M; its lane's part of sum p       */
-        float code_sum[RT][kGroups];   /* its part of sum of the rounded p s               */
-        float bias_sum[F16 ? RT : 1][kGroups];  /* fp16: its part of sum p (b + centre s)  */
-        f32x4_t bias[F16 ? 1 : RT];    /* bf16: the same as a matrix product, column 2 g + part */
+        f32x4_t bias[RT];              /* what the biases add, column 2 g + part           */
         float unit[RT];                /* score units to log2                              */
         uint32_t mask[RT];             /* block rows that the row sees                     */
     };
@@ -460,20 +513,14 @@ struct Attention {
      * to where its largest is 2^11. */
     template <bool MASKED>
     static __device__ __forceinline__ void weigh(const Job& job, int t, int lane,
-                                                 const char* v, const Scales& sc, Rows& st,
-                                                 float (&z)[RT][8]) {
+                                                 const char* v, Scales& sc, const Far& far,
+                                                 Rows& st, float (&z)[RT][8]) {
         const int c = lane >> 4;
         Values in;
-        float size[8], vb[8];
-        uint32_t mid[4];
+        float size[8];
+        uint32_t ratio[4];
         tokens_of(sc.size, c, size);
-        if constexpr (!F16) {
-            const uint16_t* p = sc.parts[lane & 15 & (2 * kGroups - 1)] + 4 * c;
-            __builtin_memcpy(mid, __builtin_assume_aligned(p, 8), 8);
-            __builtin_memcpy(mid + 2, __builtin_assume_aligned(p + 16, 8), 8);
-        } else {
-            tokens_of(sc.vb[0], c, vb);
-        }
+        parts_of(sc.ratio, lane, ratio);
         read_values(v, sc, 0, lane, in);
         __builtin_amdgcn_sched_barrier(0);
         float most = size[0];
@@ -506,14 +553,9 @@ struct Attention {
                 st.off[rt] = next;
                 st.sum[rt] *= keep;
 #pragma unroll
-                for (int g = 0; g < kGroups; ++g) {
-                    st.code_sum[rt][g] *= keep;
-                    if constexpr (F16) st.bias_sum[rt][g] *= keep;
-                }
-#pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const float f = __shfl(keep, 4 * c + r);
-                    if constexpr (!F16) st.bias[rt][r] *= f;
+                    st.bias[rt][r] *= f;
 #pragma unroll
                     for (int i = 0; i < kDim / 16; ++i) st.o[rt][i][r] *= f;
                 }
@@ -524,19 +566,33 @@ struct Attention {
                 st.sum[rt] += z[rt][j];
             }
         }
-        if constexpr (!F16) {
-            /* sum p (b + centre s) of all groups at once.  p is rounded to bf16 here, so this
-             * term, and no other, is off by 2^-9 a token: less than the output's own rounding. */
-            const u32x4_t b = {mid[0], mid[1], mid[2], mid[3]};
+        if (far.any) {
+            /* sum p m of all groups at once, p and m in two bf16 parts each */
+            wave_order();
+            if (lane >= 32)
+#pragma unroll
+                for (int g = 0; g < kGroups; ++g) {
+                    sc.far[2 * g][lane & 31] = (uint16_t)far.m[g];
+                    sc.far[2 * g + 1][lane & 31] = (uint16_t)(far.m[g] >> 16);
+                }
+            wave_order();
+            uint32_t m[4];
+            parts_of(sc.far, lane, m);
+            const u32x4_t b = {m[0], m[1], m[2], m[3]};
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                u32x4_t a;
+                u32x4_t hi, lo;
 #pragma unroll
                 for (int jp = 0; jp < 4; ++jp) {
                     const f32x2_t x = {z[rt][2 * jp], z[rt][2 * jp + 1]};
-                    a[jp] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2_t));
+                    const bf16x2_t h = __builtin_convertvector(x, bf16x2_t);
+                    const f32x2_t rest = {x[0] - (float)h[0], x[1] - (float)h[1]};
+                    hi[jp] = __builtin_bit_cast(uint32_t, h);
+                    lo[jp] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, bf16x2_t));
                 }
-                st.bias[rt] = mfma(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
+                st.bias[rt] = mfma(__builtin_bit_cast(bf16x8_t, hi), __builtin_bit_cast(bf16x8_t, b),
+                                   st.bias[rt]);
+                st.bias[rt] = mfma(__builtin_bit_cast(bf16x8_t, lo), __builtin_bit_cast(bf16x8_t, b),
                                    st.bias[rt]);
             }
         }
@@ -544,16 +600,16 @@ struct Attention {
         for (int g = 0; g < kGroups; ++g) {
             f16x8_t w[kTiles];
             v_operands(in, w);
-            float s[8], b[8];
+            float s[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                s[j] = in.s[j];
-                if constexpr (F16) b[j] = vb[j];
-            }
+            for (int j = 0; j < 8; ++j) s[j] = in.s[j];
+            /* the other groups' columns of the product with the ratios stay as they are */
+            const bool mine = (lane & 15) >> 1 == g;
+            const f16x8_t r = as_f16x8(mine ? ratio[0] : 0, mine ? ratio[1] : 0,
+                                       mine ? ratio[2] : 0, mine ? ratio[3] : 0);
             __builtin_amdgcn_sched_barrier(0);
             if (g + 1 < kGroups) {
                 read_values(v, sc, g + 1, lane, in);
-                if constexpr (F16) tokens_of(sc.vb[g + 1], c, vb);
                 __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
@@ -567,20 +623,16 @@ struct Attention {
                         if (!sees(job, st.mask[rt], tok)) x[0] = 0.0f;
                         if (!sees(job, st.mask[rt], tok + 1)) x[1] = 0.0f;
                     }
-                    if constexpr (F16) {
-                        st.bias_sum[rt][g] = fmaf(z[rt][2 * jp], b[2 * jp], st.bias_sum[rt][g]);
-                        st.bias_sum[rt][g] =
-                            fmaf(z[rt][2 * jp + 1], b[2 * jp + 1], st.bias_sum[rt][g]);
-                    }
-                    const f16x2_t h = __builtin_convertvector(x, f16x2_t);
-                    ps[jp] = __builtin_bit_cast(uint32_t, h);
-                    const f16x2_t one = {(_Float16)1.0f, (_Float16)1.0f};
-                    st.code_sum[rt][g] = __builtin_amdgcn_fdot2(h, one, st.code_sum[rt][g], false);
+                    ps[jp] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2_t));
                 }
-                const f16x8_t a = as_f16x8(ps[0], ps[1], ps[2], ps[3]);
+                f16x8_t a = as_f16x8(ps[0], ps[1], ps[2], ps[3]);
 #pragma unroll
                 for (int i = 0; i < kTiles; ++i)
                     st.o[rt][g * kTiles + i] = mfma(a, w[i], st.o[rt][g * kTiles + i]);
+                if (far.nan)   /* stays in its own group */
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) a[j] = a[j] == a[j] ? a[j] : (_Float16)0.0f;
+                st.bias[rt] = mfma(a, r, st.bias[rt]);
             }
         }
     }
@@ -598,11 +650,9 @@ struct Attention {
             };
             struct {
                 f32x4_t merge[kWaves][kDim / 16][RT][64];
-                /* by row: offset, sum; what the centre and (fp16) the biases add to a group's
-                 * channels; with bf16 the biases' two parts */
+                /* by row: offset, sum, and the two parts of what the biases add to a group */
                 float offs[kWaves][kRows], sums[kWaves][kRows];
-                float fix[kWaves][kGroups][kRows];
-                float bias[F16 ? 0 : kWaves][2 * kGroups][kRows];
+                float bias[kWaves][2 * kGroups][kRows];
             };
         };
     };
@@ -721,12 +771,7 @@ struct Attention {
             st.sum[rt] = 0.0f;
             st.unit[rt] = lds.units[r];
             st.mask[rt] = lds.masks[r];
-#pragma unroll
-            for (int g = 0; g < kGroups; ++g) {
-                st.code_sum[rt][g] = 0.0f;
-                if constexpr (F16) st.bias_sum[rt][g] = 0.0f;
-            }
-            if constexpr (!F16) st.bias[rt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            st.bias[rt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int d = 0; d < kDim / 16; ++d) st.o[rt][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
         }
@@ -738,7 +783,8 @@ struct Attention {
         while (t < job.t1) {
             const int next = t + 32 * kWaves, other = kBufs == 2 ? buf ^ 1 : 0;
             loaded<0>();
-            stage_scales(scale, lane, sc);
+            Far far;
+            stage_scales(scale, lane, sc, far);
             if (next < job.t1) load_scales(job, next, lane, scale);
             if constexpr (kBufs == 2) {
                 if (next < job.t1) {
@@ -760,15 +806,15 @@ struct Attention {
                     loaded<0>();
                 }
             }
-            if (masked) weigh<true>(job, t, lane, v[buf], sc, st, z);
-            else weigh<false>(job, t, lane, v[buf], sc, st, z);
+            if (masked) weigh<true>(job, t, lane, v[buf], sc, far, st, z);
+            else weigh<false>(job, t, lane, v[buf], sc, far, st, z);
             read_done();
             buf = other;
             t = next;
         }
 
-        /* The waves' rows together: their outputs, offsets, sums and what the codes' centre and
-         * the biases add meet in LDS.  A wave then adds up every fourth column tile, each of its
+        /* The waves' rows together: their outputs, offsets, sums and what the biases add meet in
+         * LDS.  A wave then adds up every fourth column tile, each of its
          * lanes with the weights of its four rows. */
         __syncthreads();
 #pragma unroll
@@ -783,16 +829,8 @@ struct Attention {
                 lds.offs[wave][r] = st.off[rt];
                 lds.sums[wave][r] = sum;
             }
-#pragma unroll
-            for (int g = 0; g < kGroups; ++g) {
-                float f = -kCentre * st.code_sum[rt][g];
-                if constexpr (F16) f += st.bias_sum[rt][g];
-                f = quarters_sum(f);
-                if (lane < 16) lds.fix[wave][g][r] = f;
-            }
-            if constexpr (!F16)
-                if ((lane & 15) < 2 * kGroups)
-                    *(f32x4_t*)&lds.bias[wave][lane & 15][row] = st.bias[rt];
+            if ((lane & 15) < 2 * kGroups)
+                *(f32x4_t*)&lds.bias[wave][lane & 15][row] = st.bias[rt];
         }
         __syncthreads();
         const int64_t nrows = (int64_t)p.batch * p.rows.by * p.group.by;
@@ -846,13 +884,11 @@ struct Attention {
 #pragma unroll
                 for (int w = 0; w < kWaves; ++w) {
                     const f32x4_t x = lds.merge[w][d][rt][lane];
-                    f32x4_t fix = *(const f32x4_t*)&lds.fix[w][g][row];
-                    if constexpr (!F16)
-                        fix += *(const f32x4_t*)&lds.bias[w][2 * g][row] +
-                               *(const f32x4_t*)&lds.bias[w][2 * g + 1][row];
+                    const f32x4_t bias = *(const f32x4_t*)&lds.bias[w][2 * g][row] +
+                                         *(const f32x4_t*)&lds.bias[w][2 * g + 1][row];
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        y[i] = fmaf(fmaf(x[i], back, fix[i]), weight[w][i], y[i]);
+                        y[i] = fmaf(fmaf(x[i], back, bias[i]), weight[w][i], y[i]);
                 }
                 if (alone) {
                     const int channel = g * GS + (lane & 15) * kTiles + d % kTiles;
