@@ -169,7 +169,7 @@ struct Attention {
             uint16_t far[2 * kGroups][32];     /* later: V's far middles in two bf16 parts  */
         };
         float v[kGroups][32];                  /* V scales                                  */
-        float size[32];                        /* a token's largest V scale                 */
+        float size[32];                        /* log2 of a token's largest V scale         */
         uint16_t kb[32 * kGroups];             /* K biases                                  */
         uint16_t ratio[2 * kGroups][32];       /* what is added to V's codes, in two fp16 parts */
     };
@@ -230,7 +230,7 @@ struct Attention {
                 sc.v[g][tok] = s;
                 put_ratio(sc, g, tok, b * __builtin_amdgcn_rcpf(s));
             }
-            sc.size[tok] = size;
+            sc.size[tok] = log2_above(size);
         }
         far.any = far.nan = false;
 #pragma unroll
@@ -257,12 +257,17 @@ struct Attention {
                     seen |= far.m[g];
                     nan |= !fine;
                 }
-                sc.size[tok] = size;
+                sc.size[tok] = log2_above(size);
             }
             far.any = __any(seen != 0);
             far.nan = __any(nan);
         }
         wave_order();
+    }
+    /* log2 of a scale, rounded up to a whole number; the least is -64, so that sums of weights stay
+     * finite where the scales are 0. */
+    static __device__ __forceinline__ float log2_above(float size) {
+        return fmaxf((float)((int)(__float_as_uint(size) >> 23) - 126), -64.0f);
     }
     /* Whether a group's middle is within twice its codes' half range: false where the scale is 0
      * (or under 2^-100, whose reciprocal may not be finite), infinite or NaN. */
@@ -510,7 +515,8 @@ struct Attention {
     /* Softmax weights of the tile's scores and their product with V.  A row's offset M is kept
      * so that p s stays below 2^15: p s is rounded to fp16 for the matrix cores, whose 2^-14
      * least normal number then lies 2^-29 under it.  M rises only when a tile would pass 2^15,
-     * to where its largest is 2^11. */
+     * to where its largest is 2^11.  It goes by each token's own score and scale: a token of huge
+     * values and no weight does not move it. */
     template <bool MASKED>
     static __device__ __forceinline__ void weigh(const Job& job, int t, int lane,
                                                  const char* v, Scales& sc, const Far& far,
@@ -523,32 +529,15 @@ struct Attention {
         parts_of(sc.ratio, lane, ratio);
         read_values(v, sc, 0, lane, in);
         __builtin_amdgcn_sched_barrier(0);
-        float most = size[0];
-#pragma unroll
-        for (int j = 1; j < 8; ++j) most = fmaxf(most, size[j]);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            float top = z[rt][0];
+            float top = fmaf(z[rt][0], st.unit[rt], size[0]);
 #pragma unroll
-            for (int j = 1; j < 8; ++j) top = fmaxf(top, z[rt][j]);
-            if constexpr (MASKED) {
-                most = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int tok = t + 16 * (j >> 2) + 4 * c + (j & 3);
-                    if (sees(job, st.mask[rt], tok)) most = fmaxf(most, size[j]);
-                }
-            }
-            /* log2 of the scale, rounded up to a whole number */
-            const float up = fmaxf((float)((int)(__float_as_uint(most) >> 23) - 126), -40.0f);
-            const float high = fmaf(top, st.unit[rt], up);
-            if (__any(high > st.off[rt] + 15.0f)) {
-                float all = fmaf(top, st.unit[rt], 0.0f), allup = up;
-                all = fmaxf(all, __shfl_xor(all, 16));
-                all = fmaxf(all, __shfl_xor(all, 32));
-                allup = fmaxf(allup, __shfl_xor(allup, 16));
-                allup = fmaxf(allup, __shfl_xor(allup, 32));
-                const float next = fmaxf(st.off[rt], all + allup - 11.0f);
+            for (int j = 1; j < 8; ++j) top = fmaxf(top, fmaf(z[rt][j], st.unit[rt], size[j]));
+            if (__any(top > st.off[rt] + 15.0f)) {
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float next = fmaxf(st.off[rt], top - 11.0f);
                 const float keep = next == st.off[rt] ? 1.0f : exp2f(st.off[rt] - next);
                 st.off[rt] = next;
                 st.sum[rt] *= keep;

@@ -112,3 +112,42 @@ def test_groups_far_from_zero(ctx, bits, gs, dim, dt):
     c = One(q, arrays_of(k, bits, gs), arrays_of(v.flatten(-2).to(DTYPES[dt]), bits, gs), bits, gs)
     announce(f"attention far groups bits={bits} gs={gs} dim={dim} {dt}")
     c.check(*c.run(ctx))
+
+
+def aimed(q, scores, scale):
+    """K rows [tokens, dim] whose products with the one query q are `scores`."""
+    f = q.double()
+    return torch.tensor(scores).double()[:, None] * f / (scale * (f @ f))
+
+
+def one_query(seed, dim, dt, scores):
+    """A single row and head, and K rows with about these scores."""
+    q = normal(seed, 1, 1, dim).to(DTYPES[dt])
+    return q, aimed(q[0, 0], scores, dim ** -0.5)[None, None].to(DTYPES[dt])
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("power", [28, 34, 60])
+@pytest.mark.parametrize("at", [3, 290])
+def test_a_token_of_no_weight_and_huge_values(ctx, at, power, bits):
+    """One token that the row sees has values 2^power times the others' and a weight 2^-power - 40
+    of theirs: nothing of it reaches the outputs."""
+    n, dim, gs = 400, 128, 64
+    scores = normal(7, n)
+    scores[at] = -(power + 40) * math.log(2.0)
+    q, k = one_query(8, dim, "bf16", scores.tolist())
+    v = normal(9, 1, 1, n, dim)
+    v[0, 0, at] *= 2.0 ** power
+    c = One(q, arrays_of(k, bits, gs), arrays_of(v.bfloat16(), bits, gs), bits, gs)
+    announce(f"attention huge token at {at} 2^{power} bits={bits}")
+    c.check(*c.run(ctx))
+
+
+@pytest.mark.parametrize("size", [1e-24, 1e-12, 1e12, 1e30])
+def test_small_and_large_values(ctx, size):
+    q = (1.5 * normal(15, 4, 2, 128)).bfloat16()
+    k = normal(16, 1, 2, 300, 128).bfloat16()
+    v = (size * normal(17, 1, 2, 300, 128)).bfloat16()
+    c = One(q, arrays_of(k, 4, 64), arrays_of(v, 4, 64), 4, 64)
+    announce(f"attention values of size {size}")
+    c.check(*c.run(ctx))
