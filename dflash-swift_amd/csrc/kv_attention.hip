@@ -196,7 +196,8 @@ struct Attention {
      * Where the middle b + centre s is more than twice the codes' half range (or s is 0), h would
      * carry most of the value in a number that may be small beside the other groups'.  There r is
      * -centre, codes count from the middle, which is no larger than the value, and the far middle
-     * meets p itself, both in two bf16 parts (16 bits).
+     * meets p itself, both in two bf16 parts (16 bits).  The offset of a row's weights keeps p m
+     * below 2^35 as it keeps h below 2^15: for it, a far middle counts as a scale of 2^-20 of it.
      * A V group whose scale or bias is not finite (or the middle of its range past bf16) counts as
      * a NaN scale and no bias: the rows that see it get NaN, and the others, whose weight is 0,
      * nothing. */
@@ -250,6 +251,7 @@ struct Attention {
                     if (!is_near(s, b)) {
                         put_ratio(sc, g, tok, -kCentre);
                         const float m = fine ? mid : 0.0f;
+                        size = fmaxf(size, fabsf(m) * 0x1p-20f);
                         const __bf16 top = (__bf16)m, rest = (__bf16)(m - (float)top);
                         far.m[g] = __builtin_bit_cast(uint16_t, top) |
                                    (uint32_t)__builtin_bit_cast(uint16_t, rest) << 16;

@@ -151,3 +151,15 @@ def test_small_and_large_values(ctx, size):
     c = One(q, arrays_of(k, 4, 64), arrays_of(v, 4, 64), 4, 64)
     announce(f"attention values of size {size}")
     c.check(*c.run(ctx))
+
+
+@pytest.mark.parametrize("value", [1e-30, 5.0, 1e25, -3e38])
+@pytest.mark.parametrize("tokens", [1, 300])
+def test_values_all_the_same(ctx, tokens, value):
+    """Groups of equal elements have no scale, only a bias."""
+    q = normal(13, 1, 2, 128).bfloat16()
+    k = normal(14, 1, 2, tokens, 128).bfloat16()
+    v = torch.full((1, 2, tokens, 128), value, dtype=torch.bfloat16)
+    c = One(q, arrays_of(k, 4, 64), arrays_of(v, 4, 64), 4, 64)
+    announce(f"attention equal values {value} tokens={tokens}")
+    c.check(*c.run(ctx))
