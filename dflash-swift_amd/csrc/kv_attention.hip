@@ -721,7 +721,8 @@ struct Attention {
                     for (int j = kGroups; j < 8; ++j) to[j] = 0;
             }
             if (piece == 0) {
-                lds.units[r] = ldexpf(p.scale_log2e, 8 + e - 14);
+                /* never 0: a hidden token's -inf stays one */
+                lds.units[r] = fmaxf(ldexpf(p.scale_log2e, 8 + e - 14), 0x1p-149f);
                 lds.masks[r] = in.mask[i];
             }
             /* nibble order of k_operand: operand element j is channel j/2 + 4 (j%2) */

@@ -163,3 +163,14 @@ def test_values_all_the_same(ctx, tokens, value):
     c = One(q, arrays_of(k, 4, 64), arrays_of(v, 4, 64), 4, 64)
     announce(f"attention equal values {value} tokens={tokens}")
     c.check(*c.run(ctx))
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-38])
+def test_no_scores_and_hidden_tokens(ctx, scale):
+    """Queries of zero and a tiny scale: every score is 0, and the draft chain's mask still holds."""
+    q = torch.zeros(6, 2, 128, dtype=torch.bfloat16)
+    k = normal(18, 1, 2, 50, 128).bfloat16()
+    v = normal(19, 1, 2, 50, 128).bfloat16()
+    c = One(q, arrays_of(k, 4, 64), arrays_of(v, 4, 64), 4, 64, scale=scale)
+    announce(f"attention no scores scale={scale}")
+    c.check(*c.run(ctx))
