@@ -37,7 +37,7 @@ namespace {
 
 constexpr int kDim = DFQ_HEAD_DIM;
 constexpr int kWaves = DFQ_KV_THREADS / 64;
-constexpr float kNever = -1e30f;      /* the offset of a row that has seen nothing */
+constexpr float kNever = -__FLT_MAX__;   /* the offset of a row that has seen nothing */
 
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
@@ -436,6 +436,8 @@ struct Attention {
         float off[RT], sum[RT];        /* a row's offset M; its lane's part of sum p       */
         f32x4_t bias[RT];              /* what the biases add, column 2 g + part           */
         float unit[RT];                /* score units to log2                              */
+        float from[RT];                /* what a row's scores are counted from, mostly 0   */
+        bool moved;                    /* whether any is not                               */
         uint32_t mask[RT];             /* block rows that the row sees                     */
     };
 
@@ -514,11 +516,22 @@ struct Attention {
         return tok < job.clear || (tok < job.n && (mask >> (tok - job.first) & 1));
     }
 
+    static __device__ __forceinline__ float largest_product(const float (&z)[8], float unit,
+                                                            const float (&size)[8]) {
+        float top = fmaf(z[0], unit, size[0]);
+#pragma unroll
+        for (int j = 1; j < 8; ++j) top = fmaxf(top, fmaf(z[j], unit, size[j]));
+        return top;
+    }
+
     /* Softmax weights of the tile's scores and their product with V.  A row's offset M is kept
      * so that p s stays below 2^15: p s is rounded to fp16 for the matrix cores, whose 2^-14
      * least normal number then lies 2^-29 under it.  M rises only when a tile would pass 2^15,
      * to where its largest is 2^11.  It goes by each token's own score and scale: a token of huge
-     * values and no weight does not move it. */
+     * values and no weight does not move it.
+     * Where M would pass 2^10 in size, the row's scores are counted from the tile's largest, and M
+     * with them: an M of 2^26 could not be placed within the 2^4 that p s has above 2^11, and past
+     * that p would be infinite or 0 throughout. */
     template <bool MASKED>
     static __device__ __forceinline__ void weigh(const Job& job, int t, int lane,
                                                  const char* v, Scales& sc, const Far& far,
@@ -533,14 +546,29 @@ struct Attention {
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            float top = fmaf(z[rt][0], st.unit[rt], size[0]);
+            if (st.moved)
 #pragma unroll
-            for (int j = 1; j < 8; ++j) top = fmaxf(top, fmaf(z[rt][j], st.unit[rt], size[j]));
+                for (int j = 0; j < 8; ++j) z[rt][j] -= st.from[rt];
+            float top = largest_product(z[rt], st.unit[rt], size);
             if (__any(top > st.off[rt] + 15.0f)) {
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                const float next = fmaxf(st.off[rt], top - 11.0f);
-                const float keep = next == st.off[rt] ? 1.0f : exp2f(st.off[rt] - next);
+                top = quarters_largest(top);
+                float off = st.off[rt], next = fmaxf(off, top - 11.0f);
+                const bool move = next > off && fabsf(next) > 0x1p10f;
+                if (__any(move)) {
+                    float by = z[rt][0];
+#pragma unroll
+                    for (int j = 1; j < 8; ++j) by = fmaxf(by, z[rt][j]);
+                    by = quarters_largest(by);
+                    by = move && fabsf(by) < __builtin_inff() ? by : 0.0f;
+                    st.from[rt] += by;
+                    st.moved = true;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) z[rt][j] -= by;
+                    top = quarters_largest(largest_product(z[rt], st.unit[rt], size));
+                    off = off == kNever ? off : fmaf(-by, st.unit[rt], off);
+                    next = fmaxf(off, top - 11.0f);
+                }
+                const float keep = next == off ? 1.0f : exp2f(off - next);
                 st.off[rt] = next;
                 st.sum[rt] *= keep;
 #pragma unroll
@@ -756,10 +784,12 @@ struct Attention {
         __syncthreads();
 
         Rows st;
+        st.moved = false;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const int r = rt * 16 + (lane & 15);
             st.off[rt] = kNever;
+            st.from[rt] = 0.0f;
             st.sum[rt] = 0.0f;
             st.unit[rt] = lds.units[r];
             st.mask[rt] = lds.masks[r];
@@ -818,7 +848,9 @@ struct Attention {
             const int r = rt * 16 + (lane & 15), row = rt * 16 + 4 * (lane >> 4);
             const float sum = quarters_sum(st.sum[rt]);
             if (lane < 16) {
-                lds.offs[wave][r] = st.off[rt];
+                lds.offs[wave][r] = st.off[rt] == kNever
+                                        ? kNever
+                                        : fmaf(st.from[rt], st.unit[rt], st.off[rt]);
                 lds.sums[wave][r] = sum;
             }
             if ((lane & 15) < 2 * kGroups)

@@ -174,3 +174,38 @@ def test_no_scores_and_hidden_tokens(ctx, scale):
     c = One(q, arrays_of(k, 4, 64), arrays_of(v, 4, 64), 4, 64, scale=scale)
     announce(f"attention no scores scale={scale}")
     c.check(*c.run(ctx))
+
+
+def test_scores_far_below_zero(ctx):
+    """A row whose scores all lie below -1e30 has a softmax as any other."""
+    n, dim = 70, 64
+    scores = [-1e33 * (2 + i % 7) for i in range(n)]
+    scores[41] = -5e32
+    q, k = one_query(20, dim, "bf16", scores)
+    v = normal(21, 1, 1, n, dim).bfloat16()
+    c = One(q, arrays_of(k, 8, 64), arrays_of(v, 8, 64), 8, 64)
+    announce("attention scores far below zero")
+    y, lse = c.run(ctx)
+    want_y, want_lse, _, _ = c.expected()
+    assert ((lse - want_lse) / want_lse).abs().max() < 1e-4
+    assert ((y - want_y).abs() <= 2.0 ** -8 * want_y.abs() + 2.0 ** -18 * v.abs().max()).all()
+
+
+@pytest.mark.parametrize("bits,dt", [(4, "bf16"), (8, "f16")])
+@pytest.mark.parametrize("size", [1e3, 1e6, 1e8, 1e9, 1e12])
+def test_large_scores(ctx, size, bits, dt):
+    """Scores of either sign far past what fp32 holds in whole numbers: the largest alone counts,
+    and lies apart from the others by more than any sum's rounding."""
+    n, dim = 500, 128
+    scores = (size * normal(22, n)).clamp(-2 * size, 2 * size)
+    scores[77], scores[401] = 3 * size, 4 * size
+    q, k = one_query(23, dim, "bf16" if size > 1e3 else dt, scores.tolist())
+    dt = "bf16" if size > 1e3 else dt
+    v = normal(24, 1, 1, n, dim).to(DTYPES[dt])
+    c = One(q, arrays_of(k, bits, 64), arrays_of(v, bits, 64), bits, 64)
+    announce(f"attention large scores {size} bits={bits} {dt}")
+    y, lse = c.run(ctx)
+    want_y, want_lse, _, _ = c.expected()
+    ulp = 2.0 ** -8 if dt == "bf16" else 2.0 ** -11
+    assert ((lse - want_lse) / want_lse).abs().max() < 1e-4
+    assert ((y - want_y).abs() <= ulp * want_y.abs() + 2.0 ** -18 * v.abs().max()).all()
