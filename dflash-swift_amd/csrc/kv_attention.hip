@@ -74,6 +74,9 @@ __device__ __forceinline__ f32x4_t mfma(bf16x8_t a, bf16x8_t b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
+/* A condition whose code is kept out of the others' way. */
+__device__ __forceinline__ bool rarely(bool b) { return __builtin_expect(b, false); }
+
 /* A pointer that is the same in every lane, in scalar registers. */
 __device__ __forceinline__ const char* uniform(const void* p) {
     const uint64_t a = (uint64_t)(uintptr_t)p;
@@ -186,6 +189,64 @@ struct Attention {
         __builtin_memcpy(out.b, job.bias + (int64_t)tok * kGroups, 2 * kGroups);
     }
 
+    struct Rows {
+        f32x4_t o[RT][kDim / 16];      /* rows 4 c + r of a tile, one column a lane        */
+        float off[RT], sum[RT];        /* a row's offset M; its lane's part of sum p       */
+        f32x4_t bias[RT];              /* what the biases add, column 2 g + part           */
+        float unit[RT];                /* score units to log2                              */
+        float from[RT];                /* what a row's scores are counted from, mostly 0   */
+        bool moved;                    /* whether any is not                               */
+        uint64_t apart;                /* what even_groups took from a group's scales, log2, a
+                                        * byte each                                        */
+        uint32_t mask[RT];             /* block rows that the row sees                     */
+    };
+
+    static __device__ __forceinline__ bool sees(const Job& job, uint32_t mask, int tok) {
+        return tok < job.clear || (tok < job.n && (mask >> (tok - job.first) & 1));
+    }
+
+    /* Where the groups' V scales are 2^8 and more apart, they are brought to one size, that of the
+     * smallest group: h of one group would be denormal beside another's 2^20 times as large.  A
+     * group's size is the mean exponent of its scales over the wave's first tile, of the tokens that
+     * all rows see (what a row does not see may not move its roundings); zeros count as their
+     * token's largest. */
+    static constexpr uint32_t kApart = 8;
+    static __device__ __forceinline__ uint64_t even_groups(const Job& job, int t, int lane,
+                                                           const Scales& sc, const Rows& st) {
+        uint32_t all = ~0u;
+        if (t + 32 > job.clear) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+                if (rt * 16 + (lane & 15) < job.nrows) all &= st.mask[rt];
+            all = group_of<16>(all, [](uint32_t a, uint32_t b) { return a & b; });
+        }
+        const bool counts = lane >= 32 && sees(job, all, t + (lane & 31));
+        const int n = max(__popcll(__ballot(counts)), 1);
+        const auto exponent = [&](int g) { return __float_as_uint(sc.v[g][lane & 31]) >> 23 & 255u; };
+        uint32_t most = 0;
+#pragma unroll 1
+        for (int g = 0; g < kGroups; ++g) most = max(most, exponent(g));
+        uint64_t means = 0;   /* a byte each */
+        uint32_t least = 255;
+#pragma unroll 1
+        for (int g = 0; g < kGroups; ++g) {
+            const uint32_t e = exponent(g);
+            const uint32_t v = group_of<16>(counts ? e ? e : most : 0u,
+                                            [](uint32_t x, uint32_t y) { return x + y; });
+            const uint32_t sum = __builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48);
+            const uint32_t mean = __builtin_amdgcn_readfirstlane(sum / n);
+            means |= (uint64_t)mean << 8 * g;
+            least = min(least, mean);
+        }
+        uint64_t apart = 0;
+#pragma unroll 1
+        for (int g = 0; g < kGroups; ++g) {
+            const uint32_t by = (uint32_t)(means >> 8 * g & 255u) - least;
+            if (by >= kApart) apart |= (uint64_t)min(by, 60u) << 8 * g;
+        }
+        return apart;
+    }
+
     /* What V's biases add.  The matrix cores take a token's weight and scale as h = p s rounded to
      * fp16, and h meets the codes and, in the same form, the ratio r = b / s: h (c + r) is off by
      * what h is, 2^-12 of the value itself.  With the bias met by p instead, codes and bias cancel
@@ -210,10 +271,11 @@ struct Attention {
         sc.ratio[2 * g][tok] = __builtin_bit_cast(uint16_t, hi);
         sc.ratio[2 * g + 1][tok] = __builtin_bit_cast(uint16_t, lo);
     }
-    static __device__ __forceinline__ void stage_scales(const TokenScales& in, int lane,
-                                                        Scales& sc, Far& far) {
+    static __device__ __forceinline__ void stage_scales(const Job& job, int t, bool first,
+                                                        const TokenScales& in, int lane,
+                                                        Scales& sc, Far& far, Rows& st) {
         const int tok = lane & 31;
-        bool all_near = true;
+        bool plain = true;   /* near middles, scales of one size */
         wave_order();
         if (lane < 32) {
 #pragma unroll
@@ -222,23 +284,29 @@ struct Attention {
             __builtin_memcpy(__builtin_assume_aligned(sc.kb + tok * kGroups, 2 * kGroups), in.b,
                              2 * kGroups);
         } else {
-            float size = 0.0f;
+            float size = 0.0f, least = __builtin_inff();
 #pragma unroll
             for (int g = 0; g < kGroups; ++g) {
                 const float s = elem_to_f32<F16>(in.s[g]), b = elem_to_f32<F16>(in.b[g]);
-                all_near &= is_near(s, b);
+                plain &= is_near(s, b);
                 size = fmaxf(size, fabsf(s));
+                least = fminf(least, fabsf(s));
                 sc.v[g][tok] = s;
                 put_ratio(sc, g, tok, b * __builtin_amdgcn_rcpf(s));
             }
+            plain &= size < least * (float)(1 << (kApart - 1));
             sc.size[tok] = log2_above(size);
         }
         far.any = far.nan = false;
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) far.m[g] = 0;
-        if (!__all(all_near)) {
+        if (rarely(!__all(plain) || st.apart)) {
             bool nan = false;
             uint32_t seen = 0;
+            if (kGroups > 1 && first) {
+                wave_order();
+                st.apart = even_groups(job, t, lane, sc, st);
+            }
             if (lane >= 32) {
                 float size = 0.0f;
 #pragma unroll
@@ -246,11 +314,12 @@ struct Attention {
                     const float s = elem_to_f32<F16>(in.s[g]), b = elem_to_f32<F16>(in.b[g]);
                     const float mid = fmaf(kCentre, s, b);
                     const bool fine = fabsf(s) < __builtin_inff() && fabsf(mid) < kMost;
-                    if (fine) size = fmaxf(size, fabsf(s));
-                    else sc.v[g][tok] = __builtin_nanf("");
+                    const int by = (int)(st.apart >> 8 * g & 255u);
+                    sc.v[g][tok] = fine ? ldexpf(s, -by) : __builtin_nanf("");
+                    if (fine) size = fmaxf(size, ldexpf(fabsf(s), -by));
                     if (!is_near(s, b)) {
                         put_ratio(sc, g, tok, -kCentre);
-                        const float m = fine ? mid : 0.0f;
+                        const float m = fine ? ldexpf(mid, -by) : 0.0f;
                         size = fmaxf(size, fabsf(m) * 0x1p-20f);
                         const __bf16 top = (__bf16)m, rest = (__bf16)(m - (float)top);
                         far.m[g] = __builtin_bit_cast(uint16_t, top) |
@@ -431,16 +500,6 @@ struct Attention {
         for (int i = 0; i < kTiles; ++i) out[i] = as_f16x8(o[i][0], o[i][1], o[i][2], o[i][3]);
     }
 
-    struct Rows {
-        f32x4_t o[RT][kDim / 16];      /* rows 4 c + r of a tile, one column a lane        */
-        float off[RT], sum[RT];        /* a row's offset M; its lane's part of sum p       */
-        f32x4_t bias[RT];              /* what the biases add, column 2 g + part           */
-        float unit[RT];                /* score units to log2                              */
-        float from[RT];                /* what a row's scores are counted from, mostly 0   */
-        bool moved;                    /* whether any is not                               */
-        uint32_t mask[RT];             /* block rows that the row sees                     */
-    };
-
     /* One tile of 32 tokens: scores from k, then the next tile's K, then the values. */
     template <bool MASKED>
     static __device__ __forceinline__ void scores(const Job& job, int t, int lane,
@@ -512,10 +571,6 @@ struct Attention {
         }
     }
 
-    static __device__ __forceinline__ bool sees(const Job& job, uint32_t mask, int tok) {
-        return tok < job.clear || (tok < job.n && (mask >> (tok - job.first) & 1));
-    }
-
     static __device__ __forceinline__ float largest_product(const float (&z)[8], float unit,
                                                             const float (&size)[8]) {
         float top = fmaf(z[0], unit, size[0]);
@@ -546,7 +601,7 @@ struct Attention {
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            if (st.moved)
+            if (rarely(st.moved))
 #pragma unroll
                 for (int j = 0; j < 8; ++j) z[rt][j] -= st.from[rt];
             float top = largest_product(z[rt], st.unit[rt], size);
@@ -554,7 +609,7 @@ struct Attention {
                 top = quarters_largest(top);
                 float off = st.off[rt], next = fmaxf(off, top - 11.0f);
                 const bool move = next > off && fabsf(next) > 0x1p10f;
-                if (__any(move)) {
+                if (rarely(__any(move))) {
                     float by = z[rt][0];
 #pragma unroll
                     for (int j = 1; j < 8; ++j) by = fmaxf(by, z[rt][j]);
@@ -585,7 +640,7 @@ struct Attention {
                 st.sum[rt] += z[rt][j];
             }
         }
-        if (far.any) {
+        if (rarely(far.any)) {
             /* sum p m of all groups at once, p and m in two bf16 parts each */
             wave_order();
             if (lane >= 32)
@@ -648,7 +703,7 @@ struct Attention {
 #pragma unroll
                 for (int i = 0; i < kTiles; ++i)
                     st.o[rt][g * kTiles + i] = mfma(a, w[i], st.o[rt][g * kTiles + i]);
-                if (far.nan)   /* stays in its own group */
+                if (rarely(far.nan))   /* stays in its own group */
 #pragma unroll
                     for (int j = 0; j < 8; ++j) a[j] = a[j] == a[j] ? a[j] : (_Float16)0.0f;
                 st.bias[rt] = mfma(a, r, st.bias[rt]);
@@ -672,6 +727,7 @@ struct Attention {
                 /* by row: offset, sum, and the two parts of what the biases add to a group */
                 float offs[kWaves][kRows], sums[kWaves][kRows];
                 float bias[kWaves][2 * kGroups][kRows];
+                uint64_t apart[kWaves];
             };
         };
     };
@@ -785,6 +841,7 @@ struct Attention {
 
         Rows st;
         st.moved = false;
+        st.apart = 0;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const int r = rt * 16 + (lane & 15);
@@ -806,7 +863,7 @@ struct Attention {
             const int next = t + 32 * kWaves, other = kBufs == 2 ? buf ^ 1 : 0;
             loaded<0>();
             Far far;
-            stage_scales(scale, lane, sc, far);
+            stage_scales(job, t, t < job.t0 + 32 * kWaves, scale, lane, sc, far, st);
             if (next < job.t1) load_scales(job, next, lane, scale);
             if constexpr (kBufs == 2) {
                 if (next < job.t1) {
@@ -843,6 +900,7 @@ struct Attention {
         for (int d = 0; d < kDim / 16; ++d)
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) lds.merge[wave][d][rt][lane] = st.o[rt][d];
+        if (lane == 0) lds.apart[wave] = st.apart;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const int r = rt * 16 + (lane & 15), row = rt * 16 + 4 * (lane >> 4);
@@ -910,9 +968,10 @@ struct Attention {
                     const f32x4_t x = lds.merge[w][d][rt][lane];
                     const f32x4_t bias = *(const f32x4_t*)&lds.bias[w][2 * g][row] +
                                          *(const f32x4_t*)&lds.bias[w][2 * g + 1][row];
+                    const int by = (int)(lds.apart[w] >> 8 * g & 255u);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        y[i] = fmaf(fmaf(x[i], back, bias[i]), weight[w][i], y[i]);
+                        y[i] = fmaf(ldexpf(fmaf(x[i], back, bias[i]), by), weight[w][i], y[i]);
                 }
                 if (alone) {
                     const int channel = g * GS + (lane & 15) * kTiles + d % kTiles;

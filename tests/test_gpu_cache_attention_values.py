@@ -209,3 +209,17 @@ def test_large_scores(ctx, size, bits, dt):
     ulp = 2.0 ** -8 if dt == "bf16" else 2.0 ** -11
     assert ((lse - want_lse) / want_lse).abs().max() < 1e-4
     assert ((y - want_y).abs() <= ulp * want_y.abs() + 2.0 ** -18 * v.abs().max()).all()
+
+
+@pytest.mark.parametrize("dim,gs", [(64, 32), (128, 64), (256, 32)])
+@pytest.mark.parametrize("power", [-50, -28, 28, 50])
+def test_groups_of_very_different_size(ctx, power, dim, gs):
+    """The values of every other group are 2^power times their neighbours'."""
+    heads, rows, n, bits = 2, 4, 333, 4
+    q = (1.5 * normal(10, rows, heads, dim)).bfloat16()
+    k = normal(11, 1, heads, n, dim).bfloat16()
+    v = normal(12, 1, heads, n, dim).unflatten(-1, (-1, gs))
+    v[..., 1::2, :] *= 2.0 ** power
+    c = One(q, arrays_of(k, bits, gs), arrays_of(v.flatten(-2).bfloat16(), bits, gs), bits, gs)
+    announce(f"attention groups apart by 2^{power} dim={dim} gs={gs}")
+    c.check(*c.run(ctx))
