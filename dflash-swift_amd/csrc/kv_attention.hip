@@ -389,9 +389,13 @@ struct Attention {
                 const int tok = t + i * kEach + row;
                 a -= (uint32_t)(tok < n ? 0 : tok - n + 1) * kRowBytes;
             }
-            __asm__ volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-                             :: "v"(a), "s"(base),
-                                "s"(__builtin_amdgcn_readfirstlane(lds + i * 1024)) : "memory");
+            uint32_t m0;   /* the compiler's own, which no clobber list can name */
+            __asm__ volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\t"
+                             "global_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                             : "=&s"(m0)
+                             : "v"(a), "s"(base),
+                               "s"(__builtin_amdgcn_readfirstlane(lds + i * 1024))
+                             : "memory");
         }
     }
 
