@@ -26,7 +26,7 @@
  *
  * Measured and not taken: unpacking codes once a workgroup into fp16 tiles in LDS for up to 64 rows
  * (half the vector instructions, but a barrier a round and two waves a SIMD: 112 us where this took
- * 111); three and four row tiles (registers spill).
+ * 111); three and four row tiles (103 and 137 KB of LDS at heads of 128: a workgroup a CU).
  */
 #include <type_traits>
 
@@ -1130,7 +1130,10 @@ __device__ __forceinline__ void join(const KvAttnParams& p) {
 }  // namespace
 
 /* Built for the row tiles that attention_tiles (verify_ops.cpp) asks for; per_4 and per_8 are the
- * waves that a SIMD has registers and LDS for with 4 and 8 bits. */
+ * waves that a SIMD has registers and LDS for with 4 and 8 bits.  One kernel spills at them: heads of
+ * 64 with 4 bits in groups of 64, bf16, two tiles, 12 bytes a lane.  With two waves a SIMD it does not,
+ * and takes 363 us for 294 (32 sequences of 8 rows of 64 heads over 30000 shared tokens); nor with the
+ * rows' masks read again for each tile, 299. */
 #define DFQ_ATTN(bits, gs, name, f16, rt, per_simd)                                            \
     extern "C" __global__ __launch_bounds__(DFQ_KV_THREADS, per_simd) void                     \
         dfq_cache_attention_b##bits##_g##gs##_##name##_r##rt(KvAttnParams p) {                 \

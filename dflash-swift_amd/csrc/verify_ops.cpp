@@ -61,7 +61,7 @@ static dfq_status hip_error(hipError_t e, const char* what) {
  * codes once for both: 16 sequences of 8 rows of 40 heads over a shared 16384-token prefix take
  * 102 us, one tile 118.  At heads of 256 their outputs leave a CU room for one workgroup of two
  * tiles and two of one: 16 rows of 16 heads over 16000 tokens 44.8 us against 35.7, so there it
- * is one.  Three and four spill at any width. */
+ * is one.  Three and four would take 103 and 137 KB of LDS at heads of 128, a workgroup a CU. */
 static int attention_tiles(int dim) { return dim == 256 ? 1 : 2; }
 
 static dfq_status resolve(VerifyOps* o) {
