@@ -246,7 +246,6 @@ class Context:
         # replaces the old, which is kept (a graph or another stream may still hold it)
         self._ws = {}
         self._scratch = {}
-        self._need = ctypes.c_size_t()
         self._retired = []
 
     def close(self):
@@ -544,10 +543,11 @@ class Context:
             if st != _ERR_WORKSPACE or not again:
                 break
             # the scratch is as large as any call on the stream needed so far: ask, and grow it
+            need = ctypes.c_size_t()
             _check(self.lib.dfq_cache_attention_workspace_bytes(
-                self.handle, pd, prefix_length, cd, max_length, batch, rows, heads, self._need),
-                "dfq_cache_attention_workspace_bytes")
-            ws = self.workspace_uncleared(self._need.value, stream)
+                self.handle, pd, prefix_length, cd, max_length, batch, rows, heads,
+                ctypes.byref(need)), "dfq_cache_attention_workspace_bytes")
+            ws = self.workspace_uncleared(need.value, stream)
         if st:
             _check(st, "dfq_cache_attention")
         return out, lse
@@ -585,10 +585,11 @@ class Context:
                 ws.numel(), stream)
             if st != _ERR_WORKSPACE or not again:
                 break
+            need = ctypes.c_size_t()
             _check(self.lib.dfq_token_logprobs_workspace_bytes(self.handle, M, V, top_k,
-                                                               self._need),
+                                                               ctypes.byref(need)),
                    "dfq_token_logprobs_workspace_bytes")
-            ws = self.workspace_uncleared(self._need.value, stream)
+            ws = self.workspace_uncleared(need.value, stream)
         if st:
             _check(st, "dfq_token_logprobs")
         return lp, entropy, ids, top
