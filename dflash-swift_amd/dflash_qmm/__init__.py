@@ -19,8 +19,10 @@ raw integer device pointers.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
+import threading
 
 __all__ = [
     "BF16", "F16", "F32", "DfqError", "Context", "KVCache", "PackedWeight",
@@ -233,6 +235,9 @@ def dtype_code(t) -> int:
     return _dtype_codes[getattr(t, "dtype", t)]
 
 
+_no_lock = contextlib.nullcontext()
+
+
 class Context:
     """A dfq_ctx: the gfx950 code object loaded on one device."""
 
@@ -247,6 +252,9 @@ class Context:
         self._ws = {}
         self._scratch = {}
         self._retired = []
+        # held from taking one of them to the end of the call: the launches of two threads' calls
+        # on a stream (both on the default one, say) may not alternate over one workspace
+        self._lock = threading.RLock()
 
     def close(self):
         if self.handle:
@@ -360,11 +368,12 @@ class Context:
         if out is None:
             out = torch.empty((M, N), dtype=x.dtype, device=x.device)
         need = self.workspace_bytes(M, N, K, bits, gs)
-        if ws is None:
-            ws = self.workspace(need, stream)
-        self.qmm_raw(x, w, scales, biases, out, M, N, K, bits, gs, dt, dtype_code(scales), dt,
-                     lbias=lbias, ws=ws, ws_bytes=(ws.numel() if ws is not None else 0),
-                     stream=stream)
+        with self._lock if ws is None else _no_lock:
+            if ws is None:
+                ws = self.workspace(need, stream)
+            self.qmm_raw(x, w, scales, biases, out, M, N, K, bits, gs, dt, dtype_code(scales), dt,
+                         lbias=lbias, ws=ws, ws_bytes=(ws.numel() if ws is not None else 0),
+                         stream=stream)
         return out
 
     def qmm_silu_gate_up(self, x, w_gu, scales_gu, biases_gu, bits, gs, lbias=None, out=None,
@@ -379,12 +388,13 @@ class Context:
         if out is None:
             out = torch.empty((M, H), dtype=x.dtype, device=x.device)
         need = self.workspace_bytes(M, 2 * H, K, bits, gs)
-        if ws is None:
-            ws = self.workspace(need, stream)
-        _check(self.lib.dfq_qmm_silu_gate_up(
-            self.handle, _ptr(x), _ptr(w_gu), _ptr(scales_gu), _ptr(biases_gu), _ptr(lbias),
-            _ptr(out), M, H, K, bits, gs, dtype_code(x), _ptr(ws),
-            ws.numel() if ws is not None else 0, _stream(stream)), "dfq_qmm_silu_gate_up")
+        with self._lock if ws is None else _no_lock:
+            if ws is None:
+                ws = self.workspace(need, stream)
+            _check(self.lib.dfq_qmm_silu_gate_up(
+                self.handle, _ptr(x), _ptr(w_gu), _ptr(scales_gu), _ptr(biases_gu), _ptr(lbias),
+                _ptr(out), M, H, K, bits, gs, dtype_code(x), _ptr(ws),
+                ws.numel() if ws is not None else 0, _stream(stream)), "dfq_qmm_silu_gate_up")
         return out
 
     def interleave_gate_up(self, gate, up, stream=None):
@@ -533,21 +543,22 @@ class Context:
         cd = cache.desc if cache is not None else None
         stream = self._stream_of(stream)
         own_ws = ws is None
-        if own_ws:
-            ws = self.workspace_uncleared(1, stream)
-        for again in (own_ws, False):
-            st = self.lib.dfq_cache_attention(
-                self.handle, pd, prefix_length, cd, d_lengths, max_length, d_tree, q.data_ptr(),
-                _row_stride(q), out.data_ptr(), lse.data_ptr(), batch, rows, heads, scale,
-                ws.data_ptr(), ws.numel(), stream)
-            if st != _ERR_WORKSPACE or not again:
-                break
-            # the scratch is as large as any call on the stream needed so far: ask, and grow it
-            need = ctypes.c_size_t()
-            _check(self.lib.dfq_cache_attention_workspace_bytes(
-                self.handle, pd, prefix_length, cd, max_length, batch, rows, heads,
-                ctypes.byref(need)), "dfq_cache_attention_workspace_bytes")
-            ws = self.workspace_uncleared(need.value, stream)
+        with self._lock if own_ws else _no_lock:
+            if own_ws:
+                ws = self.workspace_uncleared(1, stream)
+            for again in (own_ws, False):
+                st = self.lib.dfq_cache_attention(
+                    self.handle, pd, prefix_length, cd, d_lengths, max_length, d_tree,
+                    q.data_ptr(), _row_stride(q), out.data_ptr(), lse.data_ptr(), batch, rows,
+                    heads, scale, ws.data_ptr(), ws.numel(), stream)
+                if st != _ERR_WORKSPACE or not again:
+                    break
+                # the scratch is as large as any call on the stream needed so far: ask, grow it
+                need = ctypes.c_size_t()
+                _check(self.lib.dfq_cache_attention_workspace_bytes(
+                    self.handle, pd, prefix_length, cd, max_length, batch, rows, heads,
+                    ctypes.byref(need)), "dfq_cache_attention_workspace_bytes")
+                ws = self.workspace_uncleared(need.value, stream)
         if st:
             _check(st, "dfq_cache_attention")
         return out, lse
@@ -575,21 +586,22 @@ class Context:
             top = None
         stream = self._stream_of(stream)
         own_ws = ws is None
-        if own_ws:
-            ws = self.workspace_uncleared(1, stream)
-        for again in (own_ws, False):
-            st = self.lib.dfq_token_logprobs(
-                self.handle, logits.data_ptr(), logits.stride(0) if M > 1 else V, M, V,
-                dtype_code(logits), d_tokens, top_k, p + 4 * M if tokens is not None else None, p,
-                ids.data_ptr() if more else None, p + 8 * M if more else None, ws.data_ptr(),
-                ws.numel(), stream)
-            if st != _ERR_WORKSPACE or not again:
-                break
-            need = ctypes.c_size_t()
-            _check(self.lib.dfq_token_logprobs_workspace_bytes(self.handle, M, V, top_k,
-                                                               ctypes.byref(need)),
-                   "dfq_token_logprobs_workspace_bytes")
-            ws = self.workspace_uncleared(need.value, stream)
+        with self._lock if own_ws else _no_lock:
+            if own_ws:
+                ws = self.workspace_uncleared(1, stream)
+            for again in (own_ws, False):
+                st = self.lib.dfq_token_logprobs(
+                    self.handle, logits.data_ptr(), logits.stride(0) if M > 1 else V, M, V,
+                    dtype_code(logits), d_tokens, top_k,
+                    p + 4 * M if tokens is not None else None, p, ids.data_ptr() if more else None,
+                    p + 8 * M if more else None, ws.data_ptr(), ws.numel(), stream)
+                if st != _ERR_WORKSPACE or not again:
+                    break
+                need = ctypes.c_size_t()
+                _check(self.lib.dfq_token_logprobs_workspace_bytes(self.handle, M, V, top_k,
+                                                                   ctypes.byref(need)),
+                       "dfq_token_logprobs_workspace_bytes")
+                ws = self.workspace_uncleared(need.value, stream)
         if st:
             _check(st, "dfq_token_logprobs")
         return lp, entropy, ids, top
@@ -642,10 +654,11 @@ class Context:
         M = x.shape[0]
         if out is None:
             out = torch.empty((M, pw.N), dtype=x.dtype, device=x.device)
-        if ws is None:
-            ws = self.workspace(self.workspace_bytes(M, pw.N, pw.K, pw.bits, pw.gs), stream)
-        self.qmm_packed_raw(x, pw, out, M, lbias=lbias, ws=ws,
-                            ws_bytes=ws.numel() if ws is not None else 0, stream=stream)
+        with self._lock if ws is None else _no_lock:
+            if ws is None:
+                ws = self.workspace(self.workspace_bytes(M, pw.N, pw.K, pw.bits, pw.gs), stream)
+            self.qmm_packed_raw(x, pw, out, M, lbias=lbias, ws=ws,
+                                ws_bytes=ws.numel() if ws is not None else 0, stream=stream)
         return out
 
     def qmm_silu_gate_up_packed(self, x, pw, lbias=None, out=None, ws=None, stream=None):
@@ -655,12 +668,13 @@ class Context:
         H = pw.N // 2
         if out is None:
             out = torch.empty((M, H), dtype=x.dtype, device=x.device)
-        if ws is None:
-            ws = self.workspace(self.workspace_bytes(M, pw.N, K, pw.bits, pw.gs), stream)
-        _check(self.lib.dfq_qmm_silu_gate_up_packed(
-            self.handle, _ptr(x), _ptr(pw.data), _ptr(lbias), _ptr(out), M, H, K, pw.bits,
-            pw.gs, pw.dtype, _ptr(ws), ws.numel() if ws is not None else 0, _stream(stream)),
-            "dfq_qmm_silu_gate_up_packed")
+        with self._lock if ws is None else _no_lock:
+            if ws is None:
+                ws = self.workspace(self.workspace_bytes(M, pw.N, K, pw.bits, pw.gs), stream)
+            _check(self.lib.dfq_qmm_silu_gate_up_packed(
+                self.handle, _ptr(x), _ptr(pw.data), _ptr(lbias), _ptr(out), M, H, K, pw.bits,
+                pw.gs, pw.dtype, _ptr(ws), ws.numel() if ws is not None else 0, _stream(stream)),
+                "dfq_qmm_silu_gate_up_packed")
         return out
 
     def qmm_argmax_accept_packed(self, x, pw, proposals=None, lbias=None, logits=None,
@@ -903,12 +917,13 @@ class QuantizedLinear:
         nb = ctypes.c_size_t()
         _check(self.lib.dfq_linear_workspace_bytes(self._h, rows, ctypes.byref(nb)),
                "dfq_linear_workspace_bytes")
-        ws = self.ctx.workspace(nb.value, stream)
         took = ctypes.c_int(0)
-        _check(self.lib.dfq_linear_forward(
-            self._h, _ptr(flat), dtype_code(x), rows, _ptr(y), _ptr(ws),
-            ws.numel() if ws is not None else 0, _stream(stream), ctypes.byref(took)),
-            "dfq_linear_forward")
+        with self.ctx._lock:
+            ws = self.ctx.workspace(nb.value, stream)
+            _check(self.lib.dfq_linear_forward(
+                self._h, _ptr(flat), dtype_code(x), rows, _ptr(y), _ptr(ws),
+                ws.numel() if ws is not None else 0, _stream(stream), ctypes.byref(took)),
+                "dfq_linear_forward")
         self.last_took_kernel = bool(took.value)
         return y.reshape(*lead, self.out_features)
 

@@ -35,6 +35,12 @@ class Fake:
     def is_contiguous(self):
         return True
 
+    def contiguous(self):
+        return self
+
+    def reshape(self, *shape):
+        return Fake(shape, self.dtype, self.device, self.address)
+
     def element_size(self):
         return torch.empty(0, dtype=self.dtype).element_size()
 
@@ -57,7 +63,7 @@ class Library:
             return b"recorded"
         self.calls.append((name, args))
         if name.endswith("workspace_bytes"):
-            rows = args[1] if name == "dfq_token_logprobs_workspace_bytes" else args[6]
+            rows = args[6] if name.startswith("dfq_cache") else args[1]
             n = getattr(args[-1], "_obj", args[-1])
             n.value = self.need(rows)
             self.during(name, args)
@@ -114,3 +120,58 @@ def test_threads_growing_their_workspaces_do_not_see_each_others_size(lib):
     in_threads(lambda: ctx.token_logprobs(Fake((5, 8)), stream=1),
                lambda: ctx.token_logprobs(Fake((2, 8)), stream=2))
     assert ctx._scratch[1].numel() == 5 << 20 and ctx._scratch[2].numel() == 2 << 20
+
+
+def cache(device="cuda:0"):
+    """A cache of one slot of one head of 64, capacity 64, 4 bits in groups of 64."""
+    codes, rest = (1, 1, 64, 8), (1, 1, 64, 1)
+    a = lambda at: (Fake(codes, torch.int32, device, at), Fake(rest, device=device),  # noqa: E731
+                    Fake(rest, device=device))
+    return dflash_qmm.KVCache.from_arrays(a(1 << 21), a(1 << 22), 4, 64)
+
+
+def packed():
+    return dflash_qmm.PackedWeight(Fake((64,), torch.uint8), 64, 512, 4, 64, 0)
+
+
+def linear(ctx):
+    return dflash_qmm.QuantizedLinear(ctx, Fake((64, 64), torch.int32), Fake((64, 8)),
+                                      Fake((64, 8)), _handle=1)
+
+
+# name -> a call with a workspace of the context's
+SHARED = {
+    "token_logprobs": lambda ctx: ctx.token_logprobs(Fake((5, 8)), stream=1),
+    "cache_attention": lambda ctx: ctx.cache_attention(Fake((1, 1, 64)), cache(), stream=1),
+    "qmm": lambda ctx: ctx.qmm(Fake((2, 512)), Fake((64, 64)), Fake((64, 8)), Fake((64, 8)), 4, 64,
+                               stream=1),
+    "qmm_silu_gate_up": lambda ctx: ctx.qmm_silu_gate_up(
+        Fake((2, 512)), Fake((64, 64)), Fake((64, 8)), Fake((64, 8)), 4, 64, stream=1),
+    "linear_forward": lambda ctx: linear(ctx)(Fake((2, 512)), stream=1),
+    "qmm_packed": lambda ctx: ctx.qmm_packed(Fake((2, 512)), packed(), stream=1),
+    "qmm_silu_gate_up_packed": lambda ctx: ctx.qmm_silu_gate_up_packed(Fake((2, 512)), packed(),
+                                                                       stream=1),
+}
+
+
+@pytest.mark.parametrize("first", sorted(SHARED))
+def test_calls_on_one_stream_do_not_share_a_workspace_at_once(lib, first):
+    """A call makes several launches that meet in the workspace; another thread's on the same
+    stream may come before or after all of them, not between."""
+    ctx = dflash_qmm.Context(0)
+    lib.need = lambda rows: 1 << 20
+    state = {"inside": set(), "met": []}
+
+    def during(name, args):
+        # the addresses of the context's workspaces in the call
+        known = {t.data_ptr() for d in (ctx._ws, ctx._scratch) for t in d.values()}
+        mine = known & {a for a in args if isinstance(a, int)}
+        if name.endswith("bytes") or not mine:
+            return
+        state["met"] += [name] if mine & state["inside"] else []
+        state["inside"] |= mine
+        time.sleep(0.05)
+        state["inside"] -= mine
+    lib.during = during
+    in_threads(*[lambda: SHARED[first](ctx)] * 2)
+    assert not state["met"] and any(name == "dfq_" + first for name, _ in lib.calls)
