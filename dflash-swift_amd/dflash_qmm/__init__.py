@@ -482,6 +482,9 @@ class Context:
         """The values (k, v) [batch, rows, heads, head_dim] of a span of `cache`, in its dtype
         or fp32; batch defaults to that of starts, else to all slots."""
         import torch
+        if stream is not None and self._is_other(stream):
+            with self._current(stream):
+                return self.cache_read(cache, rows, start, starts, batch, dtype, k, v)
         if batch is None:
             batch = cache.slots if starts is None else starts.shape[0]
         dt = cache.dtype if dtype is None else dtype
@@ -512,6 +515,10 @@ class Context:
         prefix's capacity, scale to head_dim ** -0.5.  tree [batch, rows] int32 holds the rows
         of the block that each row sees (bit j: row j); without it the block is a chain."""
         import torch
+        if stream is not None and self._is_other(stream):
+            with self._current(stream):
+                return self.cache_attention(q, cache, lengths, max_length, prefix, prefix_length,
+                                            tree, scale, out, lse, ws)
         fmt = cache if cache is not None else prefix
         if fmt is None:
             raise ValueError("cache_attention needs a cache or a prefix")
@@ -567,6 +574,9 @@ class Context:
         """(logprobs [M], entropy [M], top_tokens [M, top_k], top_logprobs [M, top_k]) of logits
         [M, V] (rows may be strided) and tokens [M] int32; what is not asked for is None."""
         import torch
+        if stream is not None and self._is_other(stream):
+            with self._current(stream):
+                return self.token_logprobs(logits, tokens, top_k, ws)
         if logits.dim() != 2 or logits.stride(1) != 1:
             raise ValueError("logits are [M, V] with contiguous rows")
         M, V = logits.shape
@@ -605,6 +615,18 @@ class Context:
         if st:
             _check(st, "dfq_token_logprobs")
         return lp, entropy, ids, top
+
+    def _is_other(self, stream) -> bool:
+        return (_stream(stream) or 0) != _current_stream(self.device)
+
+    def _current(self, stream):
+        """torch.cuda.stream of a launch's stream: what the call allocates is that stream's, so that
+        neither work queued on torch's current one still uses the memory, nor, dropped early, is
+        it the current one's next allocation while the launch has still to write it."""
+        import torch
+        handle = _stream(stream)
+        return torch.cuda.stream(torch.cuda.ExternalStream(handle, device=self.device) if handle
+                                 else torch.cuda.default_stream(self.device))
 
     def _stream_of(self, stream):
         """A stream's handle: the one given, or torch's current one on this context's device."""

@@ -42,7 +42,7 @@ class Fake:
         return Fake(shape, self.dtype, self.device, self.address)
 
     def element_size(self):
-        return torch.empty(0, dtype=self.dtype).element_size()
+        return self.dtype.itemsize
 
 
 class Library:
@@ -76,6 +76,19 @@ class Library:
         return 0
 
 
+class Stream:
+    """Enters as torch.cuda.stream's context manager does."""
+
+    def __init__(self, lib, handle):
+        self.lib, self.cuda_stream = lib, handle
+
+    def __enter__(self):
+        self.before, self.lib.current = self.lib.current, self.cuda_stream
+
+    def __exit__(self, *args):
+        self.lib.current = self.before
+
+
 @pytest.fixture
 def lib(monkeypatch):
     """The recording library, with outputs in host memory and stream 0 current."""
@@ -90,6 +103,10 @@ def lib(monkeypatch):
         fake.calls.append(("allocate", (t.data_ptr(), fake.current)))
         return t
     monkeypatch.setattr(torch, "empty", allocate)
+    monkeypatch.setattr(torch.cuda, "ExternalStream",
+                        lambda handle, device=None: Stream(fake, handle))
+    monkeypatch.setattr(torch.cuda, "default_stream", lambda device=None: Stream(fake, 0))
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: s)
     return fake
 
 
@@ -175,3 +192,28 @@ def test_calls_on_one_stream_do_not_share_a_workspace_at_once(lib, first):
     lib.during = during
     in_threads(*[lambda: SHARED[first](ctx)] * 2)
     assert not state["met"] and any(name == "dfq_" + first for name, _ in lib.calls)
+
+
+LAUNCHES = {
+    "dfq_token_logprobs": lambda ctx, **kw: ctx.token_logprobs(
+        Fake((5, 8)), Fake((5,), torch.int32), top_k=3, **kw),
+    "dfq_cache_attention": lambda ctx, **kw: ctx.cache_attention(Fake((1, 1, 64)), cache(), **kw),
+    "dfq_cache_read": lambda ctx, **kw: ctx.cache_read(cache(), 2, **kw),
+}
+
+
+@pytest.mark.parametrize("name", sorted(LAUNCHES))
+@pytest.mark.parametrize("form", ["handle", "stream", "default"])
+def test_outputs_and_workspaces_belong_to_the_stream_of_the_launch(lib, name, form):
+    """What a call allocates on another stream than the current one may be dropped, and be the
+    current stream's next allocation, while the launch has still to write it."""
+    ctx = dflash_qmm.Context(0)
+    lib.need = lambda rows: 3 << 20
+    lib.current, launch = (9, 0) if form == "default" else (0, 7)
+    given = Stream(lib, 7) if form == "stream" else launch
+    before = lib.current
+    outputs = LAUNCHES[name](ctx, stream=given)
+    assert lib.current == before and outputs
+    made = [args[1] for what, args in lib.calls if what == "allocate"]
+    assert made and set(made) == {launch}
+    assert [args[-1] or 0 for what, args in lib.calls if what == name][-1] == launch
