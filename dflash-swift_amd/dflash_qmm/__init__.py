@@ -471,6 +471,7 @@ class Context:
             raise ValueError("k and v must have the same strides")
         if k.dtype != cache.dtype or v.dtype != cache.dtype:
             raise ValueError(f"the cache holds {cache.dtype}")
+        self._check_here(cache, k, v, starts)
         st = self.lib.dfq_cache_append(
             self.handle, cache.desc, k.data_ptr(), v.data_ptr(), stride, shape[0], shape[1], start,
             _check_int32("starts", starts, shape[:1]), self._stream_of(stream))
@@ -492,6 +493,7 @@ class Context:
         for a in (k, v):
             if a is not None and (a.shape != shape or a.dtype != dt or not a.is_contiguous()):
                 raise ValueError(f"outputs are contiguous {shape} of {dt}")
+        self._check_here(cache, k, v, starts)
         if k is None:
             k = torch.empty(shape, dtype=dt, device=cache.device)
         if v is None:
@@ -510,6 +512,7 @@ class Context:
         sequences' own caches (dfq_cache_attention): y [batch, rows, q_heads*head_dim] in q's
         dtype, lse fp32 [batch, rows, q_heads].
 
+        All arrays are on this context's GPU.
         lengths [batch] int32 counts each sequence's own tokens, the block's rows included;
         max_length bounds them (the capacity when left out).  prefix_length defaults to the
         prefix's capacity, scale to head_dim ** -0.5.  tree [batch, rows] int32 holds the rows
@@ -529,6 +532,7 @@ class Context:
         heads = width // fmt.head_dim
         if q.dtype != fmt.dtype:
             raise ValueError(f"the cache holds {fmt.dtype}, got {q.dtype}")
+        self._check_here(cache, prefix, q, lengths, tree, out, lse, ws)
         d_lengths = _check_int32("lengths", lengths, (batch,))
         d_tree = _check_int32("tree", tree, (batch, rows))
         if max_length is None:
@@ -580,6 +584,7 @@ class Context:
         if logits.dim() != 2 or logits.stride(1) != 1:
             raise ValueError("logits are [M, V] with contiguous rows")
         M, V = logits.shape
+        self._check_here(logits, tokens, ws)
         d_tokens = _check_int32("tokens", tokens, (M,))
         # the fp32 outputs of one allocation, as wide as they are asked for
         more = top_k if top_k > 0 else 0
@@ -615,6 +620,13 @@ class Context:
         if st:
             _check(st, "dfq_token_logprobs")
         return lp, entropy, ids, top
+
+    def _check_here(self, *arrays):
+        """Refuses tensors and caches (or None) that are not on this context's GPU: a kernel
+        would take a host address for one of its own."""
+        for a in arrays:
+            if a is not None and a.get_device() != self.device:
+                raise ValueError(f"all arrays are on cuda:{self.device}, got one on {a.device}")
 
     def _is_other(self, stream) -> bool:
         return (_stream(stream) or 0) != _current_stream(self.device)
@@ -827,9 +839,16 @@ class KVCache:
                         a.dtype != self.dtype for a in (scales, biases)) or \
                     not all(a.is_contiguous() for a in (codes, scales, biases)):
                 raise ValueError("the cache's arrays do not agree in shape and dtype")
+            if any(a.device != self.device for a in (codes, scales, biases)):
+                raise ValueError("the cache's arrays are on one device")
         d = _KVCacheDesc(*(a.data_ptr() for a in (*k, *v)), self.slots, self.heads,
                          self.capacity, self.head_dim, bits, group_size, dtype_code(self.dtype))
         self._desc, self.desc = d, ctypes.addressof(d)
+        self._index = k[0].get_device()
+
+    def get_device(self) -> int:
+        """The GPU's index; -1 for a cache in host memory, which no call takes."""
+        return self._index
 
 
 class PackedWeight:

@@ -35,6 +35,9 @@ class Fake:
     def is_contiguous(self):
         return True
 
+    def get_device(self):
+        return self.device.index if self.is_cuda else -1
+
     def contiguous(self):
         return self
 
@@ -217,3 +220,47 @@ def test_outputs_and_workspaces_belong_to_the_stream_of_the_launch(lib, name, fo
     made = [args[1] for what, args in lib.calls if what == "allocate"]
     assert made and set(made) == {launch}
     assert [args[-1] or 0 for what, args in lib.calls if what == name][-1] == launch
+
+
+def ints(*shape, device="cuda:0"):
+    return Fake(shape, torch.int32, device)
+
+
+# call, and its arrays by name with a maker of each for a device
+TAKES = {
+    "cache_append": (lambda ctx, **a: ctx.cache_append(a.pop("cache"), a.pop("k"), a.pop("v"), **a), {
+        "cache": cache, "k": lambda d: Fake((1, 2, 64), device=d),
+        "v": lambda d: Fake((1, 2, 64), device=d), "starts": lambda d: ints(1, device=d)}),
+    "cache_read": (lambda ctx, **a: ctx.cache_read(a.pop("cache"), 2, **a), {
+        "cache": cache, "starts": lambda d: ints(1, device=d),
+        "k": lambda d: Fake((1, 2, 1, 64), device=d), "v": lambda d: Fake((1, 2, 1, 64), device=d)}),
+    "cache_attention": (lambda ctx, **a: ctx.cache_attention(**a), {
+        "q": lambda d: Fake((1, 2, 64), device=d), "cache": cache, "prefix": cache,
+        "lengths": lambda d: ints(1, device=d), "tree": lambda d: ints(1, 2, device=d),
+        "out": lambda d: Fake((1, 2, 64), device=d),
+        "lse": lambda d: Fake((1, 2, 1), torch.float32, d)}),
+    "token_logprobs": (lambda ctx, **a: ctx.token_logprobs(**a), {
+        "logits": lambda d: Fake((3, 9), device=d), "tokens": lambda d: ints(3, device=d)}),
+}
+
+
+@pytest.mark.parametrize("name", sorted(TAKES))
+@pytest.mark.parametrize("where", ["cpu", "cuda:1"])
+def test_arrays_that_are_not_on_the_gpu_are_refused(lib, name, where):
+    """Each array of each call in host memory, or on another GPU: an error, and nothing is called."""
+    ctx = dflash_qmm.Context(0)
+    call, takes = TAKES[name]
+    call(ctx, **{k: make("cuda:0") for k, make in takes.items()})
+    assert any(what == "dfq_" + name for what, _ in lib.calls)
+    for bad in takes:
+        lib.calls.clear()
+        with pytest.raises(ValueError):
+            call(ctx, **{k: make(where if k == bad else "cuda:0") for k, make in takes.items()})
+        assert not any(what.startswith("dfq_") for what, _ in lib.calls), bad
+
+
+def test_a_cache_lies_on_one_device():
+    part = (Fake((1, 1, 64, 8), torch.int32), Fake((1, 1, 64, 1)), Fake((1, 1, 64, 1)))
+    other = (part[0], part[1], Fake((1, 1, 64, 1), device="cpu"))
+    with pytest.raises(ValueError):
+        dflash_qmm.KVCache.from_arrays(part, other, 4, 64)
