@@ -472,6 +472,7 @@ class Context:
         if k.dtype != cache.dtype or v.dtype != cache.dtype:
             raise ValueError(f"the cache holds {cache.dtype}")
         self._check_here(cache, k, v, starts)
+        _check_ints(shape[0], shape[1], start)
         st = self.lib.dfq_cache_append(
             self.handle, cache.desc, k.data_ptr(), v.data_ptr(), stride, shape[0], shape[1], start,
             _check_int32("starts", starts, shape[:1]), self._stream_of(stream))
@@ -488,6 +489,7 @@ class Context:
                 return self.cache_read(cache, rows, start, starts, batch, dtype, k, v)
         if batch is None:
             batch = cache.slots if starts is None else starts.shape[0]
+        _check_ints(batch, rows, start)
         dt = cache.dtype if dtype is None else dtype
         shape = (batch, rows, cache.heads, cache.head_dim)
         for a in (k, v):
@@ -539,6 +541,7 @@ class Context:
             max_length = cache.capacity if cache is not None else 0
         if prefix_length is None:
             prefix_length = prefix.capacity if prefix is not None else 0
+        _check_ints(batch, rows, max_length, prefix_length)
         if scale is None:
             scale = fmt.head_dim ** -0.5
         if out is None:
@@ -585,6 +588,7 @@ class Context:
             raise ValueError("logits are [M, V] with contiguous rows")
         M, V = logits.shape
         self._check_here(logits, tokens, ws)
+        _check_ints(M, V, top_k)
         d_tokens = _check_int32("tokens", tokens, (M,))
         # the fp32 outputs of one allocation, as wide as they are asked for
         more = top_k if top_k > 0 else 0
@@ -792,6 +796,13 @@ def _row_stride(t) -> int:
     return stride
 
 
+def _check_ints(*values):
+    """Refuses what a C int does not hold: ctypes would pass its low 32 bits."""
+    for v in values:
+        if not -0x80000000 <= v <= 0x7fffffff:
+            raise ValueError(f"{v} is out of range")
+
+
 def _check_int32(name, t, shape):
     if t is None:
         return None
@@ -830,6 +841,7 @@ class KVCache:
     def _set(self, k, v, bits, group_size):
         self.k, self.v, self.bits, self.group_size = k, v, bits, group_size
         self.slots, self.heads, self.capacity, words = k[0].shape
+        _check_ints(self.slots, self.heads, self.capacity)
         self.head_dim = words * 32 // bits
         self.dtype, self.device = k[1].dtype, k[0].device
         lead = (self.slots, self.heads, self.capacity)

@@ -264,3 +264,33 @@ def test_a_cache_lies_on_one_device():
     other = (part[0], part[1], Fake((1, 1, 64, 1), device="cpu"))
     with pytest.raises(ValueError):
         dflash_qmm.KVCache.from_arrays(part, other, 4, 64)
+
+
+BIG = 1 << 32
+OUT_OF_RANGE = {
+    "start of an append": lambda ctx: ctx.cache_append(cache(), Fake((1, 1, 64)), Fake((1, 1, 64)),
+                                                       start=BIG),
+    "rows of an append": lambda ctx: ctx.cache_append(cache(), Fake((1, BIG + 1, 64)),
+                                                      Fake((1, BIG + 1, 64))),
+    "start of a read": lambda ctx: ctx.cache_read(cache(), 1, start=-BIG),
+    "rows of a read": lambda ctx: ctx.cache_read(cache(), BIG + 1, k=Fake((1, BIG + 1, 1, 64)),
+                                                 v=Fake((1, BIG + 1, 1, 64))),
+    "max_length": lambda ctx: ctx.cache_attention(Fake((1, 1, 64)), cache(), max_length=BIG + 5),
+    "prefix_length": lambda ctx: ctx.cache_attention(Fake((1, 1, 64)), prefix=cache(),
+                                                     prefix_length=BIG),
+    "vocabulary": lambda ctx: ctx.token_logprobs(Fake((1, BIG + 7))),
+    "rows of logits": lambda ctx: ctx.token_logprobs(Fake((BIG, 7))),
+    "alternatives": lambda ctx: ctx.token_logprobs(Fake((1, 7)), top_k=BIG + 1),
+    "capacity": lambda ctx: dflash_qmm.KVCache.from_arrays(
+        *[(Fake((1, 1, BIG + 64, 8), torch.int32), *[Fake((1, 1, BIG + 64, 1))] * 2)] * 2, 4, 64),
+}
+
+
+@pytest.mark.parametrize("name", sorted(OUT_OF_RANGE))
+def test_numbers_that_a_c_int_does_not_hold_are_refused(lib, monkeypatch, name):
+    """Not taken modulo 2^32: a start of 2^32 would write position 0."""
+    monkeypatch.setattr(torch, "empty", lambda *shape, **kw: pytest.fail("allocated"))
+    ctx = dflash_qmm.Context(0)
+    with pytest.raises(ValueError):
+        OUT_OF_RANGE[name](ctx)
+    assert not any(what == "dfq_cache_append" for what, _ in lib.calls)
