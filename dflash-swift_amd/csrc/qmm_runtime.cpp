@@ -8,6 +8,7 @@
 #include <hip/hip_runtime_api.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -151,7 +152,8 @@ struct dfq_ctx {
     hipFunction_t read_stream = nullptr; // the plain streaming read (bandwidth reference)
     hipFunction_t read_units = nullptr;  // the fast kernel's own loads with no compute
     hipFunction_t read_units_packed = nullptr;  // the same over the packed layout
-    dfq::VerifyOps* verify = nullptr;    // cache, attention and log-probability kernels
+    std::atomic<dfq::VerifyOps*> verify{nullptr};  // cache, attention, log probabilities
+    std::mutex verify_mu;                // held while they are loaded
     void* scratch = nullptr;             // the fixed scratch of dfq_qmm_noalloc (this device)
     std::mutex mu;
     std::unordered_map<PlanKey, dfq::Plan, PlanKeyHash> plans;
@@ -203,7 +205,24 @@ struct DeviceGuard {
 
 int ctx_device(const dfq_ctx* ctx) { return ctx->device; }
 
-VerifyOps* ctx_verify_ops(const dfq_ctx* ctx) { return ctx->verify; }
+dfq_status ctx_verify_ops(dfq_ctx* ctx, const VerifyOps** out) {
+    VerifyOps* ops = ctx->verify.load(std::memory_order_acquire);
+    if (!ops) {
+        std::lock_guard<std::mutex> lock(ctx->verify_mu);
+        if (!(ops = ctx->verify.load(std::memory_order_relaxed))) {
+            DeviceGuard g(ctx->device);
+            /* the first call may be one that a graph captures; loading is no part of the graph */
+            hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+            const hipError_t e = hipThreadExchangeStreamCaptureMode(&mode);
+            const dfq_status st = verify_ops_load(&ops);
+            if (e == hipSuccess) (void)hipThreadExchangeStreamCaptureMode(&mode);
+            if (st != DFQ_OK) return st;
+            ctx->verify.store(ops, std::memory_order_release);
+        }
+    }
+    *out = ops;
+    return DFQ_OK;
+}
 
 DeviceScope::DeviceScope(const dfq_ctx* ctx) : dev_(ctx_device(ctx)) {
     if (hipGetDevice(&prev_) != hipSuccess) prev_ = -1;
@@ -721,10 +740,8 @@ dfq_status dfq_init(int device, dfq_ctx** out) {
         return hip_fail(e, "hipModuleGetFunction");
     }
     dfq_status st = load_gemm(ctx);
-    if (st == DFQ_OK) st = verify_ops_load(&ctx->verify);
     if (st == DFQ_OK) st = scratch_setup(device, &ctx->scratch);
     if (st != DFQ_OK) {
-        verify_ops_unload(ctx->verify);
         if (ctx->gemm_module) (void)hipModuleUnload(ctx->gemm_module);
         (void)hipModuleUnload(ctx->module);
         delete ctx;
@@ -738,7 +755,7 @@ dfq_status dfq_destroy(dfq_ctx* ctx) {
     if (!ctx) return DFQ_OK;
     {
         DeviceGuard g(ctx->device);
-        verify_ops_unload(ctx->verify);
+        verify_ops_unload(ctx->verify.load());
         if (ctx->gemm_module) (void)hipModuleUnload(ctx->gemm_module);
         if (ctx->module) (void)hipModuleUnload(ctx->module);
     }

@@ -203,9 +203,9 @@ dfq_status check_span(const dfq_kv_cache* c, int batch, int rows) {
     return DFQ_OK;
 }
 
-const CacheKernels& kernels_of(const dfq_ctx* ctx, const dfq_kv_cache* c) {
-    return ctx_verify_ops(ctx)->cache[dim_index(c->head_dim)][c->bits == 8]
-                                     [group_index(c->group_size)][c->dtype == DFQ_F16];
+const CacheKernels& kernels_of(const VerifyOps* ops, const dfq_kv_cache* c) {
+    return ops->cache[dim_index(c->head_dim)][c->bits == 8][group_index(c->group_size)]
+                     [c->dtype == DFQ_F16];
 }
 
 KvArrays arrays_of(const dfq_kv_cache* c, bool v) {
@@ -324,8 +324,8 @@ struct Card {
     }
 };
 
-AttentionPlan plan_attention(dfq_ctx* ctx, const dfq_kv_cache* fmt, int prefix_length,
-                             int max_length, int batch, int rows, int q_heads) {
+AttentionPlan plan_attention(int cus, const CacheKernels& kernels, const dfq_kv_cache* fmt,
+                             int prefix_length, int max_length, int batch, int rows, int q_heads) {
     AttentionPlan a;
     const int group = q_heads / fmt->heads;
     const int64_t own_rows = (int64_t)rows * group, all_rows = own_rows * batch;
@@ -337,7 +337,7 @@ AttentionPlan plan_attention(dfq_ctx* ctx, const dfq_kv_cache* fmt, int prefix_l
                                        ((prefix_length ? all_rows : own_rows) + 15) / 16);
     double best = 0;
     for (int tiles = 1; tiles <= most; ++tiles) {
-        const Card card = {dfq_num_cus(ctx), kernels_of(ctx, fmt).resident[tiles - 1]};
+        const Card card = {cus, kernels.resident[tiles - 1]};
         const int64_t pb = (all_rows + 16 * tiles - 1) / (16 * tiles);
         const int64_t ob = (own_rows + 16 * tiles - 1) / (16 * tiles);
         const int64_t pn = fmt->heads * pb, on = fmt->heads * ob * batch;
@@ -404,10 +404,12 @@ dfq_status dfq_cache_append(dfq_ctx* ctx, const dfq_kv_cache* cache, const void*
     KvAppendParams p{{arrays_of(cache, false), arrays_of(cache, true)},
                      {(const uint16_t*)k, (const uint16_t*)v}, starts, row_stride, start, rows,
                      cache->heads, cache->capacity};
+    const VerifyOps* ops;
+    if ((s = ctx_verify_ops(ctx, &ops))) return s;
     DeviceScope scope(ctx);
     void* args[] = {&p};
     const hipError_t e = hipModuleLaunchKernel(
-        kernels_of(ctx, cache).append, (unsigned)row_blocks(cache, rows), 1, (unsigned)batch,
+        kernels_of(ops, cache).append, (unsigned)row_blocks(cache, rows), 1, (unsigned)batch,
         DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
     return e == hipSuccess ? DFQ_OK : hip_error(e, "launch dfq_cache_append");
 }
@@ -426,10 +428,12 @@ dfq_status dfq_cache_read(dfq_ctx* ctx, const dfq_kv_cache* cache, void* k, void
     KvReadParams p{{arrays_of(cache, false), arrays_of(cache, true)}, {k, v}, starts, start, rows,
                    cache->heads, cache->capacity};
     int dt = (int)dtype;
+    const VerifyOps* ops;
+    if ((s = ctx_verify_ops(ctx, &ops))) return s;
     DeviceScope scope(ctx);
     void* args[] = {&p, &dt};
     const hipError_t e = hipModuleLaunchKernel(
-        kernels_of(ctx, cache).read, (unsigned)row_blocks(cache, rows), 1, 2u * batch,
+        kernels_of(ops, cache).read, (unsigned)row_blocks(cache, rows), 1, 2u * batch,
         DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
     return e == hipSuccess ? DFQ_OK : hip_error(e, "launch dfq_cache_read");
 }
@@ -444,8 +448,10 @@ dfq_status dfq_cache_attention_workspace_bytes(dfq_ctx* ctx, const dfq_kv_cache*
     const dfq_kv_cache* fmt;
     dfq_status s =
         check_attention(prefix, prefix_length, cache, max_length, batch, rows, q_heads, &fmt);
-    if (s) return s;
-    *bytes = plan_attention(ctx, fmt, prefix_length, max_length, batch, rows, q_heads)
+    const VerifyOps* ops;
+    if (s || (s = ctx_verify_ops(ctx, &ops))) return s;
+    *bytes = plan_attention(dfq_num_cus(ctx), kernels_of(ops, fmt), fmt, prefix_length, max_length,
+                            batch, rows, q_heads)
                  .bytes;
     return DFQ_OK;
 }
@@ -470,8 +476,11 @@ dfq_status dfq_cache_attention(dfq_ctx* ctx, const dfq_kv_cache* prefix, int pre
         return fail(DFQ_ERR_INVALID_ARGUMENT, "q_stride is smaller than a row");
     if (!(scale > 0.0f) || !std::isfinite(scale))
         return fail(DFQ_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
-    const AttentionPlan a =
-        plan_attention(ctx, fmt, prefix_length, max_length, batch, rows, q_heads);
+    const VerifyOps* ops;
+    if ((s = ctx_verify_ops(ctx, &ops))) return s;
+    const CacheKernels& fn = kernels_of(ops, fmt);
+    const AttentionPlan a = plan_attention(dfq_num_cus(ctx), fn, fmt, prefix_length, max_length,
+                                           batch, rows, q_heads);
     const int64_t groups = a.groups(fmt->heads, batch);
     const int group = q_heads / fmt->heads;
     if (groups > INT32_MAX || (int64_t)batch * rows * group > INT32_MAX)
@@ -512,7 +521,6 @@ dfq_status dfq_cache_attention(dfq_ctx* ctx, const dfq_kv_cache* prefix, int pre
      * a wave each 12.5) */
     p.join_rows = a.prefix_splits + a.own_splits <= 8 ? DFQ_KV_THREADS / 64 : 1;
     p.scale_log2e = scale * 1.44269504088896340736f;
-    const CacheKernels& fn = kernels_of(ctx, fmt);
     DeviceScope scope(ctx);
     void* args[] = {&p};
     hipError_t e = hipSuccess;
@@ -597,7 +605,8 @@ dfq_status dfq_token_logprobs(dfq_ctx* ctx, const void* logits, int64_t row_stri
                     (uint64_t*)workspace,
                     (float*)((char*)workspace + logprob_keys_bytes(M, splits, top_k)), row_stride,
                     M, V, top_k, splits};
-    const VerifyOps* ops = ctx_verify_ops(ctx);
+    const VerifyOps* ops;
+    if ((s = ctx_verify_ops(ctx, &ops))) return s;
     DeviceScope scope(ctx);
     void* args[] = {&p};
     hipError_t e = hipModuleLaunchKernel(ops->logprobs_part[(int)dtype], (unsigned)M * splits, 1,
