@@ -254,10 +254,9 @@ struct Attention {
      * stands apart from its group's others): 64 tokens with one of 64 channels off by 16 of their
      * 0.3, the others' errors were 9 (8 bits, 25) times the output's own rounding, and with p in
      * 16 bits still 2.  r comes in two fp16 parts, 22 bits.
-     * Where the middle b + centre s is more than twice the codes' half range (or s is 0), h would
-     * carry most of the value in a number that may be small beside the other groups'.  There r is
-     * -centre, codes count from the middle, which is no larger than the value, and the far middle
-     * meets p itself, both in two bf16 parts (16 bits).  The offset of a row's weights keeps p m
+     * Where the middle b + centre s is more than 128 times the codes' half range (or s is 0), r would
+     * pass fp16.  There r is -centre, codes count from the middle, which they change little, and the
+     * far middle meets p itself, both in two bf16 parts (16 bits).  The offset of a row's weights keeps p m
      * below 2^35 as it keeps h below 2^15: for it, a far middle counts as a scale of 2^-20 of it.
      * A V group whose scale or bias is not finite (or the middle of its range past bf16) counts as
      * a NaN scale and no bias: the rows that see it get NaN, and the others, whose weight is 0,
@@ -340,10 +339,10 @@ struct Attention {
     static __device__ __forceinline__ float log2_above(float size) {
         return fmaxf((float)((int)(__float_as_uint(size) >> 23) - 126), -64.0f);
     }
-    /* Whether a group's middle is within twice its codes' half range: false where the scale is 0
+    /* Whether a group's middle is within 128 times its codes' half range: false where the scale is 0
      * (or under 2^-100, whose reciprocal may not be finite), infinite or NaN. */
     static __device__ __forceinline__ bool is_near(float s, float b) {
-        return fabsf(fmaf(kCentre, s, b)) < fmaf(2.0f * kCentre, fabsf(s), -0x1p-100f);
+        return fabsf(fmaf(kCentre, s, b)) < fmaf(128.0f * kCentre, fabsf(s), -0x1p-100f);
     }
 
     /* A lane's 8 tokens of one array and group: 4 c + 0..3 of each half of the tile. */

@@ -100,15 +100,15 @@ def test_an_outlying_channel_spoils_no_other(ctx, offset, bits, gs, dim, dt):
 @pytest.mark.parametrize("dt", ["bf16", "f16"])
 @pytest.mark.parametrize("bits,gs,dim", [(4, 64, 128), (8, 32, 256)])
 def test_groups_far_from_zero(ctx, bits, gs, dim, dt):
-    """V whose groups lie near zero, at 3 and 40 times their half range from it, and on one value,
-    by token and group in turn."""
+    """V whose groups lie near zero, at 3, 40 and (bf16 holds two numbers there) 200 times their half
+    range from it, and on one value, by token and group in turn."""
     heads, rows, n = 2, 5, 300
     q = (1.5 * normal(4, rows, heads, dim)).to(DTYPES[dt])
     k = normal(5, 1, heads, n, dim).to(DTYPES[dt])
     v = normal(6, 1, heads, n, dim).clamp(-1, 1).unflatten(-1, (-1, gs))
-    at = torch.tensor([0.0, 3.0, -40.0, 5.0])
+    at = torch.tensor([0.0, 3.0, -40.0, 200.0, 5.0])
     kind = torch.arange(n)[:, None] * 3 + torch.arange(dim // gs)
-    v = torch.where((kind % 4 == 3)[..., None], 0.0, v) + at[kind % 4][..., None]
+    v = torch.where((kind % 5 == 4)[..., None], 0.0, v) + at[kind % 5][..., None]
     c = One(q, arrays_of(k, bits, gs), arrays_of(v.flatten(-2).to(DTYPES[dt]), bits, gs), bits, gs)
     announce(f"attention far groups bits={bits} gs={gs} dim={dim} {dt}")
     c.check(*c.run(ctx))
