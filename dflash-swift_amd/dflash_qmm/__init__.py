@@ -236,6 +236,7 @@ def dtype_code(t) -> int:
 
 
 _no_lock = contextlib.nullcontext()
+_INT_MAX = 0x7fffffff   # past it ctypes would pass a number's low 32 bits
 
 
 class Context:
@@ -471,8 +472,11 @@ class Context:
             raise ValueError("k and v must have the same strides")
         if k.dtype != cache.dtype or v.dtype != cache.dtype:
             raise ValueError(f"the cache holds {cache.dtype}")
-        self._check_here(cache, k, v, starts)
-        _check_ints(shape[0], shape[1], start)
+        if not (cache.index == k.get_device() == v.get_device() == self.device) or \
+                starts is not None and starts.get_device() != self.device:
+            self._elsewhere(cache.k[0], k, v, starts)
+        if max(shape[0], shape[1], start, -start) > _INT_MAX:
+            raise ValueError("batch, rows or start past a C int")
         st = self.lib.dfq_cache_append(
             self.handle, cache.desc, k.data_ptr(), v.data_ptr(), stride, shape[0], shape[1], start,
             _check_int32("starts", starts, shape[:1]), self._stream_of(stream))
@@ -489,13 +493,18 @@ class Context:
                 return self.cache_read(cache, rows, start, starts, batch, dtype, k, v)
         if batch is None:
             batch = cache.slots if starts is None else starts.shape[0]
-        _check_ints(batch, rows, start)
+        if max(batch, rows, start, -start) > _INT_MAX:
+            raise ValueError("batch, rows or start past a C int")
         dt = cache.dtype if dtype is None else dtype
         shape = (batch, rows, cache.heads, cache.head_dim)
         for a in (k, v):
             if a is not None and (a.shape != shape or a.dtype != dt or not a.is_contiguous()):
                 raise ValueError(f"outputs are contiguous {shape} of {dt}")
-        self._check_here(cache, k, v, starts)
+        if cache.index != self.device or \
+                starts is not None and starts.get_device() != self.device or \
+                k is not None and k.get_device() != self.device or \
+                v is not None and v.get_device() != self.device:
+            self._elsewhere(cache.k[0], k, v, starts)
         if k is None:
             k = torch.empty(shape, dtype=dt, device=cache.device)
         if v is None:
@@ -534,14 +543,23 @@ class Context:
         heads = width // fmt.head_dim
         if q.dtype != fmt.dtype:
             raise ValueError(f"the cache holds {fmt.dtype}, got {q.dtype}")
-        self._check_here(cache, prefix, q, lengths, tree, out, lse, ws)
+        device = self.device
+        if not (q.get_device() == fmt.index == device) or \
+                prefix is not None and prefix.index != device or \
+                lengths is not None and lengths.get_device() != device or \
+                tree is not None and tree.get_device() != device or \
+                out is not None and out.get_device() != device or \
+                lse is not None and lse.get_device() != device or \
+                ws is not None and ws.get_device() != device:
+            self._elsewhere(q, fmt.k[0], prefix and prefix.k[0], lengths, tree, out, lse, ws)
         d_lengths = _check_int32("lengths", lengths, (batch,))
         d_tree = _check_int32("tree", tree, (batch, rows))
         if max_length is None:
             max_length = cache.capacity if cache is not None else 0
         if prefix_length is None:
             prefix_length = prefix.capacity if prefix is not None else 0
-        _check_ints(batch, rows, max_length, prefix_length)
+        if max(batch, rows, max_length, prefix_length, -max_length, -prefix_length) > _INT_MAX:
+            raise ValueError("batch, rows or a length past a C int")
         if scale is None:
             scale = fmt.head_dim ** -0.5
         if out is None:
@@ -587,8 +605,12 @@ class Context:
         if logits.dim() != 2 or logits.stride(1) != 1:
             raise ValueError("logits are [M, V] with contiguous rows")
         M, V = logits.shape
-        self._check_here(logits, tokens, ws)
-        _check_ints(M, V, top_k)
+        if logits.get_device() != self.device or \
+                tokens is not None and tokens.get_device() != self.device or \
+                ws is not None and ws.get_device() != self.device:
+            self._elsewhere(logits, tokens, ws)
+        if max(M, V, top_k, -top_k) > _INT_MAX:
+            raise ValueError("M, V or top_k past a C int")
         d_tokens = _check_int32("tokens", tokens, (M,))
         # the fp32 outputs of one allocation, as wide as they are asked for
         more = top_k if top_k > 0 else 0
@@ -625,12 +647,11 @@ class Context:
             _check(st, "dfq_token_logprobs")
         return lp, entropy, ids, top
 
-    def _check_here(self, *arrays):
-        """Refuses tensors and caches (or None) that are not on this context's GPU: a kernel
-        would take a host address for one of its own."""
-        for a in arrays:
-            if a is not None and a.get_device() != self.device:
-                raise ValueError(f"all arrays are on cuda:{self.device}, got one on {a.device}")
+    def _elsewhere(self, *arrays):
+        """The refusal of tensors that are not on this context's GPU: a kernel would take a host
+        address for one of its own."""
+        where = {str(a.device) for a in arrays if a is not None}
+        raise ValueError(f"all arrays are on cuda:{self.device}, got {sorted(where)}")
 
     def _is_other(self, stream) -> bool:
         return (_stream(stream) or 0) != _current_stream(self.device)
@@ -796,13 +817,6 @@ def _row_stride(t) -> int:
     return stride
 
 
-def _check_ints(*values):
-    """Refuses what a C int does not hold: ctypes would pass its low 32 bits."""
-    for v in values:
-        if not -0x80000000 <= v <= 0x7fffffff:
-            raise ValueError(f"{v} is out of range")
-
-
 def _check_int32(name, t, shape):
     if t is None:
         return None
@@ -841,7 +855,8 @@ class KVCache:
     def _set(self, k, v, bits, group_size):
         self.k, self.v, self.bits, self.group_size = k, v, bits, group_size
         self.slots, self.heads, self.capacity, words = k[0].shape
-        _check_ints(self.slots, self.heads, self.capacity)
+        if max(self.slots, self.heads, self.capacity) > _INT_MAX:
+            raise ValueError("slots, heads or capacity past a C int")
         self.head_dim = words * 32 // bits
         self.dtype, self.device = k[1].dtype, k[0].device
         lead = (self.slots, self.heads, self.capacity)
@@ -856,11 +871,7 @@ class KVCache:
         d = _KVCacheDesc(*(a.data_ptr() for a in (*k, *v)), self.slots, self.heads,
                          self.capacity, self.head_dim, bits, group_size, dtype_code(self.dtype))
         self._desc, self.desc = d, ctypes.addressof(d)
-        self._index = k[0].get_device()
-
-    def get_device(self) -> int:
-        """The GPU's index; -1 for a cache in host memory, which no call takes."""
-        return self._index
+        self.index = k[0].get_device()   # the GPU's; -1 in host memory, which no call takes
 
 
 class PackedWeight:
