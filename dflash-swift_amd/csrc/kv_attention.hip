@@ -53,14 +53,6 @@ template <int BITS>
 constexpr float kKScaleOf = BITS == 4 ? kScaleUnit / 16.0f : kScaleUnit;
 constexpr float kMost = 3.38e38f;     /* finite numbers below it stay so in bf16 */
 
-template <bool F16>
-__device__ __forceinline__ float half_of(uint32_t word, bool high) {
-    if constexpr (F16)
-        return (float)__builtin_bit_cast(f16x2_t, word)[high ? 1 : 0];
-    else
-        return __uint_as_float(high ? word & 0xffff0000u : word << 16);
-}
-
 __device__ __forceinline__ f16x8_t as_f16x8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     u32x4_t v = {a, b, c, d};
     return __builtin_bit_cast(f16x8_t, v);
@@ -427,8 +419,10 @@ struct Attention {
         }
     }
 
-    /* Whether column tile i holds its codes times 16.  (V's may stay in the low nibble: 2^-20 of a
-     * sum is far under the outputs' own rounding.) */
+    /* Whether column tile i holds its codes times 16.  V's others stay in the low nibble, where a
+     * sum keeps 2^-21 of the group's extent: under the outputs' rounding, but for a channel that
+     * stands still 2^6 (fp16; bf16 2^9) under its group's others (4096 tokens, 4 bits, one channel
+     * off by 16 of 0.3: 0.9 of the fp16 rounding more, the other tiles' channels 0.2). */
     static constexpr __device__ bool odd_tile(int i) { return BITS == 4 && (i & 1); }
 
     /* What a lane reads for one chunk of steps: its quarter's 8-channel pieces of tokens l % 16
