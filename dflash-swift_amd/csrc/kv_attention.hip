@@ -18,11 +18,11 @@
  * there is more than one.
  *
  * What bounds it.  Long caches and shared prefixes: issue of vector instructions.  A tile of 32
- * rows and 32 tokens with heads of 128 is some 430 of them at 4.3 cycles and 38 matrix steps at 16
- * on each SIMD; it takes 2650 cycles.  16 sequences of 8 rows of 40 heads over 16384 shared tokens
- * (44 GFLOP) 99 us, 440 TFLOP/s; 8 rows over 32776 tokens of their own 27.8 us, 38 MB at 1.4 TB/s.
- * Few tokens: a launch and code that each CU runs once (up to 128 tokens 6.4 us with heads of 64,
- * 7.5 of 128, 10.7 of 256; where a join follows, 8.4, 9.9 and 13).
+ * rows and 32 tokens with heads of 128 is some 435 of them at 4.3 cycles and 40 matrix steps at 16
+ * on each SIMD; it takes 2700 cycles.  16 sequences of 8 rows of 40 heads over 16384 shared tokens
+ * (44 GFLOP) 100 us, 440 TFLOP/s; 8 rows over 32776 tokens of their own 28 us, 38 MB at 1.4 TB/s.
+ * Few tokens: a launch and code that each CU runs once (up to 128 tokens 6.5 us with heads of 64,
+ * 7.5 of 128, 10.8 of 256; where a join follows, 8.8, 10.4 and 14).
  *
  * Measured and not taken: unpacking codes once a workgroup into fp16 tiles in LDS for up to 64 rows
  * (half the vector instructions, but a barrier a round and two waves a SIMD: 112 us where this took
@@ -149,8 +149,8 @@ struct Attention {
     static constexpr int kTileBytes = 32 * kRowBytes;    /* codes of 32 tokens         */
     static constexpr int kLoads = kTileBytes / 1024;     /* wave loads of them         */
     /* K and V tiles in LDS: two of each, or one where two would leave a CU fewer workgroups.  One
-     * row a sequence of 16 over 8192 tokens 36.4 us with one, 35.5 with two; at rows of 128 bytes,
-     * 16 rows of 4 heads over 16000 tokens 37.7 with one, 47.9 with two. */
+     * row of 16 sequences over 8192 tokens 34.9 us with one, 32.7 with two; at rows of 128 bytes, 16
+     * rows of 16 heads of 256 over 16000 tokens 26.1 with one, 31.0 with two. */
     static constexpr int kBufs = kRowBytes <= 64 ? 2 : 1;
     static constexpr float kCentre = BITS == 4 ? 8.0f : 128.0f;
     static constexpr int kRows = 16 * RT;

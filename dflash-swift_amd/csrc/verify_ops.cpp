@@ -59,8 +59,8 @@ static dfq_status hip_error(hipError_t e, const char* what) {
 
 /* The most tiles of 16 rows that attention kernels take in one pass.  Two read and unpack the
  * codes once for both: 16 sequences of 8 rows of 40 heads over a shared 16384-token prefix take
- * 102 us, one tile 118.  At heads of 256 their outputs leave a CU room for one workgroup of two
- * tiles and two of one: 16 rows of 16 heads over 16000 tokens 44.8 us against 35.7, so there it
+ * 102 us, one tile 119.  At heads of 256 their outputs leave a CU room for one workgroup of two
+ * tiles and two of one: 16 rows of 16 heads over 16000 tokens 32.5 us against 26.1, so there it
  * is one.  Three and four would take 103 and 137 KB of LDS at heads of 128, a workgroup a CU. */
 static int attention_tiles(int dim) { return dim == 256 ? 1 : 2; }
 
@@ -278,14 +278,14 @@ constexpr int kRoundTokens = DFQ_KV_THREADS / 2;
  * costs besides its rounds (staging the queries, joining its waves); what each workgroup more on
  * a CU adds to a round of all (they wait for memory, then for issue); what two tiles cost against
  * one; and what one more range costs the join.  Over the plans of sixteen shapes (heads of 64, 128
- * and 256, 1..32 sequences, own caches and shared prefixes) the one that these numbers choose is
- * within 7 % of the fastest, mostly the fastest itself. */
+ * and 256, 1..32 sequences, own caches and shared prefixes, groups of 32, 64 and 128) the one that
+ * these numbers choose is within 2 % of the fastest, mostly the fastest itself. */
 constexpr double kFixedRounds = 1.5, kAnother = 0.45, kTwoTiles = 1.7, kRangeRounds = 0.02;
 /* And the join itself, a launch that a single range does without; a round of heads of 256 is twice
  * one of 128.  Device time of 8 rows of 4 sequences (a caller that launches one call after the other
  * saves 2.5 us of its own besides), one range / 128 tokens a range:
- *   heads of 128: 128 tokens 7.5 / 9.9 us, 512 10.7 / 9.9;  64: 6.4 / 8.4, 8.6 / 8.5;
- *   heads of 256: 10.6 / 13.0, 16.1 / 13.0. */
+ *   heads of 128: 129 tokens 8.6 / 10.4 us, 512 11.2 / 10.7;  64: 7.2 / 8.8, 8.9 / 9.2;
+ *   heads of 256: 12.6 / 14.0, 17.2 / 15.2. */
 double join_rounds(int dim) { return dim > 128 ? 1.5 : 3.0; }
 
 /* The workgroups of `blocks` row blocks over `rounds` rounds in ranges of at most `each`, as even

@@ -306,7 +306,10 @@ dfq_status dfq_qmm_argmax_accept(dfq_ctx* ctx, const void* x, const uint32_t* w,
  * [slots][heads][capacity][head_dim/group_size] in the cache's dtype (bf16 or fp16).  head_dim is
  * 64, 128 or 256 and group_size divides it.  A slot holds one sequence's tokens by position.  The
  * arrays are the caller's; codes are 16-byte aligned, the others 2-byte; one slot of one head is
- * under 2 GiB in each array.  The reference's caches are its target's (a snapshot is taken and
+ * under 2 GiB in each array.  The layout is MLX's, the quantiser is not: dfq_cache_append takes a
+ * group's least and greatest elements, where MLX starts from the edge that is larger in size and
+ * keeps zero exact, so that codes differ from those of a cache that MLX wrote.  Reads and attention
+ * take either (any scale and bias).  The reference's caches are its target's (a snapshot is taken and
  * restored whole, Sources/DFlashKit/PrefixCache.swift:86-141); a prompt's tokens that several
  * sequences share are one cache of one slot here, read in place by all of them. */
 typedef struct dfq_kv_cache {
@@ -358,8 +361,13 @@ dfq_status dfq_cache_read(dfq_ctx* ctx, const dfq_kv_cache* cache, void* k, void
  * heads side by side (any element alignment); y is dense [batch][rows][q_heads*head_dim] in that
  * dtype; lse fp32 [batch][rows][q_heads] or NULL.  prefix and cache agree in heads, head_dim,
  * bits, group_size and dtype.  scale is positive and finite.  Scores, softmax sums and outputs
- * are summed in fp32; the same call gives the same bits every time.  The workspace
- * (dfq_cache_attention_workspace_bytes for the same sizes, 16-byte aligned) needs no clearing.
+ * are summed in fp32.  A token's softmax weight times its V scale is rounded to fp16 before it meets
+ * the token's codes and bias: by 2^-12 of itself, or, if that is more, 2^-35 of the row's largest
+ * such product in any group of the head (groups 2^8 and more apart in size are first brought to one,
+ * from the first tokens of a range).  Query elements under 2^-29 of their row's largest lose bits.
+ * The same call gives the same bits every time.  The workspace
+ * (dfq_cache_attention_workspace_bytes for the same sizes, 16-byte aligned) needs no clearing; two
+ * calls that may run at once, or that threads may launch on one stream at once, need one each.
  * Asynchronous on `stream`. */
 dfq_status dfq_cache_attention_workspace_bytes(dfq_ctx* ctx, const dfq_kv_cache* prefix,
                                                int prefix_length, const dfq_kv_cache* cache,
@@ -382,7 +390,8 @@ dfq_status dfq_cache_attention(dfq_ctx* ctx, const dfq_kv_cache* prefix, int pre
  * A logit of -inf has probability 0.  A row with a NaN or +inf, or with nothing above -inf, has
  * NaN for its probabilities and entropy.  What a sampler's client is told of the tokens that the
  * greedy accept takes (acceptedPrefix, DFlashSpeculativeGenerator.swift:555-571, keeps the tokens
- * alone).  The workspace (16-byte aligned; none where its size is 0) needs no clearing.
+ * alone).  The workspace (16-byte aligned; none where its size is 0) needs no clearing, and is
+ * shared no more than dfq_cache_attention's.
  * Asynchronous on `stream`. */
 dfq_status dfq_token_logprobs_workspace_bytes(dfq_ctx* ctx, int M, int V, int top_k,
                                               size_t* bytes);
