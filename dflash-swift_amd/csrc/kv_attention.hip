@@ -149,8 +149,8 @@ struct Attention {
     static constexpr int kTileBytes = 32 * kRowBytes;    /* codes of 32 tokens         */
     static constexpr int kLoads = kTileBytes / 1024;     /* wave loads of them         */
     /* K and V tiles in LDS: two of each, or one where two would leave a CU fewer workgroups.  One
-     * row of 16 sequences over 8192 tokens 34.9 us with one, 32.7 with two; at rows of 128 bytes, 16
-     * rows of 16 heads of 256 over 16000 tokens 26.1 with one, 31.0 with two. */
+     * row of 16 sequences over 8192 tokens 34.9 us with one, 32.7 with two; at rows of 128 bytes,
+     * 16 rows of 16 heads of 256 over 16000 tokens 26.1 with one, 31.0 with two. */
     static constexpr int kBufs = kRowBytes <= 64 ? 2 : 1;
     static constexpr float kCentre = BITS == 4 ? 8.0f : 128.0f;
     static constexpr int kRows = 16 * RT;
@@ -199,8 +199,8 @@ struct Attention {
 
     /* Where the groups' V scales are 2^8 and more apart, they are brought to one size, that of the
      * smallest group: h of one group would be denormal beside another's 2^20 times as large.  A
-     * group's size is the mean exponent of its scales over the wave's first tile, of the tokens that
-     * all rows see (what a row does not see may not move its roundings); zeros count as their
+     * group's size is the mean exponent of its scales over the wave's first tile, of the tokens
+     * that all rows see (what a row does not see may not move its roundings); zeros count as their
      * token's largest. */
     static constexpr uint32_t kApart = 8;
     static __device__ __forceinline__ uint64_t even_groups(const Job& job, int t, int lane,
@@ -246,10 +246,11 @@ struct Attention {
      * stands apart from its group's others): 64 tokens with one of 64 channels off by 16 of their
      * 0.3, the others' errors were 9 (8 bits, 25) times the output's own rounding, and with p in
      * 16 bits still 2.  r comes in two fp16 parts, 22 bits.
-     * Where the middle b + centre s is more than 128 times the codes' half range (or s is 0), r would
-     * pass fp16.  There r is -centre, codes count from the middle, which they change little, and the
-     * far middle meets p itself, both in two bf16 parts (16 bits).  The offset of a row's weights keeps p m
-     * below 2^35 as it keeps h below 2^15: for it, a far middle counts as a scale of 2^-20 of it.
+     * Where the middle b + centre s is more than 128 times the codes' half range (or s is 0), r
+     * would pass fp16.  There r is -centre, codes count from the middle, which they change little,
+     * and the far middle meets p itself, both in two bf16 parts (16 bits).  The offset of a row's
+     * weights keeps p m below 2^35 as it keeps h below 2^15: for it, a far middle counts as a scale
+     * of 2^-20 of it.
      * A V group whose scale or bias is not finite (or the middle of its range past bf16) counts as
      * a NaN scale and no bias: the rows that see it get NaN, and the others, whose weight is 0,
      * nothing. */
