@@ -1,6 +1,6 @@
 /*
- * kv_params.h -- kernel arguments shared by the cache, attention and log-probability kernels
- * and the host code that launches them.
+ * kv_params.h -- kernel arguments shared by the cache, attention, log-probability, rotation and
+ * sampled-accept kernels and the host code that launches them.
  */
 #ifndef DFQ_KV_PARAMS_H
 #define DFQ_KV_PARAMS_H
@@ -74,6 +74,68 @@ struct LogprobParams {
     int64_t row_stride;
     int rows, vocab, top;
     int splits;              /* workgroups, and parts, a row                                */
+};
+
+/* What a workgroup of dfq_sample_accept's first kernel makes of its range of a row. */
+struct AcceptPart {
+    float top;               /* the largest logit, NaN passed over; -inf where there is none */
+    float sum;               /* of e^((x - max(top, -FLT_MAX)) / T)                          */
+    int32_t at;              /* the first that is the largest, -1 where all are NaN          */
+    int32_t pad;
+};
+
+/* What is left to draw of a sequence: from p, p without its draft, or max(p - q, 0). */
+enum { DFQ_DRAW_NONE = 0, DFQ_DRAW_P = 1, DFQ_DRAW_OTHER = 2, DFQ_DRAW_REST = 3 };
+struct AcceptDraw {
+    int32_t mode, row;       /* the target's row, and the place of the token         */
+    int32_t draft;           /* DFQ_DRAW_OTHER: the token left out                    */
+    float p_top, q_top;      /* largest logits of the rows                            */
+    int32_t pad;
+};
+
+struct AcceptParams {
+    const void* logits;
+    const void* draft_logits;   /* or NULL: drafts are certain                     */
+    const int32_t* drafts;      /* [batch][rows - 1]                               */
+    const int32_t* lengths;     /* drafts of each sequence, or NULL: rows - 1      */
+    const float* uniforms;      /* [batch][rows]                                   */
+    const float* temperatures;  /* [batch], or NULL: `temperature`                 */
+    const float* draft_temperatures;
+    int32_t* tokens;            /* [batch][rows]                                   */
+    int32_t* accepted;          /* [batch]                                         */
+    float* chances;             /* [batch][rows - 1] or NULL                       */
+    AcceptPart* parts;          /* [batch][rows, then draft rows][splits]          */
+    AcceptDraw* draws;          /* [batch]                                         */
+    double* totals;             /* [batch][2][chunks]: sums of e^((x - top) / T)   */
+    double* weights;            /* [batch][chunks]: sums of what is drawn from     */
+    int64_t batch_stride, row_stride, draft_batch_stride, draft_row_stride;
+    float temperature, draft_temperature;
+    int batch, rows, all_rows, vocab;
+    int splits;                 /* workgroups, and parts, a row                    */
+    int chunks;                 /* pieces of DFQ_KV_THREADS lanes' 16 bytes a row  */
+};
+
+#define DFQ_ROPE_DIM 512     /* widest head */
+
+struct RopeTensor {
+    const void* in;
+    void* out;
+    const void* weight;      /* [dim] or NULL                                    */
+    int64_t in_batch, in_row, in_head, out_batch, out_row, out_head;   /* elements */
+    int heads;
+};
+
+struct RopeParams {
+    RopeTensor t[2];         /* queries, keys (0 heads: none)                    */
+    const uint64_t* turns;   /* [pairs] 2^-64 turns a position                   */
+    const int32_t* starts;   /* first position of each sequence, added to start  */
+    const int32_t* positions;   /* [batch][rows], in place of those, or NULL     */
+    int64_t slots;           /* heads of all tokens                              */
+    int start, dim, pairs;
+    int lanes;               /* that hold a head (rotate_heads)                  */
+    int inverse, interleaved, weight_f32;
+    float amplitude, eps, offset;
+    Divisor all_heads, rows;
 };
 
 #endif

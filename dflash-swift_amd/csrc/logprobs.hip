@@ -17,7 +17,7 @@
  * alternatives 7.3 and 4.3 us.
  */
 #include "kv_params.h"
-#include "qmm_device.h"
+#include "logit_piece.h"
 
 namespace {
 
@@ -26,8 +26,6 @@ constexpr int kWaves = DFQ_KV_THREADS / 64;
 constexpr int kKept = 64;            /* candidates that stay without being sorted      */
 constexpr int kPiece = 8;            /* most logits (or keys) that a lane brings at once */
 constexpr int kRoom = kKept + 64 * kPiece;
-
-typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
 /* Order of a logit: larger first, then the lower index; NaN below every number (0). */
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -188,46 +186,11 @@ struct Sums {
 };
 
 template <int DT>
-struct Pieces {
-    static constexpr int kN = DT == 2 ? 4 : 8;       /* logits of 16 bytes              */
+struct Pieces : LogitPiece<DT> {
+    using LogitPiece<DT>::kN, LogitPiece<DT>::load, LogitPiece<DT>::widen,
+        LogitPiece<DT>::largest;
     static constexpr int kLow = DT == 2 ? 4 : 16;    /* bits that reach() leaves        */
     static constexpr int kAhead = 4;                 /* loads in flight a lane          */
-
-    static __device__ __forceinline__ u32x4_t load(const char* row, int i, int end) {
-        constexpr int kSize = 16 / kN;
-        if (i + kN <= end) return *(const u32x4_any*)(row + (int64_t)i * kSize);
-        u32x4_t v;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if constexpr (DT == 2) {
-                v[j] = i + j < end ? *(const uint32_t*)(row + (int64_t)(i + j) * 4) : 0xff800000u;
-            } else {
-                constexpr uint32_t kInf = DT == 1 ? 0xfc00u : 0xff80u;
-                const uint16_t* p = (const uint16_t*)row + i + 2 * j;
-                v[j] = (i + 2 * j < end ? p[0] : kInf) | (i + 2 * j + 1 < end ? p[1] : kInf) << 16;
-            }
-        }
-        return v;
-    }
-
-    static __device__ __forceinline__ void widen(u32x4_t v, float (&x)[kN]) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if constexpr (DT == 2) {
-                x[j] = __uint_as_float(v[j]);
-            } else {
-                x[2 * j] = elem_to_f32<DT == 1>(v[j] & 0xffffu);
-                x[2 * j + 1] = elem_to_f32<DT == 1>(v[j] >> 16);
-            }
-        }
-    }
-
-    static __device__ __forceinline__ float largest(const float (&x)[kN]) {
-        float m = x[0];
-#pragma unroll
-        for (int j = 1; j < kN; ++j) m = fmaxf(m, x[j]);
-        return m;
-    }
 
     /* The logits of 64 lanes' pieces into the sums and, where any may be among the best, into
      * them. */

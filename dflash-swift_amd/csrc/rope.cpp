@@ -1,0 +1,199 @@
+/*
+ * rope.cpp -- the C ABI of the rotary positions: frequency tables (host only), argument checks and
+ * launches of rope.hip.
+ */
+#include <cmath>
+#include <cstdint>
+
+#include "verify_ops.h"
+
+using namespace dfq;
+
+namespace {
+
+constexpr double kTurn = 6.28318530717958647692528676655900577;
+
+bool good(double v) { return v > 0 && std::isfinite(v); }
+
+dfq_status check_heads(const dfq_heads* t, const char* name, dfq_dtype dtype) {
+    if (!t->in || !t->out) return fail(DFQ_ERR_INVALID_ARGUMENT, "null %s", name);
+    if (!aligned(t->in, dtype_size(dtype)) || !aligned(t->out, dtype_size(dtype)))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "misaligned %s", name);
+    if (t->heads < 1) return fail(DFQ_ERR_INVALID_ARGUMENT, "%s has no heads", name);
+    return DFQ_OK;
+}
+
+RopeTensor tensor_of(const dfq_heads* t, const void* weight) {
+    return {t->in, t->out, weight, t->in_batch, t->in_row, t->in_head,
+            t->out_batch, t->out_row, t->out_head, t->heads};
+}
+
+struct Norms {
+    const void* q_weight;
+    const void* k_weight;
+    dfq_dtype weight_dtype;
+    float eps, offset;
+};
+
+/* Both entry points; norms is NULL for the rotation alone. */
+dfq_status rotate(dfq_ctx* ctx, const dfq_rope_table* rope, const dfq_heads* q, const dfq_heads* k,
+                  const Norms* norms, int head_dim, dfq_dtype dtype, int batch, int rows, int start,
+                  const int32_t* starts, const int32_t* positions, int inverse, void* stream,
+                  const char* what) {
+    if (!ctx) return fail(DFQ_ERR_INVALID_ARGUMENT, "null context");
+    if (!q) return fail(DFQ_ERR_INVALID_ARGUMENT, "null q");
+    if (dtype != DFQ_BF16 && dtype != DFQ_F16 && dtype != DFQ_F32)
+        return fail(DFQ_ERR_UNSUPPORTED, "heads are bf16, fp16 or fp32");
+    if (head_dim < 2 || head_dim > DFQ_ROPE_DIM || head_dim % 2)
+        return fail(DFQ_ERR_UNSUPPORTED, "head_dim must be even and at most %d (got %d)",
+                    DFQ_ROPE_DIM, head_dim);
+    if (batch < 1 || rows < 1) return fail(DFQ_ERR_INVALID_ARGUMENT, "batch and rows must be >= 1");
+    if (!rope && !norms) return fail(DFQ_ERR_INVALID_ARGUMENT, "null rope table");
+    if (rope) {
+        if (!rope->turns || !aligned(rope->turns, 8))
+            return fail(DFQ_ERR_INVALID_ARGUMENT, "null or misaligned turns");
+        if (rope->rotary_dim < 2 || rope->rotary_dim % 2 || rope->rotary_dim > head_dim)
+            return fail(DFQ_ERR_UNSUPPORTED, "rotary_dim must be even and at most the head's %d "
+                        "(got %d)", head_dim, rope->rotary_dim);
+        if (!std::isfinite(rope->amplitude))
+            return fail(DFQ_ERR_INVALID_ARGUMENT, "amplitude must be finite");
+    }
+    dfq_status s = check_heads(q, "q", dtype);
+    if (s || (k && (s = check_heads(k, "k", dtype)))) return s;
+    if (!aligned(starts, 4) || !aligned(positions, 4))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "misaligned starts or positions");
+    if (positions && (starts || start))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "positions take the place of start and starts");
+    RopeParams p{};
+    p.t[0] = tensor_of(q, norms ? norms->q_weight : nullptr);
+    if (k) p.t[1] = tensor_of(k, norms ? norms->k_weight : nullptr);
+    if (norms) {
+        if (norms->weight_dtype != dtype && norms->weight_dtype != DFQ_F32)
+            return fail(DFQ_ERR_UNSUPPORTED, "weights are in the heads' dtype or fp32");
+        const size_t a = dtype_size(norms->weight_dtype);
+        if (!aligned(norms->q_weight, a) || !aligned(norms->k_weight, a))
+            return fail(DFQ_ERR_INVALID_ARGUMENT, "misaligned weights");
+        if (!(norms->eps >= 0.0f) || !std::isfinite(norms->eps) || !std::isfinite(norms->offset))
+            return fail(DFQ_ERR_INVALID_ARGUMENT, "eps must be finite and >= 0, the offset finite");
+        p.weight_f32 = norms->weight_dtype == DFQ_F32;
+        p.eps = norms->eps;
+        p.offset = norms->offset;
+    }
+    const int64_t all = (int64_t)q->heads + (k ? k->heads : 0), tokens = (int64_t)batch * rows;
+    if (all > INT32_MAX || tokens > INT32_MAX / all)
+        return fail(DFQ_ERR_UNSUPPORTED, "grid too large");
+    p.turns = rope ? rope->turns : nullptr;
+    p.pairs = rope ? rope->rotary_dim / 2 : 0;
+    p.amplitude = rope ? rope->amplitude : 1.0f;
+    p.interleaved = rope && rope->interleaved;
+    p.starts = starts;
+    p.positions = positions;
+    p.start = start;
+    p.inverse = inverse != 0;
+    p.slots = tokens * all;
+    p.dim = head_dim;
+    p.all_heads = divisor((int)all);
+    p.rows = divisor(rows);
+    /* Chunks of 8 channels hold both channels of their pairs where a head is 16 n wide and, with
+     * pairs half the rotated width apart, that half is a multiple of 8. */
+    const bool chunks = head_dim % 16 == 0 && (p.interleaved || p.pairs % 8 == 0);
+    const int way = chunks ? (p.interleaved ? 1 : 0) : 2;
+    p.lanes = 64;
+    if (chunks)
+        for (p.lanes = 1; p.lanes * 16 < head_dim; p.lanes *= 2) {}
+    const VerifyOps* ops;
+    if ((s = ctx_verify_ops(ctx, &ops))) return s;
+    DeviceScope scope(ctx);
+    const int64_t per = DFQ_KV_THREADS / p.lanes;
+    void* args[] = {&p};
+    const hipError_t e = hipModuleLaunchKernel(
+        ops->rotate[norms != nullptr][way][(int)dtype], (unsigned)((p.slots + per - 1) / per), 1, 1,
+        DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
+    return e == hipSuccess ? DFQ_OK : hip_error(e, what);
+}
+
+}  // namespace
+
+extern "C" {
+
+dfq_status dfq_rope_frequencies(const dfq_rope_desc* d, double* frequencies, float* amplitude) {
+    if (!d || !frequencies) return fail(DFQ_ERR_INVALID_ARGUMENT, "null argument");
+    const int R = d->rotary_dim, n = R / 2;
+    if (R < 2 || R % 2 || R > DFQ_ROPE_DIM)
+        return fail(DFQ_ERR_UNSUPPORTED, "rotary_dim must be even and at most %d (got %d)",
+                    DFQ_ROPE_DIM, R);
+    if (!(d->base > 1.0) || !std::isfinite(d->base))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "base must be finite and above 1");
+    if (d->scaling < DFQ_ROPE_PLAIN || d->scaling > DFQ_ROPE_YARN)
+        return fail(DFQ_ERR_UNSUPPORTED, "unknown scaling %d", (int)d->scaling);
+    if (d->scaling != DFQ_ROPE_PLAIN && !good(d->factor))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "factor must be positive and finite");
+    const bool bands = d->scaling == DFQ_ROPE_BANDS, yarn = d->scaling == DFQ_ROPE_YARN;
+    if ((bands || yarn) && !good(d->original_length))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "original_length must be positive and finite");
+    if (bands && !(good(d->low_freq_factor) && good(d->high_freq_factor) &&
+                   d->low_freq_factor < d->high_freq_factor))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "0 < low_freq_factor < high_freq_factor");
+    if (yarn && !(good(d->beta_fast) && good(d->beta_slow) && d->beta_slow < d->beta_fast))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "0 < beta_slow < beta_fast");
+    double base = d->base;
+    if (d->scaling == DFQ_ROPE_NTK) base *= std::pow(d->factor, (double)R / (R > 2 ? R - 2 : 1));
+    double low = 0, high = 0;
+    if (yarn) {
+        /* the pair that turns `beta` times over the original length */
+        const auto edge = [&](double beta) {
+            return R * std::log(d->original_length / (beta * kTurn)) / (2 * std::log(base));
+        };
+        low = std::fmax(std::floor(edge(d->beta_fast)), 0.0);
+        high = std::fmin(std::ceil(edge(d->beta_slow)), R - 1.0);
+    }
+    for (int i = 0; i < n; ++i) {
+        const double f = std::pow(base, -2.0 * i / R);
+        double keep = 1.0;   /* of the frequency; the rest is divided by the factor */
+        if (d->scaling == DFQ_ROPE_LINEAR) keep = 0.0;
+        if (bands)
+            keep = (d->original_length * f / kTurn - d->low_freq_factor) /
+                   (d->high_freq_factor - d->low_freq_factor);
+        if (yarn) keep = 1.0 - (i - low) / std::fmax(high - low, 0.001);
+        keep = std::fmin(std::fmax(keep, 0.0), 1.0);
+        frequencies[i] = keep == 1.0 ? f : keep * f + (1.0 - keep) * f / d->factor;
+    }
+    if (amplitude)
+        *amplitude = yarn && d->factor > 1.0 ? (float)(0.1 * std::log(d->factor) + 1.0) : 1.0f;
+    return DFQ_OK;
+}
+
+dfq_status dfq_rope_turns(const double* frequencies, int count, uint64_t* turns) {
+    if (!frequencies || !turns) return fail(DFQ_ERR_INVALID_ARGUMENT, "null argument");
+    if (count < 1) return fail(DFQ_ERR_INVALID_ARGUMENT, "count must be >= 1");
+    for (int i = 0; i < count; ++i) {
+        if (!std::isfinite(frequencies[i]))
+            return fail(DFQ_ERR_INVALID_ARGUMENT, "frequency %d is not finite", i);
+        /* a double's 53 bits over 2 pi in the 64 of a long double, its whole turns dropped */
+        const long double turn = (long double)frequencies[i] / 6.28318530717958647692528676655900577L;
+        const long double part = turn - std::floor(turn);
+        const long double scaled = std::floor(part * 18446744073709551616.0L + 0.5L);
+        turns[i] = scaled >= 18446744073709551616.0L ? 0 : (uint64_t)scaled;
+    }
+    return DFQ_OK;
+}
+
+dfq_status dfq_rope(dfq_ctx* ctx, const dfq_rope_table* rope, const dfq_heads* q,
+                    const dfq_heads* k, int head_dim, dfq_dtype dtype, int batch, int rows,
+                    int start, const int32_t* starts, const int32_t* positions, int inverse,
+                    void* stream) {
+    return rotate(ctx, rope, q, k, nullptr, head_dim, dtype, batch, rows, start, starts, positions,
+                  inverse, stream, "launch dfq_rope");
+}
+
+dfq_status dfq_qk_norm_rope(dfq_ctx* ctx, const dfq_rope_table* rope, const dfq_heads* q,
+                            const dfq_heads* k, const void* q_weight, const void* k_weight,
+                            dfq_dtype weight_dtype, float eps, float weight_offset, int head_dim,
+                            dfq_dtype dtype, int batch, int rows, int start, const int32_t* starts,
+                            const int32_t* positions, void* stream) {
+    const Norms norms = {q_weight, k_weight, weight_dtype, eps, weight_offset};
+    return rotate(ctx, rope, q, k, &norms, head_dim, dtype, batch, rows, start, starts, positions, 0,
+                  stream, "launch dfq_qk_norm_rope");
+}
+
+}  // extern "C"

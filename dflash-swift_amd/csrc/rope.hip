@@ -1,0 +1,254 @@
+/*
+ * rope.hip -- gfx950 kernels of the rotary positions of queries and keys, alone and behind the RMS
+ * norm of each head.
+ *
+ * With f the frequencies (radians a position) of a head's R/2 rotated pairs, position p turns the
+ * pair (a, b) i by the angle t = p f_i:
+ *   a' = A (a cos t - b sin t),   b' = A (b cos t + a sin t),
+ * channels behind R stay.  Pairs are (i, i + R/2) or, interleaved, (2i, 2i + 1).  The norm in front
+ * is x (w + offset) / sqrt(mean x^2 + eps) over a head's channels.  All of it in fp32, rounded once.
+ *
+ * The angle of a far position has no room in fp32 (position 10^6 at a frequency of 1 is known to
+ * 0.06), so frequencies are whole numbers F of 2^-64 turns: p F mod 2^64, in whole arithmetic, is
+ * the angle's place in its turn, whatever p, and its upper 32 bits leave an error of 2^-32 turns.
+ * Sine and cosine are their Taylor sums over an eighth of a turn to both sides of the nearest
+ * quarter: the first terms left out are x^11 / 11! < 1.8e-9 and x^12 / 12! < 1.2e-10.
+ */
+#include "kv_params.h"
+#include "qmm_device.h"
+
+namespace {
+
+/* 16 bytes at any element's address (heads cut from a fused projection have any offset). */
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+
+/* Two numbers to nearest even, the first in the low half. */
+template <bool F16>
+__device__ __forceinline__ uint32_t rounded2(float a, float b) {
+    if constexpr (F16) return __builtin_bit_cast(uint32_t, f16x2_t{(_Float16)a, (_Float16)b});
+    else return __builtin_bit_cast(uint32_t, bf16x2_t{(__bf16)a, (__bf16)b});
+}
+
+/* Sine and cosine of t 2^-32 turns. */
+__device__ __forceinline__ void turn_of(uint32_t t, float& sine, float& cosine) {
+    const uint32_t quarter = (t + 0x20000000u) >> 30;
+    const float x = (float)(int32_t)(t - (quarter << 30)) * (6.28318530717958647692f * 0x1p-32f);
+    const float y = x * x;
+    float s = fmaf(y, 1.0f / 362880.0f, -1.0f / 5040.0f);
+    s = fmaf(y, s, 1.0f / 120.0f);
+    s = fmaf(y, s, -1.0f / 6.0f);
+    s = fmaf(x * y, s, x);
+    float c = fmaf(y, -1.0f / 3628800.0f, 1.0f / 40320.0f);
+    c = fmaf(y, c, -1.0f / 720.0f);
+    c = fmaf(y, c, 1.0f / 24.0f);
+    c = fmaf(y, c, -0.5f);
+    c = fmaf(y, c, 1.0f);
+    sine = quarter & 1 ? c : s;
+    cosine = quarter & 1 ? s : c;
+    if (quarter & 2) sine = -sine;
+    if ((quarter + 1) & 2) cosine = -cosine;
+}
+
+/* The position of row m of sequence b, negated where the rotation is undone. */
+__device__ __forceinline__ uint64_t position(const RopeParams& p, int b, int m) {
+    const int64_t pos = p.positions ? (int64_t)p.positions[(int64_t)b * p.rows.by + m]
+                                    : (int64_t)p.start + (p.starts ? p.starts[b] : 0) + m;
+    return (uint64_t)(p.inverse ? -pos : pos);
+}
+
+/* Pair i turned by its angle at `pos`. */
+__device__ __forceinline__ void turn_pair(const RopeParams& p, uint64_t pos, int i, float& a,
+                                          float& b) {
+    float sine, cosine;
+    turn_of((uint32_t)(pos * p.turns[i] >> 32), sine, cosine);
+    sine *= p.amplitude;
+    cosine *= p.amplitude;
+    const float c = a;
+    a = c * cosine - b * sine;
+    b = b * cosine + c * sine;
+}
+
+template <int DT>
+struct Chunk {
+    static constexpr int kSize = DT == 2 ? 4 : 2;
+    /* 8 neighbouring elements as fp32, and back. */
+    static __device__ __forceinline__ void load(const void* base, int64_t at, float (&f)[8]) {
+        const char* a = (const char*)base + at * kSize;
+        if constexpr (DT == 2) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const u32x4_t v = *(const u32x4_any*)(a + 16 * i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f[4 * i + j] = __uint_as_float(v[j]);
+            }
+        } else {
+            const u32x4_t v = *(const u32x4_any*)a;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f[2 * i] = elem_to_f32<DT == 1>(v[i] & 0xffffu);
+                f[2 * i + 1] = elem_to_f32<DT == 1>(v[i] >> 16);
+            }
+        }
+    }
+    static __device__ __forceinline__ void store(void* base, int64_t at, const float (&f)[8]) {
+        char* a = (char*)base + at * kSize;
+        if constexpr (DT == 2) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                u32x4_t v;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = __float_as_uint(f[4 * i + j]);
+                *(u32x4_any*)(a + 16 * i) = v;
+            }
+        } else {
+            u32x4_t v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = rounded2<DT == 1>(f[2 * i], f[2 * i + 1]);
+            *(u32x4_any*)a = v;
+        }
+    }
+};
+
+__device__ __forceinline__ int divided(int n, const Divisor& d) {
+    return (int)((n + (uint64_t)((uint64_t)(uint32_t)n * d.mul >> 32)) >> d.shift);
+}
+
+/* The sum over the `lanes` (a power of two up to 32) that hold a head. */
+__device__ __forceinline__ float head_sum(float v, int lanes) {
+    for (int d = 1; d < lanes; d *= 2) v += __shfl_xor(v, d);
+    return v;
+}
+
+/* Heads of 16 n channels: a lane holds two chunks of 8, so that it has both channels of each of
+ * its 8 pairs.  `lanes` lanes a head, the heads of one token side by side. */
+template <int DT, bool NORM, bool INTERLEAVED>
+__device__ __forceinline__ void rotate_heads(const RopeParams& p) {
+    const int lane = threadIdx.x % p.lanes;
+    const int64_t slot = (int64_t)blockIdx.x * (DFQ_KV_THREADS / p.lanes) + threadIdx.x / p.lanes;
+    if (slot >= p.slots) return;
+    const int token = divided((int)slot, p.all_heads);
+    int head = (int)slot - token * p.all_heads.by;
+    const int b = divided(token, p.rows), m = token - b * p.rows.by;
+    const bool k = head >= p.t[0].heads;
+    const RopeTensor& t = p.t[k];
+    if (k) head -= p.t[0].heads;
+    const bool active = lane * 16 < p.dim;
+    /* the lane's chunks: of a rotated half and its partner, or neighbours */
+    const bool halves = !INTERLEAVED && lane * 8 < p.pairs;
+    const int at0 = halves ? lane * 8 : lane * 16;
+    const int at1 = halves ? at0 + p.pairs : at0 + 8;
+    float x[2][8] = {};
+    if (active) {
+        const int64_t from = b * t.in_batch + m * t.in_row + head * t.in_head;
+        Chunk<DT>::load(t.in, from + at0, x[0]);
+        Chunk<DT>::load(t.in, from + at1, x[1]);
+    }
+    if constexpr (NORM) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum = fmaf(x[0][i], x[0][i], fmaf(x[1][i], x[1][i], sum));
+        sum = head_sum(sum, p.lanes);
+        if (!active) return;
+        const float scale = rsqrtf(sum / (float)p.dim + p.eps);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[c][i] *= scale;
+            if (!t.weight) continue;
+            float w[8];
+            if (p.weight_f32) Chunk<2>::load(t.weight, c ? at1 : at0, w);
+            else Chunk<DT>::load(t.weight, c ? at1 : at0, w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[c][i] *= w[i] + p.offset;
+        }
+    }
+    if (!active) return;
+    const uint64_t pos = position(p, b, m);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        /* channels behind the rotated ones stay as they are, infinities and NaN among them */
+        if (lane * 8 + i >= p.pairs) break;
+        if constexpr (INTERLEAVED)
+            turn_pair(p, pos, lane * 8 + i, x[i / 4][2 * (i % 4)], x[i / 4][2 * (i % 4) + 1]);
+        else
+            turn_pair(p, pos, lane * 8 + i, x[0][i], x[1][i]);
+    }
+    const int64_t to = b * t.out_batch + m * t.out_row + head * t.out_head;
+    Chunk<DT>::store(t.out, to + at0, x[0]);
+    Chunk<DT>::store(t.out, to + at1, x[1]);
+}
+
+/* Any even head and any number of pairs: a wave a head, a lane a pair at a time. */
+template <int DT, bool NORM>
+__device__ __forceinline__ void rotate_any(const RopeParams& p) {
+    const int lane = threadIdx.x % 64;
+    const int64_t slot = (int64_t)blockIdx.x * (DFQ_KV_THREADS / 64) + threadIdx.x / 64;
+    if (slot >= p.slots) return;
+    const int token = divided((int)slot, p.all_heads);
+    int head = (int)slot - token * p.all_heads.by;
+    const int b = divided(token, p.rows), m = token - b * p.rows.by;
+    const bool k = head >= p.t[0].heads;
+    const RopeTensor& t = p.t[k];
+    if (k) head -= p.t[0].heads;
+    const int64_t from = b * t.in_batch + m * t.in_row + head * t.in_head;
+    const int64_t to = b * t.out_batch + m * t.out_row + head * t.out_head;
+    const uint64_t pos = position(p, b, m);
+    constexpr int kMost = DFQ_ROPE_DIM / 128;   /* pairs a lane */
+    float x[kMost][2];
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kMost; ++j) {
+        const int i = lane + 64 * j;
+        x[j][0] = x[j][1] = 0.0f;
+        if (2 * i < p.dim) {
+            const bool apart = !p.interleaved && i < p.pairs;
+            x[j][0] = load_any(t.in, DT, from + (apart ? i : 2 * i));
+            x[j][1] = load_any(t.in, DT, from + (apart ? i + p.pairs : 2 * i + 1));
+        }
+        sum = fmaf(x[j][0], x[j][0], fmaf(x[j][1], x[j][1], sum));
+    }
+    float scale = 1.0f;
+    if constexpr (NORM) scale = rsqrtf(head_sum(sum, 64) / (float)p.dim + p.eps);
+#pragma unroll
+    for (int j = 0; j < kMost; ++j) {
+        const int i = lane + 64 * j;
+        if (2 * i >= p.dim) continue;
+        const bool apart = !p.interleaved && i < p.pairs;
+        const int at0 = apart ? i : 2 * i, at1 = apart ? i + p.pairs : 2 * i + 1;
+        float a = x[j][0], c = x[j][1];
+        if constexpr (NORM) {
+            const int wt = p.weight_f32 ? 2 : DT;
+            a *= scale;
+            c *= scale;
+            if (t.weight) {
+                a *= load_any(t.weight, wt, at0) + p.offset;
+                c *= load_any(t.weight, wt, at1) + p.offset;
+            }
+        }
+        if (i < p.pairs) turn_pair(p, pos, i, a, c);
+        store_any(t.out, DT, to + at0, a);
+        store_any(t.out, DT, to + at1, c);
+    }
+}
+
+}  // namespace
+
+#define DFQ_ROPE_KERNELS(op, norm, name, dt)                                                \
+    extern "C" __global__ __launch_bounds__(DFQ_KV_THREADS) void dfq_##op##_halves_##name(  \
+        RopeParams p) {                                                                     \
+        rotate_heads<dt, norm, false>(p);                                                   \
+    }                                                                                       \
+    extern "C" __global__ __launch_bounds__(DFQ_KV_THREADS) void dfq_##op##_pairs_##name(   \
+        RopeParams p) {                                                                     \
+        rotate_heads<dt, norm, true>(p);                                                    \
+    }                                                                                       \
+    extern "C" __global__ __launch_bounds__(DFQ_KV_THREADS) void dfq_##op##_any_##name(     \
+        RopeParams p) {                                                                     \
+        rotate_any<dt, norm>(p);                                                            \
+    }
+#define DFQ_ROPE_TYPES(op, norm)          \
+    DFQ_ROPE_KERNELS(op, norm, bf16, 0)   \
+    DFQ_ROPE_KERNELS(op, norm, f16, 1)    \
+    DFQ_ROPE_KERNELS(op, norm, f32, 2)
+DFQ_ROPE_TYPES(rope, false)
+DFQ_ROPE_TYPES(norm_rope, true)

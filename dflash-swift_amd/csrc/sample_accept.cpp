@@ -1,0 +1,151 @@
+/*
+ * sample_accept.cpp -- the C ABI of the sampled accept: argument checks, work split and launches of
+ * sample_accept.hip.
+ */
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "verify_ops.h"
+
+using namespace dfq;
+
+namespace {
+
+dfq_status check_sizes(int batch, int rows, int V, dfq_dtype dtype) {
+    if (batch < 1 || rows < 1 || V < 1)
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "batch, rows and V must be >= 1");
+    if (rows > DFQ_ACCEPT_ROWS)
+        return fail(DFQ_ERR_UNSUPPORTED, "at most %d rows (got %d)", DFQ_ACCEPT_ROWS, rows);
+    if (V > 0x7fffffff / 2) return fail(DFQ_ERR_UNSUPPORTED, "V too large");
+    if (dtype != DFQ_BF16 && dtype != DFQ_F16 && dtype != DFQ_F32)
+        return fail(DFQ_ERR_UNSUPPORTED, "logits are bf16, fp16 or fp32");
+    return DFQ_OK;
+}
+
+struct AcceptPlan {
+    int all_rows, splits, chunks;
+    size_t draws, totals, weights, bytes;   /* offsets; the parts come first */
+};
+
+/* Workgroups a row as the log probabilities take them: ranges of 1024 logits a wave or more, five
+ * workgroups a CU. */
+AcceptPlan plan_accept(int cus, int batch, int rows, int V, dfq_dtype dtype, bool drafted) {
+    AcceptPlan a;
+    a.all_rows = drafted ? 2 * rows - 1 : rows;
+    const int64_t M = (int64_t)batch * a.all_rows;
+    const int64_t most = std::max<int64_t>(1, 5 * cus / M);
+    a.splits = (int)std::min({most, ((int64_t)V + 4095) / 4096, (int64_t)64});
+    const int chunk = DFQ_KV_THREADS * (dtype == DFQ_F32 ? 4 : 8);
+    a.chunks = (V + chunk - 1) / chunk;
+    const auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    a.draws = up((size_t)M * a.splits * sizeof(AcceptPart));
+    a.totals = a.draws + up((size_t)batch * sizeof(AcceptDraw));
+    a.weights = a.totals + (drafted ? up((size_t)batch * 2 * a.chunks * 8) : 0);
+    a.bytes = a.weights + (size_t)batch * a.chunks * 8;
+    return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+dfq_status dfq_sample_accept_workspace_bytes(dfq_ctx* ctx, int batch, int rows, int V,
+                                             dfq_dtype dtype, int drafted, size_t* bytes) {
+    if (!bytes) return fail(DFQ_ERR_INVALID_ARGUMENT, "null bytes");
+    *bytes = 0;
+    if (!ctx) return fail(DFQ_ERR_INVALID_ARGUMENT, "null context");
+    const dfq_status s = check_sizes(batch, rows, V, dtype);
+    if (s) return s;
+    *bytes = plan_accept(dfq_num_cus(ctx), batch, rows, V, dtype, drafted && rows > 1).bytes;
+    return DFQ_OK;
+}
+
+dfq_status dfq_sample_accept(dfq_ctx* ctx, const void* logits, int64_t batch_stride,
+                             int64_t row_stride, const void* draft_logits,
+                             int64_t draft_batch_stride, int64_t draft_row_stride, int batch,
+                             int rows, int V, dfq_dtype dtype, const int32_t* drafts,
+                             const int32_t* draft_lengths, const float* uniforms,
+                             const float* temperatures, float temperature,
+                             const float* draft_temperatures, float draft_temperature,
+                             int32_t* tokens, int32_t* accepted, float* chances, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+    if (!ctx) return fail(DFQ_ERR_INVALID_ARGUMENT, "null context");
+    dfq_status s = check_sizes(batch, rows, V, dtype);
+    if (s) return s;
+    if (!logits || !uniforms || !tokens || !accepted)
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "null logits, uniforms, tokens or accepted");
+    if (rows > 1 && !drafts) return fail(DFQ_ERR_INVALID_ARGUMENT, "null drafts");
+    if ((rows > 1 && row_stride < V) || (batch > 1 && batch_stride < V))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "a stride is smaller than a row");
+    const bool drafted = draft_logits && rows > 1;
+    if (drafted && ((rows > 2 && draft_row_stride < V) || (batch > 1 && draft_batch_stride < V)))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "a draft stride is smaller than a row");
+    const size_t size = dtype_size(dtype);
+    if (!aligned(logits, size) || !aligned(draft_logits, size) || !aligned(drafts, 4) ||
+        !aligned(draft_lengths, 4) || !aligned(uniforms, 4) || !aligned(temperatures, 4) ||
+        !aligned(draft_temperatures, 4) || !aligned(tokens, 4) || !aligned(accepted, 4) ||
+        !aligned(chances, 4))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "misaligned buffer");
+    if ((!temperatures && !(temperature >= 0.0f && std::isfinite(temperature))) ||
+        (drafted && !draft_temperatures &&
+         !(draft_temperature >= 0.0f && std::isfinite(draft_temperature))))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "temperatures are finite and not negative");
+    const AcceptPlan a = plan_accept(dfq_num_cus(ctx), batch, rows, V, dtype, drafted);
+    const int64_t ranges = (int64_t)batch * a.all_rows * a.splits;
+    const int64_t chunks = (int64_t)batch * a.chunks;
+    if (ranges > INT32_MAX || chunks > INT32_MAX)
+        return fail(DFQ_ERR_UNSUPPORTED, "grid too large");
+    if (!workspace || workspace_bytes < a.bytes)
+        return fail(DFQ_ERR_WORKSPACE, "workspace of %zu bytes needed (got %zu)", a.bytes,
+                    workspace ? workspace_bytes : (size_t)0);
+    if (!aligned(workspace, 16))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
+    char* const ws = (char*)workspace;
+    AcceptParams p{};
+    p.logits = logits;
+    p.draft_logits = drafted ? draft_logits : nullptr;
+    p.drafts = drafts;
+    p.lengths = draft_lengths;
+    p.uniforms = uniforms;
+    p.temperatures = temperatures;
+    p.draft_temperatures = draft_temperatures;
+    p.tokens = tokens;
+    p.accepted = accepted;
+    p.chances = chances;
+    p.parts = (AcceptPart*)ws;
+    p.draws = (AcceptDraw*)(ws + a.draws);
+    p.totals = (double*)(ws + a.totals);
+    p.weights = (double*)(ws + a.weights);
+    p.batch_stride = batch_stride;
+    p.row_stride = row_stride;
+    p.draft_batch_stride = draft_batch_stride;
+    p.draft_row_stride = draft_row_stride;
+    p.temperature = temperature;
+    p.draft_temperature = draft_temperature;
+    p.batch = batch;
+    p.rows = rows;
+    p.all_rows = a.all_rows;
+    p.vocab = V;
+    p.splits = a.splits;
+    p.chunks = a.chunks;
+    const VerifyOps* ops;
+    if ((s = ctx_verify_ops(ctx, &ops))) return s;
+    DeviceScope scope(ctx);
+    const AcceptKernels& fn = ops->accept[(int)dtype];
+    void* args[] = {&p};
+    hipError_t e = hipSuccess;
+    const auto launch = [&](hipFunction_t f, int64_t groups, int threads) {
+        if (e == hipSuccess)
+            e = hipModuleLaunchKernel(f, (unsigned)groups, 1, 1, threads, 1, 1, 0,
+                                      (hipStream_t)stream, args, nullptr);
+    };
+    launch(fn.sums, ranges, DFQ_KV_THREADS);
+    launch(fn.decide, batch, 64);
+    if (drafted) launch(fn.totals, chunks, DFQ_KV_THREADS);
+    launch(fn.weights, chunks, DFQ_KV_THREADS);
+    launch(fn.pick, batch, DFQ_KV_THREADS);
+    return e == hipSuccess ? DFQ_OK : hip_error(e, "launch dfq_sample_accept");
+}
+
+}  // extern "C"

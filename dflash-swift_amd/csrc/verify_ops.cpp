@@ -13,11 +13,12 @@
 
 #include "dflash_qmm.h"
 #include "kv_params.h"
-#include "qmm_internal.h"
+#include "verify_ops.h"
 
 #if !defined(DFQ_KV_HSACO_PATH) || !defined(DFQ_LOGPROBS_HSACO_PATH) || \
     !defined(DFQ_ATTN64_HSACO_PATH) || !defined(DFQ_ATTN128_HSACO_PATH) || \
-    !defined(DFQ_ATTN256_HSACO_PATH)
+    !defined(DFQ_ATTN256_HSACO_PATH) || !defined(DFQ_ROPE_HSACO_PATH) || \
+    !defined(DFQ_ACCEPT_HSACO_PATH)
 #error "DFQ_*_HSACO_PATH must name the gfx950 code objects to embed"
 #endif
 
@@ -36,26 +37,10 @@ DFQ_EMBED(dfq_logprobs_hsaco, DFQ_LOGPROBS_HSACO_PATH)
 DFQ_EMBED(dfq_attn64_hsaco, DFQ_ATTN64_HSACO_PATH)
 DFQ_EMBED(dfq_attn128_hsaco, DFQ_ATTN128_HSACO_PATH)
 DFQ_EMBED(dfq_attn256_hsaco, DFQ_ATTN256_HSACO_PATH)
+DFQ_EMBED(dfq_rope_hsaco, DFQ_ROPE_HSACO_PATH)
+DFQ_EMBED(dfq_accept_hsaco, DFQ_ACCEPT_HSACO_PATH)
 
 namespace dfq {
-
-/* One format of a cache: [head_dim 64/128/256][bits 4/8][group 32/64/128][bf16/f16]; groups wider
- * than the head have no kernels. */
-struct CacheKernels {
-    hipFunction_t append = nullptr, read = nullptr, join = nullptr;
-    hipFunction_t attention[2] = {};  // up to 1 and 2 row tiles (see attention_tiles)
-    int resident[2] = {};             // their workgroups that a CU holds at once
-};
-
-struct VerifyOps {
-    hipModule_t kv = nullptr, logprobs = nullptr, attention[3] = {};
-    CacheKernels cache[3][2][3][2];
-    hipFunction_t logprobs_part[3] = {}, logprobs_join[3] = {};  // [bf16/f16/f32]
-};
-
-static dfq_status hip_error(hipError_t e, const char* what) {
-    return fail(DFQ_ERR_HIP, "%s: %s (%d)", what, hipGetErrorString(e), (int)e);
-}
 
 /* The most tiles of 16 rows that attention kernels take in one pass.  Two read and unpack the
  * codes once for both: 16 sequences of 8 rows of 40 heads over a shared 16384-token prefix take
@@ -112,6 +97,30 @@ static dfq_status resolve(VerifyOps* o) {
         if ((e = hipModuleGetFunction(&o->logprobs_join[t], o->logprobs, name)) != hipSuccess)
             return hip_error(e, name);
     }
+    if ((e = hipModuleLoadData(&o->rope, dfq_rope_hsaco)) != hipSuccess)
+        return hip_error(e, "hipModuleLoadData(gfx950 rotation object)");
+    static const char* kWay[3] = {"halves", "pairs", "any"};
+    for (int n = 0; n < 2; ++n)
+        for (int w = 0; w < 3; ++w)
+            for (int t = 0; t < 3; ++t) {
+                snprintf(name, sizeof name, "dfq_%s_%s_%s", n ? "norm_rope" : "rope", kWay[w],
+                         kDt[t]);
+                if ((e = hipModuleGetFunction(&o->rotate[n][w][t], o->rope, name)) != hipSuccess)
+                    return hip_error(e, name);
+            }
+    if ((e = hipModuleLoadData(&o->sample, dfq_accept_hsaco)) != hipSuccess)
+        return hip_error(e, "hipModuleLoadData(gfx950 sampled-accept object)");
+    for (int t = 0; t < 3; ++t) {
+        AcceptKernels& a = o->accept[t];
+        const struct { const char* op; hipFunction_t* fn; } parts[] = {
+            {"sums", &a.sums}, {"decide", &a.decide}, {"totals", &a.totals},
+            {"weights", &a.weights}, {"pick", &a.pick}};
+        for (const auto& part : parts) {
+            snprintf(name, sizeof name, "dfq_accept_%s_%s", part.op, kDt[t]);
+            if ((e = hipModuleGetFunction(part.fn, o->sample, name)) != hipSuccess)
+                return hip_error(e, name);
+        }
+    }
     return DFQ_OK;
 }
 
@@ -132,6 +141,8 @@ void verify_ops_unload(VerifyOps* o) {
     if (!o) return;
     if (o->kv) (void)hipModuleUnload(o->kv);
     if (o->logprobs) (void)hipModuleUnload(o->logprobs);
+    if (o->rope) (void)hipModuleUnload(o->rope);
+    if (o->sample) (void)hipModuleUnload(o->sample);
     for (hipModule_t m : o->attention)
         if (m) (void)hipModuleUnload(m);
     delete o;
@@ -143,13 +154,8 @@ using namespace dfq;
 
 namespace {
 
-bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
-
 int dim_index(int dim) { return dim == 64 ? 0 : dim == 128 ? 1 : dim == 256 ? 2 : -1; }
 int group_index(int gs) { return gs == 32 ? 0 : gs == 64 ? 1 : gs == 128 ? 2 : -1; }
-
-/* The launch grid's limits in y and z. */
-constexpr int kMostGrid = 65535;
 
 dfq_status check_format(const dfq_kv_cache* c) {
     if (c->dtype != DFQ_BF16 && c->dtype != DFQ_F16)
@@ -263,14 +269,6 @@ struct AttentionPlan {
                                  (int64_t)batch * own_splits * own_blocks);
     }
 };
-
-/* by 0: of a part of the call that is not there, and nothing is divided */
-Divisor divisor(int by) {
-    const uint64_t d = by > 0 ? by : 1;
-    int shift = 0;
-    while ((1ull << shift) < d) ++shift;
-    return {(uint32_t)by, (uint32_t)((((1ull << shift) - d) << 32) / d + 1), shift};
-}
 
 /* Tokens that a workgroup takes in one round, 32 a wave. */
 constexpr int kRoundTokens = DFQ_KV_THREADS / 2;

@@ -22,10 +22,11 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import struct
 import threading
 
 __all__ = [
-    "BF16", "F16", "F32", "DfqError", "Context", "KVCache", "PackedWeight",
+    "BF16", "F16", "F32", "DfqError", "Context", "KVCache", "PackedWeight", "Rope",
     "SmallMQuantizedMatmul",
     "QuantizedLinear",
     "SmallMQuantizedLinear", "Model", "enable_small_m_quantized_matmul", "library_path",
@@ -69,6 +70,21 @@ class _KVCacheDesc(ctypes.Structure):
         ("head_dim", ctypes.c_int), ("bits", ctypes.c_int), ("group_size", ctypes.c_int),
         ("dtype", ctypes.c_int),
     ]
+
+
+class _RopeTable(ctypes.Structure):
+    _fields_ = [("turns", ctypes.c_void_p), ("rotary_dim", ctypes.c_int),
+                ("interleaved", ctypes.c_int), ("amplitude", ctypes.c_float)]
+
+
+class _RopeDesc(ctypes.Structure):
+    _fields_ = [("base", ctypes.c_double), ("rotary_dim", ctypes.c_int),
+                ("scaling", ctypes.c_int)] + [
+        (n, ctypes.c_double) for n in ("factor", "original_length", "low_freq_factor",
+                                       "high_freq_factor", "beta_fast", "beta_slow")]
+
+
+_pack_heads = struct.Struct("@PPqqqqqqi4x").pack   # dfq_heads
 
 
 class _TensorInfo(ctypes.Structure):
@@ -174,6 +190,15 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         "dfq_cache_attention_workspace_bytes": ([P, P, I, P, I, I, I, I, Z], I),
         "dfq_cache_attention": ([P, P, I, P, P, I, P, P, L, P, P, I, I, I,
                                  ctypes.c_float, P, S, P], I),
+        "dfq_rope_frequencies": ([ctypes.POINTER(_RopeDesc), ctypes.POINTER(ctypes.c_double),
+                                  ctypes.POINTER(ctypes.c_float)], I),
+        "dfq_rope_turns": ([ctypes.POINTER(ctypes.c_double), I, P], I),
+        "dfq_rope": ([P, P, P, P, I, I, I, I, I, P, P, I, P], I),
+        "dfq_qk_norm_rope": ([P, P, P, P, P, P, I, ctypes.c_float, ctypes.c_float, I, I, I, I, I,
+                              P, P, P], I),
+        "dfq_sample_accept_workspace_bytes": ([P, I, I, I, I, I, Z], I),
+        "dfq_sample_accept": ([P, P, L, L, P, L, L, I, I, I, I, P, P, P, P, ctypes.c_float, P,
+                               ctypes.c_float, P, P, P, P, S, P], I),
         "dfq_token_logprobs_workspace_bytes": ([P, I, I, I, Z], I),
         "dfq_token_logprobs": ([P, P, L, I, I, I, P, I, P, P, P, P, P, S, P], I),
     }
@@ -595,6 +620,90 @@ class Context:
             _check(st, "dfq_cache_attention")
         return out, lse
 
+    # ---- rotary positions ------------------------------------------------------------------
+    def rope(self, rope, q, k=None, start=0, starts=None, positions=None, inverse=False,
+             q_out=None, k_out=None, stream=None):
+        """q (and k) [batch, rows, heads, head_dim] turned to their positions by a Rope table:
+        row m of sequence b is at start + starts[b] + m (starts: int32 [batch] on the device) or
+        at positions[b, m] (int32 [batch, rows]).  inverse turns back.  Heads may be cut from a
+        fused output (any strides, contiguous channels); q_out and k_out may be q and k.  Returns
+        q_out, or (q_out, k_out) with k."""
+        return self._rotate(rope, q, k, None, start, starts, positions, inverse, q_out, k_out,
+                            stream)
+
+    def qk_norm_rope(self, rope, q, k=None, q_weight=None, k_weight=None, eps=1e-6,
+                     weight_offset=0.0, start=0, starts=None, positions=None, q_out=None,
+                     k_out=None, stream=None):
+        """The RMS norm of each head of q (and k), x (weight + weight_offset) / sqrt(mean x^2 +
+        eps), and its rotation, in one pass; otherwise as `rope`.  Weights [head_dim] are in q's
+        dtype or both fp32 (None: ones); rope None takes the norms alone."""
+        return self._rotate(rope, q, k, (q_weight, k_weight, eps, weight_offset), start, starts,
+                            positions, False, q_out, k_out, stream)
+
+    def _rotate(self, rope, q, k, norms, start, starts, positions, inverse, q_out, k_out, stream):
+        import torch
+        if stream is not None and self._is_other(stream):
+            with self._current(stream):
+                return self._rotate(rope, q, k, norms, start, starts, positions, inverse, q_out,
+                                    k_out, None)
+        shape, device = q.shape, self.device
+        if len(shape) != 4:
+            raise ValueError("q is [batch, rows, heads, head_dim]")
+        batch, rows, heads, dim = shape
+        if q.get_device() != device or \
+                k is not None and k.get_device() != device or \
+                rope is not None and rope.index != device or \
+                starts is not None and starts.get_device() != device or \
+                positions is not None and positions.get_device() != device or \
+                q_out is not None and q_out.get_device() != device or \
+                k_out is not None and k_out.get_device() != device:
+            self._elsewhere(q, k, rope and rope.turns, starts, positions, q_out, k_out)
+        if max(batch, rows, heads, dim, start, -start) > _INT_MAX:
+            raise ValueError("batch, rows, heads, head_dim or start past a C int")
+        if q_out is None:
+            q_out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        packed_q, packed_k = _heads("q", q, q_out, q), None
+        if k is not None:
+            if len(k.shape) != 4 or k.shape[0] != batch or k.shape[1] != rows or \
+                    k.shape[3] != dim or k.dtype != q.dtype:
+                raise ValueError("k is [batch, rows, heads, head_dim], with q's but for heads, in "
+                                 "q's dtype")
+            if k_out is None:
+                k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+            packed_k = _heads("k", k, k_out, k)
+        elif k_out is not None:
+            raise ValueError("k_out without k")
+        d_starts = _check_int32("starts", starts, (batch,))
+        d_positions = _check_int32("positions", positions, (batch, rows))
+        table = rope.table if rope is not None else None
+        dt = dtype_code(q)
+        if norms is None:
+            st = self.lib.dfq_rope(self.handle, table, packed_q, packed_k, dim, dt, batch, rows,
+                                   start, d_starts, d_positions, inverse, self._stream_of(stream))
+            if st:
+                _check(st, "dfq_rope")
+            return q_out if k is None else (q_out, k_out)
+        q_weight, k_weight, eps, offset = norms
+        wt = dt
+        for t in (q_weight, k_weight):
+            if t is None:
+                continue
+            if t.get_device() != device:
+                self._elsewhere(q, t)
+            kind = t.dtype
+            if t.shape != (dim,) or not t.is_contiguous() or \
+                    kind is not q.dtype and kind is not torch.float32:
+                raise ValueError("weights are contiguous [head_dim] in q's dtype or fp32")
+            wt = dtype_code(kind)
+        if q_weight is not None and k_weight is not None and q_weight.dtype is not k_weight.dtype:
+            raise ValueError("both weights have one dtype")
+        st = self.lib.dfq_qk_norm_rope(self.handle, table, packed_q, packed_k, _ptr(q_weight),
+                                       _ptr(k_weight), wt, eps, offset, dim, dt, batch, rows,
+                                       start, d_starts, d_positions, self._stream_of(stream))
+        if st:
+            _check(st, "dfq_qk_norm_rope")
+        return q_out if k is None else (q_out, k_out)
+
     def token_logprobs(self, logits, tokens=None, top_k=0, ws=None, stream=None):
         """(logprobs [M], entropy [M], top_tokens [M, top_k], top_logprobs [M, top_k]) of logits
         [M, V] (rows may be strided) and tokens [M] int32; what is not asked for is None."""
@@ -646,6 +755,77 @@ class Context:
         if st:
             _check(st, "dfq_token_logprobs")
         return lp, entropy, ids, top
+
+    def sample_accept(self, logits, uniforms, drafts=None, draft_logits=None, temperature=1.0,
+                      draft_temperature=None, draft_lengths=None, ws=None, stream=None):
+        """(tokens [batch, rows], accepted [batch], chances [batch, rows-1]) of drafts verified
+        against the probabilities of logits [batch, rows, V] (dfq_sample_accept): drafts int32
+        [batch, rows-1] (None where rows is 1), of which draft_lengths int32 [batch] count;
+        draft_logits [batch, rows-1, V] are what they were drawn from, None where each was
+        certain.  uniforms fp32 [batch, rows] are the random numbers.  Temperatures are numbers or
+        fp32 [batch]; draft_temperature defaults to temperature."""
+        import torch
+        if stream is not None and self._is_other(stream):
+            with self._current(stream):
+                return self.sample_accept(logits, uniforms, drafts, draft_logits, temperature,
+                                          draft_temperature, draft_lengths, ws)
+        device, shape = self.device, logits.shape
+        if len(shape) != 3:
+            raise ValueError("logits are [batch, rows, V]")
+        batch, rows, V = shape
+        if draft_temperature is None:
+            draft_temperature = temperature
+        t, dt = (x if isinstance(x, torch.Tensor) else None
+                 for x in (temperature, draft_temperature))
+        for a in (logits, uniforms, drafts, draft_logits, t, dt, draft_lengths, ws):
+            if a is not None and a.get_device() != device:
+                self._elsewhere(logits, uniforms, drafts, draft_logits, t, dt, draft_lengths, ws)
+        if max(batch, rows, V) > _INT_MAX:
+            raise ValueError("batch, rows or V past a C int")
+        s, one = logits.stride()[:2], logits.stride(2)
+        if one != 1 and V > 1:
+            raise ValueError("a row's logits must be contiguous")
+        if (drafts is None) != (rows == 1):
+            raise ValueError("a block of rows has rows - 1 drafts")
+        d_drafts = _check_int32("drafts", drafts, (batch, rows - 1))
+        d_lengths = _check_int32("draft_lengths", draft_lengths, (batch,))
+        d_uniforms = _check_f32("uniforms", uniforms, (batch, rows))
+        d_t = _check_f32("temperature", t, (batch,))
+        d_dt = _check_f32("draft_temperature", dt, (batch,))
+        p_draft, ds = None, (0, 0)
+        if draft_logits is not None:
+            if draft_logits.shape != (batch, rows - 1, V) or draft_logits.dtype != logits.dtype:
+                raise ValueError("draft_logits are [batch, rows-1, V] in the logits' dtype")
+            ds = draft_logits.stride()
+            if ds[2] != 1 and V > 1:
+                raise ValueError("a row's draft logits must be contiguous")
+            p_draft = draft_logits.data_ptr() if rows > 1 else None
+        tokens = torch.empty((batch, rows), dtype=torch.int32, device=logits.device)
+        accepted = torch.empty(batch, dtype=torch.int32, device=logits.device)
+        chances = torch.empty((batch, rows - 1), dtype=torch.float32, device=logits.device)
+        code = dtype_code(logits)
+        stream = self._stream_of(stream)
+        own_ws = ws is None
+        with self._lock if own_ws else _no_lock:
+            if own_ws:
+                ws = self.workspace_uncleared(1, stream)
+            for again in (own_ws, False):
+                st = self.lib.dfq_sample_accept(
+                    self.handle, logits.data_ptr(), s[0], s[1], p_draft, ds[0], ds[1], batch, rows,
+                    V, code, d_drafts, d_lengths, d_uniforms, d_t, 0.0 if d_t else temperature,
+                    d_dt, 0.0 if d_dt else draft_temperature, tokens.data_ptr(),
+                    accepted.data_ptr(), chances.data_ptr() if rows > 1 else None, ws.data_ptr(),
+                    ws.numel(), stream)
+                if st != _ERR_WORKSPACE or not again:
+                    break
+                need = ctypes.c_size_t()
+                _check(self.lib.dfq_sample_accept_workspace_bytes(
+                    self.handle, batch, rows, V, code, p_draft is not None, ctypes.byref(need)),
+                    "dfq_sample_accept_workspace_bytes")
+                ws = self.workspace_uncleared(need.value, stream)
+        if st:
+            _check(st, "dfq_sample_accept")
+        return tokens, accepted, chances
 
     def _elsewhere(self, *arrays):
         """The refusal of tensors that are not on this context's GPU: a kernel would take a host
@@ -824,6 +1004,86 @@ def _check_int32(name, t, shape):
     if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} is a contiguous int32 tensor of shape {shape}")
     return t.data_ptr()
+
+
+def _check_f32(name, t, shape):
+    if t is None:
+        return None
+    import torch
+    if t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} is a contiguous fp32 tensor of shape {shape}")
+    return t.data_ptr()
+
+
+def _heads(name, t, out, like):
+    """dfq_heads of t [batch, rows, heads, head_dim] into out."""
+    a, b = t.stride(), out.stride()
+    if t.shape[3] > 1 and (a[3] != 1 or b[3] != 1):
+        raise ValueError(f"{name}: a head's channels must be contiguous")
+    if out.shape != like.shape or out.dtype != like.dtype:
+        raise ValueError(f"{name}_out is of {name}'s shape and dtype")
+    if not out.is_contiguous():
+        # heads that share elements would be written by several lanes
+        room = out.shape[3]
+        for stride, n in sorted((s, n) for s, n in zip(b[:3], out.shape) if n > 1):
+            if stride < room:
+                raise ValueError(f"{name}_out has heads that overlap")
+            room = stride * n
+    return _pack_heads(t.data_ptr(), out.data_ptr(), a[0], a[1], a[2], b[0], b[1], b[2],
+                       t.shape[2])
+
+
+class Rope:
+    """A table of rotary frequencies (dfq_rope_table): `turns` int64 [rotary_dim/2] on the device,
+    2^-64 turns a position each.
+
+    scaling is None or a dict of "type" -- linear, ntk, bands or yarn (dfq_rope_scaling) -- and the
+    numbers that it takes: factor, original_length, low_freq_factor and high_freq_factor (bands),
+    beta_fast and beta_slow (yarn; 32 and 1 where they are left out).  frequencies takes radians a
+    position of each pair instead of base and scaling.  amplitude is the factor of the rotated
+    channels, where it is not what the scaling says."""
+
+    _kinds = {"linear": 1, "ntk": 2, "bands": 3, "yarn": 4}
+
+    def __init__(self, rotary_dim, base=10000.0, interleaved=False, scaling=None,
+                 frequencies=None, amplitude=None, device="cuda"):
+        import torch
+        n = rotary_dim // 2
+        lib = load_library()
+        if rotary_dim < 2 or rotary_dim % 2 or rotary_dim > _INT_MAX:
+            raise ValueError("rotary_dim is even and at least 2")
+        f, a = (ctypes.c_double * n)(), ctypes.c_float(1.0)
+        if frequencies is not None:
+            if scaling is not None:
+                raise ValueError("frequencies take the place of base and scaling")
+            values = [float(x) for x in frequencies]
+            if len(values) != n:
+                raise ValueError(f"{n} frequencies for {rotary_dim} channels")
+            f[:] = values
+        else:
+            given = dict(scaling or {})
+            kind = given.pop("type", None)
+            if kind is not None and kind not in self._kinds or kind is None and given:
+                raise ValueError(f"scaling is of type {', '.join(self._kinds)}, got {kind!r}")
+            d = _RopeDesc(base=base, rotary_dim=rotary_dim, scaling=self._kinds.get(kind, 0),
+                          beta_fast=32.0, beta_slow=1.0)
+            known = {name for name, _ in _RopeDesc._fields_[3:]}
+            for name, value in given.items():
+                if name not in known:
+                    raise ValueError(f"scaling has no {name!r}")
+                setattr(d, name, value)
+            _check(lib.dfq_rope_frequencies(ctypes.byref(d), f, ctypes.byref(a)),
+                   "dfq_rope_frequencies")
+        self.frequencies = list(f)
+        turns = (ctypes.c_int64 * n)()
+        _check(lib.dfq_rope_turns(f, n, turns), "dfq_rope_turns")
+        self.rotary_dim, self.interleaved = rotary_dim, bool(interleaved)
+        self.amplitude = a.value if amplitude is None else float(amplitude)
+        self.turns = torch.tensor(list(turns), dtype=torch.int64).to(device)
+        self.index = self.turns.get_device()   # the GPU's; -1 in host memory, which no call takes
+        self._table = _RopeTable(self.turns.data_ptr(), rotary_dim, self.interleaved,
+                                 self.amplitude)
+        self.table = ctypes.addressof(self._table)
 
 
 class KVCache:

@@ -379,6 +379,79 @@ dfq_status dfq_cache_attention(dfq_ctx* ctx, const dfq_kv_cache* prefix, int pre
                                float* lse, int batch, int rows, int q_heads, float scale,
                                void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- rotary positions of a verify pass's queries and keys --------------------------------- */
+/* Position p turns pair i of a head's rotary_dim/2 rotated pairs by p * frequency[i] radians:
+ * (a, b) -> amplitude * (a cos - b sin, b cos + a sin).  Pair i is (i, i + rotary_dim/2) or,
+ * interleaved, (2i, 2i + 1); the channels behind rotary_dim stay as they are.  `turns` (device
+ * memory, 8-byte aligned) are the frequencies as fractions of a turn in units of 2^-64
+ * (dfq_rope_turns), so that an angle is right to 2^-32 turns at every position.  The reference's
+ * target rotates its queries and keys in the model library (mlx-swift-lm), between the projections
+ * that the swap replaces (Sources/DFlashKit/SmallMQuantizedMatmul.swift:303-317). */
+typedef struct dfq_rope_table {
+    const uint64_t* turns;    /* [rotary_dim/2]                                             */
+    int rotary_dim;           /* even, 2 .. head_dim                                        */
+    int interleaved;
+    float amplitude;          /* factor of the rotated channels (1, but for dfq_rope_frequencies') */
+} dfq_rope_table;
+
+typedef enum dfq_rope_scaling {
+    DFQ_ROPE_PLAIN = 0,  /* base^(-2i/rotary_dim)                                               */
+    DFQ_ROPE_LINEAR = 1, /* those divided by `factor`                                           */
+    DFQ_ROPE_NTK = 2,    /* the base times factor^(R/(R-2)), R = rotary_dim                     */
+    DFQ_ROPE_BANDS = 3,  /* divided by `factor` where a pair turns low_freq_factor times or less
+                          * over original_length, kept from high_freq_factor times on, mixed
+                          * between them in proportion                                          */
+    DFQ_ROPE_YARN = 4    /* kept up to the pair that turns beta_fast times over original_length,
+                          * divided by `factor` from that of beta_slow on, mixed between them by
+                          * the pair's index; amplitude 0.1 ln(factor) + 1 (1 for factor <= 1)  */
+} dfq_rope_scaling;
+
+typedef struct dfq_rope_desc {
+    double base;              /* above 1                                                    */
+    int rotary_dim;
+    dfq_rope_scaling scaling;
+    double factor, original_length, low_freq_factor, high_freq_factor, beta_fast, beta_slow;
+} dfq_rope_desc;
+
+/* Host only: frequencies[rotary_dim/2] in radians a position, and the amplitude (may be NULL).
+ * Fields that the scaling does not use are not looked at. */
+dfq_status dfq_rope_frequencies(const dfq_rope_desc* desc, double* frequencies, float* amplitude);
+/* Host only: any finite frequencies as turns in host memory, to be copied to the device. */
+dfq_status dfq_rope_turns(const double* frequencies, int count, uint64_t* turns);
+
+/* The heads of one tensor, channels side by side: channel 0 of head h of row m of sequence b is
+ * at b*in_batch + m*in_row + h*in_head elements of `in`, and likewise of `out` (any strides that
+ * keep the heads of `out` apart; any element alignment).  `out` is `in` with the same strides, or
+ * memory that no input overlaps. */
+typedef struct dfq_heads {
+    const void* in;
+    void* out;
+    int64_t in_batch, in_row, in_head, out_batch, out_row, out_head;
+    int heads;
+} dfq_heads;
+
+/* Rotates the heads of q and k (k may be NULL) in one launch; inverse != 0 turns back (the
+ * rotation's transpose).  Row m of sequence b is at position start + starts[b] + m (starts:
+ * device memory, may be NULL for zeros) or at positions[b*rows + m] (device memory, as draft
+ * trees need them; then start is 0 and starts NULL).  Positions may be negative.  head_dim is even
+ * and at most 512; bf16, fp16 or fp32, in fp32 and rounded once.  Asynchronous on `stream`. */
+dfq_status dfq_rope(dfq_ctx* ctx, const dfq_rope_table* rope, const dfq_heads* q,
+                    const dfq_heads* k, int head_dim, dfq_dtype dtype, int batch, int rows,
+                    int start, const int32_t* starts, const int32_t* positions, int inverse,
+                    void* stream);
+
+/* The RMS norm of each head, x * (weight + weight_offset) / sqrt(mean(x^2) + eps), and the
+ * rotation of its result, in one pass and rounded once.  q_weight and k_weight [head_dim] in
+ * weight_dtype (the heads' or fp32; NULL: factors of 1, without the offset); weight_offset is 0,
+ * or 1 for weights held as their distance from 1.  rope may be NULL (norms alone).  The squares
+ * are summed in fp32: a head whose sum passes 3.4e38 comes out as 0, or NaN where it holds an
+ * infinity.  Otherwise as dfq_rope. */
+dfq_status dfq_qk_norm_rope(dfq_ctx* ctx, const dfq_rope_table* rope, const dfq_heads* q,
+                            const dfq_heads* k, const void* q_weight, const void* k_weight,
+                            dfq_dtype weight_dtype, float eps, float weight_offset, int head_dim,
+                            dfq_dtype dtype, int batch, int rows, int start, const int32_t* starts,
+                            const int32_t* positions, void* stream);
+
 /* ---- log probabilities of a verify pass's logits ----------------------------------------- */
 #define DFQ_TOP_MAX 32 /* most alternatives of a row */
 /* For each of M rows of V logits (bf16, fp16 or fp32, row_stride elements apart), in fp32:
@@ -399,6 +472,46 @@ dfq_status dfq_token_logprobs(dfq_ctx* ctx, const void* logits, int64_t row_stri
                               dfq_dtype dtype, const int32_t* tokens, int top_k, float* logprobs,
                               float* entropy, int32_t* top_tokens, float* top_logprobs,
                               void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- sampled accept of a verify pass ------------------------------------------------------ */
+#define DFQ_ACCEPT_ROWS 64 /* most rows of a block */
+/* Verifies the drafts of `batch` sequences against the target's probabilities, and draws the token
+ * behind them.  Row i < rows-1 of a sequence's logits [batch][rows][V] judges its draft i
+ * (drafts [batch][rows-1]; draft_lengths [batch] counts those that it brings, rows-1 where NULL,
+ * clamped to 0..rows-1), row n the token behind n drafts; rows = 1 draws a token of each row.  With
+ * p = softmax(logits / T) and q = softmax(draft_logits / Td) of the draft's own logits
+ * [batch][rows-1][V], or q(draft) = 1 where draft_logits is NULL or Td is 0:
+ *   chances[b][i]   min(1, p_i(draft i) / q_i(draft i)) (1 where q is 0 and p is not); 0 behind the
+ *                   sequence's drafts (may be NULL)
+ *   accepted[b]     the drafts in front of the first with u[b][i] * q_i >= p_i, all where there
+ *                   is none
+ *   tokens[b][..]   those drafts, then the token drawn from max(p - q, 0) of the refusing row (of
+ *                   p where that is 0 throughout), or from p of the row behind the drafts, then -1
+ * A token is drawn as the first whose running sum of probabilities exceeds u[b][rows-1] times their
+ * sum.  uniforms u [batch][rows] are in [0, 1) and the caller's, so that a call with the same
+ * numbers gives the same tokens, distributed as p (chances are right to 2^-20 of themselves, the
+ * drawn token is that of 64-bit sums).  temperatures and draft_temperatures [batch] are in device
+ * memory; NULL: `temperature`, `draft_temperature` for all.  T = 0 takes p = 1 for the row's
+ * argmax, as dfq_argmax_accept finds it.  A logit of -inf has probability 0.  A row with a NaN or
+ * +inf, with nothing above -inf, or with a temperature of its sequence that is negative or not
+ * finite has no distribution: a draft judged by such a row of the target or the draft is refused
+ * (chance 0), and the token in its place is -1.  So is refused a draft outside 0..V-1 (the token is
+ * then drawn as for q = 0 in all of p, or from p - q).  All strides in elements, rows contiguous.
+ * The workspace (dfq_sample_accept_workspace_bytes, drafted != 0 with draft logits; 16-byte
+ * aligned) needs no clearing, and is shared no more than dfq_cache_attention's.  The reference
+ * accepts greedily alone (acceptedPrefix, DFlashSpeculativeGenerator.swift:555-571;
+ * dfq_argmax_accept).  Asynchronous on `stream`. */
+dfq_status dfq_sample_accept_workspace_bytes(dfq_ctx* ctx, int batch, int rows, int V,
+                                             dfq_dtype dtype, int drafted, size_t* bytes);
+dfq_status dfq_sample_accept(dfq_ctx* ctx, const void* logits, int64_t batch_stride,
+                             int64_t row_stride, const void* draft_logits,
+                             int64_t draft_batch_stride, int64_t draft_row_stride, int batch,
+                             int rows, int V, dfq_dtype dtype, const int32_t* drafts,
+                             const int32_t* draft_lengths, const float* uniforms,
+                             const float* temperatures, float temperature,
+                             const float* draft_temperatures, float draft_temperature,
+                             int32_t* tokens, int32_t* accepted, float* chances, void* workspace,
+                             size_t workspace_bytes, void* stream);
 
 /* ---- the drop-in layer (SmallMQuantizedMatmul.swift:227-317) -------------------------- */
 
