@@ -76,11 +76,10 @@ dfq_status dfq_sample_accept(dfq_ctx* ctx, const void* logits, int64_t batch_str
     if (!logits || !uniforms || !tokens || !accepted)
         return fail(DFQ_ERR_INVALID_ARGUMENT, "null logits, uniforms, tokens or accepted");
     if (rows > 1 && !drafts) return fail(DFQ_ERR_INVALID_ARGUMENT, "null drafts");
-    if ((rows > 1 && row_stride < V) || (batch > 1 && batch_stride < V))
-        return fail(DFQ_ERR_INVALID_ARGUMENT, "a stride is smaller than a row");
     const bool drafted = draft_logits && rows > 1;
-    if (drafted && ((rows > 2 && draft_row_stride < V) || (batch > 1 && draft_batch_stride < V)))
-        return fail(DFQ_ERR_INVALID_ARGUMENT, "a draft stride is smaller than a row");
+    if (batch_stride < 0 || row_stride < 0 ||
+        (drafted && (draft_batch_stride < 0 || draft_row_stride < 0)))
+        return fail(DFQ_ERR_INVALID_ARGUMENT, "negative stride");
     const size_t size = dtype_size(dtype);
     if (!aligned(logits, size) || !aligned(draft_logits, size) || !aligned(drafts, 4) ||
         !aligned(draft_lengths, 4) || !aligned(uniforms, 4) || !aligned(temperatures, 4) ||

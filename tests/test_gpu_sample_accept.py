@@ -1,0 +1,353 @@
+"""The sampled accept against its definition in 64 bits: shapes, types, temperatures, masks, rows
+without a distribution, borders, strides, and the law that its tokens follow."""
+import itertools
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import dflash_qmm
+from gpu_util import announce
+from rotation_util import DTYPES, accept
+
+pytestmark = pytest.mark.gpu
+
+# A draft's chance: exponentials of up to 2^7 binary places with differences rounded to 24 bits,
+# 2^-24 * 64 of each term that counts (those within 2^-64 of the largest), but as errors of either
+# sign in sums of positive terms and in one common factor (the rate's 2^-25 times the mean of the
+# exponents, under 32); the hardware's exponential and the sums' roundings 2^-22 together.
+CHANCE = 2.0 ** -19
+
+
+def inputs(seed, batch, rows, vocab, name, drafted, spread=3.0, mixed=False):
+    gen = torch.Generator().manual_seed(seed)
+    dt = DTYPES[name]
+    x = (spread * torch.randn(batch, rows, vocab, generator=gen)).to(dt)
+    s = {"logits": x, "uniforms": torch.rand(batch, rows, generator=gen), "drafts": None,
+         "draft_logits": None, "draft_lengths": None,
+         "temperature": 0.3 + torch.rand(batch, generator=gen)}
+    if mixed:
+        s["temperature"][::2] = 0
+    if rows > 1:
+        top = x[:, :-1].float().argmax(-1)
+        other = torch.randint(0, vocab, top.shape, generator=gen)
+        s["drafts"] = torch.where(torch.rand(top.shape, generator=gen) < 0.7, top,
+                                  other).to(torch.int32)
+        s["draft_lengths"] = torch.randint(-1, 3 * rows, (batch,), generator=gen).to(torch.int32)
+        if drafted:
+            y = x[:, :-1].float() + torch.randn(batch, rows - 1, vocab, generator=gen)
+            s["draft_logits"] = y.to(dt)
+    return s
+
+
+def on_gpu(s):
+    return {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in s.items()}
+
+
+def oracle(s):
+    batch = s["logits"].shape[0]
+
+    def numbers(t):
+        return t.double().numpy() if isinstance(t, torch.Tensor) else [float(t)] * batch
+    td = s.get("draft_temperature")
+    return accept(s["logits"].double().numpy(), s["uniforms"].numpy().astype(np.float64),
+                  None if s["drafts"] is None else s["drafts"].numpy(),
+                  None if s["draft_lengths"] is None else s["draft_lengths"].numpy(),
+                  None if s["draft_logits"] is None else s["draft_logits"].double().numpy(),
+                  numbers(s["temperature"]), numbers(s["temperature"] if td is None else td))
+
+
+def check(ctx, s, margin=1e-5):
+    """One call against the definition; no decision of the inputs may lie nearer to its border
+    than the arithmetic's bound."""
+    tokens, accepted, chances, near = oracle(s)
+    assert near > margin, f"these inputs decide by {near}: take others"
+    got = ctx.sample_accept(**on_gpu(s))
+    torch.cuda.synchronize()
+    assert got[0].cpu().tolist() == tokens.tolist()
+    assert got[1].cpu().tolist() == accepted.tolist()
+    off = np.abs(got[2].double().cpu().numpy() - chances)
+    assert (off <= CHANCE * chances + 1e-37).all(), off.max()
+    return got
+
+
+SIZES = [(1, 1, 1), (1, 1, 2), (3, 2, 1), (2, 3, 7), (1, 8, 300), (5, 1, 1000), (1, 4, 2048),
+         (2, 5, 2049), (3, 16, 5000), (2, 64, 257), (33, 1, 4097), (1, 2, 33000), (70, 3, 64)]
+
+
+@pytest.mark.parametrize("batch,rows,vocab", SIZES)
+@pytest.mark.parametrize("name", sorted(DTYPES))
+def test_sizes(ctx, batch, rows, vocab, name):
+    for drafted, mixed in itertools.product((False, True), (False, True)):
+        announce(f"accept {batch} {rows} {vocab} {name} {drafted} {mixed}")
+        check(ctx, inputs(vocab + rows, batch, rows, vocab, name, drafted, mixed=mixed))
+
+
+@pytest.mark.parametrize("name", sorted(DTYPES))
+def test_a_large_vocabulary(ctx, name):
+    for drafted in (False, True):
+        announce(f"accept 151936 {name} {drafted}")
+        s = inputs(3, 2, 3, 151936, name, drafted)
+        s["logits"][:, :, 7::40000] += 12
+        check(ctx, s)
+
+
+@pytest.mark.parametrize("temperature", [1e-40, 1e-30, 1e-4, 0.01, 50.0, 1e20])
+def test_extreme_temperatures(ctx, temperature):
+    for name, drafted in itertools.product(sorted(DTYPES), (False, True)):
+        announce(f"accept T {temperature} {name} {drafted}")
+        s = inputs(17, 4, 4, 500, name, drafted)
+        s["temperature"] = torch.full((4,), temperature)
+        check(ctx, s, margin=0)
+
+
+def test_scalar_and_separate_temperatures(ctx):
+    for t, td in ((0.8, None), (0.7, 1.3), (0.0, None), (0.9, 0.0), (0.0, 0.6),
+                  (torch.tensor([0.5, 0.0, 1.5]), torch.tensor([0.0, 0.7, 0.9])),
+                  (1.0, torch.tensor([0.5, 0.0, 1.5])), (torch.tensor([0.5, 0.0, 1.5]), 0.8)):
+        for drafted in (False, True):
+            s = inputs(18, 3, 5, 400, "f32", drafted)
+            s["temperature"], s["draft_temperature"] = t, td
+            announce(f"accept T {t} {td}")
+            check(ctx, s)
+
+
+def test_greedy_is_the_argmax_accept(ctx):
+    for name in ("bf16", "f16"):   # the types that argmax_accept takes
+        s = inputs(19, 1, 8, 3001, name, False)
+        s["logits"] = s["logits"].round()   # many equal logits
+        s["logits"][0, 3, 5] = math.nan
+        s["drafts"] = s["logits"][:, :-1].float().nan_to_num(-100).argmax(-1).to(torch.int32)
+        s["drafts"][0, 6] = 9
+        s["draft_lengths"] = None
+        s["temperature"] = 0.0
+        g = on_gpu(s)
+        tokens, accepted, _ = ctx.sample_accept(**g)
+        want, count = ctx.argmax_accept(g["logits"][0], g["drafts"][0])
+        n = int(count)
+        assert int(accepted) == n
+        assert tokens[0, :n + 1].tolist() == want[:n + 1].tolist()
+        assert (tokens[0, n + 1:] == -1).all()
+
+
+@pytest.mark.parametrize("name", sorted(DTYPES))
+def test_masked_logits(ctx, name):
+    """-inf and the type's lowest value in most places, and rows that are all the lowest value."""
+    low = torch.finfo(DTYPES[name]).min
+    for mask, drafted in itertools.product((-math.inf, low), (False, True)):
+        announce(f"accept masked {name} {mask}")
+        s = inputs(20, 4, 4, 3000, name, drafted)
+        keep = torch.rand(s["logits"].shape, generator=torch.Generator().manual_seed(1)) < 0.01
+        keep[..., 77] = True
+        s["logits"][~keep] = mask
+        if drafted:
+            s["draft_logits"][~keep[:, :-1]] = mask
+        check(ctx, s)
+        if mask == low:
+            s["logits"][1, 0] = low
+            s["logits"][2] = low
+            check(ctx, s)
+        s["temperature"] = 0.0
+        check(ctx, s)
+
+
+def test_a_draft_that_its_own_distribution_rules_out(ctx):
+    s = inputs(21, 2, 3, 100, "f32", True)
+    s["draft_lengths"] = None
+    for b in range(2):
+        s["draft_logits"][b, 0, int(s["drafts"][b, 0])] = -math.inf
+    s["logits"][1, 0, int(s["drafts"][1, 0])] = -math.inf
+    got = check(ctx, s)
+    assert got[2][0, 0] == 1 and got[2][1, 0] == 0
+
+
+def test_rows_without_a_distribution(ctx):
+    """NaN, +inf, nothing above -inf, and temperatures that are none: the draft is refused and no
+    token is drawn; other sequences are not touched by it."""
+    for drafted, name in itertools.product((False, True), sorted(DTYPES)):
+        s = inputs(22, 8, 4, 700, name, drafted)
+        s["draft_lengths"] = None
+        s["logits"][0, 0, 5] = math.nan
+        s["logits"][1, 1, 699] = math.inf
+        s["logits"][2, 2] = -math.inf
+        s["logits"][3, 3, 0] = math.nan
+        s["temperature"][4:7] = torch.tensor([-1.0, math.inf, math.nan])
+        if drafted:
+            s["draft_logits"][7, 1, 3] = math.nan
+        else:
+            s["logits"][7, 1] = math.nan
+        announce(f"accept without {name} {drafted}")
+        got = check(ctx, s)
+        assert got[0][0].tolist() == [-1] * 4 and got[0][4:7].tolist() == [[-1] * 4] * 3
+        s["temperature"][:] = 0
+        check(ctx, s)
+    s["logits"][3, 0] = math.nan
+    s["temperature"][:] = 0
+    assert check(ctx, s)[0][3].tolist() == [-1] * 4
+
+
+def test_drafts_outside_the_vocabulary(ctx):
+    for drafted in (False, True):
+        s = inputs(23, 3, 3, 900, "bf16", drafted)
+        s["drafts"][:, 0] = torch.tensor([-1, 900, 2 ** 31 - 1])
+        s["draft_lengths"] = None
+        assert check(ctx, s)[1].tolist() == [0, 0, 0]
+        s["temperature"][:] = 0
+        check(ctx, s)
+
+
+def test_the_edges_of_the_random_numbers(ctx):
+    """0 takes any draft that can be and the first token that can be; 1 - 2^-24 the last."""
+    last = 1 - 2.0 ** -24
+    s = inputs(24, 2, 3, 5000, "f32", False)
+    s["draft_lengths"] = torch.tensor([2, 0], dtype=torch.int32)
+    s["logits"][:, :, :17] = -math.inf
+    s["logits"][:, :, 4990:] = -math.inf
+    s["logits"][:, 2, 4989] = s["logits"][:, 0, 4989] = 9.0
+    s["uniforms"][:] = 0
+    tokens, accepted, _ = ctx.sample_accept(**on_gpu(s))
+    assert accepted.tolist() == [2, 0] and tokens[0, 2] == 17 and tokens[1, 0] == 17
+    s["uniforms"][:] = last
+    tokens, accepted, _ = ctx.sample_accept(**on_gpu(s))
+    want = oracle(s)
+    assert accepted.tolist() == want[1].tolist() and tokens.tolist() == want[0].tolist()
+    # numbers outside [0, 1) are the caller's mistake, and still give tokens of the row
+    for u in (1.0, 7.0, -3.0, math.nan):
+        s["uniforms"][:] = u
+        tokens, accepted, _ = ctx.sample_accept(**on_gpu(s))
+        assert ((tokens >= -1) & (tokens < 4990)).all() and tokens[1, 0] >= 17
+
+
+def test_a_draw_at_its_border(ctx):
+    """Two equal tokens: the first's running sum is the half, and u = 0.5 is not passed by it."""
+    for name in sorted(DTYPES):
+        x = torch.full((2, 1, 4000), -math.inf, dtype=DTYPES[name])
+        x[..., 100] = x[..., 3900] = 1.5
+        u = torch.tensor([[0.5], [0.5 - 2.0 ** -25]])
+        tokens, _, _ = ctx.sample_accept(x.cuda(), u.cuda())
+        assert tokens[:, 0].tolist() == [3900, 100]
+
+
+def test_equal_distributions_accept_everything(ctx):
+    """p = q: chances of 1, whatever the numbers are below 1."""
+    s = inputs(25, 6, 9, 6000, "bf16", True)
+    s["draft_logits"] = s["logits"][:, :-1].clone()
+    s["draft_lengths"] = None
+    s["uniforms"][:, :-1] = 1 - 2.0 ** -24
+    tokens, accepted, chances = ctx.sample_accept(**on_gpu(s))
+    assert accepted.tolist() == [8] * 6 and (chances == 1).all()
+
+
+@pytest.mark.parametrize("drafted", (False, True))
+def test_tokens_follow_the_target(ctx, drafted):
+    """Over a grid of random numbers the first token of a block is distributed as p: drafts drawn
+    from q (every token as often as q has it) and refused, accepted or redrawn.  Steps of the grid
+    leave each of the 6 tokens at most 2 borders a draft, off by a step of 1/256 each."""
+    n, vocab = 256, 6
+    gen = torch.Generator().manual_seed(2)
+    p_logits, q_logits = 1.5 * torch.randn(2, vocab, generator=gen)
+    p, q = p_logits.double().softmax(0), q_logits.double().softmax(0)
+    grid = (torch.arange(n) + 0.5) / n
+    u = torch.stack((grid.repeat_interleave(n), grid.repeat(n)), 1)
+    law = torch.zeros(vocab, dtype=torch.float64)
+    for d in range(vocab):
+        if not drafted and d:
+            break
+        x = torch.stack((p_logits, torch.zeros(vocab)))
+        tokens, _, _ = ctx.sample_accept(
+            x.cuda().expand(n * n, -1, -1), u.cuda(),
+            drafts=torch.full((n * n, 1), d, dtype=torch.int32, device="cuda"),
+            draft_logits=q_logits.cuda().expand(n * n, 1, -1) if drafted else None)
+        counts = tokens[:, 0].long().cpu().bincount(minlength=vocab).double() / (n * n)
+        law += counts * (q[d] if drafted else 1.0)
+    assert (law - p).abs().max() <= 4.0 / n
+
+
+def test_strides(ctx):
+    """Rows and sequences apart, at odd offsets; logits and draft logits of one tensor."""
+    for name in sorted(DTYPES):
+        s = inputs(26, 3, 4, 2500, name, True)
+        room = torch.zeros(3, 9, 2611, dtype=DTYPES[name])
+        room[:, ::2, 3:2503][:, :4] = s["logits"]
+        room[:, 1::2, 111:][:, :3, :2500] = s["draft_logits"]
+        want = check(ctx, s)
+        g = on_gpu(s)
+        far = room.cuda()
+        g["logits"] = far[:, ::2, 3:2503][:, :4]
+        g["draft_logits"] = far[:, 1::2, 111:][:, :3, :2500]
+        announce(f"accept strides {name}")
+        got = ctx.sample_accept(**g)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_offsets_past_32_bits(ctx):
+    s = inputs(27, 2, 2, 5000, "bf16", False)
+    s["draft_lengths"] = None
+    want = check(ctx, s)
+    g = on_gpu(s)
+    far = 2 ** 31 + 64
+    big = torch.empty(far + 2 * 5000, dtype=torch.bfloat16, device="cuda")
+    view = big.as_strided((2, 2, 5000), (far, 5000, 1))
+    view.copy_(g["logits"])
+    g["logits"] = view
+    announce("accept far sequences")
+    assert all(torch.equal(a, b) for a, b in zip(ctx.sample_accept(**g), want))
+    view = big.as_strided((1, 2, 5000), (far, far, 1))
+    one = {k: v[:1].contiguous() if isinstance(v, torch.Tensor) else v
+           for k, v in on_gpu(s).items()}
+    view.copy_(one["logits"])
+    one["logits"] = view
+    announce("accept far rows")
+    assert all(torch.equal(a, b[:1]) for a, b in zip(ctx.sample_accept(**one), want))
+
+
+def test_the_same_call_gives_the_same_bits(ctx):
+    s = on_gpu(inputs(28, 20, 6, 30000, "bf16", True))
+    first = ctx.sample_accept(**s)
+    for _ in range(4):
+        assert all(torch.equal(a, b) for a, b in zip(ctx.sample_accept(**s), first))
+
+
+def test_captured_and_replayed(ctx):
+    s = on_gpu(inputs(29, 5, 4, 9000, "f16", True))
+    ws = torch.empty(8 << 20, dtype=torch.uint8, device="cuda")
+    ctx.sample_accept(**s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ctx.sample_accept(**s, ws=ws)
+    for n in range(4):
+        s["uniforms"].copy_(torch.rand(5, 4, generator=torch.Generator().manual_seed(n)))
+        for a in got:
+            a.fill_(7)
+        ws.fill_(n * 85)    # what a workspace holds does not matter
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, ctx.sample_accept(**s)))
+
+
+def test_two_streams_at_once(ctx):
+    cases = [on_gpu(inputs(30 + i, 6, 5, 40000, "bf16", True)) for i in range(2)]
+    want = [ctx.sample_accept(**s) for s in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for s, stream in zip(cases, streams):
+            got.append(ctx.sample_accept(**s, stream=stream))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i % 2]))
+
+
+def test_a_given_workspace(ctx):
+    s = on_gpu(inputs(32, 2, 3, 5000, "f32", True))
+    want = ctx.sample_accept(**s)
+    small = torch.empty(64, dtype=torch.uint8, device="cuda")
+    with pytest.raises(dflash_qmm.DfqError) as e:
+        ctx.sample_accept(**s, ws=small)
+    assert e.value.status == 3
+    ws = torch.full((4 << 20,), 255, dtype=torch.uint8, device="cuda")
+    assert all(torch.equal(a, b) for a, b in zip(ctx.sample_accept(**s, ws=ws), want))
