@@ -76,21 +76,23 @@ struct LogprobParams {
     int splits;              /* workgroups, and parts, a row                                */
 };
 
-/* What a workgroup of dfq_sample_accept's first kernel makes of its range of a row. */
+/* What a wave of dfq_sample_accept's first kernel makes of its range of a row. */
 struct AcceptPart {
-    float top;               /* the largest logit, NaN passed over; -inf where there is none */
-    float sum;               /* of e^((x - max(top, -FLT_MAX)) / T)                          */
-    int32_t at;              /* the first that is the largest, -1 where all are NaN          */
-    int32_t pad;
+    float top;               /* the largest logit; NaN where there is one (T > 0)         */
+    uint32_t sum;            /* T > 0: the fp32 sum of e^((x - top) / T), 0 where top is not
+                              * finite; T = 0: the first place of top, 2^31 - 1 where all
+                              * are NaN                                                   */
 };
 
-/* What is left to draw of a sequence: from p, p without its draft, or max(p - q, 0). */
+#define DFQ_ACCEPT_PIECES 8  /* 16-byte pieces that a lane takes of a range              */
+
+/* What is left to draw of a sequence: nothing, or a token from p, from p without its draft, or
+ * from max(p - q, 0). */
 enum { DFQ_DRAW_NONE = 0, DFQ_DRAW_P = 1, DFQ_DRAW_OTHER = 2, DFQ_DRAW_REST = 3 };
 struct AcceptDraw {
-    int32_t mode, row;       /* the target's row, and the place of the token         */
-    int32_t draft;           /* DFQ_DRAW_OTHER: the token left out                    */
-    float p_top, q_top;      /* largest logits of the rows                            */
-    int32_t pad;
+    int32_t mode, row;       /* the target's row, and the place of the token */
+    int32_t draft, token;    /* the row's draft; the token of DFQ_DRAW_NONE  */
+    float p_top, q_top;      /* largest logits of the rows                   */
 };
 
 struct AcceptParams {
@@ -104,15 +106,18 @@ struct AcceptParams {
     int32_t* tokens;            /* [batch][rows]                                   */
     int32_t* accepted;          /* [batch]                                         */
     float* chances;             /* [batch][rows - 1] or NULL                       */
-    AcceptPart* parts;          /* [batch][rows, then draft rows][splits]          */
-    AcceptDraw* draws;          /* [batch]                                         */
-    double* totals;             /* [batch][2][chunks]: sums of e^((x - top) / T)   */
-    double* weights;            /* [batch][chunks]: sums of what is drawn from     */
+    AcceptPart* parts;          /* [batch][rows, then draft rows][ranges]          */
+    AcceptDraw* draws;          /* [batch], with draft logits                      */
+    double* totals;             /* [batch][chunks][2]: both rows' sums             */
+    uint64_t* sums;             /* [batch][units]: what is drawn from, as doubles' bits */
+    int32_t* arrived;           /* [batch]: workgroups whose sums are there        */
     int64_t batch_stride, row_stride, draft_batch_stride, draft_row_stride;
     float temperature, draft_temperature;
-    int batch, rows, all_rows, vocab;
-    int splits;                 /* workgroups, and parts, a row                    */
-    int chunks;                 /* pieces of DFQ_KV_THREADS lanes' 16 bytes a row  */
+    int rows, vocab;
+    int jobs;                   /* ranges of all rows                              */
+    int units;                  /* 64 lanes' 16 bytes each, of a row               */
+    Divisor all_rows, ranges;   /* rows and draft rows of a sequence; ranges a row */
+    Divisor chunks;             /* workgroups of a sequence in the later kernels   */
 };
 
 #define DFQ_ROPE_DIM 512     /* widest head */

@@ -24,25 +24,26 @@ dfq_status check_sizes(int batch, int rows, int V, dfq_dtype dtype) {
 }
 
 struct AcceptPlan {
-    int all_rows, splits, chunks;
-    size_t draws, totals, weights, bytes;   /* offsets; the parts come first */
+    int all_rows, ranges, units, chunks;
+    size_t sums, totals, draws, arrived, bytes;   /* offsets; the parts come first */
 };
 
-/* Workgroups a row as the log probabilities take them: ranges of 1024 logits a wave or more, five
- * workgroups a CU. */
+constexpr int kWaves = DFQ_KV_THREADS / 64;
+
 AcceptPlan plan_accept(int cus, int batch, int rows, int V, dfq_dtype dtype, bool drafted) {
     AcceptPlan a;
     a.all_rows = drafted ? 2 * rows - 1 : rows;
-    const int64_t M = (int64_t)batch * a.all_rows;
-    const int64_t most = std::max<int64_t>(1, 5 * cus / M);
-    a.splits = (int)std::min({most, ((int64_t)V + 4095) / 4096, (int64_t)64});
-    const int chunk = DFQ_KV_THREADS * (dtype == DFQ_F32 ? 4 : 8);
-    a.chunks = (V + chunk - 1) / chunk;
+    const int unit = 64 * (dtype == DFQ_F32 ? 4 : 8);
+    a.units = (V + unit - 1) / unit;
+    a.ranges = (V + DFQ_ACCEPT_PIECES * unit - 1) / (DFQ_ACCEPT_PIECES * unit);
+    /* a wave a unit, and no more workgroups than four a CU: each decides its sequence's drafts */
+    a.chunks = std::clamp(4 * cus / batch, 1, (a.units + kWaves - 1) / kWaves);
     const auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
-    a.draws = up((size_t)M * a.splits * sizeof(AcceptPart));
-    a.totals = a.draws + up((size_t)batch * sizeof(AcceptDraw));
-    a.weights = a.totals + (drafted ? up((size_t)batch * 2 * a.chunks * 8) : 0);
-    a.bytes = a.weights + (size_t)batch * a.chunks * 8;
+    a.sums = up((size_t)batch * a.all_rows * a.ranges * sizeof(AcceptPart));
+    a.totals = a.sums + up((size_t)batch * a.units * 8);
+    a.draws = a.totals + (drafted ? up((size_t)batch * a.chunks * 16) : 0);
+    a.arrived = a.draws + (drafted ? up((size_t)batch * sizeof(AcceptDraw)) : 0);
+    a.bytes = a.arrived + (size_t)batch * 4;
     return a;
 }
 
@@ -91,9 +92,9 @@ dfq_status dfq_sample_accept(dfq_ctx* ctx, const void* logits, int64_t batch_str
          !(draft_temperature >= 0.0f && std::isfinite(draft_temperature))))
         return fail(DFQ_ERR_INVALID_ARGUMENT, "temperatures are finite and not negative");
     const AcceptPlan a = plan_accept(dfq_num_cus(ctx), batch, rows, V, dtype, drafted);
-    const int64_t ranges = (int64_t)batch * a.all_rows * a.splits;
+    const int64_t jobs = (int64_t)batch * a.all_rows * a.ranges;
     const int64_t chunks = (int64_t)batch * a.chunks;
-    if (ranges > INT32_MAX || chunks > INT32_MAX)
+    if (jobs > INT32_MAX || chunks > INT32_MAX)
         return fail(DFQ_ERR_UNSUPPORTED, "grid too large");
     if (!workspace || workspace_bytes < a.bytes)
         return fail(DFQ_ERR_WORKSPACE, "workspace of %zu bytes needed (got %zu)", a.bytes,
@@ -113,37 +114,35 @@ dfq_status dfq_sample_accept(dfq_ctx* ctx, const void* logits, int64_t batch_str
     p.accepted = accepted;
     p.chances = chances;
     p.parts = (AcceptPart*)ws;
-    p.draws = (AcceptDraw*)(ws + a.draws);
+    p.sums = (uint64_t*)(ws + a.sums);
     p.totals = (double*)(ws + a.totals);
-    p.weights = (double*)(ws + a.weights);
+    p.draws = drafted ? (AcceptDraw*)(ws + a.draws) : nullptr;
+    p.arrived = (int32_t*)(ws + a.arrived);
     p.batch_stride = batch_stride;
     p.row_stride = row_stride;
     p.draft_batch_stride = draft_batch_stride;
     p.draft_row_stride = draft_row_stride;
     p.temperature = temperature;
     p.draft_temperature = draft_temperature;
-    p.batch = batch;
     p.rows = rows;
-    p.all_rows = a.all_rows;
     p.vocab = V;
-    p.splits = a.splits;
-    p.chunks = a.chunks;
+    p.jobs = (int)jobs;
+    p.units = a.units;
+    p.all_rows = divisor(a.all_rows);
+    p.ranges = divisor(a.ranges);
+    p.chunks = divisor(a.chunks);
     const VerifyOps* ops;
     if ((s = ctx_verify_ops(ctx, &ops))) return s;
     DeviceScope scope(ctx);
     const AcceptKernels& fn = ops->accept[(int)dtype];
     void* args[] = {&p};
-    hipError_t e = hipSuccess;
-    const auto launch = [&](hipFunction_t f, int64_t groups, int threads) {
-        if (e == hipSuccess)
-            e = hipModuleLaunchKernel(f, (unsigned)groups, 1, 1, threads, 1, 1, 0,
+    hipError_t e = hipModuleLaunchKernel(fn.sums, (unsigned)((jobs + kWaves - 1) / kWaves), 1, 1,
+                                         DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args,
+                                         nullptr);
+    for (hipFunction_t f : {fn.weigh, drafted ? fn.rest : nullptr})
+        if (f && e == hipSuccess)
+            e = hipModuleLaunchKernel(f, (unsigned)chunks, 1, 1, DFQ_KV_THREADS, 1, 1, 0,
                                       (hipStream_t)stream, args, nullptr);
-    };
-    launch(fn.sums, ranges, DFQ_KV_THREADS);
-    launch(fn.decide, batch, 64);
-    if (drafted) launch(fn.totals, chunks, DFQ_KV_THREADS);
-    launch(fn.weights, chunks, DFQ_KV_THREADS);
-    launch(fn.pick, batch, DFQ_KV_THREADS);
     return e == hipSuccess ? DFQ_OK : hip_error(e, "launch dfq_sample_accept");
 }
 

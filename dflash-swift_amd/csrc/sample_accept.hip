@@ -8,9 +8,18 @@
  * first t whose running sum passes u times the whole.  That keeps the tokens distributed as p.  A
  * temperature of 0 stands for the largest logit alone (the first of equal ones).
  *
- * The draw is a whole number that a sum's last bits decide, so all that it comes from is 64 bits
- * wide: sums of 2^x over the row, and the running sum.  The accept's sums over all rows are fp32:
- * a draft's chance is then right to some 2^-21 of itself.
+ * Tokens and counts are whole numbers that a sum's last bits decide, and come out as 64-bit
+ * arithmetic has them (exponentials to 8e-13): draws sum and search in 64 bits, and a draft whose
+ * u q is within 2^-16 of p, more than the fp32 sums of its rows can be off, is decided again from
+ * 64-bit sums.  Other drafts need no more than fp32, in which a logit costs 8 instructions against
+ * 20: all rows in 64 bits took 93 us at 64 sequences of seven drafts for 151936 tokens, the rows
+ * of the draws apart.
+ *
+ * The first launch reads all rows once: a wave takes a range of one row in registers, finds its
+ * largest logit and the sum of e^((x - largest) / T).  In the second each workgroup joins its
+ * sequence's ranges and decides its drafts (alike in all of them, so that nothing has to be waited
+ * for), then weighs its part of the row that is drawn from; the last to come finds the token.
+ * Where the draw is from p - q the second sums both rows, and a third weighs and finds.
  */
 #include "kv_params.h"
 #include "logit_piece.h"
@@ -19,25 +28,41 @@ namespace {
 
 constexpr int kWaves = DFQ_KV_THREADS / 64;
 constexpr double kLog2e = 1.44269504088896340736;
+constexpr int kNone = 0x7fffffff;
 
-/* 2^a for a <= 0: the Taylor sum of the part behind the whole number, whose first term left out
- * is (ln 2 / 2)^12 / 12! < 7e-15. */
-__device__ __forceinline__ double power_of_2(double a) {
-    a = fmax(a, -1100.0);
-    const double n = rint(a), x = (a - n) * 0.693147180559945309417;
-    double s = 1.0 / 39916800.0;
-    s = fma(x, s, 1.0 / 3628800.0);
-    s = fma(x, s, 1.0 / 362880.0);
-    s = fma(x, s, 1.0 / 40320.0);
-    s = fma(x, s, 1.0 / 5040.0);
-    s = fma(x, s, 1.0 / 720.0);
-    s = fma(x, s, 1.0 / 120.0);
-    s = fma(x, s, 1.0 / 24.0);
-    s = fma(x, s, 1.0 / 6.0);
-    s = fma(x, s, 0.5);
-    s = fma(x, s, 1.0);
-    s = fma(x, s, 1.0);
-    return __builtin_ldexp(s, (int)n);
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
+/* 2^f for |f| <= 1/2: the polynomial of degree 8 whose largest relative error, 7.8e-13, is least
+ * (its nine alternating extremes found by exchange). */
+__device__ __forceinline__ double power_of_part(double f) {
+    double s = 0x1.61afcebc3eb7bp-20;
+    s = fma(f, s, 0x1.00dad25030da9p-16);
+    s = fma(f, s, 0x1.430acca345de3p-13);
+    s = fma(f, s, 0x1.5d87483855d3ep-10);
+    s = fma(f, s, 0x1.3b2ab5c52926cp-7);
+    s = fma(f, s, 0x1.c6b08dd46d38ep-5);
+    s = fma(f, s, 0x1.ebfbdff9319e1p-3);
+    s = fma(f, s, 0x1.62e42fef8615ep-1);
+    return fma(f, s, 0x1.ffffffffff7a3p-1);
+}
+
+constexpr double kWhole = 6755399441055744.0;   /* 1.5 2^52: sums with it are whole numbers */
+
+/* 2^(d rate) for d <= 0; 0 for d = -inf and past 2^-1074. */
+__device__ __forceinline__ double power(double d, double rate) {
+    const double a = fmax(d * rate, -1100.0), n = rint(a);
+    return __builtin_ldexp(power_of_part(a - n), (int)n);
+}
+
+/* The same down to 2^-1022, which stands for all that is less: `least` is -1022 / rate.  A sum
+ * of such numbers beside a 1 does not hold them. */
+__device__ __forceinline__ double power_in_sum(double d, double rate, double least) {
+    d = fmax(d, least);
+    const double t = fma(d, rate, kWhole);
+    const double v = power_of_part(fma(d, rate, kWhole - t));
+    u32x2_t w = __builtin_bit_cast(u32x2_t, v);
+    w[1] += __builtin_bit_cast(u32x2_t, t)[0] << 20;
+    return __builtin_bit_cast(double, w);
 }
 
 /* Temperatures below the least normal number are taken for it: their reciprocal is finite, and
@@ -67,9 +92,44 @@ __device__ __forceinline__ Sequence sequence_of(const AcceptParams& p, int b) {
     return s;
 }
 
+__device__ __forceinline__ int divided(int n, const Divisor& d) {
+    return (int)((n + (uint64_t)((uint64_t)(uint32_t)n * d.mul >> 32)) >> d.shift);
+}
+
+/* Exchanges over a wave: within rows of 16 lanes by DPP, then across. */
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)u, CTRL, 0xF, 0xF, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum(double v) {
+    v += dpp_f64<0xB1>(v);
+    v += dpp_f64<0x4E>(v);
+    v += dpp_f64<0x141>(v);
+    v += dpp_f64<0x140>(v);
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+template <typename Op>
+__device__ __forceinline__ float wave_of(float v, Op op) {
+    const auto bits = [&](uint32_t a, uint32_t b) {
+        return __float_as_uint(op(__uint_as_float(a), __uint_as_float(b)));
+    };
+    v = __uint_as_float(group_of<16>(__float_as_uint(v), bits));
+    v = op(v, __shfl_xor(v, 16));
+    return op(v, __shfl_xor(v, 32));
+}
+
+/* Of two numbers the larger, NaN where one is NaN. */
+__device__ __forceinline__ float larger(float a, float b) {
+    return __builtin_elementwise_maximum(a, b);
+}
+
 __device__ __forceinline__ double block_sum(double v) {
     __shared__ double waves[kWaves];
-    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
+    v = wave_sum(v);
     if (threadIdx.x % 64 == 0) waves[threadIdx.x / 64] = v;
     __syncthreads();
     double s = 0.0;
@@ -79,34 +139,115 @@ __device__ __forceinline__ double block_sum(double v) {
     return s;
 }
 
-/* The largest logit with its place, and the sum of e^((x - max(top, -FLT_MAX)) / T). */
-struct RowSums {
-    float m, l, top;
-    int at;
-    __device__ __forceinline__ void start() {
-        m = -__FLT_MAX__;   /* not -inf: differences with it stay numbers */
-        l = 0.0f;
-        top = -__builtin_inff();
-        at = -1;
+/* The sum over the threads in front of this one; `all` gets that over all. */
+__device__ __forceinline__ double block_before(double v, double& all) {
+    __shared__ double waves[kWaves];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    double run = v;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const double o = __shfl_up(run, d);
+        if (lane >= d) run += o;
     }
-    __device__ __forceinline__ void join(const RowSums& o, float rate) {
-        const float to = fmaxf(m, o.m);
-        l = l * __builtin_amdgcn_exp2f((m - to) * rate) +
-            o.l * __builtin_amdgcn_exp2f((o.m - to) * rate);
-        m = to;
-        if (o.at >= 0 && (at < 0 || o.top > top || (o.top == top && o.at < at))) {
-            top = o.top;
-            at = o.at;
+    if (lane == 63) waves[wave] = run;
+    __syncthreads();
+    double before = 0.0;
+    all = 0.0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        if (w < wave) before += waves[w];
+        all += waves[w];
+    }
+    __syncthreads();
+    return before + (run - v);
+}
+
+/* Of 512 weights, two neighbours a thread: where their running sum, counted from `from`, first
+ * passes the goal, or the last that weighs anything, or kNone; `front` gets the sum in front of it.
+ * A goal below 0 stands for u times the sum of all, and is set.  The threads' answers meet by
+ * ballots (256 lanes' minimum by LDS atomics took 2.5 us). */
+struct Search {
+    double goal, front;
+    int place;
+};
+__device__ __noinline__ Search search(double a, double b, double from, double goal, double u) {
+    __shared__ int firsts[kWaves], lasts[kWaves], place;
+    __shared__ double front;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    double all;
+    const double run = from + block_before(a + b, all);
+    if (goal < 0.0) goal = u * all;
+    const uint64_t some = __ballot(a + b > 0.0);
+    const uint64_t past = __ballot(a + b > 0.0 && run + (a + b) > goal);
+    if (lane == 0) {
+        firsts[wave] = past ? (int)__builtin_ctzll(past) : -1;
+        lasts[wave] = some ? 63 - (int)__builtin_clzll(some) : -1;
+    }
+    if (threadIdx.x == 0) place = kNone;
+    __syncthreads();
+    int first = kNone, last = -1;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        if (first == kNone && firsts[w] >= 0) first = 64 * w + firsts[w];
+        if (lasts[w] >= 0) last = 64 * w + lasts[w];
+    }
+    if ((int)threadIdx.x == (first != kNone ? first : last)) {
+        const bool second = a <= 0.0 || (b > 0.0 && run + a <= goal);
+        place = 2 * (int)threadIdx.x + second;
+        front = second ? run + a : run;
+    }
+    __syncthreads();
+    return {goal, front, place};
+}
+
+/* The place among n weights where their running sum passes u times their sum (goal < 0), or the
+ * goal, counted from `from`: cut into 512 parts until a part is one weight. */
+template <typename Weight>
+__device__ __forceinline__ Search find(int n, Weight weight, double from, double goal, double u) {
+    int lo = 0;
+    for (;;) {
+        const int each = (n + 2 * DFQ_KV_THREADS - 1) / (2 * DFQ_KV_THREADS);
+        double w[2] = {};
+        if (each == 1) {
+            /* both loads under way at once: behind a branch each they came one after the other */
+            const int i = 2 * (int)threadIdx.x;
+            w[0] = weight(lo + min(i, n - 1));
+            w[1] = weight(lo + min(i + 1, n - 1));
+            w[0] = i < n ? w[0] : 0.0;
+            w[1] = i + 1 < n ? w[1] : 0.0;
+        } else {
+            for (int k = 0; k < 2; ++k) {
+                const int64_t begin = (2 * (int64_t)threadIdx.x + k) * each;
+                for (int64_t i = begin; i < begin + each && i < n; ++i) w[k] += weight(lo + (int)i);
+            }
         }
+        Search s = search(w[0], w[1], from, goal, u);
+        if (s.place == kNone) return s;
+        lo += s.place * each;
+        n = min(each, n - s.place * each);
+        if (each == 1) {
+            s.place = lo;
+            return s;
+        }
+        from = s.front;
+        goal = s.goal;
+        __syncthreads();
     }
+}
+
+/* What is known of a row: its largest logit, and the sum of 2^((x - top) rate) or (T = 0) where
+ * it is first. */
+struct Row {
+    float top, sum;
+    int at;
 };
 
 template <int DT>
 struct Accept : LogitPiece<DT> {
-    using LogitPiece<DT>::kN, LogitPiece<DT>::load, LogitPiece<DT>::widen,
-        LogitPiece<DT>::largest;
-    static constexpr int kSize = 16 / kN, kAhead = 4;
-    static constexpr int kChunk = DFQ_KV_THREADS * kN;
+    using LogitPiece<DT>::kN, LogitPiece<DT>::load, LogitPiece<DT>::widen;
+    static constexpr int kSize = 16 / kN;
+    static constexpr int kUnit = 64 * kN;           /* logits of a wave's load          */
+    static constexpr int kPieces = DFQ_ACCEPT_PIECES, kRange = kPieces * kUnit;
 
     static __device__ __forceinline__ const char* target_row(const AcceptParams& p, int b, int r) {
         return (const char*)p.logits + (b * p.batch_stride + r * p.row_stride) * kSize;
@@ -116,299 +257,402 @@ struct Accept : LogitPiece<DT> {
                (b * p.draft_batch_stride + r * p.draft_row_stride) * kSize;
     }
 
-    /* One range of one row. */
+    /* One range of one row by one wave. */
     static __device__ __forceinline__ void sums(const AcceptParams& p) {
-        const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-        const int split = blockIdx.x % p.splits, row = blockIdx.x / p.splits;
-        const int b = row / p.all_rows, r = row % p.all_rows;
+        const int lane = threadIdx.x % 64;
+        const int job = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + threadIdx.x / 64);
+        if (job >= p.jobs) return;
+        const int row = divided(job, p.ranges), range = job - row * p.ranges.by;
+        const int b = divided(row, p.all_rows), r = row - b * p.all_rows.by;
+        if (r == 0 && range == 0 && lane == 0) p.arrived[b] = 0;
         const bool draft = r >= p.rows;
         const Sequence q = sequence_of(p, b);
         /* rows behind a sequence's drafts, and draft rows that do not matter */
         if (draft ? r - p.rows >= q.drafts || !q.drafted : r > q.drafts) return;
         const char* at_row = draft ? draft_row(p, b, r - p.rows) : target_row(p, b, r);
         const float t = draft ? q.dt : q.t;
-        const float rate = t > 0.0f ? (float)rate_of(t) : 0.0f;
-        constexpr int kStep = 64 * kN;
-        const int steps = (p.vocab + kStep - 1) / kStep, parts = p.splits * kWaves;
-        const int each = (steps + parts - 1) / parts, part = split * kWaves + wave;
-        const int from = (int64_t)part * each * kStep < p.vocab ? part * each * kStep : p.vocab;
-        const int end = each * kStep < p.vocab - from ? from + each * kStep : p.vocab;
-        RowSums s;
-        s.start();
-        for (int at = from; at < end; at += kAhead * kStep) {
-            u32x4_t v[kAhead];
+        const int from = range * kRange + lane * kN;
+        const bool whole = (range + 1) * kRange <= p.vocab;
+        u32x4_t v[kPieces];
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) v[u] = load(at_row, at + u * kStep + lane * kN, end);
+        for (int i = 0; i < kPieces; ++i) {
+            const int at = from + i * kUnit;
+            v[i] = whole ? *(const u32x4_any*)(at_row + (int64_t)at * kSize)
+                         : load(at_row, at, p.vocab);
+        }
+        AcceptPart part = {-__builtin_inff(), 0};
+        if (t == 0.0f) {
+            /* the first of the largest, NaN passed over */
+            float top = __builtin_nanf("");
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int i = at + u * kStep + lane * kN;
+            for (int i = 0; i < kPieces; ++i) {
                 float x[kN];
-                widen(v[u], x);
-                const float m = largest(x);
-                if (m > s.top || (s.at < 0 && m == s.top && i < end)) {
-                    s.top = m;
+                widen(v[i], x);
 #pragma unroll
-                    for (int j = kN - 1; j >= 0; --j)
-                        if (x[j] == m && i + j < end) s.at = i + j;
-                    if (m > s.m) {
-                        s.l *= __builtin_amdgcn_exp2f((s.m - m) * rate);
-                        s.m = m;
-                    }
+                for (int j = 0; j < kN; ++j) top = fmaxf(top, x[j]);
+            }
+            top = wave_of(top, [](float a, float c) { return fmaxf(a, c); });
+            int at = kNone;
+#pragma unroll
+            for (int i = kPieces - 1; i >= 0; --i) {
+                float x[kN];
+                widen(v[i], x);
+#pragma unroll
+                for (int j = kN - 1; j >= 0; --j)
+                    if (x[j] == top && from + i * kUnit + j < p.vocab) at = from + i * kUnit + j;
+            }
+            for (int d = 1; d < 64; d *= 2) at = min(at, __shfl_xor(at, d));
+            part = {top, (uint32_t)at};
+        } else {
+            float top = -__builtin_inff();
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                float x[kN];
+                widen(v[i], x);
+#pragma unroll
+                for (int j = 0; j < kN; ++j) top = larger(top, x[j]);
+            }
+            top = wave_of(top, [](float a, float c) { return larger(a, c); });
+            part.top = top;
+            if (fabsf(top) < __builtin_inff()) {
+                const float rate = (float)rate_of(t);
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) {
+                    float x[kN];
+                    widen(v[i], x);
+#pragma unroll
+                    for (int j = 0; j < kN; ++j)
+                        x[j] = __builtin_amdgcn_exp2f((x[j] - top) * rate);
+                    /* in pairs: fewer roundings in a row */
+#pragma unroll
+                    for (int d = kN / 2; d; d /= 2)
+#pragma unroll
+                        for (int j = 0; j < d; ++j) x[j] += x[j + d];
+                    sum += x[0];
                 }
-#pragma unroll
-                for (int j = 0; j < kN; ++j)
-                    s.l += __builtin_amdgcn_exp2f((x[j] - s.m) * rate);
+                part.sum = __float_as_uint(wave_of(sum, [](float a, float c) { return a + c; }));
             }
         }
-        for (int d = 1; d < 64; d *= 2) {
-            const RowSums o = {__shfl_xor(s.m, d), __shfl_xor(s.l, d), __shfl_xor(s.top, d),
-                               __shfl_xor(s.at, d)};
-            s.join(o, rate);
-        }
-        __shared__ RowSums waves[kWaves];
-        if (lane == 0) waves[wave] = s;
-        __syncthreads();
-        if (threadIdx.x) return;
-        for (int w = 1; w < kWaves; ++w) s.join(waves[w], rate);
-        p.parts[blockIdx.x] = AcceptPart{s.top, s.l, s.at, 0};
+        if (lane == 0) p.parts[job] = part;
     }
 
-    /* A row's parts together; sum is NaN or 0 where the row has no distribution. */
-    struct Row {
-        float top;
-        double sum;
-        int at;
-    };
+    /* A row's ranges together, by 16 lanes.  NaN, +inf or nothing above -inf leaves a sum that is
+     * not positive and finite. */
     static __device__ __forceinline__ Row row_of(const AcceptParams& p, int b, int r, float t) {
-        const AcceptPart* part = p.parts + ((int64_t)b * p.all_rows + r) * p.splits;
-        Row row = {-__builtin_inff(), 0.0, -1};
-        for (int i = 0; i < p.splits; ++i)
-            if (part[i].at >= 0 && (row.at < 0 || part[i].top > row.top)) {
-                row.top = part[i].top;
-                row.at = part[i].at;
+        const int lane = threadIdx.x % 16, n = p.ranges.by;
+        const AcceptPart* part = p.parts + ((int64_t)b * p.all_rows.by + r) * n;
+        Row row = {-__builtin_inff(), 0.0f, kNone};
+        const float rate = (float)rate_of(t);
+        constexpr int kOnce = 4;   /* loads on their way together */
+        for (int from = 0; from < n; from += 16 * kOnce) {
+            AcceptPart v[kOnce];
+#pragma unroll
+            for (int j = 0; j < kOnce; ++j) {
+                const int i = from + 16 * j + lane;
+                v[j] = {-__builtin_inff(), t == 0.0f ? kNone : 0u};
+                if (i < n) v[j] = part[i];
             }
-        const double rate = t > 0.0f ? rate_of(t) : 0.0;
-        const float top = fmaxf(row.top, -__FLT_MAX__);
-        for (int i = 0; i < p.splits; ++i)
-            row.sum += part[i].sum *
-                       power_of_2(((double)fmaxf(part[i].top, -__FLT_MAX__) - top) * rate);
-        return row;
+            if (t == 0.0f) {
+#pragma unroll
+                for (int j = 0; j < kOnce; ++j)
+                    if ((int)v[j].sum != kNone && (row.at == kNone || v[j].top > row.top)) {
+                        row.top = v[j].top;
+                        row.at = (int)v[j].sum;
+                    }
+                continue;
+            }
+            float to = row.top;
+#pragma unroll
+            for (int j = 0; j < kOnce; ++j) to = larger(to, v[j].top);
+            if (fabsf(to) < __builtin_inff()) {
+                row.sum *= __builtin_amdgcn_exp2f((row.top - to) * rate);
+#pragma unroll
+                for (int j = 0; j < kOnce; ++j)
+                    row.sum += __uint_as_float(v[j].sum) *
+                               __builtin_amdgcn_exp2f((v[j].top - to) * rate);
+            }
+            row.top = to;
+        }
+        if (t == 0.0f) {
+#pragma unroll
+            for (int d = 1; d < 16; d *= 2) {
+                const float top = __shfl_xor(row.top, d);
+                const int at = __shfl_xor(row.at, d);
+                if (at != kNone && (row.at == kNone || top > row.top ||
+                                    (top == row.top && at < row.at))) {
+                    row.top = top;
+                    row.at = at;
+                }
+            }
+            return row;
+        }
+        const float top = __uint_as_float(
+            group_of<16>(__float_as_uint(row.top), [](uint32_t a, uint32_t c) {
+                return __float_as_uint(larger(__uint_as_float(a), __uint_as_float(c)));
+            }));
+        float sum = __builtin_nanf("");
+        if (fabsf(top) < __builtin_inff())
+            sum = row.sum * __builtin_amdgcn_exp2f((row.top - top) * rate);
+        sum = __uint_as_float(group_of<16>(__float_as_uint(sum), [](uint32_t a, uint32_t c) {
+            return __float_as_uint(__uint_as_float(a) + __uint_as_float(c));
+        }));
+        return {top, sum, kNone};
     }
 
-    /* What a wave decides of a sequence: lane i looks at draft i. */
-    static __device__ __forceinline__ void decide(const AcceptParams& p) {
-        const int b = blockIdx.x, lane = threadIdx.x;
-        const Sequence s = sequence_of(p, b);
+    /* The sum of a whole row in 64 bits, by a workgroup alone. */
+    static __device__ __noinline__ double whole_row(const char* row, int vocab, float top,
+                                                    float t) {
+        const double rate = rate_of(t), least = -1022.0 / rate;
+        double sum = 0.0;
+        for (int i = threadIdx.x * kN; i < vocab; i += DFQ_KV_THREADS * kN) {
+            float x[kN];
+            widen(load(row, i, vocab), x);
+#pragma unroll
+            for (int j = 0; j < kN; ++j) sum += power_in_sum((double)x[j] - top, rate, least);
+        }
+        return block_sum(sum);
+    }
+
+    /* Decides the drafts of sequence b, by a workgroup: 16 lanes join a row, lane i of the first
+     * wave looks at draft i.  `writes` stores what is known without a draw. */
+    static __device__ __forceinline__ AcceptDraw decide(const AcceptParams& p, const Sequence& s,
+                                                        int b, bool writes) {
+        __shared__ Row rows[2 * 64];
+        __shared__ AcceptDraw made;
+        __shared__ uint64_t again;
+        const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
         const bool greedy = s.t == 0.0f;
-        Row row = {0.0f, 0.0, -1}, other = row;
-        float chance = 0.0f;
-        bool some = true, taken = false;   /* some: both rows have a distribution */
+        /* what the first wave will need of the drafts is on its way meanwhile */
         int draft = -1;
-        if (lane <= s.drafts) {
-            row = row_of(p, b, lane, s.t);
-            some = greedy ? row.at >= 0 : row.sum > 0.0 && row.sum < __builtin_inf() &&
-                                              is_temperature(s.t);
+        float x = 0.0f, y = 0.0f, u = 0.0f;
+        bool known = false;
+        if (wave == 0 && lane < s.drafts) {
+            draft = p.drafts[(int64_t)b * (p.rows - 1) + lane];
+            u = p.uniforms[(int64_t)b * p.rows + lane];
+            known = draft >= 0 && draft < p.vocab;
+            if (known) {
+                x = load_any(target_row(p, b, lane), DT, draft);
+                if (s.drafted) y = load_any(draft_row(p, b, lane), DT, draft);
+            }
+        }
+        const int joined = s.drafts + 1 + (s.drafted ? s.drafts : 0);
+        for (int i = threadIdx.x / 16; i < joined; i += DFQ_KV_THREADS / 16) {
+            const bool q = i > s.drafts;
+            const Row row = row_of(p, b, q ? p.rows + i - s.drafts - 1 : i, q ? s.dt : s.t);
+            if (lane % 16 == 0) rows[i] = row;
+        }
+        __syncthreads();
+        Row row = {0.0f, 0.0f, kNone}, other = row;
+        bool some = true, taken = false;   /* some: both rows have a distribution */
+        double mine = 0.0, theirs = 1.0;
+        if (wave == 0) {
+            if (lane <= s.drafts) {
+                row = rows[lane];
+                some = greedy ? row.at != kNone
+                              : row.sum > 0.0f && row.sum < __builtin_inff() &&
+                                    is_temperature(s.t);
+            }
             if (lane < s.drafts) {
-                draft = p.drafts[(int64_t)b * (p.rows - 1) + lane];
-                const bool known = draft >= 0 && draft < p.vocab;
-                double mine = 0.0, theirs = 1.0;
                 if (s.drafted) {
-                    other = row_of(p, b, p.rows + lane, s.dt);
-                    some = some && other.sum > 0.0 && other.sum < __builtin_inf() &&
+                    other = rows[s.drafts + 1 + lane];
+                    some = some && other.sum > 0.0f && other.sum < __builtin_inff() &&
                            is_temperature(s.dt);
                 }
-                if (known && some) {
-                    if (greedy)
-                        mine = draft == row.at;
-                    else
-                        mine = power_of_2(((double)load_any(target_row(p, b, lane), DT, draft) -
-                                           row.top) * rate_of(s.t)) / row.sum;
+                known = known && some;
+                if (known) {
+                    if (greedy) mine = draft == row.at;
+                    else mine = power((double)x - row.top, rate_of(s.t)) / row.sum;
                     if (s.drafted)
-                        theirs = power_of_2(((double)load_any(draft_row(p, b, lane), DT, draft) -
-                                             other.top) * rate_of(s.dt)) / other.sum;
-                    taken = (double)p.uniforms[(int64_t)b * p.rows + lane] * theirs < mine;
-                    chance = theirs > 0.0 ? (float)fmin(mine / theirs, 1.0) : mine > 0.0;
+                        theirs = power((double)y - other.top, rate_of(s.dt)) / other.sum;
+                    taken = u * theirs < mine;
                 }
             }
+            const uint64_t near =
+                __ballot(known && mine > 0.0 && fabs(u * theirs - mine) < 0x1p-16 * mine);
+            if (lane == 0) again = near;
         }
-        if (p.chances && lane < p.rows - 1)
-            p.chances[(int64_t)b * (p.rows - 1) + lane] = chance;
-        const uint64_t refused = ~__ballot(taken);
-        const int n = __builtin_ctzll(refused);   /* at most 63 drafts: some bit is set */
-        int token = lane < n ? draft : -1;
-        if (lane == n) {
-            AcceptDraw d = {DFQ_DRAW_NONE, n, draft, row.top, other.top, 0};
-            if (!some) {
-                token = -1;
-            } else if (greedy) {
-                token = row.at;
-            } else if (n == s.drafts) {
-                d.mode = DFQ_DRAW_P;
-            } else {
-                d.mode = s.drafted ? DFQ_DRAW_REST : DFQ_DRAW_OTHER;
+        __syncthreads();
+        /* drafts next to the border: fewer than one in ten thousand */
+        for (uint64_t near = again; near; near &= near - 1) {
+            const int i = __builtin_ctzll(near);
+            double p_sum = 0.0, q_sum = 0.0;
+            if (!greedy) p_sum = whole_row(target_row(p, b, i), p.vocab, rows[i].top, s.t);
+            if (s.drafted)
+                q_sum = whole_row(draft_row(p, b, i), p.vocab, rows[s.drafts + 1 + i].top, s.dt);
+            if (wave == 0 && lane == i) {
+                if (!greedy) mine = power((double)x - row.top, rate_of(s.t)) / p_sum;
+                if (s.drafted) theirs = power((double)y - other.top, rate_of(s.dt)) / q_sum;
+                taken = u * theirs < mine;
             }
-            p.draws[b] = d;
-            p.accepted[b] = n;
         }
-        if (lane < p.rows) p.tokens[(int64_t)b * p.rows + lane] = token;
+        if (wave == 0) {
+            const uint64_t refused = ~__ballot(taken);
+            const int n = __builtin_ctzll(refused);   /* at most 63 drafts: some bit is set */
+            if (lane == n) {
+                AcceptDraw d = {DFQ_DRAW_NONE, n, draft, -1, row.top, other.top};
+                if (some && greedy) d.token = row.at;
+                else if (some && n == s.drafts) d.mode = DFQ_DRAW_P;
+                else if (some) d.mode = s.drafted ? DFQ_DRAW_REST : DFQ_DRAW_OTHER;
+                made = d;
+                if (writes) p.accepted[b] = n;
+            }
+            if (writes) {
+                if (p.chances && lane < p.rows - 1) {
+                    float chance = 0.0f;
+                    if (known) chance = theirs > 0.0 ? (float)fmin(mine / theirs, 1.0) : mine > 0.0;
+                    p.chances[(int64_t)b * (p.rows - 1) + lane] = chance;
+                }
+                if (lane < p.rows && lane != n)
+                    p.tokens[(int64_t)b * p.rows + lane] = lane < n ? draft : -1;
+            }
+        }
+        __syncthreads();
+        return made;
     }
 
-    /* Terms of the sums over a chunk's lane: e^((x - top) / T) in 64 bits. */
-    static __device__ __forceinline__ void terms(const char* row, int i, int end, float top,
-                                                 double rate, double (&w)[kN]) {
-        float x[kN];
-        widen(load(row, i, end), x);
+    /* Weighs the row that sequence b is drawn from: waves sum units of it, and the last of the
+     * sequence's workgroups to come finds the token, -1 in the others.  `weight` gets a token and
+     * its logits in both rows (`other` NULL: one). */
+    template <typename Weight>
+    static __device__ __forceinline__ int drawn(const AcceptParams& p, int b, int chunk,
+                                                const char* row, const char* other, double u,
+                                                Weight weight) {
+        const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+        uint64_t* sums = p.sums + (int64_t)b * p.units;
+        for (int unit = chunk * kWaves + wave; unit < p.units; unit += p.chunks.by * kWaves) {
+            const int i = unit * kUnit + lane * kN;
+            float x[kN], y[kN] = {};
+            const u32x4_t v = load(row, i, p.vocab);
+            if (other) widen(load(other, i, p.vocab), y);
+            widen(v, x);
+            double sum = 0.0;
 #pragma unroll
-        for (int j = 0; j < kN; ++j) w[j] = power_of_2(((double)x[j] - top) * rate);
+            for (int j = 0; j < kN; ++j) sum += weight(i + j, x[j], y[j]);
+            sum = wave_sum(sum);
+            if (lane == 0)
+                (void)__hip_atomic_exchange(&sums[unit], __builtin_bit_cast(uint64_t, sum),
+                                            __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        /* Sums and count are met in memory by device-scope atomics, past the caches: a wave's
+         * exchanges have completed before its workgroup counts.  (Fences that write back and
+         * drop the L2 instead made 16 sequences' draw take 77 us.) */
+        __shared__ int arrived;
+        __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (threadIdx.x == 0)
+            arrived = __hip_atomic_fetch_add(&p.arrived[b], 1, __ATOMIC_RELAXED,
+                                             __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (arrived != (int)p.chunks.by - 1) return -1;
+        const Search unit = find(p.units, [&](int i) {
+            return __builtin_bit_cast(
+                double, __hip_atomic_load(&sums[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+        }, 0.0, -1.0, u);
+        if (unit.place == kNone) return kNone;
+        const int from = unit.place * kUnit;
+        return from + find(min(kUnit, p.vocab - from), [&](int i) {
+            return weight(from + i, load_any(row, DT, from + i),
+                          other ? load_any(other, DT, from + i) : 0.0f);
+        }, unit.front, unit.goal, u).place;
     }
 
-    /* Both rows' sums over a chunk, where the draw is from their difference. */
-    static __device__ __forceinline__ void totals(const AcceptParams& p) {
-        const int b = blockIdx.x / p.chunks, chunk = blockIdx.x % p.chunks;
+    static __device__ __forceinline__ void weigh(const AcceptParams& p) {
+        const int b = divided(blockIdx.x, p.chunks), chunk = blockIdx.x - b * p.chunks.by;
+        const Sequence s = sequence_of(p, b);
+        const double u = p.uniforms[(int64_t)b * p.rows + p.rows - 1];
+        const AcceptDraw d = decide(p, s, b, chunk == 0);
+        if (p.draws && chunk == 0 && threadIdx.x == 0) p.draws[b] = d;
+        int32_t* out = p.tokens + (int64_t)b * p.rows + d.row;
+        const char* row = target_row(p, b, d.row);
+        const double rate = rate_of(s.t), top = d.p_top;
+        if (d.mode == DFQ_DRAW_NONE) {
+            if (chunk == 0 && threadIdx.x == 0) *out = d.token;
+        } else if (d.mode == DFQ_DRAW_REST) {
+            /* both rows' sums */
+            const char* other = draft_row(p, b, d.row);
+            const double draft_rate = rate_of(s.dt), draft_top = d.q_top;
+            const double least = -1022.0 / rate, draft_least = -1022.0 / draft_rate;
+            double p_sum = 0.0, q_sum = 0.0;
+            for (int unit = chunk * kWaves + (int)threadIdx.x / 64; unit < p.units;
+                 unit += p.chunks.by * kWaves) {
+                const int i = unit * kUnit + (int)threadIdx.x % 64 * kN;
+                const u32x4_t v = load(row, i, p.vocab), w = load(other, i, p.vocab);
+                float x[kN], y[kN];
+                widen(v, x);
+                widen(w, y);
+#pragma unroll
+                for (int j = 0; j < kN; ++j) {
+                    p_sum += power_in_sum((double)x[j] - top, rate, least);
+                    q_sum += power_in_sum((double)y[j] - draft_top, draft_rate, draft_least);
+                }
+            }
+            p_sum = block_sum(p_sum);
+            q_sum = block_sum(q_sum);
+            if (threadIdx.x == 0) {
+                double* t = p.totals + 2 * ((int64_t)b * p.chunks.by + chunk);
+                t[0] = p_sum;
+                t[1] = q_sum;
+            }
+        } else {
+            const int without = d.mode == DFQ_DRAW_OTHER ? d.draft : -1;
+            const int token = drawn(p, b, chunk, row, nullptr, u, [&](int i, float x, float) {
+                return i == without ? 0.0 : power((double)x - top, rate);
+            });
+            /* kNone: the draft has all of p */
+            if (token >= 0 && threadIdx.x == 0) *out = token == kNone ? d.draft : token;
+        }
+    }
+
+    static __device__ __forceinline__ void rest(const AcceptParams& p) {
+        const int b = divided(blockIdx.x, p.chunks), chunk = blockIdx.x - b * p.chunks.by;
         const AcceptDraw d = p.draws[b];
         if (d.mode != DFQ_DRAW_REST) return;
         const Sequence s = sequence_of(p, b);
-        const int i = chunk * kChunk + (int)threadIdx.x * kN;
-        for (int k = 0; k < 2; ++k) {
-            double w[kN], sum = 0.0;
-            terms(k ? draft_row(p, b, d.row) : target_row(p, b, d.row), i, p.vocab,
-                  k ? d.q_top : d.p_top, rate_of(k ? s.dt : s.t), w);
-#pragma unroll
-            for (int j = 0; j < kN; ++j) sum += w[j];
-            sum = block_sum(sum);
-            if (threadIdx.x == 0) p.totals[((int64_t)b * 2 + k) * p.chunks + chunk] = sum;
+        const double u = p.uniforms[(int64_t)b * p.rows + p.rows - 1];
+        const char* row = target_row(p, b, d.row);
+        const char* other = draft_row(p, b, d.row);
+        double p_sum = 0.0, q_sum = 0.0;
+        for (int i = threadIdx.x; i < (int)p.chunks.by; i += DFQ_KV_THREADS) {
+            const double* t = p.totals + 2 * ((int64_t)b * p.chunks.by + i);
+            p_sum += t[0];
+            q_sum += t[1];
         }
-    }
-
-    /* The sum of a sequence's chunks. */
-    static __device__ __forceinline__ double sum_of(const double* sums, int chunks) {
-        double v = 0.0;
-        for (int i = threadIdx.x; i < chunks; i += DFQ_KV_THREADS) v += sums[i];
-        return block_sum(v);
-    }
-
-    /* What a lane's logits of a chunk weigh in the draw; p_by and q_by are 1 / sums (REST). */
-    static __device__ __forceinline__ void weigh(const AcceptParams& p, const AcceptDraw& d,
-                                                 const Sequence& s, int b, int chunk, double p_by,
-                                                 double q_by, double (&w)[kN]) {
-        const int i = chunk * kChunk + (int)threadIdx.x * kN;
-        terms(target_row(p, b, d.row), i, p.vocab, d.p_top, rate_of(s.t), w);
-        if (d.mode == DFQ_DRAW_OTHER) {
-#pragma unroll
-            for (int j = 0; j < kN; ++j)
-                if (i + j == d.draft) w[j] = 0.0;
+        p_sum = block_sum(p_sum);
+        q_sum = block_sum(q_sum);
+        const double rate = rate_of(s.t), draft_rate = rate_of(s.dt);
+        const double top = d.p_top, draft_top = d.q_top;
+        const double by = 1.0 / p_sum, draft_by = 1.0 / q_sum;
+        int token = drawn(p, b, chunk, row, other, u, [&](int, float x, float y) {
+            return fmax(power((double)x - top, rate) * by -
+                        power((double)y - draft_top, draft_rate) * draft_by, 0.0);
+        });
+        if (token < 0) return;
+        if (token == kNone) {
+            /* p = q to the last bit, and yet refused (a random number that is not below 1): p */
+            token = find(p.vocab, [&](int i) {
+                return power((double)load_any(row, DT, i) - top, rate);
+            }, 0.0, -1.0, u).place;
         }
-        if (d.mode == DFQ_DRAW_REST) {
-            double q[kN];
-            terms(draft_row(p, b, d.row), i, p.vocab, d.q_top, rate_of(s.dt), q);
-#pragma unroll
-            for (int j = 0; j < kN; ++j) w[j] = fmax(w[j] * p_by - q[j] * q_by, 0.0);
-        }
-    }
-
-    static __device__ __forceinline__ void weights(const AcceptParams& p) {
-        const int b = blockIdx.x / p.chunks, chunk = blockIdx.x % p.chunks;
-        const AcceptDraw d = p.draws[b];
-        if (d.mode == DFQ_DRAW_NONE) return;
-        const Sequence s = sequence_of(p, b);
-        double p_by = 0.0, q_by = 0.0;
-        if (d.mode == DFQ_DRAW_REST) {
-            const double* t = p.totals + (int64_t)b * 2 * p.chunks;
-            p_by = 1.0 / sum_of(t, p.chunks);
-            q_by = 1.0 / sum_of(t + p.chunks, p.chunks);
-        }
-        double w[kN], sum = 0.0;
-        weigh(p, d, s, b, chunk, p_by, q_by, w);
-#pragma unroll
-        for (int j = 0; j < kN; ++j) sum += w[j];
-        sum = block_sum(sum);
-        if (threadIdx.x == 0) p.weights[(int64_t)b * p.chunks + chunk] = sum;
-    }
-
-    /* The token of a sequence, by one workgroup: its chunk, then its place in it. */
-    static __device__ __forceinline__ void pick(const AcceptParams& p) {
-        const int b = blockIdx.x;
-        AcceptDraw d = p.draws[b];
-        if (d.mode == DFQ_DRAW_NONE) return;
-        const Sequence s = sequence_of(p, b);
-        const double* sums = p.weights + (int64_t)b * p.chunks;
-        const double* t = p.totals + (int64_t)b * 2 * p.chunks;
-        int32_t* out = p.tokens + (int64_t)b * p.rows + d.row;
-        double all = sum_of(sums, p.chunks), p_by = 0.0, q_by = 0.0;
-        if (d.mode == DFQ_DRAW_REST) {
-            if (all > 0.0) {
-                p_by = 1.0 / sum_of(t, p.chunks);
-                q_by = 1.0 / sum_of(t + p.chunks, p.chunks);
-            } else {   /* p = q: nothing is left of p */
-                d.mode = DFQ_DRAW_P;
-                sums = t;
-                all = sum_of(sums, p.chunks);
-            }
-        }
-        if (d.mode == DFQ_DRAW_OTHER && !(all > 0.0)) {   /* the draft has all of p */
-            if (threadIdx.x == 0) *out = d.draft;
-            return;
-        }
-        const double goal = (double)p.uniforms[(int64_t)b * p.rows + p.rows - 1] * all;
-        __shared__ int chunk, place[2];
-        __shared__ double before;
-        if (threadIdx.x == 0) {
-            /* the first whose running sum passes the goal, or the last that weighs anything */
-            double sum = 0.0;
-            chunk = 0;
-            before = 0.0;
-            for (int i = 0; i < p.chunks; ++i) {
-                if (sums[i] > 0.0) {
-                    chunk = i;
-                    before = sum;
-                }
-                sum += sums[i];
-                if (sum > goal) break;
-            }
-            place[0] = 0x7fffffff;
-            place[1] = 0;
-        }
-        __syncthreads();
-        double w[kN], sum = 0.0;
-        weigh(p, d, s, b, chunk, p_by, q_by, w);
-#pragma unroll
-        for (int j = 0; j < kN; ++j) sum += w[j];
-        /* the lanes' sums in order */
-        __shared__ double lanes[DFQ_KV_THREADS];
-        lanes[threadIdx.x] = sum;
-        __syncthreads();
-        double run = before;
-        for (int i = 0; i < (int)threadIdx.x; ++i) run += lanes[i];
-        int first = 0x7fffffff, last = 0;
-#pragma unroll
-        for (int j = 0; j < kN; ++j) {
-            const int i = chunk * kChunk + (int)threadIdx.x * kN + j;
-            run += w[j];
-            if (w[j] > 0.0) {
-                last = i;
-                if (run > goal && first == 0x7fffffff) first = i;
-            }
-        }
-        atomicMin(&place[0], first);
-        atomicMax(&place[1], last);
-        __syncthreads();
-        if (threadIdx.x == 0) *out = place[0] != 0x7fffffff ? place[0] : place[1];
+        if (threadIdx.x == 0) p.tokens[(int64_t)b * p.rows + d.row] = token;
     }
 };
 
 }  // namespace
 
-#define DFQ_ACCEPT_KERNEL(op, name, dt, threads)                                   \
-    extern "C" __global__ __launch_bounds__(threads) void dfq_accept_##op##_##name( \
-        AcceptParams p) {                                                          \
-        Accept<dt>::op(p);                                                         \
+#define DFQ_ACCEPT_KERNELS(name, dt)                                              \
+    extern "C" __global__ __launch_bounds__(DFQ_KV_THREADS) void                  \
+        dfq_accept_sums_##name(AcceptParams p) {                                  \
+        Accept<dt>::sums(p);                                                      \
+    }                                                                             \
+    extern "C" __global__ __launch_bounds__(DFQ_KV_THREADS) void                  \
+        dfq_accept_weigh_##name(AcceptParams p) {                                 \
+        Accept<dt>::weigh(p);                                                     \
+    }                                                                             \
+    extern "C" __global__ __launch_bounds__(DFQ_KV_THREADS) void                  \
+        dfq_accept_rest_##name(AcceptParams p) {                                  \
+        Accept<dt>::rest(p);                                                      \
     }
-#define DFQ_ACCEPT_KERNELS(name, dt)                    \
-    DFQ_ACCEPT_KERNEL(sums, name, dt, DFQ_KV_THREADS)   \
-    DFQ_ACCEPT_KERNEL(decide, name, dt, 64)             \
-    DFQ_ACCEPT_KERNEL(totals, name, dt, DFQ_KV_THREADS) \
-    DFQ_ACCEPT_KERNEL(weights, name, dt, DFQ_KV_THREADS) \
-    DFQ_ACCEPT_KERNEL(pick, name, dt, DFQ_KV_THREADS)
 DFQ_ACCEPT_KERNELS(bf16, 0)
 DFQ_ACCEPT_KERNELS(f16, 1)
 DFQ_ACCEPT_KERNELS(f32, 2)

@@ -24,8 +24,7 @@ struct CacheKernels {
 };
 
 struct AcceptKernels {
-    hipFunction_t sums = nullptr, decide = nullptr, totals = nullptr, weights = nullptr,
-                  pick = nullptr;
+    hipFunction_t sums = nullptr, weigh = nullptr, rest = nullptr;
 };
 
 struct VerifyOps {
