@@ -84,6 +84,7 @@ struct AcceptPart {
                               * are NaN                                                   */
 };
 
+#define DFQ_ACCEPT_APART 32  /* counters lie a cache line apart                          */
 #define DFQ_ACCEPT_PIECES 8  /* 16-byte pieces that a lane takes of a range              */
 
 /* What is left to draw of a sequence: nothing, or a token from p, from p without its draft, or
@@ -110,7 +111,7 @@ struct AcceptParams {
     AcceptDraw* draws;          /* [batch], with draft logits                      */
     double* totals;             /* [batch][chunks][2]: both rows' sums             */
     uint64_t* sums;             /* [batch][units]: what is drawn from, as doubles' bits */
-    int32_t* arrived;           /* [batch]: workgroups whose sums are there        */
+    int32_t* arrived;           /* [batch][DFQ_ACCEPT_APART]: workgroups whose sums are there */
     int64_t batch_stride, row_stride, draft_batch_stride, draft_row_stride;
     float temperature, draft_temperature;
     int rows, vocab;

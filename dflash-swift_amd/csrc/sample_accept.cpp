@@ -36,14 +36,19 @@ AcceptPlan plan_accept(int cus, int batch, int rows, int V, dfq_dtype dtype, boo
     const int unit = 64 * (dtype == DFQ_F32 ? 4 : 8);
     a.units = (V + unit - 1) / unit;
     a.ranges = (V + DFQ_ACCEPT_PIECES * unit - 1) / (DFQ_ACCEPT_PIECES * unit);
-    /* a wave a unit, and no more workgroups than four a CU: each decides its sequence's drafts */
-    a.chunks = std::clamp(4 * cus / batch, 1, (a.units + kWaves - 1) / kWaves);
+    /* Workgroups of a sequence: as many units a wave as leave no more than six workgroups a CU,
+     * which are there at once, and as few workgroups as that many units take: each decides its
+     * sequence's drafts first. */
+    const auto groups = [&](int each) { return (a.units + kWaves * each - 1) / (kWaves * each); };
+    int each = 1;
+    while (groups(each) > std::max(1, 6 * cus / batch)) ++each;
+    a.chunks = groups(each);
     const auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
     a.sums = up((size_t)batch * a.all_rows * a.ranges * sizeof(AcceptPart));
     a.totals = a.sums + up((size_t)batch * a.units * 8);
     a.draws = a.totals + (drafted ? up((size_t)batch * a.chunks * 16) : 0);
     a.arrived = a.draws + (drafted ? up((size_t)batch * sizeof(AcceptDraw)) : 0);
-    a.bytes = a.arrived + (size_t)batch * 4;
+    a.bytes = a.arrived + (size_t)batch * DFQ_ACCEPT_APART * 4;
     return a;
 }
 

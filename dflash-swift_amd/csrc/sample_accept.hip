@@ -47,16 +47,11 @@ __device__ __forceinline__ double power_of_part(double f) {
 }
 
 constexpr double kWhole = 6755399441055744.0;   /* 1.5 2^52: sums with it are whole numbers */
+/* Powers stop at 2^-1022, which stands for all that is less; what weighs no more than this is 0. */
+constexpr double kNothing = 0x1p-1000;
 
-/* 2^(d rate) for d <= 0; 0 for d = -inf and past 2^-1074. */
-__device__ __forceinline__ double power(double d, double rate) {
-    const double a = fmax(d * rate, -1100.0), n = rint(a);
-    return __builtin_ldexp(power_of_part(a - n), (int)n);
-}
-
-/* The same down to 2^-1022, which stands for all that is less: `least` is -1022 / rate.  A sum
- * of such numbers beside a 1 does not hold them. */
-__device__ __forceinline__ double power_in_sum(double d, double rate, double least) {
+/* 2^(d rate) for d <= 0, down to 2^-1022; `least` is -1022 / rate. */
+__device__ __forceinline__ double power(double d, double rate, double least) {
     d = fmax(d, least);
     const double t = fma(d, rate, kWhole);
     const double v = power_of_part(fma(d, rate, kWhole - t));
@@ -70,6 +65,15 @@ __device__ __forceinline__ double power_in_sum(double d, double rate, double lea
 __device__ __forceinline__ double rate_of(float t) {
     return kLog2e / (double)fmaxf(t, 1.17549435e-38f);
 }
+/* A row's exponentials: of its logits x, 2^((x - top) rate). */
+struct Powers {
+    double rate, least, top;
+    __device__ __forceinline__ Powers(float t, float largest)
+        : rate(rate_of(t)), least(-1022.0 / rate), top(largest) {}
+    __device__ __forceinline__ double operator()(float x) const {
+        return power((double)x - top, rate, least);
+    }
+};
 __device__ __forceinline__ bool is_temperature(float t) {
     return t >= 0.0f && t < __builtin_inff();
 }
@@ -177,8 +181,8 @@ __device__ __noinline__ Search search(double a, double b, double from, double go
     double all;
     const double run = from + block_before(a + b, all);
     if (goal < 0.0) goal = u * all;
-    const uint64_t some = __ballot(a + b > 0.0);
-    const uint64_t past = __ballot(a + b > 0.0 && run + (a + b) > goal);
+    const uint64_t some = __ballot(a + b > kNothing);
+    const uint64_t past = __ballot(a + b > kNothing && run + (a + b) > goal);
     if (lane == 0) {
         firsts[wave] = past ? (int)__builtin_ctzll(past) : -1;
         lasts[wave] = some ? 63 - (int)__builtin_clzll(some) : -1;
@@ -192,7 +196,7 @@ __device__ __noinline__ Search search(double a, double b, double from, double go
         if (lasts[w] >= 0) last = 64 * w + lasts[w];
     }
     if ((int)threadIdx.x == (first != kNone ? first : last)) {
-        const bool second = a <= 0.0 || (b > 0.0 && run + a <= goal);
+        const bool second = a <= kNothing || (b > kNothing && run + a <= goal);
         place = 2 * (int)threadIdx.x + second;
         front = second ? run + a : run;
     }
@@ -264,7 +268,7 @@ struct Accept : LogitPiece<DT> {
         if (job >= p.jobs) return;
         const int row = divided(job, p.ranges), range = job - row * p.ranges.by;
         const int b = divided(row, p.all_rows), r = row - b * p.all_rows.by;
-        if (r == 0 && range == 0 && lane == 0) p.arrived[b] = 0;
+        if (r == 0 && range == 0 && lane == 0) p.arrived[b * DFQ_ACCEPT_APART] = 0;
         const bool draft = r >= p.rows;
         const Sequence q = sequence_of(p, b);
         /* rows behind a sequence's drafts, and draft rows that do not matter */
@@ -403,15 +407,21 @@ struct Accept : LogitPiece<DT> {
     /* The sum of a whole row in 64 bits, by a workgroup alone. */
     static __device__ __noinline__ double whole_row(const char* row, int vocab, float top,
                                                     float t) {
-        const double rate = rate_of(t), least = -1022.0 / rate;
+        const Powers e(t, top);
         double sum = 0.0;
         for (int i = threadIdx.x * kN; i < vocab; i += DFQ_KV_THREADS * kN) {
             float x[kN];
             widen(load(row, i, vocab), x);
 #pragma unroll
-            for (int j = 0; j < kN; ++j) sum += power_in_sum((double)x[j] - top, rate, least);
+            for (int j = 0; j < kN; ++j) sum += e(x[j]);
         }
         return block_sum(sum);
+    }
+
+    /* A logit's share of its row. */
+    static __device__ __forceinline__ double part_of(float x, float t, float top, double sum) {
+        const double v = Powers(t, top)(x);
+        return v > kNothing ? v / sum : 0.0;
     }
 
     /* Decides the drafts of sequence b, by a workgroup: 16 lanes join a row, lane i of the first
@@ -462,9 +472,8 @@ struct Accept : LogitPiece<DT> {
                 known = known && some;
                 if (known) {
                     if (greedy) mine = draft == row.at;
-                    else mine = power((double)x - row.top, rate_of(s.t)) / row.sum;
-                    if (s.drafted)
-                        theirs = power((double)y - other.top, rate_of(s.dt)) / other.sum;
+                    else mine = part_of(x, s.t, row.top, row.sum);
+                    if (s.drafted) theirs = part_of(y, s.dt, other.top, other.sum);
                     taken = u * theirs < mine;
                 }
             }
@@ -481,8 +490,8 @@ struct Accept : LogitPiece<DT> {
             if (s.drafted)
                 q_sum = whole_row(draft_row(p, b, i), p.vocab, rows[s.drafts + 1 + i].top, s.dt);
             if (wave == 0 && lane == i) {
-                if (!greedy) mine = power((double)x - row.top, rate_of(s.t)) / p_sum;
-                if (s.drafted) theirs = power((double)y - other.top, rate_of(s.dt)) / q_sum;
+                if (!greedy) mine = part_of(x, s.t, row.top, p_sum);
+                if (s.drafted) theirs = part_of(y, s.dt, other.top, q_sum);
                 taken = u * theirs < mine;
             }
         }
@@ -531,30 +540,30 @@ struct Accept : LogitPiece<DT> {
             for (int j = 0; j < kN; ++j) sum += weight(i + j, x[j], y[j]);
             sum = wave_sum(sum);
             if (lane == 0)
-                (void)__hip_atomic_exchange(&sums[unit], __builtin_bit_cast(uint64_t, sum),
-                                            __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(&sums[unit], __builtin_bit_cast(uint64_t, sum),
+                                   __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        /* Sums and count are met in memory by device-scope atomics, past the caches: a wave's
-         * exchanges have completed before its workgroup counts.  (Fences that write back and
+        /* Sums and count meet in memory, past the caches, by device-scope atomics: a wave's stores
+         * have completed before its workgroup counts.  (Fences that write back and
          * drop the L2 instead made 16 sequences' draw take 77 us.) */
         __shared__ int arrived;
         __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (threadIdx.x == 0)
-            arrived = __hip_atomic_fetch_add(&p.arrived[b], 1, __ATOMIC_RELAXED,
+            arrived = __hip_atomic_fetch_add(&p.arrived[b * DFQ_ACCEPT_APART], 1, __ATOMIC_RELAXED,
                                              __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
         if (arrived != (int)p.chunks.by - 1) return -1;
-        const Search unit = find(p.units, [&](int i) {
+        const Search found = find(p.units, [&](int i) {
             return __builtin_bit_cast(
                 double, __hip_atomic_load(&sums[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
         }, 0.0, -1.0, u);
-        if (unit.place == kNone) return kNone;
-        const int from = unit.place * kUnit;
+        if (found.place == kNone) return kNone;
+        const int from = found.place * kUnit;
         return from + find(min(kUnit, p.vocab - from), [&](int i) {
             return weight(from + i, load_any(row, DT, from + i),
                           other ? load_any(other, DT, from + i) : 0.0f);
-        }, unit.front, unit.goal, u).place;
+        }, found.front, found.goal, u).place;
     }
 
     static __device__ __forceinline__ void weigh(const AcceptParams& p) {
@@ -565,14 +574,13 @@ struct Accept : LogitPiece<DT> {
         if (p.draws && chunk == 0 && threadIdx.x == 0) p.draws[b] = d;
         int32_t* out = p.tokens + (int64_t)b * p.rows + d.row;
         const char* row = target_row(p, b, d.row);
-        const double rate = rate_of(s.t), top = d.p_top;
+        const Powers e(s.t, d.p_top);
         if (d.mode == DFQ_DRAW_NONE) {
             if (chunk == 0 && threadIdx.x == 0) *out = d.token;
         } else if (d.mode == DFQ_DRAW_REST) {
             /* both rows' sums */
             const char* other = draft_row(p, b, d.row);
-            const double draft_rate = rate_of(s.dt), draft_top = d.q_top;
-            const double least = -1022.0 / rate, draft_least = -1022.0 / draft_rate;
+            const Powers f(s.dt, d.q_top);
             double p_sum = 0.0, q_sum = 0.0;
             for (int unit = chunk * kWaves + (int)threadIdx.x / 64; unit < p.units;
                  unit += p.chunks.by * kWaves) {
@@ -583,8 +591,8 @@ struct Accept : LogitPiece<DT> {
                 widen(w, y);
 #pragma unroll
                 for (int j = 0; j < kN; ++j) {
-                    p_sum += power_in_sum((double)x[j] - top, rate, least);
-                    q_sum += power_in_sum((double)y[j] - draft_top, draft_rate, draft_least);
+                    p_sum += e(x[j]);
+                    q_sum += f(y[j]);
                 }
             }
             p_sum = block_sum(p_sum);
@@ -597,7 +605,7 @@ struct Accept : LogitPiece<DT> {
         } else {
             const int without = d.mode == DFQ_DRAW_OTHER ? d.draft : -1;
             const int token = drawn(p, b, chunk, row, nullptr, u, [&](int i, float x, float) {
-                return i == without ? 0.0 : power((double)x - top, rate);
+                return i == without ? 0.0 : e(x);
             });
             /* kNone: the draft has all of p */
             if (token >= 0 && threadIdx.x == 0) *out = token == kNone ? d.draft : token;
@@ -620,18 +628,16 @@ struct Accept : LogitPiece<DT> {
         }
         p_sum = block_sum(p_sum);
         q_sum = block_sum(q_sum);
-        const double rate = rate_of(s.t), draft_rate = rate_of(s.dt);
-        const double top = d.p_top, draft_top = d.q_top;
+        const Powers e(s.t, d.p_top), f(s.dt, d.q_top);
         const double by = 1.0 / p_sum, draft_by = 1.0 / q_sum;
         int token = drawn(p, b, chunk, row, other, u, [&](int, float x, float y) {
-            return fmax(power((double)x - top, rate) * by -
-                        power((double)y - draft_top, draft_rate) * draft_by, 0.0);
+            return fmax(fma(e(x), by, -(f(y) * draft_by)), 0.0);
         });
         if (token < 0) return;
         if (token == kNone) {
             /* p = q to the last bit, and yet refused (a random number that is not below 1): p */
             token = find(p.vocab, [&](int i) {
-                return power((double)load_any(row, DT, i) - top, rate);
+                return e(load_any(row, DT, i));
             }, 0.0, -1.0, u).place;
         }
         if (threadIdx.x == 0) p.tokens[(int64_t)b * p.rows + d.row] = token;

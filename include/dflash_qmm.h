@@ -492,7 +492,8 @@ dfq_status dfq_token_logprobs(dfq_ctx* ctx, const void* logits, int64_t row_stri
  * numbers gives the same tokens, distributed as p (chances are right to 2^-20 of themselves, the
  * drawn token is that of 64-bit sums).  temperatures and draft_temperatures [batch] are in device
  * memory; NULL: `temperature`, `draft_temperature` for all.  T = 0 takes p = 1 for the row's
- * argmax, as dfq_argmax_accept finds it.  A logit of -inf has probability 0.  A row with a NaN or
+ * argmax, as dfq_argmax_accept finds it.  A logit of -inf has probability 0, as have probabilities
+ * under 2^-1000 of the row's largest.  A row with a NaN or
  * +inf, with nothing above -inf, or with a temperature of its sequence that is negative or not
  * finite has no distribution: a draft judged by such a row of the target or the draft is refused
  * (chance 0), and the token in its place is -1.  So is refused a draft outside 0..V-1 (the token is
