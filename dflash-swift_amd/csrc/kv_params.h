@@ -129,19 +129,20 @@ struct RopeTensor {
     const void* weight;      /* [dim] or NULL                                    */
     int64_t in_batch, in_row, in_head, out_batch, out_row, out_head;   /* elements */
     int heads;
+    Divisor slots;           /* of a token: slot s holds heads s, s + slots, ..  */
 };
 
 struct RopeParams {
-    RopeTensor t[2];         /* queries, keys (0 heads: none)                    */
+    RopeTensor t[2];         /* queries, keys                                    */
     const uint64_t* turns;   /* [pairs] 2^-64 turns a position                   */
     const int32_t* starts;   /* first position of each sequence, added to start  */
     const int32_t* positions;   /* [batch][rows], in place of those, or NULL     */
-    int64_t slots;           /* heads of all tokens                              */
-    int start, dim, pairs;
+    int tokens, start, dim, pairs;
+    int q_groups;            /* workgroups of the queries; the keys' come behind */
     int lanes;               /* that hold a head (rotate_heads)                  */
     int inverse, interleaved, weight_f32;
     float amplitude, eps, offset;
-    Divisor all_heads, rows;
+    Divisor rows;
 };
 
 #endif

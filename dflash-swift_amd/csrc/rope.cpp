@@ -2,6 +2,7 @@
  * rope.cpp -- the C ABI of the rotary positions: frequency tables (host only), argument checks and
  * launches of rope.hip.
  */
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -25,7 +26,7 @@ dfq_status check_heads(const dfq_heads* t, const char* name, dfq_dtype dtype) {
 
 RopeTensor tensor_of(const dfq_heads* t, const void* weight) {
     return {t->in, t->out, weight, t->in_batch, t->in_row, t->in_head,
-            t->out_batch, t->out_row, t->out_head, t->heads};
+            t->out_batch, t->out_row, t->out_head, t->heads, divisor(t->heads)};
 }
 
 struct Norms {
@@ -90,9 +91,8 @@ dfq_status rotate(dfq_ctx* ctx, const dfq_rope_table* rope, const dfq_heads* q, 
     p.positions = positions;
     p.start = start;
     p.inverse = inverse != 0;
-    p.slots = tokens * all;
+    p.tokens = (int)tokens;
     p.dim = head_dim;
-    p.all_heads = divisor((int)all);
     p.rows = divisor(rows);
     /* Chunks of 8 channels hold both channels of their pairs where a head is 16 n wide and, with
      * pairs half the rotated width apart, that half is a multiple of 8. */
@@ -104,10 +104,20 @@ dfq_status rotate(dfq_ctx* ctx, const dfq_rope_table* rope, const dfq_heads* q, 
     const VerifyOps* ops;
     if ((s = ctx_verify_ops(ctx, &ops))) return s;
     DeviceScope scope(ctx);
+    /* Heads a lane, whose angles are found once: as many as leave every SIMD two waves, up to 16
+     * (one in rotate_any). */
+    const int64_t waves = tokens * all * p.lanes / 64;
+    const int each = chunks ? (int)std::clamp<int64_t>(waves / (8 * dfq_num_cus(ctx)), 1, 16) : 1;
     const int64_t per = DFQ_KV_THREADS / p.lanes;
+    const auto groups = [&](RopeTensor& t) {
+        t.slots = divisor((t.heads + each - 1) / each);
+        return (tokens * t.slots.by + per - 1) / per;
+    };
+    p.q_groups = (int)groups(p.t[0]);
+    const int64_t k_groups = k ? groups(p.t[1]) : 0;
     void* args[] = {&p};
     const hipError_t e = hipModuleLaunchKernel(
-        ops->rotate[norms != nullptr][way][(int)dtype], (unsigned)((p.slots + per - 1) / per), 1, 1,
+        ops->rotate[norms != nullptr][way][(int)dtype], (unsigned)(p.q_groups + k_groups), 1, 1,
         DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
     return e == hipSuccess ? DFQ_OK : hip_error(e, what);
 }

@@ -56,55 +56,50 @@ __device__ __forceinline__ uint64_t position(const RopeParams& p, int b, int m) 
     return (uint64_t)(p.inverse ? -pos : pos);
 }
 
-/* Pair i turned by its angle at `pos`. */
-__device__ __forceinline__ void turn_pair(const RopeParams& p, uint64_t pos, int i, float& a,
-                                          float& b) {
-    float sine, cosine;
+/* Sine and cosine of pair i at `pos`, times the amplitude. */
+__device__ __forceinline__ void pair_turn(const RopeParams& p, uint64_t pos, int i, float& sine,
+                                          float& cosine) {
     turn_of((uint32_t)(pos * p.turns[i] >> 32), sine, cosine);
     sine *= p.amplitude;
     cosine *= p.amplitude;
+}
+
+__device__ __forceinline__ void turn(float& a, float& b, float sine, float cosine) {
     const float c = a;
     a = c * cosine - b * sine;
     b = b * cosine + c * sine;
 }
 
+/* 8 neighbouring elements, as they lie in memory and as fp32. */
 template <int DT>
 struct Chunk {
-    static constexpr int kSize = DT == 2 ? 4 : 2;
-    /* 8 neighbouring elements as fp32, and back. */
-    static __device__ __forceinline__ void load(const void* base, int64_t at, float (&f)[8]) {
-        const char* a = (const char*)base + at * kSize;
-        if constexpr (DT == 2) {
+    static constexpr int kSize = DT == 2 ? 4 : 2, kWords = kSize / 2;
+    u32x4_t raw[kWords];
+    __device__ __forceinline__ void load(const void* base, int64_t at) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const u32x4_t v = *(const u32x4_any*)(a + 16 * i);
+        for (int i = 0; i < kWords; ++i)
+            raw[i] = *(const u32x4_any*)((const char*)base + at * kSize + 16 * i);
+    }
+    __device__ __forceinline__ void store(void* base, int64_t at) const {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) f[4 * i + j] = __uint_as_float(v[j]);
-            }
-        } else {
-            const u32x4_t v = *(const u32x4_any*)a;
+        for (int i = 0; i < kWords; ++i)
+            __builtin_nontemporal_store(raw[i],
+                                        (u32x4_any*)((char*)base + at * kSize + 16 * i));
+    }
+    __device__ __forceinline__ void widen(float (&f)[8]) const {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                f[2 * i] = elem_to_f32<DT == 1>(v[i] & 0xffffu);
-                f[2 * i + 1] = elem_to_f32<DT == 1>(v[i] >> 16);
-            }
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (DT == 2) f[i] = __uint_as_float(raw[i / 4][i % 4]);
+            else f[i] = elem_to_f32<DT == 1>(raw[0][i / 2] >> (16 * (i % 2)) & 0xffffu);
         }
     }
-    static __device__ __forceinline__ void store(void* base, int64_t at, const float (&f)[8]) {
-        char* a = (char*)base + at * kSize;
+    __device__ __forceinline__ void round(const float (&f)[8]) {
         if constexpr (DT == 2) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                u32x4_t v;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = __float_as_uint(f[4 * i + j]);
-                *(u32x4_any*)(a + 16 * i) = v;
-            }
+            for (int i = 0; i < 8; ++i) raw[i / 4][i % 4] = __float_as_uint(f[i]);
         } else {
-            u32x4_t v;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = rounded2<DT == 1>(f[2 * i], f[2 * i + 1]);
-            *(u32x4_any*)a = v;
+            for (int i = 0; i < 4; ++i) raw[0][i] = rounded2<DT == 1>(f[2 * i], f[2 * i + 1]);
         }
     }
 };
@@ -113,83 +108,128 @@ __device__ __forceinline__ int divided(int n, const Divisor& d) {
     return (int)((n + (uint64_t)((uint64_t)(uint32_t)n * d.mul >> 32)) >> d.shift);
 }
 
-/* The sum over the `lanes` (a power of two up to 32) that hold a head. */
+/* The sum over the `lanes` (a power of two) that hold a head. */
 __device__ __forceinline__ float head_sum(float v, int lanes) {
-    for (int d = 1; d < lanes; d *= 2) v += __shfl_xor(v, d);
+    const auto add = [](uint32_t a, uint32_t b) {
+        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+    };
+    uint32_t u = __float_as_uint(v);
+    if (lanes > 1) u = exchange<0xB1>(u, add);
+    if (lanes > 2) u = exchange<0x4E>(u, add);
+    if (lanes > 4) u = exchange<0x141>(u, add);
+    if (lanes > 8) u = exchange<0x140>(u, add);
+    v = __uint_as_float(u);
+    if (lanes > 16) v += __shfl_xor(v, 16);
+    if (lanes > 32) v += __shfl_xor(v, 32);
     return v;
 }
 
 /* Heads of 16 n channels: a lane holds two chunks of 8, so that it has both channels of each of
- * its 8 pairs.  `lanes` lanes a head, the heads of one token side by side. */
+ * its 8 pairs, of every `slots`-th head of one token, whose angles it finds once.  `lanes` lanes a
+ * head, neighbouring heads side by side. */
 template <int DT, bool NORM, bool INTERLEAVED>
 __device__ __forceinline__ void rotate_heads(const RopeParams& p) {
+    const bool keys = (int)blockIdx.x >= p.q_groups;
+    const RopeTensor& t = p.t[keys];
+    const int group = keys ? blockIdx.x - p.q_groups : blockIdx.x;
     const int lane = threadIdx.x % p.lanes;
-    const int64_t slot = (int64_t)blockIdx.x * (DFQ_KV_THREADS / p.lanes) + threadIdx.x / p.lanes;
-    if (slot >= p.slots) return;
-    const int token = divided((int)slot, p.all_heads);
-    int head = (int)slot - token * p.all_heads.by;
+    const int64_t slot = (int64_t)group * (DFQ_KV_THREADS / p.lanes) + threadIdx.x / p.lanes;
+    if (slot >= (int64_t)p.tokens * t.slots.by) return;
+    const int token = divided((int)slot, t.slots);
+    int head = (int)slot - token * t.slots.by;
     const int b = divided(token, p.rows), m = token - b * p.rows.by;
-    const bool k = head >= p.t[0].heads;
-    const RopeTensor& t = p.t[k];
-    if (k) head -= p.t[0].heads;
     const bool active = lane * 16 < p.dim;
     /* the lane's chunks: of a rotated half and its partner, or neighbours */
     const bool halves = !INTERLEAVED && lane * 8 < p.pairs;
     const int at0 = halves ? lane * 8 : lane * 16;
     const int at1 = halves ? at0 + p.pairs : at0 + 8;
-    float x[2][8] = {};
+    const int64_t in = b * t.in_batch + m * t.in_row, out = b * t.out_batch + m * t.out_row;
+    Chunk<DT> c[2] = {};
     if (active) {
-        const int64_t from = b * t.in_batch + m * t.in_row + head * t.in_head;
-        Chunk<DT>::load(t.in, from + at0, x[0]);
-        Chunk<DT>::load(t.in, from + at1, x[1]);
+        c[0].load(t.in, in + head * t.in_head + at0);
+        c[1].load(t.in, in + head * t.in_head + at1);
     }
+    float w[2][8];
     if constexpr (NORM) {
-        float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum = fmaf(x[0][i], x[0][i], fmaf(x[1][i], x[1][i], sum));
-        sum = head_sum(sum, p.lanes);
-        if (!active) return;
-        const float scale = rsqrtf(sum / (float)p.dim + p.eps);
+        for (int k = 0; k < 2; ++k) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+            for (int i = 0; i < 8; ++i) w[k][i] = 1.0f;
+            if (!t.weight || !active) continue;
+            if (p.weight_f32) {
+                Chunk<2> v;
+                v.load(t.weight, k ? at1 : at0);
+                v.widen(w[k]);
+            } else {
+                Chunk<DT> v;
+                v.load(t.weight, k ? at1 : at0);
+                v.widen(w[k]);
+            }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[c][i] *= scale;
-            if (!t.weight) continue;
-            float w[8];
-            if (p.weight_f32) Chunk<2>::load(t.weight, c ? at1 : at0, w);
-            else Chunk<DT>::load(t.weight, c ? at1 : at0, w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[c][i] *= w[i] + p.offset;
+            for (int i = 0; i < 8; ++i) w[k][i] += p.offset;
         }
     }
-    if (!active) return;
-    const uint64_t pos = position(p, b, m);
+    float sine[8] = {}, cosine[8] = {};
+    const int pairs = active ? p.pairs - lane * 8 : 0;   /* of this lane's 8 that turn */
+    if (pairs > 0) {
+        const uint64_t pos = position(p, b, m);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        /* channels behind the rotated ones stay as they are, infinities and NaN among them */
-        if (lane * 8 + i >= p.pairs) break;
-        if constexpr (INTERLEAVED)
-            turn_pair(p, pos, lane * 8 + i, x[i / 4][2 * (i % 4)], x[i / 4][2 * (i % 4) + 1]);
-        else
-            turn_pair(p, pos, lane * 8 + i, x[0][i], x[1][i]);
+        for (int i = 0; i < 8; ++i)
+            if (i < pairs) pair_turn(p, pos, lane * 8 + i, sine[i], cosine[i]);
     }
-    const int64_t to = b * t.out_batch + m * t.out_row + head * t.out_head;
-    Chunk<DT>::store(t.out, to + at0, x[0]);
-    Chunk<DT>::store(t.out, to + at1, x[1]);
+    for (;;) {
+        float x[2][8];
+        c[0].widen(x[0]);
+        c[1].widen(x[1]);
+        /* the next head comes meanwhile */
+        const int next = head + t.slots.by;
+        if (active && next < t.heads) {
+            c[0].load(t.in, in + next * t.in_head + at0);
+            c[1].load(t.in, in + next * t.in_head + at1);
+        }
+        if constexpr (NORM) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum = fmaf(x[0][i], x[0][i], fmaf(x[1][i], x[1][i], sum));
+            const float scale = rsqrtf(head_sum(sum, p.lanes) / (float)p.dim + p.eps);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[0][i] *= scale * w[0][i];
+                x[1][i] *= scale * w[1][i];
+            }
+        }
+        /* channels behind the rotated ones stay as they are, infinities and NaN among them */
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (i >= pairs) break;
+            if constexpr (INTERLEAVED)
+                turn(x[i / 4][2 * (i % 4)], x[i / 4][2 * (i % 4) + 1], sine[i], cosine[i]);
+            else
+                turn(x[0][i], x[1][i], sine[i], cosine[i]);
+        }
+        if (active) {
+            Chunk<DT> y[2];
+            y[0].round(x[0]);
+            y[1].round(x[1]);
+            y[0].store(t.out, out + head * t.out_head + at0);
+            y[1].store(t.out, out + head * t.out_head + at1);
+        }
+        if (next >= t.heads) return;
+        head = next;
+    }
 }
 
 /* Any even head and any number of pairs: a wave a head, a lane a pair at a time. */
 template <int DT, bool NORM>
 __device__ __forceinline__ void rotate_any(const RopeParams& p) {
     const int lane = threadIdx.x % 64;
-    const int64_t slot = (int64_t)blockIdx.x * (DFQ_KV_THREADS / 64) + threadIdx.x / 64;
-    if (slot >= p.slots) return;
-    const int token = divided((int)slot, p.all_heads);
-    int head = (int)slot - token * p.all_heads.by;
+    const bool keys = (int)blockIdx.x >= p.q_groups;
+    const RopeTensor& t = p.t[keys];
+    const int group = keys ? blockIdx.x - p.q_groups : blockIdx.x;
+    const int64_t slot = (int64_t)group * (DFQ_KV_THREADS / 64) + threadIdx.x / 64;
+    if (slot >= (int64_t)p.tokens * t.slots.by) return;
+    const int token = divided((int)slot, t.slots), head = (int)slot - token * t.slots.by;
     const int b = divided(token, p.rows), m = token - b * p.rows.by;
-    const bool k = head >= p.t[0].heads;
-    const RopeTensor& t = p.t[k];
-    if (k) head -= p.t[0].heads;
     const int64_t from = b * t.in_batch + m * t.in_row + head * t.in_head;
     const int64_t to = b * t.out_batch + m * t.out_row + head * t.out_head;
     const uint64_t pos = position(p, b, m);
@@ -225,7 +265,11 @@ __device__ __forceinline__ void rotate_any(const RopeParams& p) {
                 c *= load_any(t.weight, wt, at1) + p.offset;
             }
         }
-        if (i < p.pairs) turn_pair(p, pos, i, a, c);
+        if (i < p.pairs) {
+            float sine, cosine;
+            pair_turn(p, pos, i, sine, cosine);
+            turn(a, c, sine, cosine);
+        }
         store_any(t.out, DT, to + at0, a);
         store_any(t.out, DT, to + at1, c);
     }

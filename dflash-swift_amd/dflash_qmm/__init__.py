@@ -660,23 +660,25 @@ class Context:
             self._elsewhere(q, k, rope and rope.turns, starts, positions, q_out, k_out)
         if max(batch, rows, heads, dim, start, -start) > _INT_MAX:
             raise ValueError("batch, rows, heads, head_dim or start past a C int")
-        if q_out is None:
-            q_out = torch.empty(shape, dtype=q.dtype, device=q.device)
-        packed_q, packed_k = _heads("q", q, q_out, q), None
+        dtype = q.dtype
+        q_out, packed_q = _heads("q", q, q_out, rows, heads, dim, dtype)
+        packed_k = None
         if k is not None:
-            if len(k.shape) != 4 or k.shape[0] != batch or k.shape[1] != rows or \
-                    k.shape[3] != dim or k.dtype != q.dtype:
+            other = k.shape
+            if len(other) != 4 or other[0] != batch or other[1] != rows or other[3] != dim or \
+                    k.dtype is not dtype:
                 raise ValueError("k is [batch, rows, heads, head_dim], with q's but for heads, in "
                                  "q's dtype")
-            if k_out is None:
-                k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-            packed_k = _heads("k", k, k_out, k)
+            if other[2] > _INT_MAX:
+                raise ValueError("heads past a C int")
+            k_out, packed_k = _heads("k", k, k_out, rows, other[2], dim, dtype)
         elif k_out is not None:
             raise ValueError("k_out without k")
-        d_starts = _check_int32("starts", starts, (batch,))
-        d_positions = _check_int32("positions", positions, (batch, rows))
+        d_starts = None if starts is None else _check_int32("starts", starts, (batch,))
+        d_positions = None if positions is None else \
+            _check_int32("positions", positions, (batch, rows))
         table = rope.table if rope is not None else None
-        dt = dtype_code(q)
+        dt = dtype_code(dtype)
         if norms is None:
             st = self.lib.dfq_rope(self.handle, table, packed_q, packed_k, dim, dt, batch, rows,
                                    start, d_starts, d_positions, inverse, self._stream_of(stream))
@@ -692,7 +694,7 @@ class Context:
                 self._elsewhere(q, t)
             kind = t.dtype
             if t.shape != (dim,) or not t.is_contiguous() or \
-                    kind is not q.dtype and kind is not torch.float32:
+                    kind is not dtype and kind is not torch.float32:
                 raise ValueError("weights are contiguous [head_dim] in q's dtype or fp32")
             wt = dtype_code(kind)
         if q_weight is not None and k_weight is not None and q_weight.dtype is not k_weight.dtype:
@@ -775,15 +777,20 @@ class Context:
         batch, rows, V = shape
         if draft_temperature is None:
             draft_temperature = temperature
-        t, dt = (x if isinstance(x, torch.Tensor) else None
-                 for x in (temperature, draft_temperature))
-        for a in (logits, uniforms, drafts, draft_logits, t, dt, draft_lengths, ws):
-            if a is not None and a.get_device() != device:
-                self._elsewhere(logits, uniforms, drafts, draft_logits, t, dt, draft_lengths, ws)
+        t = temperature if isinstance(temperature, torch.Tensor) else None
+        dt = draft_temperature if isinstance(draft_temperature, torch.Tensor) else None
+        if not (logits.get_device() == uniforms.get_device() == device) or \
+                drafts is not None and drafts.get_device() != device or \
+                draft_logits is not None and draft_logits.get_device() != device or \
+                t is not None and t.get_device() != device or \
+                dt is not None and dt.get_device() != device or \
+                draft_lengths is not None and draft_lengths.get_device() != device or \
+                ws is not None and ws.get_device() != device:
+            self._elsewhere(logits, uniforms, drafts, draft_logits, t, dt, draft_lengths, ws)
         if max(batch, rows, V) > _INT_MAX:
             raise ValueError("batch, rows or V past a C int")
-        s, one = logits.stride()[:2], logits.stride(2)
-        if one != 1 and V > 1:
+        s = logits.stride()
+        if s[2] != 1 and V > 1:
             raise ValueError("a row's logits must be contiguous")
         if (drafts is None) != (rows == 1):
             raise ValueError("a block of rows has rows - 1 drafts")
@@ -791,7 +798,7 @@ class Context:
         d_lengths = _check_int32("draft_lengths", draft_lengths, (batch,))
         d_uniforms = _check_f32("uniforms", uniforms, (batch, rows))
         d_t = _check_f32("temperature", t, (batch,))
-        d_dt = _check_f32("draft_temperature", dt, (batch,))
+        d_dt = d_t if dt is t else _check_f32("draft_temperature", dt, (batch,))
         p_draft, ds = None, (0, 0)
         if draft_logits is not None:
             if draft_logits.shape != (batch, rows - 1, V) or draft_logits.dtype != logits.dtype:
@@ -800,9 +807,10 @@ class Context:
             if ds[2] != 1 and V > 1:
                 raise ValueError("a row's draft logits must be contiguous")
             p_draft = draft_logits.data_ptr() if rows > 1 else None
-        tokens = torch.empty((batch, rows), dtype=torch.int32, device=logits.device)
+        tokens = torch.empty_like(uniforms, dtype=torch.int32)
         accepted = torch.empty(batch, dtype=torch.int32, device=logits.device)
-        chances = torch.empty((batch, rows - 1), dtype=torch.float32, device=logits.device)
+        chances = torch.empty((batch, 0), dtype=torch.float32, device=logits.device) \
+            if drafts is None else torch.empty_like(drafts, dtype=torch.float32)
         code = dtype_code(logits)
         stream = self._stream_of(stream)
         own_ws = ws is None
@@ -1015,22 +1023,27 @@ def _check_f32(name, t, shape):
     return t.data_ptr()
 
 
-def _heads(name, t, out, like):
-    """dfq_heads of t [batch, rows, heads, head_dim] into out."""
-    a, b = t.stride(), out.stride()
-    if t.shape[3] > 1 and (a[3] != 1 or b[3] != 1):
+def _heads(name, t, out, rows, heads, dim, dtype):
+    """(out, dfq_heads) of t [batch, rows, heads, head_dim] into out, made where it is None."""
+    a = t.stride()
+    if out is None:
+        import torch
+        out = torch.empty_like(t, memory_format=torch.contiguous_format)
+        b = (rows * heads * dim, heads * dim, dim, 1)
+    else:
+        if out.shape != t.shape or out.dtype is not dtype:
+            raise ValueError(f"{name}_out is of {name}'s shape and dtype")
+        b = out.stride()
+        if not out.is_contiguous():
+            # heads that share elements would be written by several lanes
+            room = dim
+            for stride, n in sorted((s, n) for s, n in zip(b[:3], out.shape) if n > 1):
+                if stride < room:
+                    raise ValueError(f"{name}_out has heads that overlap")
+                room = stride * n
+    if dim > 1 and (a[3] != 1 or b[3] != 1):
         raise ValueError(f"{name}: a head's channels must be contiguous")
-    if out.shape != like.shape or out.dtype != like.dtype:
-        raise ValueError(f"{name}_out is of {name}'s shape and dtype")
-    if not out.is_contiguous():
-        # heads that share elements would be written by several lanes
-        room = out.shape[3]
-        for stride, n in sorted((s, n) for s, n in zip(b[:3], out.shape) if n > 1):
-            if stride < room:
-                raise ValueError(f"{name}_out has heads that overlap")
-            room = stride * n
-    return _pack_heads(t.data_ptr(), out.data_ptr(), a[0], a[1], a[2], b[0], b[1], b[2],
-                       t.shape[2])
+    return out, _pack_heads(t.data_ptr(), out.data_ptr(), a[0], a[1], a[2], b[0], b[1], b[2], heads)
 
 
 class Rope:

@@ -232,6 +232,13 @@ def test_accepts_that_are_refused():
 
 # ---- the wrappers --------------------------------------------------------------------------
 
+@pytest.fixture(autouse=True)
+def like(monkeypatch):
+    """torch.empty_like of such a tensor, as the recording library's fixture has torch.empty."""
+    monkeypatch.setattr(torch, "empty_like", lambda t, dtype=None, memory_format=None:
+                        torch.empty(t.shape, dtype=dtype or t.dtype, device=t.device))
+
+
 class Tensor(Fake):
     """A Fake with strides of its own, whose dtype torch knows."""
 
