@@ -118,7 +118,7 @@ struct AcceptParams {
     int jobs;                   /* ranges of all rows                              */
     int units;                  /* 64 lanes' 16 bytes each, of a row               */
     Divisor all_rows, ranges;   /* rows and draft rows of a sequence; ranges a row */
-    Divisor chunks;             /* workgroups of a sequence in the later kernels   */
+    Divisor chunks, rest_chunks;   /* workgroups of a sequence in the later kernels */
 };
 
 #define DFQ_ROPE_DIM 512     /* widest head */

@@ -24,7 +24,7 @@ dfq_status check_sizes(int batch, int rows, int V, dfq_dtype dtype) {
 }
 
 struct AcceptPlan {
-    int all_rows, ranges, units, chunks;
+    int all_rows, ranges, units, chunks, rest_chunks;
     size_t sums, totals, draws, arrived, bytes;   /* offsets; the parts come first */
 };
 
@@ -43,6 +43,7 @@ AcceptPlan plan_accept(int cus, int batch, int rows, int V, dfq_dtype dtype, boo
     int each = 1;
     while (groups(each) > std::max(1, 6 * cus / batch)) ++each;
     a.chunks = groups(each);
+    a.rest_chunks = groups(1);
     const auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
     a.sums = up((size_t)batch * a.all_rows * a.ranges * sizeof(AcceptPart));
     a.totals = a.sums + up((size_t)batch * a.units * 8);
@@ -98,8 +99,8 @@ dfq_status dfq_sample_accept(dfq_ctx* ctx, const void* logits, int64_t batch_str
         return fail(DFQ_ERR_INVALID_ARGUMENT, "temperatures are finite and not negative");
     const AcceptPlan a = plan_accept(dfq_num_cus(ctx), batch, rows, V, dtype, drafted);
     const int64_t jobs = (int64_t)batch * a.all_rows * a.ranges;
-    const int64_t chunks = (int64_t)batch * a.chunks;
-    if (jobs > INT32_MAX || chunks > INT32_MAX)
+    const int64_t chunks = (int64_t)batch * a.chunks, rest = (int64_t)batch * a.rest_chunks;
+    if (jobs > INT32_MAX || rest > INT32_MAX)
         return fail(DFQ_ERR_UNSUPPORTED, "grid too large");
     if (!workspace || workspace_bytes < a.bytes)
         return fail(DFQ_ERR_WORKSPACE, "workspace of %zu bytes needed (got %zu)", a.bytes,
@@ -136,6 +137,7 @@ dfq_status dfq_sample_accept(dfq_ctx* ctx, const void* logits, int64_t batch_str
     p.all_rows = divisor(a.all_rows);
     p.ranges = divisor(a.ranges);
     p.chunks = divisor(a.chunks);
+    p.rest_chunks = divisor(a.rest_chunks);
     const VerifyOps* ops;
     if ((s = ctx_verify_ops(ctx, &ops))) return s;
     DeviceScope scope(ctx);
@@ -144,10 +146,12 @@ dfq_status dfq_sample_accept(dfq_ctx* ctx, const void* logits, int64_t batch_str
     hipError_t e = hipModuleLaunchKernel(fn.sums, (unsigned)((jobs + kWaves - 1) / kWaves), 1, 1,
                                          DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args,
                                          nullptr);
-    for (hipFunction_t f : {fn.weigh, drafted ? fn.rest : nullptr})
-        if (f && e == hipSuccess)
-            e = hipModuleLaunchKernel(f, (unsigned)chunks, 1, 1, DFQ_KV_THREADS, 1, 1, 0,
-                                      (hipStream_t)stream, args, nullptr);
+    if (e == hipSuccess)
+        e = hipModuleLaunchKernel(fn.weigh, (unsigned)chunks, 1, 1, DFQ_KV_THREADS, 1, 1, 0,
+                                  (hipStream_t)stream, args, nullptr);
+    if (e == hipSuccess && drafted)
+        e = hipModuleLaunchKernel(fn.rest, (unsigned)rest, 1, 1, DFQ_KV_THREADS, 1, 1, 0,
+                                  (hipStream_t)stream, args, nullptr);
     return e == hipSuccess ? DFQ_OK : hip_error(e, "launch dfq_sample_accept");
 }
 

@@ -524,12 +524,12 @@ struct Accept : LogitPiece<DT> {
      * sequence's workgroups to come finds the token, -1 in the others.  `weight` gets a token and
      * its logits in both rows (`other` NULL: one). */
     template <typename Weight>
-    static __device__ __forceinline__ int drawn(const AcceptParams& p, int b, int chunk,
-                                                const char* row, const char* other, double u,
-                                                Weight weight) {
+    static __device__ __forceinline__ int drawn(const AcceptParams& p, int chunks, int b,
+                                                int chunk, const char* row, const char* other,
+                                                double u, Weight weight) {
         const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
         uint64_t* sums = p.sums + (int64_t)b * p.units;
-        for (int unit = chunk * kWaves + wave; unit < p.units; unit += p.chunks.by * kWaves) {
+        for (int unit = chunk * kWaves + wave; unit < p.units; unit += chunks * kWaves) {
             const int i = unit * kUnit + lane * kN;
             float x[kN], y[kN] = {};
             const u32x4_t v = load(row, i, p.vocab);
@@ -553,7 +553,7 @@ struct Accept : LogitPiece<DT> {
             arrived = __hip_atomic_fetch_add(&p.arrived[b * DFQ_ACCEPT_APART], 1, __ATOMIC_RELAXED,
                                              __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
-        if (arrived != (int)p.chunks.by - 1) return -1;
+        if (arrived != chunks - 1) return -1;
         const Search found = find(p.units, [&](int i) {
             return __builtin_bit_cast(
                 double, __hip_atomic_load(&sums[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
@@ -604,7 +604,8 @@ struct Accept : LogitPiece<DT> {
             }
         } else {
             const int without = d.mode == DFQ_DRAW_OTHER ? d.draft : -1;
-            const int token = drawn(p, b, chunk, row, nullptr, u, [&](int i, float x, float) {
+            const int token = drawn(p, p.chunks.by, b, chunk, row, nullptr, u,
+                                    [&](int i, float x, float) {
                 return i == without ? 0.0 : e(x);
             });
             /* kNone: the draft has all of p */
@@ -613,7 +614,8 @@ struct Accept : LogitPiece<DT> {
     }
 
     static __device__ __forceinline__ void rest(const AcceptParams& p) {
-        const int b = divided(blockIdx.x, p.chunks), chunk = blockIdx.x - b * p.chunks.by;
+        const int b = divided(blockIdx.x, p.rest_chunks);
+        const int chunk = blockIdx.x - b * p.rest_chunks.by;
         const AcceptDraw d = p.draws[b];
         if (d.mode != DFQ_DRAW_REST) return;
         const Sequence s = sequence_of(p, b);
@@ -630,7 +632,7 @@ struct Accept : LogitPiece<DT> {
         q_sum = block_sum(q_sum);
         const Powers e(s.t, d.p_top), f(s.dt, d.q_top);
         const double by = 1.0 / p_sum, draft_by = 1.0 / q_sum;
-        int token = drawn(p, b, chunk, row, other, u, [&](int, float x, float y) {
+        int token = drawn(p, p.rest_chunks.by, b, chunk, row, other, u, [&](int, float x, float y) {
             return fmax(fma(e(x), by, -(f(y) * draft_by)), 0.0);
         });
         if (token < 0) return;
