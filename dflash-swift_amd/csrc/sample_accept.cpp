@@ -39,11 +39,10 @@ AcceptPlan plan_accept(int cus, int batch, int rows, int V, dfq_dtype dtype, boo
     /* Workgroups of a sequence: as many units a wave as leave no more than six workgroups a CU,
      * which are there at once, and as few workgroups as that many units take: each decides its
      * sequence's drafts first. */
-    const auto groups = [&](int each) { return (a.units + kWaves * each - 1) / (kWaves * each); };
-    int each = 1;
-    while (groups(each) > std::max(1, 6 * cus / batch)) ++each;
-    a.chunks = groups(each);
-    a.rest_chunks = groups(1);
+    const auto parts = [](int n, int of) { return (int)(((int64_t)n + of - 1) / of); };
+    const int most = std::max(1, 6 * cus / batch);
+    a.chunks = parts(a.units, kWaves * parts(a.units, kWaves * most));
+    a.rest_chunks = parts(a.units, kWaves);   /* nothing is decided there */
     const auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
     a.sums = up((size_t)batch * a.all_rows * a.ranges * sizeof(AcceptPart));
     a.totals = a.sums + up((size_t)batch * a.units * 8);

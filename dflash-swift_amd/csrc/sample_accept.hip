@@ -10,10 +10,12 @@
  *
  * Tokens and counts are whole numbers that a sum's last bits decide, and come out as 64-bit
  * arithmetic has them (exponentials to 8e-13): draws sum and search in 64 bits, and a draft whose
- * u q is within 2^-16 of p, more than the fp32 sums of its rows can be off, is decided again from
- * 64-bit sums.  Other drafts need no more than fp32, in which a logit costs 8 instructions against
- * 20: all rows in 64 bits took 93 us at 64 sequences of seven drafts for 151936 tokens, the rows
- * of the draws apart.
+ * u q is within 2^-16 of p is decided again from 64-bit sums.  Other drafts need no more than fp32,
+ * in which a logit costs 8 instructions against 20: all rows of 64 sequences of seven drafts of
+ * 151936 tokens in 64 bits took 93 us for 46.  An fp32 sum is off by less than 2^-17 / 2 of itself:
+ * an exponent a has three roundings, 2.5 2^-24 |a|, and the mean of |a| over a row's mass is at most
+ * log2 V, which makes 34 2^-24 for 2^20 tokens and 52 for 2^30; 17 sums in a row and the
+ * exponential's last bit are 20 more.
  *
  * The first launch reads all rows once: a wave takes a range of one row in registers, finds its
  * largest logit and the sum of e^((x - largest) / T).  In the second each workgroup joins its
@@ -108,11 +110,14 @@ __device__ __forceinline__ double dpp_f64(double v) {
     const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, 0xF, 0xF, true);
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-__device__ __forceinline__ double wave_sum(double v) {
+__device__ __forceinline__ double lanes16_sum(double v) {
     v += dpp_f64<0xB1>(v);
     v += dpp_f64<0x4E>(v);
     v += dpp_f64<0x141>(v);
-    v += dpp_f64<0x140>(v);
+    return v + dpp_f64<0x140>(v);
+}
+__device__ __forceinline__ double wave_sum(double v) {
+    v = lanes16_sum(v);
     v += __shfl_xor(v, 16);
     return v + __shfl_xor(v, 32);
 }
@@ -242,8 +247,9 @@ __device__ __forceinline__ Search find(int n, Weight weight, double from, double
 /* What is known of a row: its largest logit, and the sum of 2^((x - top) rate) or (T = 0) where
  * it is first. */
 struct Row {
-    float top, sum;
+    float top;
     int at;
+    double sum;
 };
 
 template <int DT>
@@ -346,7 +352,7 @@ struct Accept : LogitPiece<DT> {
     static __device__ __forceinline__ Row row_of(const AcceptParams& p, int b, int r, float t) {
         const int lane = threadIdx.x % 16, n = p.ranges.by;
         const AcceptPart* part = p.parts + ((int64_t)b * p.all_rows.by + r) * n;
-        Row row = {-__builtin_inff(), 0.0f, kNone};
+        Row row = {-__builtin_inff(), kNone, 0.0};
         const float rate = (float)rate_of(t);
         constexpr int kOnce = 4;   /* loads on their way together */
         for (int from = 0; from < n; from += 16 * kOnce) {
@@ -373,7 +379,7 @@ struct Accept : LogitPiece<DT> {
                 row.sum *= __builtin_amdgcn_exp2f((row.top - to) * rate);
 #pragma unroll
                 for (int j = 0; j < kOnce; ++j)
-                    row.sum += __uint_as_float(v[j].sum) *
+                    row.sum += (double)__uint_as_float(v[j].sum) *
                                __builtin_amdgcn_exp2f((v[j].top - to) * rate);
             }
             row.top = to;
@@ -395,13 +401,10 @@ struct Accept : LogitPiece<DT> {
             group_of<16>(__float_as_uint(row.top), [](uint32_t a, uint32_t c) {
                 return __float_as_uint(larger(__uint_as_float(a), __uint_as_float(c)));
             }));
-        float sum = __builtin_nanf("");
+        double sum = __builtin_nan("");
         if (fabsf(top) < __builtin_inff())
             sum = row.sum * __builtin_amdgcn_exp2f((row.top - top) * rate);
-        sum = __uint_as_float(group_of<16>(__float_as_uint(sum), [](uint32_t a, uint32_t c) {
-            return __float_as_uint(__uint_as_float(a) + __uint_as_float(c));
-        }));
-        return {top, sum, kNone};
+        return {top, kNone, lanes16_sum(sum)};
     }
 
     /* The sum of a whole row in 64 bits, by a workgroup alone. */
@@ -453,20 +456,20 @@ struct Accept : LogitPiece<DT> {
             if (lane % 16 == 0) rows[i] = row;
         }
         __syncthreads();
-        Row row = {0.0f, 0.0f, kNone}, other = row;
+        Row row = {0.0f, kNone, 0.0}, other = row;
         bool some = true, taken = false;   /* some: both rows have a distribution */
         double mine = 0.0, theirs = 1.0;
         if (wave == 0) {
             if (lane <= s.drafts) {
                 row = rows[lane];
                 some = greedy ? row.at != kNone
-                              : row.sum > 0.0f && row.sum < __builtin_inff() &&
+                              : row.sum > 0.0 && row.sum < __builtin_inf() &&
                                     is_temperature(s.t);
             }
             if (lane < s.drafts) {
                 if (s.drafted) {
                     other = rows[s.drafts + 1 + lane];
-                    some = some && other.sum > 0.0f && other.sum < __builtin_inff() &&
+                    some = some && other.sum > 0.0 && other.sum < __builtin_inf() &&
                            is_temperature(s.dt);
                 }
                 known = known && some;

@@ -430,8 +430,8 @@ typedef struct dfq_heads {
     int heads;
 } dfq_heads;
 
-/* Rotates the heads of q and k (k may be NULL) in one launch; inverse != 0 turns back (the
- * rotation's transpose).  Row m of sequence b is at position start + starts[b] + m (starts:
+/* Rotates the heads of q and k (k may be NULL) in one launch; inverse != 0 turns back
+ * by the same angles.  Row m of sequence b is at position start + starts[b] + m (starts:
  * device memory, may be NULL for zeros) or at positions[b*rows + m] (device memory, as draft
  * trees need them; then start is 0 and starts NULL).  Positions may be negative.  head_dim is even
  * and at most 512; bf16, fp16 or fp32, in fp32 and rounded once.  Asynchronous on `stream`. */
@@ -489,8 +489,8 @@ dfq_status dfq_token_logprobs(dfq_ctx* ctx, const void* logits, int64_t row_stri
  *                   p where that is 0 throughout), or from p of the row behind the drafts, then -1
  * A token is drawn as the first whose running sum of probabilities exceeds u[b][rows-1] times their
  * sum.  uniforms u [batch][rows] are in [0, 1) and the caller's, so that a call with the same
- * numbers gives the same tokens, distributed as p (chances are right to 2^-20 of themselves, the
- * drawn token is that of 64-bit sums).  temperatures and draft_temperatures [batch] are in device
+ * numbers gives the same tokens, distributed as p (counts and tokens are those of 64-bit sums, with
+ * exponentials to 8e-13; chances are right to 2^-17 of themselves).  temperatures and draft_temperatures [batch] are in device
  * memory; NULL: `temperature`, `draft_temperature` for all.  T = 0 takes p = 1 for the row's
  * argmax, as dfq_argmax_accept finds it.  A logit of -inf has probability 0, as have probabilities
  * under 2^-1000 of the row's largest.  A row with a NaN or

@@ -88,7 +88,7 @@ def distribution(x, t):
 def accept(logits, uniforms, drafts, lengths, draft_logits, temperature, draft_temperature):
     """(tokens, accepted, chances, margin) by the definition, one sequence after the other; margin
     is how near the nearest decision lies to its border: of u q to p, relative to p, and of the
-    running sums to u times the whole, relative to the whole (1e6 times as near counts)."""
+    running sums to u times the whole, relative to the whole."""
     b, m, v = logits.shape
     tokens = np.full((b, m), -1, dtype=np.int32)
     accepted = np.zeros(b, dtype=np.int32)
@@ -141,5 +141,5 @@ def accept(logits, uniforms, drafts, lengths, draft_logits, temperature, draft_t
             at = int(np.nonzero(left)[0][-1])
         tokens[i, accepted[i]] = at
         if t > 0 and left[left > 0].size > 1:
-            margin = min(margin, 1e6 * np.abs(run[left > 0][:-1] / run[-1] - u).min())
+            margin = min(margin, np.abs(run[left > 0][:-1] / run[-1] - u).min())
     return tokens, accepted, chances, margin

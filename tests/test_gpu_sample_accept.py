@@ -9,15 +9,14 @@ import torch
 
 import dflash_qmm
 from gpu_util import announce
-from rotation_util import DTYPES, accept
+from rotation_util import DTYPES, accept, distribution
 
 pytestmark = pytest.mark.gpu
 
-# A draft's chance: exponentials of up to 2^7 binary places with differences rounded to 24 bits,
-# 2^-24 * 64 of each term that counts (those within 2^-64 of the largest), but as errors of either
-# sign in sums of positive terms and in one common factor (the rate's 2^-25 times the mean of the
-# exponents, under 32); the hardware's exponential and the sums' roundings 2^-22 together.
-CHANCE = 2.0 ** -19
+# A draft's chance, from two rows' fp32 sums: an exponent a of 2 has three roundings, 2.5 * 2^-24 |a|
+# together, and the mean of |a| over a row's mass is at most the logarithm of its tokens' number,
+# 20 here: 34 * 2^-24 of the sum; 17 sums in a row and the exponential's last bits are 20 more.
+CHANCE = 2.0 * 54 * 2.0 ** -24
 
 
 def inputs(seed, batch, rows, vocab, name, drafted, spread=3.0, mixed=False):
@@ -58,7 +57,11 @@ def oracle(s):
                   numbers(s["temperature"]), numbers(s["temperature"] if td is None else td))
 
 
-def check(ctx, s, margin=1e-5):
+# Exponentials are right to 8e-13 of themselves, and so are two rows' sums: 4 of them, twice over.
+NEAR = 7e-12
+
+
+def check(ctx, s, margin=NEAR):
     """One call against the definition; no decision of the inputs may lie nearer to its border
     than the arithmetic's bound."""
     tokens, accepted, chances, near = oracle(s)
@@ -351,3 +354,91 @@ def test_a_given_workspace(ctx):
     assert e.value.status == 3
     ws = torch.full((4 << 20,), 255, dtype=torch.uint8, device="cuda")
     assert all(torch.equal(a, b) for a, b in zip(ctx.sample_accept(**s, ws=ws), want))
+
+
+def at_the_border(s, first):
+    """The fp32 numbers nearest to each draft's chance, and their neighbours, as random numbers; a
+    step further where one lies within 1e-11 of the chance, which exponentials to 8e-13 in both
+    rows and both sums do not tell from it by far."""
+    _, _, chances, _ = oracle(s)
+    u = torch.from_numpy(chances).float()
+    move = torch.arange(u.numel()).view(u.shape) % 3 - 1
+    up, down = torch.full_like(u, 2.0), torch.full_like(u, -2.0)
+    u = torch.where(move > 0, torch.nextafter(u, up),
+                    torch.where(move < 0, torch.nextafter(u, down), u))
+    near = (u.double().numpy() - chances) < 1e-11 * chances
+    near &= (u.double().numpy() - chances) > -1e-11 * chances
+    u = torch.where(torch.from_numpy(near), torch.nextafter(u, up), u).clamp(0, 1 - 2.0 ** -24)
+    s["uniforms"][:, :-1] = u
+    if first:   # drafts in front of the last are taken, so that each row is judged at its border
+        s["uniforms"][:, :-2] = 0
+
+
+@pytest.mark.parametrize("name", sorted(DTYPES))
+@pytest.mark.parametrize("vocab", [50, 3000, 33000])
+def test_drafts_next_to_their_border(ctx, name, vocab):
+    """Random numbers one fp32 step around the chances, which lie some 1e-8 from them: nearer than
+    fp32 sums of the rows can tell, and decided as 64-bit sums decide them."""
+    for drafted, first in itertools.product((False, True), (False, True)):
+        s = inputs(40 + vocab, 24, 4, vocab, name, drafted)
+        s["draft_lengths"] = None
+        at_the_border(s, first)
+        announce(f"accept at the border {vocab} {name} {drafted}")
+        check(ctx, s)
+
+
+@pytest.mark.parametrize("name", sorted(DTYPES))
+def test_draws_next_to_their_border(ctx, name):
+    """Random numbers within an fp32 step of the running sum's value at some token."""
+    for drafted, rows in ((False, 1), (False, 2), (True, 2)):
+        s = inputs(50, 40, rows, 4000, name, drafted, spread=1.0)
+        s["draft_lengths"] = None
+        if rows == 2:
+            s["uniforms"][:, 0] = 1 - 2.0 ** -24   # refused, unless the chance is 1
+        tokens, accepted, _, _ = oracle(s)
+        for b in range(40):
+            n = int(accepted[b])
+            p = distribution(s["logits"][b, n].double().numpy(), float(s["temperature"][b]))
+            left = p
+            if n < rows - 1:
+                q = np.zeros_like(p)
+                q[int(s["drafts"][b, n])] = 1.0
+                if drafted:
+                    q = distribution(s["draft_logits"][b, n].double().numpy(),
+                                     float(s["temperature"][b]))
+                left = np.maximum(p - q, 0)
+            run = left.cumsum() / left.sum()
+            u = torch.tensor(run[500 + 87 * b], dtype=torch.float32)
+            u = torch.nextafter(u, torch.tensor(float(b % 3 - 1))) if b % 3 else u
+            s["uniforms"][b, -1] = u.clamp(0, 1 - 2.0 ** -24)
+        announce(f"draw at the border {name} {drafted} {rows}")
+        check(ctx, s)
+
+
+@pytest.mark.parametrize("name", sorted(DTYPES))
+def test_more_units_than_one_search_takes(ctx, name):
+    for drafted in (False, True):
+        announce(f"accept 700001 {name} {drafted}")
+        s = inputs(60, 2, 2, 700001, name, drafted)
+        s["uniforms"][0, 0] = 1 - 2.0 ** -24
+        check(ctx, s)
+
+
+def test_many_sequences(ctx):
+    for batch, rows, vocab in ((1700, 1, 5000), (900, 3, 2100)):
+        for drafted in (False, True):
+            announce(f"accept {batch} sequences {drafted}")
+            check(ctx, inputs(61, batch, rows, vocab, "bf16", drafted))
+
+
+def test_a_certain_draft_refused_by_a_number_past_1(ctx):
+    """p = q = 1 for one token, and u is not below 1: p is drawn from, which is that token."""
+    for drafted in (False, True):
+        x = torch.full((1, 2, 3000), -math.inf)
+        x[..., 1234] = 0.5
+        tokens, accepted, chances = ctx.sample_accept(
+            x.cuda(), torch.tensor([[1.0, 0.3]]).cuda(),
+            drafts=torch.tensor([[1234]], dtype=torch.int32).cuda(),
+            draft_logits=x[:, :1].cuda() if drafted else None)
+        assert tokens.tolist() == [[1234, -1]] and accepted.tolist() == [0]
+        assert chances.tolist() == [[1.0]]
