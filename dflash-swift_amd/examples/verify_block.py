@@ -5,17 +5,20 @@ A decoder of the benchmark model's shape (random weights; --small for a toy one)
 into a cache of one slot, once for all sequences, 16 rows at a time.  Then each verify pass takes a
 block of every sequence (its last token and the drafts), and
 
-  * quantises the block's K and V rows, cut from the fused q|k|v output, into the sequences' own
-    caches as it writes them (Context.cache_append),
+  * norms the heads of the block's queries and keys, cut from the fused q|k|v output, and turns
+    them to their positions (Context.qk_norm_rope),
+  * quantises the block's K and V rows into the sequences' own caches as it writes them
+    (Context.cache_append),
   * attends over the prompt, the sequence's own tokens and the block (Context.cache_attention),
   * scores the drafts and takes the model's own tokens with their log probabilities
-    (Context.token_logprobs),
+    (Context.token_logprobs), or, at a temperature, keeps drafts by their probabilities and draws
+    the token behind them (Context.sample_accept),
 
 with the quantised projections in between.  Drafts that agree with the model are kept; what was
 appended of the others is written over by the next block.  The drafts here are the model's own
 tokens with some replaced, as no draft model is loaded.
 
-    python3 dflash-swift_amd/examples/verify_block.py --small
+    python3 dflash-swift_amd/examples/verify_block.py --small [--temperature 0.8]
 """
 import argparse
 import os
@@ -46,16 +49,6 @@ def norm(x):
     return (f * torch.rsqrt(f.square().mean(-1, keepdim=True) + 1e-6)).to(x.dtype)
 
 
-def rotate(x, positions, head_dim):
-    """Rotary embedding of x [batch, rows, heads*head_dim] at positions [batch, rows]."""
-    half = head_dim // 2
-    freq = 1e6 ** (-torch.arange(half, device=x.device) / half)
-    angle = positions[..., None, None].float() * freq
-    a, b = x.unflatten(-1, (-1, 2, half)).float().unbind(-2)
-    cos, sin = angle.cos(), angle.sin()
-    return torch.stack((a * cos - b * sin, b * cos + a * sin), -2).flatten(2).to(x.dtype)
-
-
 class Decoder:
     """A decoder of `layers` blocks with quantised weights and K/V caches: `prompt` holds the
     shared tokens (one slot), `own` each sequence's."""
@@ -71,12 +64,15 @@ class Decoder:
             "o": random_linear(ctx, hidden, self.q_width, gen),
             "gate_up": random_linear(ctx, 2 * mlp, hidden, gen),
             "down": random_linear(ctx, hidden, mlp, gen),
+            "q_norm": torch.ones(head_dim, dtype=torch.bfloat16, device="cuda"),
+            "k_norm": torch.ones(head_dim, dtype=torch.bfloat16, device="cuda"),
             "prompt": dflash_qmm.KVCache(1, kv_heads, prompt_capacity, head_dim),
             "own": dflash_qmm.KVCache(sequences, kv_heads, own_capacity, head_dim),
         } for _ in range(layers)]
         self.embedding = torch.randn(vocab, hidden, device="cuda",
                                      generator=gen).to(torch.bfloat16)
         self.lm_head = random_linear(ctx, vocab, hidden, gen)
+        self.rope = dflash_qmm.Rope(head_dim, base=1e6)
         self.prompt_length = 0
 
     def forward(self, tokens, cache, starts, lengths, prompt_length, max_length):
@@ -85,18 +81,18 @@ class Decoder:
         ctx = self.ctx
         batch, rows = tokens.shape
         offset = prompt_length if cache == "own" else 0
-        positions = offset + starts[:, None] + torch.arange(rows, device="cuda")
         x = self.embedding[tokens.long()]
         for layer in self.layers:
             fused = layer["qkv"](norm(x))
             q, k, v = fused.split((self.q_width, self.kv_width, self.kv_width), -1)
             # v stays a slice of the fused rows; the rotated k goes back beside it
-            k.copy_(rotate(k, positions, self.head_dim))
+            q, heads = (t.unflatten(-1, (-1, self.head_dim)) for t in (q, k))
+            q, _ = ctx.qk_norm_rope(self.rope, q, heads, layer["q_norm"], layer["k_norm"],
+                                    start=offset, starts=starts, k_out=heads)
             ctx.cache_append(layer[cache], k, v, starts=starts)
             y, _ = ctx.cache_attention(
-                rotate(q, positions, self.head_dim), layer[cache], lengths=lengths,
-                max_length=max_length, prefix=layer["prompt"] if offset else None,
-                prefix_length=offset or None)
+                q.flatten(2), layer[cache], lengths=lengths, max_length=max_length,
+                prefix=layer["prompt"] if offset else None, prefix_length=offset or None)
             x = x + layer["o"](y)
             gate_up = layer["gate_up"](norm(x)).flatten(0, 1)
             x = x + layer["down"](ctx.silu_mul(gate_up).view(batch, rows, -1))
@@ -111,6 +107,17 @@ class Decoder:
             logits = self.forward(block, "prompt", start, start + block.shape[1], 0, end)
         self.prompt_length = tokens.shape[0]
         return logits[0, -1:]
+
+    def sample(self, blocks, starts, uniforms, temperature):
+        """One pass over blocks as in verify, whose drafts are kept by their probabilities at a
+        temperature: (tokens [batch, rows] -- the drafts kept and the token drawn behind them --,
+        how many were kept, the chance of each, the logits).  uniforms [batch, rows] are the
+        random numbers."""
+        rows = blocks.shape[1]
+        logits = self.forward(blocks, "own", starts, starts + rows, self.prompt_length,
+                              self.layers[0]["own"].capacity)
+        drafts = blocks[:, 1:].contiguous() if rows > 1 else None
+        return *self.ctx.sample_accept(logits, uniforms, drafts, temperature=temperature), logits
 
     def verify(self, blocks, starts, top_k=5):
         """One pass over blocks [batch, rows] (a sequence's last token, then its drafts) placed
@@ -142,6 +149,7 @@ def main():
     ap.add_argument("--sequences", type=int, default=4)
     ap.add_argument("--rows", type=int, default=4, help="rows of a block: a token and its drafts")
     ap.add_argument("--passes", type=int, default=4)
+    ap.add_argument("--temperature", type=float, default=0.0, help="0: the likeliest tokens")
     a = ap.parse_args()
     shape = ((512, 8, 2, 64, 1024, 2000) if a.small else (5120, 40, 8, 128, 17408, 151936))
     vocab = shape[-1]
@@ -161,6 +169,14 @@ def main():
             block = torch.cat((block, seen[:, -1:]), 1)
         if a.rows > 2:
             block[:, -1] = (block[:, -1] + 1) % vocab
+        if a.temperature > 0:
+            u = torch.rand(block.shape, generator=gen).cuda()
+            tokens, kept, chances, _ = model.sample(block, starts, u, a.temperature)
+            last = tokens.gather(1, kept.long()[:, None])[:, 0]
+            print(f"pass {n}: kept {kept.tolist()} of {a.rows - 1} drafts, next tokens "
+                  f"{last.tolist()}, chances {[[round(v, 2) for v in c] for c in chances.tolist()]}")
+            starts = starts + kept + 1
+            continue
         out = model.verify(block, starts)
         at = out["accepted"].long()[:, None]
         last = out["tokens"].gather(1, at)[:, 0]
