@@ -23,6 +23,7 @@ import contextlib
 import ctypes
 import os
 import struct
+import sys
 import threading
 
 __all__ = [
@@ -641,7 +642,6 @@ class Context:
                             positions, False, q_out, k_out, stream)
 
     def _rotate(self, rope, q, k, norms, start, starts, positions, inverse, q_out, k_out, stream):
-        import torch
         if stream is not None and self._is_other(stream):
             with self._current(stream):
                 return self._rotate(rope, q, k, norms, start, starts, positions, inverse, q_out,
@@ -658,7 +658,8 @@ class Context:
                 q_out is not None and q_out.get_device() != device or \
                 k_out is not None and k_out.get_device() != device:
             self._elsewhere(q, k, rope and rope.turns, starts, positions, q_out, k_out)
-        if max(batch, rows, heads, dim, start, -start) > _INT_MAX:
+        if batch > _INT_MAX or rows > _INT_MAX or heads > _INT_MAX or dim > _INT_MAX or \
+                not -_INT_MAX <= start <= _INT_MAX:
             raise ValueError("batch, rows, heads, head_dim or start past a C int")
         dtype = q.dtype
         q_out, packed_q = _heads("q", q, q_out, rows, heads, dim, dtype)
@@ -694,7 +695,7 @@ class Context:
                 self._elsewhere(q, t)
             kind = t.dtype
             if t.shape != (dim,) or not t.is_contiguous() or \
-                    kind is not dtype and kind is not torch.float32:
+                    kind is not dtype and _dtype_codes.get(kind) != F32:
                 raise ValueError("weights are contiguous [head_dim] in q's dtype or fp32")
             wt = dtype_code(kind)
         if q_weight is not None and k_weight is not None and q_weight.dtype is not k_weight.dtype:
@@ -1008,7 +1009,7 @@ def _row_stride(t) -> int:
 def _check_int32(name, t, shape):
     if t is None:
         return None
-    import torch
+    torch = sys.modules["torch"]
     if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} is a contiguous int32 tensor of shape {shape}")
     return t.data_ptr()
@@ -1017,7 +1018,7 @@ def _check_int32(name, t, shape):
 def _check_f32(name, t, shape):
     if t is None:
         return None
-    import torch
+    torch = sys.modules["torch"]
     if t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} is a contiguous fp32 tensor of shape {shape}")
     return t.data_ptr()
@@ -1027,7 +1028,7 @@ def _heads(name, t, out, rows, heads, dim, dtype):
     """(out, dfq_heads) of t [batch, rows, heads, head_dim] into out, made where it is None."""
     a = t.stride()
     if out is None:
-        import torch
+        torch = sys.modules["torch"]
         out = torch.empty_like(t, memory_format=torch.contiguous_format)
         b = (rows * heads * dim, heads * dim, dim, 1)
     else:
