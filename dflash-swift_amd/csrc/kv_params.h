@@ -86,6 +86,7 @@ struct AcceptPart {
 
 #define DFQ_ACCEPT_APART 32  /* counters lie a cache line apart                          */
 #define DFQ_ACCEPT_PIECES 8  /* 16-byte pieces that a lane takes of a range              */
+#define DFQ_ACCEPT_WIDE 2    /* and where their sums are 64 bits wide                    */
 
 /* What is left to draw of a sequence: nothing, or a token from p, from p without its draft, or
  * from max(p - q, 0). */
@@ -94,6 +95,7 @@ struct AcceptDraw {
     int32_t mode, row;       /* the target's row, and the place of the token */
     int32_t draft, token;    /* the row's draft; the token of DFQ_DRAW_NONE  */
     float p_top, q_top;      /* largest logits of the rows                   */
+    double p_sum, q_sum;     /* and their sums of 2^((x - top) rate)         */
 };
 
 struct AcceptParams {
@@ -108,6 +110,7 @@ struct AcceptParams {
     int32_t* accepted;          /* [batch]                                         */
     float* chances;             /* [batch][rows - 1] or NULL                       */
     AcceptPart* parts;          /* [batch][rows, then draft rows][ranges]          */
+    double* wide;               /* [batch][rows, ..][ranges]: the parts' sums in 64 bits */
     AcceptDraw* draws;          /* [batch], with draft logits                      */
     double* totals;             /* [batch][chunks][2]: both rows' sums             */
     uint64_t* sums;             /* [batch][units]: what is drawn from, as doubles' bits */

@@ -24,8 +24,8 @@ dfq_status check_sizes(int batch, int rows, int V, dfq_dtype dtype) {
 }
 
 struct AcceptPlan {
-    int all_rows, ranges, units, chunks, rest_chunks;
-    size_t sums, totals, draws, arrived, bytes;   /* offsets; the parts come first */
+    int all_rows, wide, ranges, units, chunks, rest_chunks;
+    size_t wide_sums, sums, totals, draws, arrived, bytes;   /* offsets; the parts come first */
 };
 
 constexpr int kWaves = DFQ_KV_THREADS / 64;
@@ -35,7 +35,12 @@ AcceptPlan plan_accept(int cus, int batch, int rows, int V, dfq_dtype dtype, boo
     a.all_rows = drafted ? 2 * rows - 1 : rows;
     const int unit = 64 * (dtype == DFQ_F32 ? 4 : 8);
     a.units = (V + unit - 1) / unit;
-    a.ranges = (V + DFQ_ACCEPT_PIECES * unit - 1) / (DFQ_ACCEPT_PIECES * unit);
+    /* All rows' sums in 64 bits cost up to twice the first launch and save the third, which only
+     * draft logits need.  Seven drafts of 151936 tokens each, bf16, on the device: 1 sequence
+     * 15.3 us wide and 18.3 with fp32 sums, 8 28.0 and 30.6, 12 (27 M logits) 34.0 and 33.8. */
+    a.wide = drafted && (int64_t)batch * a.all_rows * V <= 24 << 20;
+    const int range = unit * (a.wide ? DFQ_ACCEPT_WIDE : DFQ_ACCEPT_PIECES);
+    a.ranges = (V + range - 1) / range;
     /* Workgroups of a sequence: as many units a wave as leave no more than six workgroups a CU,
      * which are there at once, and as few workgroups as that many units take: each decides its
      * sequence's drafts first. */
@@ -44,7 +49,9 @@ AcceptPlan plan_accept(int cus, int batch, int rows, int V, dfq_dtype dtype, boo
     a.chunks = parts(a.units, kWaves * parts(a.units, kWaves * most));
     a.rest_chunks = parts(a.units, kWaves);   /* nothing is decided there */
     const auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
-    a.sums = up((size_t)batch * a.all_rows * a.ranges * sizeof(AcceptPart));
+    const size_t ranges = (size_t)batch * a.all_rows * a.ranges;
+    a.wide_sums = up(ranges * sizeof(AcceptPart));
+    a.sums = a.wide_sums + (a.wide ? up(ranges * 8) : 0);
     a.totals = a.sums + up((size_t)batch * a.units * 8);
     a.draws = a.totals + (drafted ? up((size_t)batch * a.chunks * 16) : 0);
     a.arrived = a.draws + (drafted ? up((size_t)batch * sizeof(AcceptDraw)) : 0);
@@ -120,6 +127,7 @@ dfq_status dfq_sample_accept(dfq_ctx* ctx, const void* logits, int64_t batch_str
     p.chances = chances;
     p.parts = (AcceptPart*)ws;
     p.sums = (uint64_t*)(ws + a.sums);
+    p.wide = (double*)(ws + a.wide_sums);
     p.totals = (double*)(ws + a.totals);
     p.draws = drafted ? (AcceptDraw*)(ws + a.draws) : nullptr;
     p.arrived = (int32_t*)(ws + a.arrived);
@@ -142,13 +150,13 @@ dfq_status dfq_sample_accept(dfq_ctx* ctx, const void* logits, int64_t batch_str
     DeviceScope scope(ctx);
     const AcceptKernels& fn = ops->accept[(int)dtype];
     void* args[] = {&p};
-    hipError_t e = hipModuleLaunchKernel(fn.sums, (unsigned)((jobs + kWaves - 1) / kWaves), 1, 1,
+    hipError_t e = hipModuleLaunchKernel(fn.sums[a.wide], (unsigned)((jobs + kWaves - 1) / kWaves), 1, 1,
                                          DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args,
                                          nullptr);
     if (e == hipSuccess)
-        e = hipModuleLaunchKernel(fn.weigh, (unsigned)chunks, 1, 1, DFQ_KV_THREADS, 1, 1, 0,
+        e = hipModuleLaunchKernel(fn.weigh[a.wide], (unsigned)chunks, 1, 1, DFQ_KV_THREADS, 1, 1, 0,
                                   (hipStream_t)stream, args, nullptr);
-    if (e == hipSuccess && drafted)
+    if (e == hipSuccess && drafted && !a.wide)
         e = hipModuleLaunchKernel(fn.rest, (unsigned)rest, 1, 1, DFQ_KV_THREADS, 1, 1, 0,
                                   (hipStream_t)stream, args, nullptr);
     return e == hipSuccess ? DFQ_OK : hip_error(e, "launch dfq_sample_accept");

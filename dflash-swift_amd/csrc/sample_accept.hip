@@ -21,7 +21,8 @@
  * largest logit and the sum of e^((x - largest) / T).  In the second each workgroup joins its
  * sequence's ranges and decides its drafts (alike in all of them, so that nothing has to be waited
  * for), then weighs its part of the row that is drawn from; the last to come finds the token.
- * Where the draw is from p - q the second sums both rows, and a third weighs and finds.
+ * Where the draw is from p - q the second sums both rows in 64 bits, and a third weighs and finds;
+ * calls of few logits sum all rows in 64 bits at once (the wide kernels) and need no third.
  */
 #include "kv_params.h"
 #include "logit_piece.h"
@@ -257,7 +258,6 @@ struct Accept : LogitPiece<DT> {
     using LogitPiece<DT>::kN, LogitPiece<DT>::load, LogitPiece<DT>::widen;
     static constexpr int kSize = 16 / kN;
     static constexpr int kUnit = 64 * kN;           /* logits of a wave's load          */
-    static constexpr int kPieces = DFQ_ACCEPT_PIECES, kRange = kPieces * kUnit;
 
     static __device__ __forceinline__ const char* target_row(const AcceptParams& p, int b, int r) {
         return (const char*)p.logits + (b * p.batch_stride + r * p.row_stride) * kSize;
@@ -267,8 +267,11 @@ struct Accept : LogitPiece<DT> {
                (b * p.draft_batch_stride + r * p.draft_row_stride) * kSize;
     }
 
-    /* One range of one row by one wave. */
+    /* One range of one row by one wave, kPieces x 16 bytes a lane; its sum in fp32 or (WIDE) in 64
+     * bits. */
+    template <int kPieces, bool WIDE>
     static __device__ __forceinline__ void sums(const AcceptParams& p) {
+        constexpr int kRange = kPieces * kUnit;
         const int lane = threadIdx.x % 64;
         const int job = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + threadIdx.x / 64);
         if (job >= p.jobs) return;
@@ -324,7 +327,21 @@ struct Accept : LogitPiece<DT> {
             }
             top = wave_of(top, [](float a, float c) { return larger(a, c); });
             part.top = top;
-            if (fabsf(top) < __builtin_inff()) {
+            if constexpr (WIDE) {
+                double sum = 0.0;
+                if (fabsf(top) < __builtin_inff()) {
+                    const Powers e(t, top);
+#pragma unroll
+                    for (int i = 0; i < kPieces; ++i) {
+                        float x[kN];
+                        widen(v[i], x);
+#pragma unroll
+                        for (int j = 0; j < kN; ++j) sum += e(x[j]);
+                    }
+                    sum = wave_sum(sum);
+                }
+                if (lane == 0) p.wide[job] = sum;
+            } else if (fabsf(top) < __builtin_inff()) {
                 const float rate = (float)rate_of(t);
                 float sum = 0.0f;
 #pragma unroll
@@ -349,19 +366,33 @@ struct Accept : LogitPiece<DT> {
 
     /* A row's ranges together, by 16 lanes.  NaN, +inf or nothing above -inf leaves a sum that is
      * not positive and finite. */
+    template <bool WIDE>
     static __device__ __forceinline__ Row row_of(const AcceptParams& p, int b, int r, float t) {
         const int lane = threadIdx.x % 16, n = p.ranges.by;
-        const AcceptPart* part = p.parts + ((int64_t)b * p.all_rows.by + r) * n;
+        const int64_t first = ((int64_t)b * p.all_rows.by + r) * n;
         Row row = {-__builtin_inff(), kNone, 0.0};
         const float rate = (float)rate_of(t);
+        const auto factor = [&](float from, float to) -> double {
+            if constexpr (WIDE) return Powers(t, to)(from);
+            else return __builtin_amdgcn_exp2f((from - to) * rate);
+        };
         constexpr int kOnce = 4;   /* loads on their way together */
         for (int from = 0; from < n; from += 16 * kOnce) {
             AcceptPart v[kOnce];
+            double sums[kOnce];
 #pragma unroll
             for (int j = 0; j < kOnce; ++j) {
-                const int i = from + 16 * j + lane;
-                v[j] = {-__builtin_inff(), t == 0.0f ? kNone : 0u};
-                if (i < n) v[j] = part[i];
+                const int64_t i = first + min(from + 16 * j + lane, n - 1);
+                v[j] = p.parts[i];
+                if constexpr (WIDE) sums[j] = p.wide[i];
+            }
+#pragma unroll
+            for (int j = 0; j < kOnce; ++j) {
+                const bool in = from + 16 * j + lane < n;
+                if constexpr (!WIDE) sums[j] = (double)__uint_as_float(v[j].sum);
+                sums[j] = in ? sums[j] : 0.0;
+                v[j].top = in ? v[j].top : -__builtin_inff();
+                v[j].sum = in ? v[j].sum : (uint32_t)kNone;
             }
             if (t == 0.0f) {
 #pragma unroll
@@ -376,11 +407,9 @@ struct Accept : LogitPiece<DT> {
 #pragma unroll
             for (int j = 0; j < kOnce; ++j) to = larger(to, v[j].top);
             if (fabsf(to) < __builtin_inff()) {
-                row.sum *= __builtin_amdgcn_exp2f((row.top - to) * rate);
+                row.sum *= factor(row.top, to);
 #pragma unroll
-                for (int j = 0; j < kOnce; ++j)
-                    row.sum += (double)__uint_as_float(v[j].sum) *
-                               __builtin_amdgcn_exp2f((v[j].top - to) * rate);
+                for (int j = 0; j < kOnce; ++j) row.sum += sums[j] * factor(v[j].top, to);
             }
             row.top = to;
         }
@@ -403,7 +432,7 @@ struct Accept : LogitPiece<DT> {
             }));
         double sum = __builtin_nan("");
         if (fabsf(top) < __builtin_inff())
-            sum = row.sum * __builtin_amdgcn_exp2f((row.top - top) * rate);
+            sum = row.sum * factor(row.top, top);
         return {top, kNone, lanes16_sum(sum)};
     }
 
@@ -429,6 +458,7 @@ struct Accept : LogitPiece<DT> {
 
     /* Decides the drafts of sequence b, by a workgroup: 16 lanes join a row, lane i of the first
      * wave looks at draft i.  `writes` stores what is known without a draw. */
+    template <bool WIDE>
     static __device__ __forceinline__ AcceptDraw decide(const AcceptParams& p, const Sequence& s,
                                                         int b, bool writes) {
         __shared__ Row rows[2 * 64];
@@ -452,7 +482,7 @@ struct Accept : LogitPiece<DT> {
         const int joined = s.drafts + 1 + (s.drafted ? s.drafts : 0);
         for (int i = threadIdx.x / 16; i < joined; i += DFQ_KV_THREADS / 16) {
             const bool q = i > s.drafts;
-            const Row row = row_of(p, b, q ? p.rows + i - s.drafts - 1 : i, q ? s.dt : s.t);
+            const Row row = row_of<WIDE>(p, b, q ? p.rows + i - s.drafts - 1 : i, q ? s.dt : s.t);
             if (lane % 16 == 0) rows[i] = row;
         }
         __syncthreads();
@@ -484,9 +514,9 @@ struct Accept : LogitPiece<DT> {
                 __ballot(known && mine > 0.0 && fabs(u * theirs - mine) < 0x1p-16 * mine);
             if (lane == 0) again = near;
         }
-        __syncthreads();
+        if constexpr (!WIDE) __syncthreads();
         /* drafts next to the border: fewer than one in ten thousand */
-        for (uint64_t near = again; near; near &= near - 1) {
+        for (uint64_t near = WIDE ? 0 : again; near; near &= near - 1) {
             const int i = __builtin_ctzll(near);
             double p_sum = 0.0, q_sum = 0.0;
             if (!greedy) p_sum = whole_row(target_row(p, b, i), p.vocab, rows[i].top, s.t);
@@ -502,7 +532,8 @@ struct Accept : LogitPiece<DT> {
             const uint64_t refused = ~__ballot(taken);
             const int n = __builtin_ctzll(refused);   /* at most 63 drafts: some bit is set */
             if (lane == n) {
-                AcceptDraw d = {DFQ_DRAW_NONE, n, draft, -1, row.top, other.top};
+                AcceptDraw d = {DFQ_DRAW_NONE, n, draft, -1, row.top, other.top, row.sum,
+                                other.sum};
                 if (some && greedy) d.token = row.at;
                 else if (some && n == s.drafts) d.mode = DFQ_DRAW_P;
                 else if (some) d.mode = s.drafted ? DFQ_DRAW_REST : DFQ_DRAW_OTHER;
@@ -569,17 +600,38 @@ struct Accept : LogitPiece<DT> {
         }, found.front, found.goal, u).place;
     }
 
+    /* The draw from p - q, both scaled to sums of 1; as drawn(). */
+    static __device__ __forceinline__ int from_rest(const AcceptParams& p, const Sequence& s,
+                                                    const AcceptDraw& d, int chunks, int b,
+                                                    int chunk, double p_sum, double q_sum,
+                                                    double u) {
+        const char* row = target_row(p, b, d.row);
+        const char* other = draft_row(p, b, d.row);
+        const Powers e(s.t, d.p_top), f(s.dt, d.q_top);
+        const double by = 1.0 / p_sum, draft_by = 1.0 / q_sum;
+        const int token = drawn(p, chunks, b, chunk, row, other, u, [&](int, float x, float y) {
+            return fmax(fma(e(x), by, -(f(y) * draft_by)), 0.0);
+        });
+        if (token != kNone) return token;
+        /* p = q to the last bit, and yet refused (a random number that is not below 1): p */
+        return find(p.vocab, [&](int i) { return e(load_any(row, DT, i)); }, 0.0, -1.0, u).place;
+    }
+
+    template <bool WIDE>
     static __device__ __forceinline__ void weigh(const AcceptParams& p) {
         const int b = divided(blockIdx.x, p.chunks), chunk = blockIdx.x - b * p.chunks.by;
         const Sequence s = sequence_of(p, b);
         const double u = p.uniforms[(int64_t)b * p.rows + p.rows - 1];
-        const AcceptDraw d = decide(p, s, b, chunk == 0);
-        if (p.draws && chunk == 0 && threadIdx.x == 0) p.draws[b] = d;
+        const AcceptDraw d = decide<WIDE>(p, s, b, chunk == 0);
+        if (!WIDE && p.draws && chunk == 0 && threadIdx.x == 0) p.draws[b] = d;
         int32_t* out = p.tokens + (int64_t)b * p.rows + d.row;
         const char* row = target_row(p, b, d.row);
         const Powers e(s.t, d.p_top);
         if (d.mode == DFQ_DRAW_NONE) {
             if (chunk == 0 && threadIdx.x == 0) *out = d.token;
+        } else if (WIDE && d.mode == DFQ_DRAW_REST) {
+            const int token = from_rest(p, s, d, p.chunks.by, b, chunk, d.p_sum, d.q_sum, u);
+            if (token >= 0 && threadIdx.x == 0) *out = token;
         } else if (d.mode == DFQ_DRAW_REST) {
             /* both rows' sums */
             const char* other = draft_row(p, b, d.row);
@@ -623,8 +675,6 @@ struct Accept : LogitPiece<DT> {
         if (d.mode != DFQ_DRAW_REST) return;
         const Sequence s = sequence_of(p, b);
         const double u = p.uniforms[(int64_t)b * p.rows + p.rows - 1];
-        const char* row = target_row(p, b, d.row);
-        const char* other = draft_row(p, b, d.row);
         double p_sum = 0.0, q_sum = 0.0;
         for (int i = threadIdx.x; i < (int)p.chunks.by; i += DFQ_KV_THREADS) {
             const double* t = p.totals + 2 * ((int64_t)b * p.chunks.by + i);
@@ -633,37 +683,24 @@ struct Accept : LogitPiece<DT> {
         }
         p_sum = block_sum(p_sum);
         q_sum = block_sum(q_sum);
-        const Powers e(s.t, d.p_top), f(s.dt, d.q_top);
-        const double by = 1.0 / p_sum, draft_by = 1.0 / q_sum;
-        int token = drawn(p, p.rest_chunks.by, b, chunk, row, other, u, [&](int, float x, float y) {
-            return fmax(fma(e(x), by, -(f(y) * draft_by)), 0.0);
-        });
-        if (token < 0) return;
-        if (token == kNone) {
-            /* p = q to the last bit, and yet refused (a random number that is not below 1): p */
-            token = find(p.vocab, [&](int i) {
-                return e(load_any(row, DT, i));
-            }, 0.0, -1.0, u).place;
-        }
-        if (threadIdx.x == 0) p.tokens[(int64_t)b * p.rows + d.row] = token;
+        const int token = from_rest(p, s, d, p.rest_chunks.by, b, chunk, p_sum, q_sum, u);
+        if (token >= 0 && threadIdx.x == 0) p.tokens[(int64_t)b * p.rows + d.row] = token;
     }
 };
 
 }  // namespace
 
-#define DFQ_ACCEPT_KERNELS(name, dt)                                              \
-    extern "C" __global__ __launch_bounds__(DFQ_KV_THREADS) void                  \
-        dfq_accept_sums_##name(AcceptParams p) {                                  \
-        Accept<dt>::sums(p);                                                      \
-    }                                                                             \
-    extern "C" __global__ __launch_bounds__(DFQ_KV_THREADS) void                  \
-        dfq_accept_weigh_##name(AcceptParams p) {                                 \
-        Accept<dt>::weigh(p);                                                     \
-    }                                                                             \
-    extern "C" __global__ __launch_bounds__(DFQ_KV_THREADS) void                  \
-        dfq_accept_rest_##name(AcceptParams p) {                                  \
-        Accept<dt>::rest(p);                                                      \
+#define DFQ_ACCEPT_KERNEL(op, name, call)                                          \
+    extern "C" __global__ __launch_bounds__(DFQ_KV_THREADS) void                   \
+        dfq_accept_##op##_##name(AcceptParams p) {                                 \
+        call(p);                                                                   \
     }
+#define DFQ_ACCEPT_KERNELS(name, dt)                                               \
+    DFQ_ACCEPT_KERNEL(sums, name, (Accept<dt>::sums<DFQ_ACCEPT_PIECES, false>))    \
+    DFQ_ACCEPT_KERNEL(weigh, name, (Accept<dt>::weigh<false>))                     \
+    DFQ_ACCEPT_KERNEL(rest, name, (Accept<dt>::rest))                              \
+    DFQ_ACCEPT_KERNEL(wide_sums, name, (Accept<dt>::sums<DFQ_ACCEPT_WIDE, true>))  \
+    DFQ_ACCEPT_KERNEL(wide_weigh, name, (Accept<dt>::weigh<true>))
 DFQ_ACCEPT_KERNELS(bf16, 0)
 DFQ_ACCEPT_KERNELS(f16, 1)
 DFQ_ACCEPT_KERNELS(f32, 2)

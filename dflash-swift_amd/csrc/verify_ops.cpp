@@ -113,7 +113,8 @@ static dfq_status resolve(VerifyOps* o) {
     for (int t = 0; t < 3; ++t) {
         AcceptKernels& a = o->accept[t];
         const struct { const char* op; hipFunction_t* fn; } parts[] = {
-            {"sums", &a.sums}, {"weigh", &a.weigh}, {"rest", &a.rest}};
+            {"sums", &a.sums[0]}, {"wide_sums", &a.sums[1]}, {"weigh", &a.weigh[0]},
+            {"wide_weigh", &a.weigh[1]}, {"rest", &a.rest}};
         for (const auto& part : parts) {
             snprintf(name, sizeof name, "dfq_accept_%s_%s", part.op, kDt[t]);
             if ((e = hipModuleGetFunction(part.fn, o->sample, name)) != hipSuccess)

@@ -24,7 +24,7 @@ struct CacheKernels {
 };
 
 struct AcceptKernels {
-    hipFunction_t sums = nullptr, weigh = nullptr, rest = nullptr;
+    hipFunction_t sums[2] = {}, weigh[2] = {}, rest = nullptr;   // [sums in fp32/64 bits]
 };
 
 struct VerifyOps {
