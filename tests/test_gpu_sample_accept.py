@@ -442,3 +442,53 @@ def test_a_certain_draft_refused_by_a_number_past_1(ctx):
             draft_logits=x[:, :1].cuda() if drafted else None)
         assert tokens.tolist() == [[1234, -1]] and accepted.tolist() == [0]
         assert chances.tolist() == [[1.0]]
+
+
+@pytest.mark.parametrize("name", sorted(DTYPES))
+@pytest.mark.parametrize("border", (False, True))
+def test_calls_whose_rows_are_summed_in_fp32(ctx, name, border):
+    """More than 24 M logits with draft logits: three launches, ragged, greedy and bad rows among
+    them, and drafts next to their border, which are decided again."""
+    s = inputs(70, 190, 4, 20003, name, True, mixed=not border)
+    if border:
+        s["draft_lengths"] = None
+        at_the_border(s, True)
+    else:
+        s["logits"][0, 0, 7] = math.nan
+        s["logits"][1, 1] = -math.inf
+        s["draft_logits"][3, 0, 20002] = math.inf
+        s["temperature"][5] = -1.0
+        s["uniforms"][9:40, 1] = 1 - 2.0 ** -24
+    announce(f"accept 27 M logits {name} {border}")
+    got = check(ctx, s)
+    again = ctx.sample_accept(**on_gpu(s))
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+def test_both_ways_agree(ctx):
+    """The same sequences in one large call and in small ones, whose rows are summed otherwise."""
+    s = on_gpu(inputs(71, 26, 5, 120011, "bf16", True))
+    whole = ctx.sample_accept(**s)
+    for at in range(0, 26, 9):
+        part = {k: v[at:at + 9] if isinstance(v, torch.Tensor) else v for k, v in s.items()}
+        got = ctx.sample_accept(**part)
+        assert torch.equal(got[0], whole[0][at:at + 9])
+        assert torch.equal(got[1], whole[1][at:at + 9])
+        off = (got[2] - whole[2][at:at + 9]).abs()
+        assert bool((off <= CHANCE * got[2]).all())
+
+
+def test_a_captured_call_of_three_launches(ctx):
+    s = on_gpu(inputs(72, 190, 4, 20003, "f16", True))
+    ws = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+    ctx.sample_accept(**s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ctx.sample_accept(**s, ws=ws)
+    for n in range(3):
+        s["uniforms"].copy_(torch.rand(190, 4, generator=torch.Generator().manual_seed(n)))
+        ws.fill_(n * 85)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, ctx.sample_accept(**s)))
