@@ -85,7 +85,7 @@ struct AcceptPart {
 };
 
 #define DFQ_ACCEPT_APART 32  /* counters lie a cache line apart                          */
-#define DFQ_ACCEPT_PIECES 8  /* 16-byte pieces that a lane takes of a range              */
+#define DFQ_ACCEPT_PIECES 4  /* 16-byte pieces that a lane takes of a range              */
 #define DFQ_ACCEPT_WIDE 2    /* and where their sums are 64 bits wide                    */
 
 /* What is left to draw of a sequence: nothing, or a token from p, from p without its draft, or

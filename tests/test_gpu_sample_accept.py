@@ -15,7 +15,7 @@ pytestmark = pytest.mark.gpu
 
 # A draft's chance, from two rows' fp32 sums: an exponent a of 2 has three roundings, 2.5 * 2^-24 |a|
 # together, and the mean of |a| over a row's mass is at most the logarithm of its tokens' number,
-# 20 here: 34 * 2^-24 of the sum; 17 sums in a row and the exponential's last bits are 20 more.
+# 20 here: 34 * 2^-24 of the sum; 13 sums in a row and the exponential's last bits are 20 more.
 CHANCE = 2.0 * 54 * 2.0 ** -24
 
 
