@@ -458,7 +458,7 @@ struct Accept : LogitPiece<DT> {
         return v > kNothing ? v / sum : 0.0;
     }
 
-    /* Decides the drafts of sequence b, by a workgroup: 16 lanes join a row, lane i of the first
+    /* Decides the drafts of sequence b, by a workgroup: 16 lanes join a row, lane i of the last
      * wave looks at draft i.  `writes` stores what is known without a draw. */
     template <bool WIDE>
     static __device__ __forceinline__ AcceptDraw decide(const AcceptParams& p, const Sequence& s,
@@ -468,30 +468,31 @@ struct Accept : LogitPiece<DT> {
         __shared__ uint64_t again;
         const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
         const bool greedy = s.t == 0.0f;
-        /* what the first wave will need of the drafts is on its way meanwhile */
+        /* The last wave decides (with few rows it has none to join), and what it will need of the
+         * drafts is on its way meanwhile.  Rows and drafts behind the sequence's own are met too:
+         * its length and temperatures need not have come before. */
+        const bool decides = wave == kWaves - 1;
         int draft = -1;
         float x = 0.0f, y = 0.0f, u = 0.0f;
         bool known = false;
-        if (wave == 0 && lane < s.drafts) {
+        if (decides && lane < p.rows - 1) {
             draft = p.drafts[(int64_t)b * (p.rows - 1) + lane];
             u = p.uniforms[(int64_t)b * p.rows + lane];
             known = draft >= 0 && draft < p.vocab;
             if (known) {
                 x = load_any(target_row(p, b, lane), DT, draft);
-                if (s.drafted) y = load_any(draft_row(p, b, lane), DT, draft);
+                if (p.draft_logits) y = load_any(draft_row(p, b, lane), DT, draft);
             }
         }
-        const int joined = s.drafts + 1 + (s.drafted ? s.drafts : 0);
-        for (int i = threadIdx.x / 16; i < joined; i += DFQ_KV_THREADS / 16) {
-            const bool q = i > s.drafts;
-            const Row row = row_of<WIDE>(p, b, q ? p.rows + i - s.drafts - 1 : i, q ? s.dt : s.t);
+        for (int i = threadIdx.x / 16; i < (int)p.all_rows.by; i += DFQ_KV_THREADS / 16) {
+            const Row row = row_of<WIDE>(p, b, i, i < p.rows ? s.t : s.dt);
             if (lane % 16 == 0) rows[i] = row;
         }
         __syncthreads();
         Row row = {0.0f, kNone, 0.0}, other = row;
         bool some = true, taken = false;   /* some: both rows have a distribution */
         double mine = 0.0, theirs = 1.0;
-        if (wave == 0) {
+        if (decides) {
             if (lane <= s.drafts) {
                 row = rows[lane];
                 some = greedy ? row.at != kNone
@@ -500,7 +501,7 @@ struct Accept : LogitPiece<DT> {
             }
             if (lane < s.drafts) {
                 if (s.drafted) {
-                    other = rows[s.drafts + 1 + lane];
+                    other = rows[p.rows + lane];
                     some = some && other.sum > 0.0 && other.sum < __builtin_inf() &&
                            is_temperature(s.dt);
                 }
@@ -512,6 +513,7 @@ struct Accept : LogitPiece<DT> {
                     taken = u * theirs < mine;
                 }
             }
+            known = known && lane < s.drafts;
             const uint64_t near =
                 __ballot(known && mine > 0.0 && fabs(u * theirs - mine) < 0x1p-16 * mine);
             if (lane == 0) again = near;
@@ -523,14 +525,14 @@ struct Accept : LogitPiece<DT> {
             double p_sum = 0.0, q_sum = 0.0;
             if (!greedy) p_sum = whole_row(target_row(p, b, i), p.vocab, rows[i].top, s.t);
             if (s.drafted)
-                q_sum = whole_row(draft_row(p, b, i), p.vocab, rows[s.drafts + 1 + i].top, s.dt);
-            if (wave == 0 && lane == i) {
+                q_sum = whole_row(draft_row(p, b, i), p.vocab, rows[p.rows + i].top, s.dt);
+            if (decides && lane == i) {
                 if (!greedy) mine = part_of(x, s.t, row.top, p_sum);
                 if (s.drafted) theirs = part_of(y, s.dt, other.top, q_sum);
                 taken = u * theirs < mine;
             }
         }
-        if (wave == 0) {
+        if (decides) {
             const uint64_t refused = ~__ballot(taken);
             const int n = __builtin_ctzll(refused);   /* at most 63 drafts: some bit is set */
             if (lane == n) {
