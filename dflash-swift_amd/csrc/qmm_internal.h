@@ -63,14 +63,15 @@ bool make_plan(int M, int N, int K, int bits, int gs, int num_cus, size_t lds_ma
 /* The device address of the fixed scratch array (qmm_scratch.hip) on `device`, which must be
  * current; taken and cleared once per device. */
 dfq_status scratch_setup(int device, void** out);
-/* The kernels of the cache, attention and log-probability calls (verify_ops.cpp), on the current
- * device. */
-struct VerifyOps;
-dfq_status verify_ops_load(VerifyOps** out);
-void verify_ops_unload(VerifyOps* ops);
-/* A context's, loaded with the first call that needs them (a program that only multiplies pays
- * nothing for them: with a context they took 4 of its 44 ms and 10 MiB). */
-dfq_status ctx_verify_ops(dfq_ctx* ctx, const VerifyOps** out);
+/* Kernels of a group of operators that a context loads with the first call that needs one of them
+ * (a program that only multiplies pays nothing for them: with a context the cache's, attention's and
+ * log probabilities' took 4 of its 44 ms and 10 MiB). */
+struct LoadedOps {
+    virtual ~LoadedOps() = default;   // unloads; the context's device is current
+};
+enum OpsGroup { kVerifyOps, kRotationOps, kAcceptOps, kOpsGroups };
+dfq_status ctx_ops(dfq_ctx* ctx, OpsGroup group, dfq_status (*load)(LoadedOps** out),
+                   const LoadedOps** out);
 /* A layer whose only copy of the weight is `packed` (the packed layout, in memory the caller
  * keeps alive); d carries its shape, format, dtype and linear bias, and no MLX arrays. */
 dfq_status make_packed_linear(dfq_ctx* ctx, const dfq_linear_desc& d, const void* packed,

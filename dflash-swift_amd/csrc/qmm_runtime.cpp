@@ -152,8 +152,8 @@ struct dfq_ctx {
     hipFunction_t read_stream = nullptr; // the plain streaming read (bandwidth reference)
     hipFunction_t read_units = nullptr;  // the fast kernel's own loads with no compute
     hipFunction_t read_units_packed = nullptr;  // the same over the packed layout
-    std::atomic<dfq::VerifyOps*> verify{nullptr};  // cache, attention, log probabilities
-    std::mutex verify_mu;                // held while they are loaded
+    std::atomic<dfq::LoadedOps*> ops[dfq::kOpsGroups] = {};  // loaded with their first calls
+    std::mutex ops_mu;                   // held while a group is loaded
     void* scratch = nullptr;             // the fixed scratch of dfq_qmm_noalloc (this device)
     std::mutex mu;
     std::unordered_map<PlanKey, dfq::Plan, PlanKeyHash> plans;
@@ -205,19 +205,20 @@ struct DeviceGuard {
 
 int ctx_device(const dfq_ctx* ctx) { return ctx->device; }
 
-dfq_status ctx_verify_ops(dfq_ctx* ctx, const VerifyOps** out) {
-    VerifyOps* ops = ctx->verify.load(std::memory_order_acquire);
+dfq_status ctx_ops(dfq_ctx* ctx, OpsGroup group, dfq_status (*load)(LoadedOps** out),
+                   const LoadedOps** out) {
+    LoadedOps* ops = ctx->ops[group].load(std::memory_order_acquire);
     if (!ops) {
-        std::lock_guard<std::mutex> lock(ctx->verify_mu);
-        if (!(ops = ctx->verify.load(std::memory_order_relaxed))) {
+        std::lock_guard<std::mutex> lock(ctx->ops_mu);
+        if (!(ops = ctx->ops[group].load(std::memory_order_relaxed))) {
             DeviceGuard g(ctx->device);
             /* the first call may be one that a graph captures; loading is no part of the graph */
             hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
             const hipError_t e = hipThreadExchangeStreamCaptureMode(&mode);
-            const dfq_status st = verify_ops_load(&ops);
+            const dfq_status st = load(&ops);
             if (e == hipSuccess) (void)hipThreadExchangeStreamCaptureMode(&mode);
             if (st != DFQ_OK) return st;
-            ctx->verify.store(ops, std::memory_order_release);
+            ctx->ops[group].store(ops, std::memory_order_release);
         }
     }
     *out = ops;
@@ -755,7 +756,7 @@ dfq_status dfq_destroy(dfq_ctx* ctx) {
     if (!ctx) return DFQ_OK;
     {
         DeviceGuard g(ctx->device);
-        verify_ops_unload(ctx->verify.load());
+        for (auto& ops : ctx->ops) delete ops.load();
         if (ctx->gemm_module) (void)hipModuleUnload(ctx->gemm_module);
         if (ctx->module) (void)hipModuleUnload(ctx->module);
     }

@@ -5,12 +5,43 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <cstdio>
 
 #include "verify_ops.h"
+
+#ifndef DFQ_ROPE_HSACO_PATH
+#error "DFQ_ROPE_HSACO_PATH must name the gfx950 code object to embed"
+#endif
+DFQ_EMBED(dfq_rope_hsaco, DFQ_ROPE_HSACO_PATH)
 
 using namespace dfq;
 
 namespace {
+
+struct RotationOps : LoadedOps {
+    static constexpr OpsGroup kGroup = kRotationOps;
+    hipModule_t module = nullptr;
+    hipFunction_t rotate[2][3][3] = {};  // [alone/with norms][halves/pairs/any][bf16/f16/f32]
+    dfq_status resolve() {
+        static const char* kDt[3] = {"bf16", "f16", "f32"};
+        static const char* kWay[3] = {"halves", "pairs", "any"};
+        hipError_t e = hipModuleLoadData(&module, dfq_rope_hsaco);
+        if (e != hipSuccess) return hip_error(e, "hipModuleLoadData(gfx950 rotation object)");
+        char name[80];
+        for (int n = 0; n < 2; ++n)
+            for (int w = 0; w < 3; ++w)
+                for (int t = 0; t < 3; ++t) {
+                    snprintf(name, sizeof name, "dfq_%s_%s_%s", n ? "norm_rope" : "rope", kWay[w],
+                             kDt[t]);
+                    if ((e = hipModuleGetFunction(&rotate[n][w][t], module, name)) != hipSuccess)
+                        return hip_error(e, name);
+                }
+        return DFQ_OK;
+    }
+    ~RotationOps() override {
+        if (module) (void)hipModuleUnload(module);
+    }
+};
 
 constexpr double kTurn = 6.28318530717958647692528676655900577;
 
@@ -101,8 +132,8 @@ dfq_status rotate(dfq_ctx* ctx, const dfq_rope_table* rope, const dfq_heads* q, 
     p.lanes = 64;
     if (chunks)
         for (p.lanes = 1; p.lanes * 16 < head_dim; p.lanes *= 2) {}
-    const VerifyOps* ops;
-    if ((s = ctx_verify_ops(ctx, &ops))) return s;
+    const RotationOps* ops;
+    if ((s = ops_of(ctx, &ops))) return s;
     DeviceScope scope(ctx);
     /* Heads a lane, whose angles are found once: as many as leave every SIMD two waves, up to 16
      * (one in rotate_any). */

@@ -5,12 +5,49 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <cstdio>
 
 #include "verify_ops.h"
+
+#ifndef DFQ_ACCEPT_HSACO_PATH
+#error "DFQ_ACCEPT_HSACO_PATH must name the gfx950 code object to embed"
+#endif
+DFQ_EMBED(dfq_accept_hsaco, DFQ_ACCEPT_HSACO_PATH)
 
 using namespace dfq;
 
 namespace {
+
+struct AcceptKernels {
+    hipFunction_t sums[2] = {}, weigh[2] = {}, rest = nullptr;   // [sums in fp32/64 bits]
+};
+
+struct AcceptOps : LoadedOps {
+    static constexpr OpsGroup kGroup = kAcceptOps;
+    hipModule_t module = nullptr;
+    AcceptKernels kernels[3];   // [bf16/f16/f32]
+    dfq_status resolve() {
+        static const char* kDt[3] = {"bf16", "f16", "f32"};
+        hipError_t e = hipModuleLoadData(&module, dfq_accept_hsaco);
+        if (e != hipSuccess) return hip_error(e, "hipModuleLoadData(gfx950 sampled-accept object)");
+        char name[80];
+        for (int t = 0; t < 3; ++t) {
+            AcceptKernels& a = kernels[t];
+            const struct { const char* op; hipFunction_t* fn; } parts[] = {
+                {"sums", &a.sums[0]}, {"wide_sums", &a.sums[1]}, {"weigh", &a.weigh[0]},
+                {"wide_weigh", &a.weigh[1]}, {"rest", &a.rest}};
+            for (const auto& part : parts) {
+                snprintf(name, sizeof name, "dfq_accept_%s_%s", part.op, kDt[t]);
+                if ((e = hipModuleGetFunction(part.fn, module, name)) != hipSuccess)
+                    return hip_error(e, name);
+            }
+        }
+        return DFQ_OK;
+    }
+    ~AcceptOps() override {
+        if (module) (void)hipModuleUnload(module);
+    }
+};
 
 dfq_status check_sizes(int batch, int rows, int V, dfq_dtype dtype) {
     if (batch < 1 || rows < 1 || V < 1)
@@ -145,10 +182,10 @@ dfq_status dfq_sample_accept(dfq_ctx* ctx, const void* logits, int64_t batch_str
     p.ranges = divisor(a.ranges);
     p.chunks = divisor(a.chunks);
     p.rest_chunks = divisor(a.rest_chunks);
-    const VerifyOps* ops;
-    if ((s = ctx_verify_ops(ctx, &ops))) return s;
+    const AcceptOps* ops;
+    if ((s = ops_of(ctx, &ops))) return s;
     DeviceScope scope(ctx);
-    const AcceptKernels& fn = ops->accept[(int)dtype];
+    const AcceptKernels& fn = ops->kernels[(int)dtype];
     void* args[] = {&p};
     hipError_t e = hipModuleLaunchKernel(fn.sums[a.wide], (unsigned)((jobs + kWaves - 1) / kWaves), 1, 1,
                                          DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args,

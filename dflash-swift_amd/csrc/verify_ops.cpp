@@ -17,39 +17,51 @@
 
 #if !defined(DFQ_KV_HSACO_PATH) || !defined(DFQ_LOGPROBS_HSACO_PATH) || \
     !defined(DFQ_ATTN64_HSACO_PATH) || !defined(DFQ_ATTN128_HSACO_PATH) || \
-    !defined(DFQ_ATTN256_HSACO_PATH) || !defined(DFQ_ROPE_HSACO_PATH) || \
-    !defined(DFQ_ACCEPT_HSACO_PATH)
+    !defined(DFQ_ATTN256_HSACO_PATH)
 #error "DFQ_*_HSACO_PATH must name the gfx950 code objects to embed"
 #endif
 
-#define DFQ_EMBED(name, path)                      \
-    __asm__(".section .rodata.dfq_verify_hsaco,\"a\",@progbits\n" \
-            ".p2align 12\n"                        \
-            ".globl " #name "\n"                   \
-            ".hidden " #name "\n"                  \
-            #name ":\n"                            \
-            ".incbin \"" path "\"\n"              \
-            ".byte 0\n"                            \
-            ".previous\n");                        \
-    extern "C" const char name[];
 DFQ_EMBED(dfq_kv_hsaco, DFQ_KV_HSACO_PATH)
 DFQ_EMBED(dfq_logprobs_hsaco, DFQ_LOGPROBS_HSACO_PATH)
 DFQ_EMBED(dfq_attn64_hsaco, DFQ_ATTN64_HSACO_PATH)
 DFQ_EMBED(dfq_attn128_hsaco, DFQ_ATTN128_HSACO_PATH)
 DFQ_EMBED(dfq_attn256_hsaco, DFQ_ATTN256_HSACO_PATH)
-DFQ_EMBED(dfq_rope_hsaco, DFQ_ROPE_HSACO_PATH)
-DFQ_EMBED(dfq_accept_hsaco, DFQ_ACCEPT_HSACO_PATH)
 
-namespace dfq {
+using namespace dfq;
+
+namespace {
+
+/* One format of a cache: [head_dim 64/128/256][bits 4/8][group 32/64/128][bf16/f16]; groups wider
+ * than the head have no kernels. */
+struct CacheKernels {
+    hipFunction_t append = nullptr, read = nullptr, join = nullptr;
+    hipFunction_t attention[2] = {};  // up to 1 and 2 row tiles (see attention_tiles)
+    int resident[2] = {};             // their workgroups that a CU holds at once
+};
+
+struct VerifyOps : LoadedOps {
+    static constexpr OpsGroup kGroup = kVerifyOps;
+    hipModule_t kv = nullptr, logprobs = nullptr, attention[3] = {};
+    CacheKernels cache[3][2][3][2];
+    hipFunction_t logprobs_part[3] = {}, logprobs_join[3] = {};  // [bf16/f16/f32]
+    dfq_status resolve();
+    ~VerifyOps() override {
+        if (kv) (void)hipModuleUnload(kv);
+        if (logprobs) (void)hipModuleUnload(logprobs);
+        for (hipModule_t m : attention)
+            if (m) (void)hipModuleUnload(m);
+    }
+};
 
 /* The most tiles of 16 rows that attention kernels take in one pass.  Two read and unpack the
  * codes once for both: 16 sequences of 8 rows of 40 heads over a shared 16384-token prefix take
  * 102 us, one tile 119.  At heads of 256 their outputs leave a CU room for one workgroup of two
  * tiles and two of one: 16 rows of 16 heads over 16000 tokens 32.5 us against 26.1, so there it
  * is one.  Three and four would take 103 and 137 KB of LDS at heads of 128, a workgroup a CU. */
-static int attention_tiles(int dim) { return dim == 256 ? 1 : 2; }
+int attention_tiles(int dim) { return dim == 256 ? 1 : 2; }
 
-static dfq_status resolve(VerifyOps* o) {
+dfq_status VerifyOps::resolve() {
+    VerifyOps* const o = this;
     static const char* kDt[3] = {"bf16", "f16", "f32"};
     hipError_t e;
     if ((e = hipModuleLoadData(&o->kv, dfq_kv_hsaco)) != hipSuccess)
@@ -97,62 +109,8 @@ static dfq_status resolve(VerifyOps* o) {
         if ((e = hipModuleGetFunction(&o->logprobs_join[t], o->logprobs, name)) != hipSuccess)
             return hip_error(e, name);
     }
-    if ((e = hipModuleLoadData(&o->rope, dfq_rope_hsaco)) != hipSuccess)
-        return hip_error(e, "hipModuleLoadData(gfx950 rotation object)");
-    static const char* kWay[3] = {"halves", "pairs", "any"};
-    for (int n = 0; n < 2; ++n)
-        for (int w = 0; w < 3; ++w)
-            for (int t = 0; t < 3; ++t) {
-                snprintf(name, sizeof name, "dfq_%s_%s_%s", n ? "norm_rope" : "rope", kWay[w],
-                         kDt[t]);
-                if ((e = hipModuleGetFunction(&o->rotate[n][w][t], o->rope, name)) != hipSuccess)
-                    return hip_error(e, name);
-            }
-    if ((e = hipModuleLoadData(&o->sample, dfq_accept_hsaco)) != hipSuccess)
-        return hip_error(e, "hipModuleLoadData(gfx950 sampled-accept object)");
-    for (int t = 0; t < 3; ++t) {
-        AcceptKernels& a = o->accept[t];
-        const struct { const char* op; hipFunction_t* fn; } parts[] = {
-            {"sums", &a.sums[0]}, {"wide_sums", &a.sums[1]}, {"weigh", &a.weigh[0]},
-            {"wide_weigh", &a.weigh[1]}, {"rest", &a.rest}};
-        for (const auto& part : parts) {
-            snprintf(name, sizeof name, "dfq_accept_%s_%s", part.op, kDt[t]);
-            if ((e = hipModuleGetFunction(part.fn, o->sample, name)) != hipSuccess)
-                return hip_error(e, name);
-        }
-    }
     return DFQ_OK;
 }
-
-dfq_status verify_ops_load(VerifyOps** out) {
-    *out = nullptr;
-    VerifyOps* o = new (std::nothrow) VerifyOps();
-    if (!o) return fail(DFQ_ERR_HIP, "out of host memory");
-    const dfq_status s = resolve(o);
-    if (s) {
-        verify_ops_unload(o);
-        return s;
-    }
-    *out = o;
-    return DFQ_OK;
-}
-
-void verify_ops_unload(VerifyOps* o) {
-    if (!o) return;
-    if (o->kv) (void)hipModuleUnload(o->kv);
-    if (o->logprobs) (void)hipModuleUnload(o->logprobs);
-    if (o->rope) (void)hipModuleUnload(o->rope);
-    if (o->sample) (void)hipModuleUnload(o->sample);
-    for (hipModule_t m : o->attention)
-        if (m) (void)hipModuleUnload(m);
-    delete o;
-}
-
-}  // namespace dfq
-
-using namespace dfq;
-
-namespace {
 
 int dim_index(int dim) { return dim == 64 ? 0 : dim == 128 ? 1 : dim == 256 ? 2 : -1; }
 int group_index(int gs) { return gs == 32 ? 0 : gs == 64 ? 1 : gs == 128 ? 2 : -1; }
@@ -403,7 +361,7 @@ dfq_status dfq_cache_append(dfq_ctx* ctx, const dfq_kv_cache* cache, const void*
                      {(const uint16_t*)k, (const uint16_t*)v}, starts, row_stride, start, rows,
                      cache->heads, cache->capacity};
     const VerifyOps* ops;
-    if ((s = ctx_verify_ops(ctx, &ops))) return s;
+    if ((s = ops_of(ctx, &ops))) return s;
     DeviceScope scope(ctx);
     void* args[] = {&p};
     const hipError_t e = hipModuleLaunchKernel(
@@ -427,7 +385,7 @@ dfq_status dfq_cache_read(dfq_ctx* ctx, const dfq_kv_cache* cache, void* k, void
                    cache->heads, cache->capacity};
     int dt = (int)dtype;
     const VerifyOps* ops;
-    if ((s = ctx_verify_ops(ctx, &ops))) return s;
+    if ((s = ops_of(ctx, &ops))) return s;
     DeviceScope scope(ctx);
     void* args[] = {&p, &dt};
     const hipError_t e = hipModuleLaunchKernel(
@@ -447,7 +405,7 @@ dfq_status dfq_cache_attention_workspace_bytes(dfq_ctx* ctx, const dfq_kv_cache*
     dfq_status s =
         check_attention(prefix, prefix_length, cache, max_length, batch, rows, q_heads, &fmt);
     const VerifyOps* ops;
-    if (s || (s = ctx_verify_ops(ctx, &ops))) return s;
+    if (s || (s = ops_of(ctx, &ops))) return s;
     *bytes = plan_attention(dfq_num_cus(ctx), kernels_of(ops, fmt), fmt, prefix_length, max_length,
                             batch, rows, q_heads)
                  .bytes;
@@ -475,7 +433,7 @@ dfq_status dfq_cache_attention(dfq_ctx* ctx, const dfq_kv_cache* prefix, int pre
     if (!(scale > 0.0f) || !std::isfinite(scale))
         return fail(DFQ_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
     const VerifyOps* ops;
-    if ((s = ctx_verify_ops(ctx, &ops))) return s;
+    if ((s = ops_of(ctx, &ops))) return s;
     const CacheKernels& fn = kernels_of(ops, fmt);
     const AttentionPlan a = plan_attention(dfq_num_cus(ctx), fn, fmt, prefix_length, max_length,
                                            batch, rows, q_heads);
@@ -604,7 +562,7 @@ dfq_status dfq_token_logprobs(dfq_ctx* ctx, const void* logits, int64_t row_stri
                     (float*)((char*)workspace + logprob_keys_bytes(M, splits, top_k)), row_stride,
                     M, V, top_k, splits};
     const VerifyOps* ops;
-    if ((s = ctx_verify_ops(ctx, &ops))) return s;
+    if ((s = ops_of(ctx, &ops))) return s;
     DeviceScope scope(ctx);
     void* args[] = {&p};
     hipError_t e = hipModuleLaunchKernel(ops->logprobs_part[(int)dtype], (unsigned)M * splits, 1,

@@ -1,6 +1,6 @@
 /*
- * verify_ops.h -- what the host sources of a verify pass's operators share: their kernels, loaded
- * together with a context's first call of one of them, and small helpers.
+ * verify_ops.h -- what the host sources of a verify pass's operators share: embedding and loading of
+ * their kernels, and small helpers.
  */
 #ifndef DFQ_VERIFY_OPS_H
 #define DFQ_VERIFY_OPS_H
@@ -9,35 +9,49 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <new>
 
 #include "kv_params.h"
 #include "qmm_internal.h"
 
+/* A gfx950 code object embedded under a name. */
+#define DFQ_EMBED(name, path)                      \
+    __asm__(".section .rodata.dfq_verify_hsaco,\"a\",@progbits\n" \
+            ".p2align 12\n"                        \
+            ".globl " #name "\n"                   \
+            ".hidden " #name "\n"                  \
+            #name ":\n"                            \
+            ".incbin \"" path "\"\n"              \
+            ".byte 0\n"                            \
+            ".previous\n");                        \
+    extern "C" const char name[];
+
 namespace dfq {
 
-/* One format of a cache: [head_dim 64/128/256][bits 4/8][group 32/64/128][bf16/f16]; groups wider
- * than the head have no kernels. */
-struct CacheKernels {
-    hipFunction_t append = nullptr, read = nullptr, join = nullptr;
-    hipFunction_t attention[2] = {};  // up to 1 and 2 row tiles (see attention_tiles)
-    int resident[2] = {};             // their workgroups that a CU holds at once
-};
-
-struct AcceptKernels {
-    hipFunction_t sums[2] = {}, weigh[2] = {}, rest = nullptr;   // [sums in fp32/64 bits]
-};
-
-struct VerifyOps {
-    hipModule_t kv = nullptr, logprobs = nullptr, attention[3] = {}, rope = nullptr,
-                sample = nullptr;
-    CacheKernels cache[3][2][3][2];
-    hipFunction_t logprobs_part[3] = {}, logprobs_join[3] = {};  // [bf16/f16/f32]
-    hipFunction_t rotate[2][3][3] = {};  // [alone/with norms][halves/pairs/any][bf16/f16/f32]
-    AcceptKernels accept[3];             // [bf16/f16/f32]
-};
 
 inline dfq_status hip_error(hipError_t e, const char* what) {
     return fail(DFQ_ERR_HIP, "%s: %s (%d)", what, hipGetErrorString(e), (int)e);
+}
+
+/* A context's kernels of one group: Ops is a LoadedOps with its kGroup and resolve(). */
+template <typename Ops>
+dfq_status load_ops(LoadedOps** out) {
+    Ops* o = new (std::nothrow) Ops();
+    if (!o) return fail(DFQ_ERR_HIP, "out of host memory");
+    const dfq_status s = o->resolve();
+    if (s) {
+        delete o;
+        return s;
+    }
+    *out = o;
+    return DFQ_OK;
+}
+template <typename Ops>
+dfq_status ops_of(dfq_ctx* ctx, const Ops** out) {
+    const LoadedOps* o;
+    const dfq_status s = ctx_ops(ctx, Ops::kGroup, load_ops<Ops>, &o);
+    if (s == DFQ_OK) *out = static_cast<const Ops*>(o);
+    return s;
 }
 
 inline bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
