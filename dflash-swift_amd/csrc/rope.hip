@@ -13,6 +13,13 @@
  * the angle's place in its turn, whatever p, and its upper 32 bits leave an error of 2^-32 turns.
  * Sine and cosine are their Taylor sums over an eighth of a turn to both sides of the nearest
  * quarter: the first terms left out are x^11 / 11! < 1.8e-9 and x^12 / 12! < 1.2e-10.
+ *
+ * Bound by memory where there are many rows, and by the launch where there are few.  A pair's angle
+ * costs 30 instructions, so that a lane turns up to 16 heads of its token by the same ones, the next
+ * head's channels on their way meanwhile; outputs go past the caches.  8192 rows of 40 + 8 heads of
+ * 128 in bf16, cut from fused rows (201 MB): 39.6 us (5.1 TB/s, a large copy's rate), with norms
+ * 40.7.  One head a lane took 57 us, up to 8 of them with plain stores 45.  One row of 8 sequences
+ * 4.0 us, 8 rows with norms 4.5, 1665 rows of 18 heads of 256 with a quarter rotated 9.7 (31 MB).
  */
 #include "kv_params.h"
 #include "qmm_device.h"

