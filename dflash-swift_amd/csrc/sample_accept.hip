@@ -619,10 +619,13 @@ struct Accept : LogitPiece<DT> {
         const Powers e(s.t, d.p_top), f(s.dt, d.q_top);
         const double by = 1.0 / p_sum, draft_by = 1.0 / q_sum;
         const int token = drawn(p, chunks, b, chunk, row, other, u, [&](int, float x, float y) {
-            return fmax(fma(e(x), by, -(f(y) * draft_by)), 0.0);
+            /* both rounded: a product fused with the difference leaves its rounding where p = q */
+#pragma clang fp contract(off)
+            return fmax(e(x) * by - f(y) * draft_by, 0.0);
         });
         if (token != kNone) return token;
-        /* p = q to the last bit, and yet refused (a random number that is not below 1): p */
+        /* p = q to the last bit, and yet refused (no token of the vocabulary, or a random number
+         * that is not below 1): p */
         return find(p.vocab, [&](int i) { return e(load_any(row, DT, i)); }, 0.0, -1.0, u).place;
     }
 

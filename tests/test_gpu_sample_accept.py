@@ -200,6 +200,18 @@ def test_drafts_outside_the_vocabulary(ctx):
         check(ctx, s)
 
 
+@pytest.mark.parametrize("batch,vocab", [(5, 900), (3, 33000), (100, 90000)])
+def test_drafts_outside_the_vocabulary_where_p_is_q(ctx, batch, vocab):
+    """p - q is 0 throughout: the token comes from p (the last size sums rows in fp32 first)."""
+    s = inputs(26, batch, 2, vocab, "bf16", True)
+    s["draft_logits"] = s["logits"][:, :-1].clone()
+    s["draft_lengths"] = None
+    s["drafts"][:] = -1
+    announce(f"accept outside, p = q {batch} {vocab}")
+    got = check(ctx, s)
+    assert (got[1] == 0).all() and (got[0][:, 0] >= 0).all()
+
+
 def test_the_edges_of_the_random_numbers(ctx):
     """0 takes any draft that can be and the first token that can be; 1 - 2^-24 the last."""
     last = 1 - 2.0 ** -24
