@@ -52,6 +52,8 @@ dfq_status check_heads(const dfq_heads* t, const char* name, dfq_dtype dtype) {
     if (!aligned(t->in, dtype_size(dtype)) || !aligned(t->out, dtype_size(dtype)))
         return fail(DFQ_ERR_INVALID_ARGUMENT, "misaligned %s", name);
     if (t->heads < 1) return fail(DFQ_ERR_INVALID_ARGUMENT, "%s has no heads", name);
+    if (t->heads > kMostGrid)
+        return fail(DFQ_ERR_UNSUPPORTED, "at most %d heads (got %d)", kMostGrid, t->heads);
     return DFQ_OK;
 }
 
@@ -112,7 +114,7 @@ dfq_status rotate(dfq_ctx* ctx, const dfq_rope_table* rope, const dfq_heads* q, 
         p.offset = norms->offset;
     }
     const int64_t all = (int64_t)q->heads + (k ? k->heads : 0), tokens = (int64_t)batch * rows;
-    if (all > INT32_MAX || tokens > INT32_MAX / all)
+    if (tokens > INT32_MAX / all)
         return fail(DFQ_ERR_UNSUPPORTED, "grid too large");
     p.turns = rope ? rope->turns : nullptr;
     p.pairs = rope ? rope->rotary_dim / 2 : 0;
@@ -132,23 +134,24 @@ dfq_status rotate(dfq_ctx* ctx, const dfq_rope_table* rope, const dfq_heads* q, 
     p.lanes = 64;
     if (chunks)
         for (p.lanes = 1; p.lanes * 16 < head_dim; p.lanes *= 2) {}
-    const RotationOps* ops;
-    if ((s = ops_of(ctx, &ops))) return s;
-    DeviceScope scope(ctx);
     /* Heads a lane, whose angles are found once: as many as leave every SIMD two waves, up to 16
      * (one in rotate_any). */
-    const int64_t waves = tokens * all * p.lanes / 64;
-    const int each = chunks ? (int)std::clamp<int64_t>(waves / (8 * dfq_num_cus(ctx)), 1, 16) : 1;
+    const int64_t waves = tokens * all * p.lanes / 64, cus = std::max(1, dfq_num_cus(ctx));
+    const int each = chunks ? (int)std::clamp<int64_t>(waves / (8 * cus), 1, 16) : 1;
     const int64_t per = DFQ_KV_THREADS / p.lanes;
     const auto groups = [&](RopeTensor& t) {
         t.slots = divisor((t.heads + each - 1) / each);
         return (tokens * t.slots.by + per - 1) / per;
     };
-    p.q_groups = (int)groups(p.t[0]);
-    const int64_t k_groups = k ? groups(p.t[1]) : 0;
+    const int64_t q_groups = groups(p.t[0]), k_groups = k ? groups(p.t[1]) : 0;
+    if (q_groups + k_groups > kMostGroups) return fail(DFQ_ERR_UNSUPPORTED, "grid too large");
+    p.q_groups = (int)q_groups;
+    const RotationOps* ops;
+    if ((s = ops_of(ctx, &ops))) return s;
+    DeviceScope scope(ctx);
     void* args[] = {&p};
     const hipError_t e = hipModuleLaunchKernel(
-        ops->rotate[norms != nullptr][way][(int)dtype], (unsigned)(p.q_groups + k_groups), 1, 1,
+        ops->rotate[norms != nullptr][way][(int)dtype], (unsigned)(q_groups + k_groups), 1, 1,
         DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
     return e == hipSuccess ? DFQ_OK : hip_error(e, what);
 }

@@ -54,6 +54,7 @@ dfq_status check_sizes(int batch, int rows, int V, dfq_dtype dtype) {
         return fail(DFQ_ERR_INVALID_ARGUMENT, "batch, rows and V must be >= 1");
     if (rows > DFQ_ACCEPT_ROWS)
         return fail(DFQ_ERR_UNSUPPORTED, "at most %d rows (got %d)", DFQ_ACCEPT_ROWS, rows);
+    if (batch > kMostGroups) return fail(DFQ_ERR_UNSUPPORTED, "too many sequences");
     if (V > 0x7fffffff / 2) return fail(DFQ_ERR_UNSUPPORTED, "V too large");
     if (dtype != DFQ_BF16 && dtype != DFQ_F16 && dtype != DFQ_F32)
         return fail(DFQ_ERR_UNSUPPORTED, "logits are bf16, fp16 or fp32");
@@ -141,9 +142,9 @@ dfq_status dfq_sample_accept(dfq_ctx* ctx, const void* logits, int64_t batch_str
          !(draft_temperature >= 0.0f && std::isfinite(draft_temperature))))
         return fail(DFQ_ERR_INVALID_ARGUMENT, "temperatures are finite and not negative");
     const AcceptPlan a = plan_accept(dfq_num_cus(ctx), batch, rows, V, dtype, drafted);
-    const int64_t jobs = (int64_t)batch * a.all_rows * a.ranges;
+    const int64_t jobs = (int64_t)batch * a.all_rows * a.ranges, groups = (jobs + kWaves - 1) / kWaves;
     const int64_t chunks = (int64_t)batch * a.chunks, rest = (int64_t)batch * a.rest_chunks;
-    if (jobs > INT32_MAX || rest > INT32_MAX)
+    if (groups > kMostGroups || chunks > kMostGroups || (drafted && rest > kMostGroups))
         return fail(DFQ_ERR_UNSUPPORTED, "grid too large");
     if (!workspace || workspace_bytes < a.bytes)
         return fail(DFQ_ERR_WORKSPACE, "workspace of %zu bytes needed (got %zu)", a.bytes,
@@ -187,9 +188,8 @@ dfq_status dfq_sample_accept(dfq_ctx* ctx, const void* logits, int64_t batch_str
     DeviceScope scope(ctx);
     const AcceptKernels& fn = ops->kernels[(int)dtype];
     void* args[] = {&p};
-    hipError_t e = hipModuleLaunchKernel(fn.sums[a.wide], (unsigned)((jobs + kWaves - 1) / kWaves), 1, 1,
-                                         DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args,
-                                         nullptr);
+    hipError_t e = hipModuleLaunchKernel(fn.sums[a.wide], (unsigned)groups, 1, 1, DFQ_KV_THREADS, 1, 1,
+                                         0, (hipStream_t)stream, args, nullptr);
     if (e == hipSuccess)
         e = hipModuleLaunchKernel(fn.weigh[a.wide], (unsigned)chunks, 1, 1, DFQ_KV_THREADS, 1, 1, 0,
                                   (hipStream_t)stream, args, nullptr);

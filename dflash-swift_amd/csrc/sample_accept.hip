@@ -12,7 +12,7 @@
  * arithmetic has them (exponentials to 8e-13): draws sum and search in 64 bits, and a draft whose
  * u q is within 2^-16 of p is decided again from 64-bit sums.  Other drafts need no more than fp32,
  * in which a logit costs 8 instructions against 20: all rows of 64 sequences of seven drafts of
- * 151936 tokens in 64 bits took 93 us for 46.  An fp32 sum is off by less than 2^-17 / 2 of itself:
+ * 151936 tokens in 64 bits took 93 us for 43.  An fp32 sum is off by less than 2^-17 / 2 of itself:
  * an exponent a has three roundings, 2.5 2^-24 |a|, and the mean of |a| over a row's mass is at most
  * log2 V, which makes 34 2^-24 for 2^20 tokens and 52 for 2^30; 13 sums in a row and the
  * exponential's last bits are 20 more.

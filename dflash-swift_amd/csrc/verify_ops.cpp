@@ -9,7 +9,6 @@
 #include <cmath>
 #include <cstdint>
 #include <cstdio>
-#include <new>
 
 #include "dflash_qmm.h"
 #include "kv_params.h"

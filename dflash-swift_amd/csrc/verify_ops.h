@@ -28,7 +28,6 @@
 
 namespace dfq {
 
-
 inline dfq_status hip_error(hipError_t e, const char* what) {
     return fail(DFQ_ERR_HIP, "%s: %s (%d)", what, hipGetErrorString(e), (int)e);
 }
@@ -58,8 +57,10 @@ inline bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
 
 inline size_t dtype_size(dfq_dtype t) { return t == DFQ_F32 ? 4 : 2; }
 
-/* The launch grid's limits in y and z. */
+/* The launch grid's limits in y and z, and of x in workgroups of DFQ_KV_THREADS: a grid has fewer
+ * than 2^32 threads along it. */
 constexpr int kMostGrid = 65535;
+constexpr int64_t kMostGroups = ((int64_t)1 << 32) / DFQ_KV_THREADS - 1;
 
 /* by 0: of a part of the call that is not there, and nothing is divided */
 inline Divisor divisor(int by) {

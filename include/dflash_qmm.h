@@ -434,7 +434,8 @@ typedef struct dfq_heads {
  * by the same angles.  Row m of sequence b is at position start + starts[b] + m (starts:
  * device memory, may be NULL for zeros) or at positions[b*rows + m] (device memory, as draft
  * trees need them; then start is 0 and starts NULL).  Positions may be negative.  head_dim is even
- * and at most 512; bf16, fp16 or fp32, in fp32 and rounded once.  Asynchronous on `stream`. */
+ * and at most 512, heads at most 65535 a token; bf16, fp16 or fp32, in fp32 and rounded once.
+ * Asynchronous on `stream`. */
 dfq_status dfq_rope(dfq_ctx* ctx, const dfq_rope_table* rope, const dfq_heads* q,
                     const dfq_heads* k, int head_dim, dfq_dtype dtype, int batch, int rows,
                     int start, const int32_t* starts, const int32_t* positions, int inverse,
@@ -490,10 +491,10 @@ dfq_status dfq_token_logprobs(dfq_ctx* ctx, const void* logits, int64_t row_stri
  * A token is drawn as the first whose running sum of probabilities exceeds u[b][rows-1] times their
  * sum.  uniforms u [batch][rows] are in [0, 1) and the caller's, so that a call with the same
  * numbers gives the same tokens, distributed as p (counts and tokens are those of 64-bit sums, with
- * exponentials to 8e-13; chances are right to 2^-17 of themselves).  temperatures and draft_temperatures [batch] are in device
- * memory; NULL: `temperature`, `draft_temperature` for all.  T = 0 takes p = 1 for the row's
- * argmax, as dfq_argmax_accept finds it.  A logit of -inf has probability 0, as have probabilities
- * under 2^-1000 of the row's largest.  A row with a NaN or
+ * exponentials to 8e-13; chances are right to 2^-17 of themselves).  temperatures and
+ * draft_temperatures [batch] are in device memory; NULL: `temperature`, `draft_temperature` for
+ * all.  T = 0 takes p = 1 for the row's argmax, as dfq_argmax_accept finds it.  A logit of -inf has
+ * probability 0, as have probabilities under 2^-1000 of the row's largest.  A row with a NaN or
  * +inf, with nothing above -inf, or with a temperature of its sequence that is negative or not
  * finite has no distribution: a draft judged by such a row of the target or the draft is refused
  * (chance 0), and the token in its place is -1.  So is refused a draft outside 0..V-1 (the token is

@@ -177,6 +177,15 @@ def test_rotations_that_are_refused(norms):
     refused(2, q=heads(MAX), k=heads(MAX))
 
 
+def test_rotations_past_a_launch_are_refused():
+    """More heads of a token than a lane's counting holds, and grids of 2^32 threads and more (a
+    wave a head where chunks do not fit)."""
+    for n in (65536, MAX):
+        assert rope_call(q=heads(n)) == 2
+        assert rope_call(k=heads(n)) == 2
+    assert rope_call(rope=table(rotary=12), dim=12, batch=1 << 13, rows=1 << 13) == 2
+
+
 def test_norms_that_are_refused():
     for norms, status in (((AT, AT, 1, 1e-6, 0.0), 2), ((AT + 1, None, 0, 1e-6, 0.0), 1),
                           ((None, AT + 2, 2, 1e-6, 0.0), 1), ((AT, AT, 0, -1e-6, 0.0), 1),
@@ -220,6 +229,10 @@ def test_accepts_that_are_refused():
     refused(3, ws_bytes=8)
     refused(1, ws=AT + 8)
     refused(2, batch=MAX, rows=1, drafts=None, V=10 ** 6, ws_bytes=1 << 62)
+    # more workgroups than a launch has
+    refused(2, batch=1 << 24, rows=1, drafts=None, V=1, ws_bytes=1 << 62)
+    refused(2, batch=1 << 23, rows=64, V=1, ws_bytes=1 << 62)
+    refused(2, batch=MAX, rows=64, V=MAX // 2, ws_bytes=1 << 62)
     c = dflash_qmm.load_library()
     n = ctypes.c_size_t(7)
     assert c.dfq_sample_accept_workspace_bytes(None, 1, 1, 9, 0, 0, ctypes.byref(n)) == 1
