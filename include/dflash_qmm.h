@@ -499,7 +499,8 @@ dfq_status dfq_token_logprobs(dfq_ctx* ctx, const void* logits, int64_t row_stri
  * finite has no distribution: a draft judged by such a row of the target or the draft is refused
  * (chance 0), and the token in its place is -1.  So is refused a draft outside 0..V-1 (the token is
  * then drawn as for q = 0 in all of p, or from p - q).  Strides are in elements, logits of a row
- * side by side; sequences or rows may share logits (a stride of 0).
+ * side by side; sequences or rows may share logits (a stride of 0).  Outputs and workspace overlap
+ * no input.
  * The workspace (dfq_sample_accept_workspace_bytes, drafted != 0 with draft logits; 16-byte
  * aligned) needs no clearing, and is shared no more than dfq_cache_attention's.  The reference
  * accepts greedily alone (acceptedPrefix, DFlashSpeculativeGenerator.swift:555-571;
