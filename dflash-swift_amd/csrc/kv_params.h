@@ -86,17 +86,6 @@ struct AcceptPart {
 
 #define DFQ_ACCEPT_APART 32  /* counters lie a cache line apart                          */
 #define DFQ_ACCEPT_PIECES 4  /* 16-byte pieces that a lane takes of a range              */
-#define DFQ_ACCEPT_WIDE 2    /* and where their sums are 64 bits wide                    */
-
-/* What is left to draw of a sequence: nothing, or a token from p, from p without its draft, or
- * from max(p - q, 0). */
-enum { DFQ_DRAW_NONE = 0, DFQ_DRAW_P = 1, DFQ_DRAW_OTHER = 2, DFQ_DRAW_REST = 3 };
-struct AcceptDraw {
-    int32_t mode, row;       /* the target's row, and the place of the token */
-    int32_t draft, token;    /* the row's draft; the token of DFQ_DRAW_NONE  */
-    float p_top, q_top;      /* largest logits of the rows                   */
-    double p_sum, q_sum;     /* and their sums of 2^((x - top) rate)         */
-};
 
 struct AcceptParams {
     const void* logits;
@@ -110,18 +99,17 @@ struct AcceptParams {
     int32_t* accepted;          /* [batch]                                         */
     float* chances;             /* [batch][rows - 1] or NULL                       */
     AcceptPart* parts;          /* [batch][rows, then draft rows][ranges]          */
-    double* wide;               /* [batch][rows, ..][ranges]: the parts' sums in 64 bits */
-    AcceptDraw* draws;          /* [batch], with draft logits                      */
-    double* totals;             /* [batch][chunks][2]: both rows' sums             */
-    uint64_t* sums;             /* [batch][units]: what is drawn from, as doubles' bits */
+    uint64_t* sums;             /* [batch][sums_apart]: of units, one or (p - q) four; doubles' bits */
+    uint64_t* totals;           /* [batch][chunks][2]: both rows' sums, with draft logits  */
     int32_t* arrived;           /* [batch][DFQ_ACCEPT_APART]: workgroups whose sums are there */
     int64_t batch_stride, row_stride, draft_batch_stride, draft_row_stride;
     float temperature, draft_temperature;
     int rows, vocab;
     int jobs;                   /* ranges of all rows                              */
     int units;                  /* 64 lanes' 16 bytes each, of a row               */
+    int sums_apart;             /* units, four times that with draft logits        */
     Divisor all_rows, ranges;   /* rows and draft rows of a sequence; ranges a row */
-    Divisor chunks, rest_chunks;   /* workgroups of a sequence in the later kernels */
+    Divisor chunks;             /* workgroups of a sequence in the second kernel   */
 };
 
 #define DFQ_ROPE_DIM 512     /* widest head */

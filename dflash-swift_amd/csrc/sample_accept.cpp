@@ -18,30 +18,21 @@ using namespace dfq;
 
 namespace {
 
-struct AcceptKernels {
-    hipFunction_t sums[2] = {}, weigh[2] = {}, rest = nullptr;   // [sums in fp32/64 bits]
-};
-
 struct AcceptOps : LoadedOps {
     static constexpr OpsGroup kGroup = kAcceptOps;
     hipModule_t module = nullptr;
-    AcceptKernels kernels[3];   // [bf16/f16/f32]
+    hipFunction_t kernels[2][3] = {};   // [sums/weigh][bf16/f16/f32]
     dfq_status resolve() {
         static const char* kDt[3] = {"bf16", "f16", "f32"};
         hipError_t e = hipModuleLoadData(&module, dfq_accept_hsaco);
         if (e != hipSuccess) return hip_error(e, "hipModuleLoadData(gfx950 sampled-accept object)");
         char name[80];
-        for (int t = 0; t < 3; ++t) {
-            AcceptKernels& a = kernels[t];
-            const struct { const char* op; hipFunction_t* fn; } parts[] = {
-                {"sums", &a.sums[0]}, {"wide_sums", &a.sums[1]}, {"weigh", &a.weigh[0]},
-                {"wide_weigh", &a.weigh[1]}, {"rest", &a.rest}};
-            for (const auto& part : parts) {
-                snprintf(name, sizeof name, "dfq_accept_%s_%s", part.op, kDt[t]);
-                if ((e = hipModuleGetFunction(part.fn, module, name)) != hipSuccess)
+        for (int k = 0; k < 2; ++k)
+            for (int t = 0; t < 3; ++t) {
+                snprintf(name, sizeof name, "dfq_accept_%s_%s", k ? "weigh" : "sums", kDt[t]);
+                if ((e = hipModuleGetFunction(&kernels[k][t], module, name)) != hipSuccess)
                     return hip_error(e, name);
             }
-        }
         return DFQ_OK;
     }
     ~AcceptOps() override {
@@ -62,8 +53,8 @@ dfq_status check_sizes(int batch, int rows, int V, dfq_dtype dtype) {
 }
 
 struct AcceptPlan {
-    int all_rows, wide, ranges, units, chunks, rest_chunks;
-    size_t wide_sums, sums, totals, draws, arrived, bytes;   /* offsets; the parts come first */
+    int all_rows, ranges, units, sums_apart, chunks;
+    size_t sums, totals, arrived, bytes;   /* offsets; the parts come first */
 };
 
 constexpr int kWaves = DFQ_KV_THREADS / 64;
@@ -73,26 +64,21 @@ AcceptPlan plan_accept(int cus, int batch, int rows, int V, dfq_dtype dtype, boo
     a.all_rows = drafted ? 2 * rows - 1 : rows;
     const int unit = 64 * (dtype == DFQ_F32 ? 4 : 8);
     a.units = (V + unit - 1) / unit;
-    /* All rows' sums in 64 bits cost up to twice the first launch and save the third, which only
-     * draft logits need.  Seven drafts of 151936 tokens each, bf16, on the device: 1 sequence
-     * 15.3 us wide and 18.3 with fp32 sums, 8 28.0 and 30.6, 12 (27 M logits) 34.0 and 33.8. */
-    a.wide = drafted && (int64_t)batch * a.all_rows * V <= 24 << 20;
-    const int range = unit * (a.wide ? DFQ_ACCEPT_WIDE : DFQ_ACCEPT_PIECES);
+    a.sums_apart = drafted ? 4 * a.units : a.units;
+    const int range = unit * DFQ_ACCEPT_PIECES;
     a.ranges = (V + range - 1) / range;
-    /* Workgroups of a sequence: as many units a wave as leave no more than six workgroups a CU,
-     * which are there at once, and as few workgroups as that many units take: each decides its
-     * sequence's drafts first. */
+    /* Workgroups of a sequence: as many units a wave as leave no more than four workgroups a CU,
+     * which are there at once (99 registers), and as few workgroups as that many units take: each
+     * decides its sequence's drafts first.  With five a CU 64 sequences of seven drafts of 151936
+     * tokens took 73.6 us for 71.9 and 16 32.3 for 29.9; eight took 33 rows of 50257 from 14.3 to
+     * 16.2. */
     const auto parts = [](int n, int of) { return (int)(((int64_t)n + of - 1) / of); };
-    const int most = std::max(1, 6 * cus / batch);
+    const int most = std::max(1, 4 * cus / batch);
     a.chunks = parts(a.units, kWaves * parts(a.units, kWaves * most));
-    a.rest_chunks = parts(a.units, kWaves);   /* nothing is decided there */
     const auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
-    const size_t ranges = (size_t)batch * a.all_rows * a.ranges;
-    a.wide_sums = up(ranges * sizeof(AcceptPart));
-    a.sums = a.wide_sums + (a.wide ? up(ranges * 8) : 0);
-    a.totals = a.sums + up((size_t)batch * a.units * 8);
-    a.draws = a.totals + (drafted ? up((size_t)batch * a.chunks * 16) : 0);
-    a.arrived = a.draws + (drafted ? up((size_t)batch * sizeof(AcceptDraw)) : 0);
+    a.sums = up((size_t)batch * a.all_rows * a.ranges * sizeof(AcceptPart));
+    a.totals = a.sums + up((size_t)batch * a.sums_apart * 8);
+    a.arrived = a.totals + (drafted ? up((size_t)batch * a.chunks * 16) : 0);
     a.bytes = a.arrived + (size_t)batch * DFQ_ACCEPT_APART * 4;
     return a;
 }
@@ -143,8 +129,8 @@ dfq_status dfq_sample_accept(dfq_ctx* ctx, const void* logits, int64_t batch_str
         return fail(DFQ_ERR_INVALID_ARGUMENT, "temperatures are finite and not negative");
     const AcceptPlan a = plan_accept(dfq_num_cus(ctx), batch, rows, V, dtype, drafted);
     const int64_t jobs = (int64_t)batch * a.all_rows * a.ranges, groups = (jobs + kWaves - 1) / kWaves;
-    const int64_t chunks = (int64_t)batch * a.chunks, rest = (int64_t)batch * a.rest_chunks;
-    if (groups > kMostGroups || chunks > kMostGroups || (drafted && rest > kMostGroups))
+    const int64_t chunks = (int64_t)batch * a.chunks;
+    if (groups > kMostGroups || chunks > kMostGroups)
         return fail(DFQ_ERR_UNSUPPORTED, "grid too large");
     if (!workspace || workspace_bytes < a.bytes)
         return fail(DFQ_ERR_WORKSPACE, "workspace of %zu bytes needed (got %zu)", a.bytes,
@@ -165,9 +151,7 @@ dfq_status dfq_sample_accept(dfq_ctx* ctx, const void* logits, int64_t batch_str
     p.chances = chances;
     p.parts = (AcceptPart*)ws;
     p.sums = (uint64_t*)(ws + a.sums);
-    p.wide = (double*)(ws + a.wide_sums);
-    p.totals = (double*)(ws + a.totals);
-    p.draws = drafted ? (AcceptDraw*)(ws + a.draws) : nullptr;
+    p.totals = (uint64_t*)(ws + a.totals);
     p.arrived = (int32_t*)(ws + a.arrived);
     p.batch_stride = batch_stride;
     p.row_stride = row_stride;
@@ -179,23 +163,19 @@ dfq_status dfq_sample_accept(dfq_ctx* ctx, const void* logits, int64_t batch_str
     p.vocab = V;
     p.jobs = (int)jobs;
     p.units = a.units;
+    p.sums_apart = a.sums_apart;
     p.all_rows = divisor(a.all_rows);
     p.ranges = divisor(a.ranges);
     p.chunks = divisor(a.chunks);
-    p.rest_chunks = divisor(a.rest_chunks);
     const AcceptOps* ops;
     if ((s = ops_of(ctx, &ops))) return s;
     DeviceScope scope(ctx);
-    const AcceptKernels& fn = ops->kernels[(int)dtype];
     void* args[] = {&p};
-    hipError_t e = hipModuleLaunchKernel(fn.sums[a.wide], (unsigned)groups, 1, 1, DFQ_KV_THREADS, 1, 1,
-                                         0, (hipStream_t)stream, args, nullptr);
+    hipError_t e = hipModuleLaunchKernel(ops->kernels[0][(int)dtype], (unsigned)groups, 1, 1,
+                                         DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
     if (e == hipSuccess)
-        e = hipModuleLaunchKernel(fn.weigh[a.wide], (unsigned)chunks, 1, 1, DFQ_KV_THREADS, 1, 1, 0,
-                                  (hipStream_t)stream, args, nullptr);
-    if (e == hipSuccess && drafted && !a.wide)
-        e = hipModuleLaunchKernel(fn.rest, (unsigned)rest, 1, 1, DFQ_KV_THREADS, 1, 1, 0,
-                                  (hipStream_t)stream, args, nullptr);
+        e = hipModuleLaunchKernel(ops->kernels[1][(int)dtype], (unsigned)chunks, 1, 1,
+                                  DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
     return e == hipSuccess ? DFQ_OK : hip_error(e, "launch dfq_sample_accept");
 }
 

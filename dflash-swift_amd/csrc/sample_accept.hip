@@ -21,13 +21,13 @@
  * largest logit and the sum of e^((x - largest) / T).  In the second each workgroup joins its
  * sequence's ranges and decides its drafts (alike in all of them, so that nothing has to be waited
  * for), then weighs its part of the row that is drawn from; the last to come finds the token.
- * Where the draw is from p - q the second sums both rows in 64 bits, and a third weighs and finds;
- * calls of few logits sum all rows in 64 bits at once (the wide kernels) and need no third.
+ * A draw from p - q needs no third launch either, though its terms are known only when both rows
+ * have been summed: nearly all tokens' signs are, from the fp32 sums (from_rest).
  *
- * 64 sequences of seven sampled drafts of 151936 tokens in bf16: 85 us in all.  The sums take 43
- * (254 MB, 5.9 TB/s), the refusing rows' sums 24 and the draws 21, of which vector instructions are
- * half and the rest what a launch's start, its decisions and its last workgroup take.  16 sequences
- * 36 us, one block of seven certain drafts 12.6, 33 plain draws from 50257 logits in fp32 14.4.
+ * 64 sequences of seven sampled drafts of 151936 tokens in bf16: 72 us in all.  The sums take 43
+ * (254 MB, 5.9 TB/s) and the draws 29, of which vector instructions are some 18 and the rest what the
+ * launch's start, its decisions and its last workgroup take.  16 sequences 29.9 us, one block of
+ * seven certain drafts 12.6, 33 plain draws from 50257 logits in fp32 14.3.
  */
 #include "kv_params.h"
 #include "logit_piece.h"
@@ -86,6 +86,18 @@ __device__ __forceinline__ bool is_temperature(float t) {
     return t >= 0.0f && t < __builtin_inff();
 }
 
+/* What is alike in all lanes, in scalar registers. */
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ float uniform(float v) {
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v)));
+}
+__device__ __forceinline__ double uniform(double v) {
+    u32x2_t w = __builtin_bit_cast(u32x2_t, v);
+    w[0] = __builtin_amdgcn_readfirstlane(w[0]);
+    w[1] = __builtin_amdgcn_readfirstlane(w[1]);
+    return __builtin_bit_cast(double, w);
+}
+
 struct Sequence {
     float t, dt;         /* temperatures                        */
     int drafts;          /* that it brings                      */
@@ -127,6 +139,13 @@ __device__ __forceinline__ double wave_sum(double v) {
     v += __shfl_xor(v, 16);
     return v + __shfl_xor(v, 32);
 }
+/* Two sums at once: a's in the lower 32 lanes, b's in the upper. */
+__device__ __forceinline__ double wave_sums(double a, double b) {
+    const bool upper = threadIdx.x % 64 >= 32;
+    const double v = (upper ? b : a) + __shfl_xor(upper ? a : b, 32);
+    const double sum = lanes16_sum(v);
+    return sum + __shfl_xor(sum, 16);
+}
 template <typename Op>
 __device__ __forceinline__ float wave_of(float v, Op op) {
     const auto bits = [&](uint32_t a, uint32_t b) {
@@ -152,6 +171,20 @@ __device__ __forceinline__ double block_sum(double v) {
     for (int w = 0; w < kWaves; ++w) s += waves[w];
     __syncthreads();
     return s;
+}
+
+__device__ __forceinline__ void block_sums(double& a, double& b) {
+    __shared__ double waves[2 * kWaves];
+    const double v = wave_sums(a, b);
+    if (threadIdx.x % 32 == 0) waves[threadIdx.x / 32] = v;
+    __syncthreads();
+    a = b = 0.0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        a += waves[2 * w];
+        b += waves[2 * w + 1];
+    }
+    __syncthreads();
 }
 
 /* The sum over the threads in front of this one; `all` gets that over all. */
@@ -192,8 +225,9 @@ __device__ __noinline__ Search search(double a, double b, double from, double go
     double all;
     const double run = from + block_before(a + b, all);
     if (goal < 0.0) goal = u * all;
-    const uint64_t some = __ballot(a + b > kNothing);
-    const uint64_t past = __ballot(a + b > kNothing && run + (a + b) > goal);
+    const bool weighs = a > kNothing || b > kNothing;
+    const uint64_t some = __ballot(weighs);
+    const uint64_t past = __ballot(weighs && run + (a + b) > goal);
     if (lane == 0) {
         firsts[wave] = past ? (int)__builtin_ctzll(past) : -1;
         lasts[wave] = some ? 63 - (int)__builtin_clzll(some) : -1;
@@ -216,9 +250,11 @@ __device__ __noinline__ Search search(double a, double b, double from, double go
 }
 
 /* The place among n weights where their running sum passes u times their sum (goal < 0), or the
- * goal, counted from `from`: cut into 512 parts until a part is one weight. */
-template <typename Weight>
-__device__ __forceinline__ Search find(int n, Weight weight, double from, double goal, double u) {
+ * goal, counted from `from`: cut into 512 parts until a part is one weight.  A weight is that of
+ * (place, what `fetch` reads of it); all threads come to each, those without one to a neighbour's. */
+template <typename Fetch, typename Weight>
+__device__ __forceinline__ Search find(int n, Fetch fetch, Weight weight, double from, double goal,
+                                       double u) {
     int lo = 0;
     for (;;) {
         const int each = (n + 2 * DFQ_KV_THREADS - 1) / (2 * DFQ_KV_THREADS);
@@ -226,14 +262,20 @@ __device__ __forceinline__ Search find(int n, Weight weight, double from, double
         if (each == 1) {
             /* both loads under way at once: behind a branch each they came one after the other */
             const int i = 2 * (int)threadIdx.x;
-            w[0] = weight(lo + min(i, n - 1));
-            w[1] = weight(lo + min(i + 1, n - 1));
+            const int at0 = lo + min(i, n - 1), at1 = lo + min(i + 1, n - 1);
+            const auto first = fetch(at0), second = fetch(at1);
+            w[0] = weight(at0, first);
+            w[1] = weight(at1, second);
             w[0] = i < n ? w[0] : 0.0;
             w[1] = i + 1 < n ? w[1] : 0.0;
         } else {
             for (int k = 0; k < 2; ++k) {
                 const int64_t begin = (2 * (int64_t)threadIdx.x + k) * each;
-                for (int64_t i = begin; i < begin + each && i < n; ++i) w[k] += weight(lo + (int)i);
+                for (int64_t i = begin; i < begin + each; ++i) {
+                    const int at = lo + (int)(i < n ? i : n - 1);
+                    const double v = weight(at, fetch(at));
+                    w[k] += i < n ? v : 0.0;
+                }
             }
         }
         Search s = search(w[0], w[1], from, goal, u);
@@ -258,6 +300,16 @@ struct Row {
     double sum;
 };
 
+/* What is left to draw of a sequence: nothing, or a token from p, from p without its draft, or from
+ * max(p - q, 0). */
+enum { kDrawNone, kDrawP, kDrawOther, kDrawRest };
+struct Draw {
+    int mode, row;          /* the target's row, and the place of the token */
+    int draft, token;       /* the row's draft; the token of kDrawNone      */
+    float p_top, q_top;     /* largest logits of the rows                   */
+    double p_sum, q_sum;    /* and their sums, right to fp32's bound        */
+};
+
 template <int DT>
 struct Accept : LogitPiece<DT> {
     using LogitPiece<DT>::kN, LogitPiece<DT>::load, LogitPiece<DT>::widen;
@@ -272,13 +324,11 @@ struct Accept : LogitPiece<DT> {
                (b * p.draft_batch_stride + r * p.draft_row_stride) * kSize;
     }
 
-    /* One range of one row by one wave, kPieces x 16 bytes a lane; its sum in fp32 or (WIDE) in 64
-     * bits.  Of 2, 3, 4, 6 and 8 pieces in fp32, 64 sequences of seven drafts took 97, 87, 85, 85
-     * and 86 us, 16 38, 36, 36, 36 and 38 (8 take 108 registers), one block 12.6, 12.2, 12.6, 12.7
-     * and 13.7. */
-    template <int kPieces, bool WIDE>
+    /* One range of one row by one wave, kPieces x 16 bytes a lane; its sum in fp32.  Of 2, 3, 4, 6
+     * and 8 pieces, 64 sequences of seven drafts took 85, 75, 72, 72 and 73 us, 16 32, 30, 30, 30 and
+     * 32 (8 take 108 registers), one block 12.7, 12.1, 12.5, 12.5 and 13.5. */
     static __device__ __forceinline__ void sums(const AcceptParams& p) {
-        constexpr int kRange = kPieces * kUnit;
+        constexpr int kPieces = DFQ_ACCEPT_PIECES, kRange = kPieces * kUnit;
         const int lane = threadIdx.x % 64;
         const int job = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + threadIdx.x / 64);
         if (job >= p.jobs) return;
@@ -334,21 +384,7 @@ struct Accept : LogitPiece<DT> {
             }
             top = wave_of(top, [](float a, float c) { return larger(a, c); });
             part.top = top;
-            if constexpr (WIDE) {
-                double sum = 0.0;
-                if (fabsf(top) < __builtin_inff()) {
-                    const Powers e(t, top);
-#pragma unroll
-                    for (int i = 0; i < kPieces; ++i) {
-                        float x[kN];
-                        widen(v[i], x);
-#pragma unroll
-                        for (int j = 0; j < kN; ++j) sum += e(x[j]);
-                    }
-                    sum = wave_sum(sum);
-                }
-                if (lane == 0) p.wide[job] = sum;
-            } else if (fabsf(top) < __builtin_inff()) {
+            if (fabsf(top) < __builtin_inff()) {
                 const float rate = (float)rate_of(t);
                 float sum = 0.0f;
 #pragma unroll
@@ -373,31 +409,25 @@ struct Accept : LogitPiece<DT> {
 
     /* A row's ranges together, by 16 lanes.  NaN, +inf or nothing above -inf leaves a sum that is
      * not positive and finite. */
-    template <bool WIDE>
     static __device__ __forceinline__ Row row_of(const AcceptParams& p, int b, int r, float t) {
         const int lane = threadIdx.x % 16, n = p.ranges.by;
         const int64_t first = ((int64_t)b * p.all_rows.by + r) * n;
         Row row = {-__builtin_inff(), kNone, 0.0};
         const float rate = (float)rate_of(t);
         const auto factor = [&](float from, float to) -> double {
-            if constexpr (WIDE) return Powers(t, to)(from);
-            else return __builtin_amdgcn_exp2f((from - to) * rate);
+            return __builtin_amdgcn_exp2f((from - to) * rate);
         };
         constexpr int kOnce = 4;   /* loads on their way together */
         for (int from = 0; from < n; from += 16 * kOnce) {
             AcceptPart v[kOnce];
             double sums[kOnce];
 #pragma unroll
-            for (int j = 0; j < kOnce; ++j) {
-                const int64_t i = first + min(from + 16 * j + lane, n - 1);
-                v[j] = p.parts[i];
-                if constexpr (WIDE) sums[j] = p.wide[i];
-            }
+            for (int j = 0; j < kOnce; ++j)
+                v[j] = p.parts[first + min(from + 16 * j + lane, n - 1)];
 #pragma unroll
             for (int j = 0; j < kOnce; ++j) {
                 const bool in = from + 16 * j + lane < n;
-                if constexpr (!WIDE) sums[j] = (double)__uint_as_float(v[j].sum);
-                sums[j] = in ? sums[j] : 0.0;
+                sums[j] = in ? (double)__uint_as_float(v[j].sum) : 0.0;
                 v[j].top = in ? v[j].top : -__builtin_inff();
                 v[j].sum = in ? v[j].sum : (uint32_t)kNone;
             }
@@ -457,19 +487,19 @@ struct Accept : LogitPiece<DT> {
         return block_sum(sum);
     }
 
+    static __device__ __forceinline__ double counted(double v) { return v > kNothing ? v : 0.0; }
+
     /* A logit's share of its row. */
     static __device__ __forceinline__ double part_of(float x, float t, float top, double sum) {
-        const double v = Powers(t, top)(x);
-        return v > kNothing ? v / sum : 0.0;
+        return counted(Powers(t, top)(x)) / sum;
     }
 
     /* Decides the drafts of sequence b, by a workgroup: 16 lanes join a row, lane i of the last
      * wave looks at draft i.  `writes` stores what is known without a draw. */
-    template <bool WIDE>
-    static __device__ __forceinline__ AcceptDraw decide(const AcceptParams& p, const Sequence& s,
+    static __device__ __forceinline__ Draw decide(const AcceptParams& p, const Sequence& s,
                                                         int b, bool writes) {
         __shared__ Row rows[2 * 64];
-        __shared__ AcceptDraw made;
+        __shared__ Draw made;
         __shared__ uint64_t again;
         const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
         const bool greedy = s.t == 0.0f;
@@ -490,7 +520,7 @@ struct Accept : LogitPiece<DT> {
             }
         }
         for (int i = threadIdx.x / 16; i < (int)p.all_rows.by; i += DFQ_KV_THREADS / 16) {
-            const Row row = row_of<WIDE>(p, b, i, i < p.rows ? s.t : s.dt);
+            const Row row = row_of(p, b, i, i < p.rows ? s.t : s.dt);
             if (lane % 16 == 0) rows[i] = row;
         }
         __syncthreads();
@@ -523,9 +553,9 @@ struct Accept : LogitPiece<DT> {
                 __ballot(known && mine > 0.0 && fabs(u * theirs - mine) < 0x1p-16 * mine);
             if (lane == 0) again = near;
         }
-        if constexpr (!WIDE) __syncthreads();
+        __syncthreads();
         /* drafts next to the border: fewer than one in ten thousand */
-        for (uint64_t near = WIDE ? 0 : again; near; near &= near - 1) {
+        for (uint64_t near = again; near; near &= near - 1) {
             const int i = __builtin_ctzll(near);
             double p_sum = 0.0, q_sum = 0.0;
             if (!greedy) p_sum = whole_row(target_row(p, b, i), p.vocab, rows[i].top, s.t);
@@ -541,11 +571,11 @@ struct Accept : LogitPiece<DT> {
             const uint64_t refused = ~__ballot(taken);
             const int n = __builtin_ctzll(refused);   /* at most 63 drafts: some bit is set */
             if (lane == n) {
-                AcceptDraw d = {DFQ_DRAW_NONE, n, draft, -1, row.top, other.top, row.sum,
+                Draw d = {kDrawNone, n, draft, -1, row.top, other.top, row.sum,
                                 other.sum};
                 if (some && greedy) d.token = row.at;
-                else if (some && n == s.drafts) d.mode = DFQ_DRAW_P;
-                else if (some) d.mode = s.drafted ? DFQ_DRAW_REST : DFQ_DRAW_OTHER;
+                else if (some && n == s.drafts) d.mode = kDrawP;
+                else if (some) d.mode = s.drafted ? kDrawRest : kDrawOther;
                 made = d;
                 if (writes) p.accepted[b] = n;
             }
@@ -560,35 +590,24 @@ struct Accept : LogitPiece<DT> {
             }
         }
         __syncthreads();
-        return made;
+        return {uniform(made.mode), uniform(made.row), uniform(made.draft), uniform(made.token),
+                uniform(made.p_top), uniform(made.q_top), uniform(made.p_sum),
+                uniform(made.q_sum)};
     }
 
-    /* Weighs the row that sequence b is drawn from: waves sum units of it, and the last of the
-     * sequence's workgroups to come finds the token, -1 in the others.  `weight` gets a token and
-     * its logits in both rows (`other` NULL: one). */
-    template <typename Weight>
-    static __device__ __forceinline__ int drawn(const AcceptParams& p, int chunks, int b,
-                                                int chunk, const char* row, const char* other,
-                                                double u, Weight weight) {
-        const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-        uint64_t* sums = p.sums + (int64_t)b * p.units;
-        for (int unit = chunk * kWaves + wave; unit < p.units; unit += chunks * kWaves) {
-            const int i = unit * kUnit + lane * kN;
-            float x[kN], y[kN] = {};
-            const u32x4_t v = load(row, i, p.vocab);
-            if (other) widen(load(other, i, p.vocab), y);
-            widen(v, x);
-            double sum = 0.0;
-#pragma unroll
-            for (int j = 0; j < kN; ++j) sum += weight(i + j, x[j], y[j]);
-            sum = wave_sum(sum);
-            if (lane == 0)
-                __hip_atomic_store(&sums[unit], __builtin_bit_cast(uint64_t, sum),
-                                   __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        /* Sums and count meet in memory, past the caches, by device-scope atomics: a wave's stores
-         * have completed before its workgroup counts.  (Fences that write back and
-         * drop the L2 instead made 16 sequences' draw take 77 us.) */
+    static __device__ __forceinline__ void put(uint64_t* at, double v) {
+        __hip_atomic_store(at, __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+    }
+    static __device__ __forceinline__ double got(const uint64_t* at) {
+        return __builtin_bit_cast(
+            double, __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    }
+    /* Whether this is the last of sequence b's workgroups to come.  Sums and count meet in memory,
+     * past the caches, by device-scope atomics: a wave's stores have completed before its workgroup
+     * counts.  (Fences that write back and drop the L2 instead made 16 sequences' draw take 77
+     * us.) */
+    static __device__ __forceinline__ bool last(const AcceptParams& p, int b) {
         __shared__ int arrived;
         __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
@@ -596,107 +615,200 @@ struct Accept : LogitPiece<DT> {
             arrived = __hip_atomic_fetch_add(&p.arrived[b * DFQ_ACCEPT_APART], 1, __ATOMIC_RELAXED,
                                              __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
-        if (arrived != chunks - 1) return -1;
-        const Search found = find(p.units, [&](int i) {
-            return __builtin_bit_cast(
-                double, __hip_atomic_load(&sums[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-        }, 0.0, -1.0, u);
-        if (found.place == kNone) return kNone;
-        const int from = found.place * kUnit;
-        return from + find(min(kUnit, p.vocab - from), [&](int i) {
-            return weight(from + i, load_any(row, DT, from + i),
-                          other ? load_any(other, DT, from + i) : 0.0f);
-        }, found.front, found.goal, u).place;
+        return arrived == p.chunks.by - 1;
     }
 
-    /* The draw from p - q, both scaled to sums of 1; as drawn(). */
+    /* A token drawn from the exponentials of the target's row, without the one at `without`: waves
+     * sum units, and the last of the sequence's workgroups finds it (kNone: nothing weighs), -1 in
+     * the others. */
+    static __device__ __forceinline__ int from_row(const AcceptParams& p, const char* row,
+                                                   const Powers& e, int without, int b, int chunk,
+                                                   double u) {
+        const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+        uint64_t* sums = p.sums + (int64_t)b * p.sums_apart;
+        const auto weight = [&](int i, float x) { return i == without ? 0.0 : e(x); };
+        for (int unit = chunk * kWaves + wave; unit < p.units; unit += p.chunks.by * kWaves) {
+            const int i = unit * kUnit + lane * kN;
+            float x[kN];
+            widen(load(row, i, p.vocab), x);
+            double sum = 0.0;
+#pragma unroll
+            for (int j = 0; j < kN; ++j) sum += weight(i + j, x[j]);
+            sum = wave_sum(sum);
+            if (lane == 0) put(&sums[unit], sum);
+        }
+        if (!last(p, b)) return -1;
+        const Search unit = find(p.units, [&](int i) { return got(&sums[i]); },
+                                 [](int, double v) { return v; }, 0.0, -1.0, u);
+        if (unit.place == kNone) return kNone;
+        const int from = unit.place * kUnit;
+        const int place = find(min(kUnit, p.vocab - from),
+                               [&](int i) { return load_any(row, DT, from + i); },
+                               [&](int i, float x) { return weight(from + i, x); },
+                               unit.front, unit.goal, u).place;
+        if (place != kNone) return from + place;
+        /* u = 0 and a unit of nothing but what counts as nothing one by one */
+        return find(p.vocab, [&](int i) { return load_any(row, DT, i); },
+                    [&](int i, float x) { return counted(weight(i, x)); }, 0.0, -1.0, u).place;
+    }
+
+    /* A token drawn from max(p - q, 0), as from_row.  The rows' sums in 64 bits are known when all
+     * their logits have been seen; in which tokens p is larger is known before, but for those where
+     * the two are within 2^-15 of each other by the fp32 sums (off by 2^-17 at most each; four or so
+     * of 151936).  So a unit's part is kept as the sums of p's and of q's exponentials over the
+     * tokens where p is surely larger, and the two of a token in between, to be scaled and
+     * subtracted when the sums are known; the last workgroup weighs units with more tokens in
+     * between again.  (Two launches instead, of both rows' sums and then of their differences,
+     * took 24 and 21 us for 64 sequences, this 29.)  Of a product with 0 or 1 in the sums: one
+     * select instead of four. */
     static __device__ __forceinline__ int from_rest(const AcceptParams& p, const Sequence& s,
-                                                    const AcceptDraw& d, int chunks, int b,
-                                                    int chunk, double p_sum, double q_sum,
-                                                    double u) {
+                                                    const Draw& d, int b, int chunk, double u) {
+        const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
         const char* row = target_row(p, b, d.row);
         const char* other = draft_row(p, b, d.row);
         const Powers e(s.t, d.p_top), f(s.dt, d.q_top);
-        const double by = 1.0 / p_sum, draft_by = 1.0 / q_sum;
-        const int token = drawn(p, chunks, b, chunk, row, other, u, [&](int, float x, float y) {
+        const double ratio = uniform(d.q_sum / d.p_sum);
+        uint64_t* sums = p.sums + (int64_t)b * p.sums_apart;
+        uint64_t* totals = p.totals + 2 * (int64_t)b * p.chunks.by;
+        const auto is_more = [&](double a, double c) { return fma(a, ratio, -c) > c * 0x1p-15; };
+        const auto is_close = [&](double a, double c) {
+            return fabs(fma(a, ratio, -c)) <= c * 0x1p-15 && a > kNothing;
+        };
+        double p_sum = 0.0, q_sum = 0.0;
+        for (int unit = chunk * kWaves + wave; unit < p.units; unit += p.chunks.by * kWaves) {
+            const int i = unit * kUnit + lane * kN;
+            const u32x4_t v = load(row, i, p.vocab), w = load(other, i, p.vocab);
+            float x[kN], y[kN];
+            widen(v, x);
+            widen(w, y);
+            double p_more = 0.0, q_more = 0.0;
+            bool close = false;
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+                const double a = e(x[j]), c = f(y[j]);
+                const double more = is_more(a, c) ? 1.0 : 0.0;
+                close |= is_close(a, c);
+                p_sum += a;
+                q_sum += c;
+                p_more = fma(a, more, p_more);
+                q_more = fma(c, more, q_more);
+            }
+            double part = wave_sums(p_more, q_more);
+            double p_one = 0.0, q_one = 0.0;
+            if (__ballot(close)) {
+                int n = 0;
+#pragma unroll 1
+                for (int j = 0; j < kN; ++j) {
+                    const float x = load_any(row, DT, min(i + j, p.vocab - 1));
+                    const float y = load_any(other, DT, min(i + j, p.vocab - 1));
+                    const double a = e(x), c = f(y);
+                    const bool is = i + j < p.vocab && is_close(a, c);
+                    const uint64_t who = __ballot(is);
+                    if (!who) continue;
+                    n += __popcll(who);
+                    p_one = __shfl(a, (int)__builtin_ctzll(who));
+                    q_one = __shfl(c, (int)__builtin_ctzll(who));
+                }
+                if (n > 1) part = -1.0;
+            }
+            /* a unit's four numbers at once: p's and q's lie in the lanes' halves */
+            const int half = lane / 32, k = lane % 32;
+            if (k == 1) part = half ? q_one : p_one;
+            if (k < 2) put(&sums[4 * (int64_t)unit + 2 * k + half], part);
+        }
+        block_sums(p_sum, q_sum);
+        if (threadIdx.x == 0) {
+            put(&totals[2 * chunk], p_sum);
+            put(&totals[2 * chunk + 1], q_sum);
+        }
+        if (!last(p, b)) return -1;
+        p_sum = q_sum = 0.0;
+        for (int i = threadIdx.x; i < p.chunks.by; i += DFQ_KV_THREADS) {
+            p_sum += got(&totals[2 * i]);
+            q_sum += got(&totals[2 * i + 1]);
+        }
+        double by = 0.0, draft_by = 0.0;
+        bool known = false;
+        const auto scale = [&] {
+            if (known) return;
+            known = true;
+            block_sums(p_sum, q_sum);
+            by = 1.0 / p_sum;
+            draft_by = 1.0 / q_sum;
+        };
+        const auto rest = [&](double a, double c) {
             /* both rounded: a product fused with the difference leaves its rounding where p = q */
 #pragma clang fp contract(off)
-            return fmax(e(x) * by - f(y) * draft_by, 0.0);
-        });
-        if (token != kNone) return token;
+            return fmax(a * by - c * draft_by, 0.0);
+        };
+        struct Part {
+            double p, q, p_one, q_one;
+        };
+        const Search unit = find(p.units, [&](int i) {
+            const uint64_t* v = &sums[4 * (int64_t)i];
+            return Part{got(v), got(v + 1), got(v + 2), got(v + 3)};
+        }, [&](int i, const Part& part) {
+            scale();   /* here: units' parts are on their way meanwhile */
+            double weight = rest(part.p, part.q) + rest(part.p_one, part.q_one);
+            uint64_t close = __ballot(part.p < 0.0);
+            while (close) {
+                const int at = __shfl(i, __builtin_ctzll(close)), first = at * kUnit + lane * kN;
+                float x[kN], y[kN];
+                widen(load(row, first, p.vocab), x);
+                widen(load(other, first, p.vocab), y);
+                double sum = 0.0;
+#pragma unroll
+                for (int j = 0; j < kN; ++j) sum += rest(e(x[j]), f(y[j]));
+                sum = wave_sum(sum);
+                if (i == at) weight = sum;
+                close &= ~__ballot(i == at);
+            }
+            return weight;
+        }, 0.0, -1.0, u);
+        if (unit.place != kNone) {
+            struct Two {
+                float x, y;
+            };
+            int from = unit.place * kUnit;
+            const auto both = [&](int i) {
+                return Two{load_any(row, DT, from + i), load_any(other, DT, from + i)};
+            };
+            int place = find(min(kUnit, p.vocab - from), both, [&](int, const Two& v) {
+                return rest(e(v.x), f(v.y));
+            }, unit.front, unit.goal, u).place;
+            if (place == kNone) {
+                from = 0;   /* as in from_row */
+                place = find(p.vocab, both, [&](int, const Two& v) {
+                    return counted(rest(e(v.x), f(v.y)));
+                }, 0.0, -1.0, u).place;
+            }
+            if (place != kNone) return from + place;
+        }
         /* p = q to the last bit, and yet refused (no token of the vocabulary, or a random number
          * that is not below 1): p */
-        return find(p.vocab, [&](int i) { return e(load_any(row, DT, i)); }, 0.0, -1.0, u).place;
+        return find(p.vocab, [&](int i) { return load_any(row, DT, i); },
+                    [&](int, float x) { return counted(e(x)); }, 0.0, -1.0, u).place;
     }
 
-    template <bool WIDE>
     static __device__ __forceinline__ void weigh(const AcceptParams& p) {
         const int b = divided(blockIdx.x, p.chunks), chunk = blockIdx.x - b * p.chunks.by;
         const Sequence s = sequence_of(p, b);
         const double u = p.uniforms[(int64_t)b * p.rows + p.rows - 1];
-        const AcceptDraw d = decide<WIDE>(p, s, b, chunk == 0);
-        if (!WIDE && p.draws && chunk == 0 && threadIdx.x == 0) p.draws[b] = d;
+        const Draw d = decide(p, s, b, chunk == 0);
         int32_t* out = p.tokens + (int64_t)b * p.rows + d.row;
-        const char* row = target_row(p, b, d.row);
-        const Powers e(s.t, d.p_top);
-        if (d.mode == DFQ_DRAW_NONE) {
+        if (d.mode == kDrawNone) {
             if (chunk == 0 && threadIdx.x == 0) *out = d.token;
-        } else if (WIDE && d.mode == DFQ_DRAW_REST) {
-            const int token = from_rest(p, s, d, p.chunks.by, b, chunk, d.p_sum, d.q_sum, u);
-            if (token >= 0 && threadIdx.x == 0) *out = token;
-        } else if (d.mode == DFQ_DRAW_REST) {
-            /* both rows' sums */
-            const char* other = draft_row(p, b, d.row);
-            const Powers f(s.dt, d.q_top);
-            double p_sum = 0.0, q_sum = 0.0;
-            for (int unit = chunk * kWaves + (int)threadIdx.x / 64; unit < p.units;
-                 unit += p.chunks.by * kWaves) {
-                const int i = unit * kUnit + (int)threadIdx.x % 64 * kN;
-                const u32x4_t v = load(row, i, p.vocab), w = load(other, i, p.vocab);
-                float x[kN], y[kN];
-                widen(v, x);
-                widen(w, y);
-#pragma unroll
-                for (int j = 0; j < kN; ++j) {
-                    p_sum += e(x[j]);
-                    q_sum += f(y[j]);
-                }
-            }
-            p_sum = block_sum(p_sum);
-            q_sum = block_sum(q_sum);
-            if (threadIdx.x == 0) {
-                double* t = p.totals + 2 * ((int64_t)b * p.chunks.by + chunk);
-                t[0] = p_sum;
-                t[1] = q_sum;
-            }
+            return;
+        }
+        int token;
+        if (d.mode == kDrawRest) {
+            token = from_rest(p, s, d, b, chunk, u);
         } else {
-            const int without = d.mode == DFQ_DRAW_OTHER ? d.draft : -1;
-            const int token = drawn(p, p.chunks.by, b, chunk, row, nullptr, u,
-                                    [&](int i, float x, float) {
-                return i == without ? 0.0 : e(x);
-            });
-            /* kNone: the draft has all of p */
-            if (token >= 0 && threadIdx.x == 0) *out = token == kNone ? d.draft : token;
+            const int without = d.mode == kDrawOther ? d.draft : -1;
+            token = from_row(p, target_row(p, b, d.row), Powers(s.t, d.p_top), without, b, chunk, u);
+            if (token == kNone) token = d.draft;   /* which has all of p */
         }
-    }
-
-    static __device__ __forceinline__ void rest(const AcceptParams& p) {
-        const int b = divided(blockIdx.x, p.rest_chunks);
-        const int chunk = blockIdx.x - b * p.rest_chunks.by;
-        const AcceptDraw d = p.draws[b];
-        if (d.mode != DFQ_DRAW_REST) return;
-        const Sequence s = sequence_of(p, b);
-        const double u = p.uniforms[(int64_t)b * p.rows + p.rows - 1];
-        double p_sum = 0.0, q_sum = 0.0;
-        for (int i = threadIdx.x; i < (int)p.chunks.by; i += DFQ_KV_THREADS) {
-            const double* t = p.totals + 2 * ((int64_t)b * p.chunks.by + i);
-            p_sum += t[0];
-            q_sum += t[1];
-        }
-        p_sum = block_sum(p_sum);
-        q_sum = block_sum(q_sum);
-        const int token = from_rest(p, s, d, p.rest_chunks.by, b, chunk, p_sum, q_sum, u);
-        if (token >= 0 && threadIdx.x == 0) p.tokens[(int64_t)b * p.rows + d.row] = token;
+        if (token >= 0 && threadIdx.x == 0) *out = token;
     }
 };
 
@@ -708,11 +820,8 @@ struct Accept : LogitPiece<DT> {
         call(p);                                                                   \
     }
 #define DFQ_ACCEPT_KERNELS(name, dt)                                               \
-    DFQ_ACCEPT_KERNEL(sums, name, (Accept<dt>::sums<DFQ_ACCEPT_PIECES, false>))    \
-    DFQ_ACCEPT_KERNEL(weigh, name, (Accept<dt>::weigh<false>))                     \
-    DFQ_ACCEPT_KERNEL(rest, name, (Accept<dt>::rest))                              \
-    DFQ_ACCEPT_KERNEL(wide_sums, name, (Accept<dt>::sums<DFQ_ACCEPT_WIDE, true>))  \
-    DFQ_ACCEPT_KERNEL(wide_weigh, name, (Accept<dt>::weigh<true>))
+    DFQ_ACCEPT_KERNEL(sums, name, (Accept<dt>::sums))                              \
+    DFQ_ACCEPT_KERNEL(weigh, name, (Accept<dt>::weigh))
 DFQ_ACCEPT_KERNELS(bf16, 0)
 DFQ_ACCEPT_KERNELS(f16, 1)
 DFQ_ACCEPT_KERNELS(f32, 2)

@@ -202,7 +202,7 @@ def test_drafts_outside_the_vocabulary(ctx):
 
 @pytest.mark.parametrize("batch,vocab", [(5, 900), (3, 33000), (100, 90000)])
 def test_drafts_outside_the_vocabulary_where_p_is_q(ctx, batch, vocab):
-    """p - q is 0 throughout: the token comes from p (the last size sums rows in fp32 first)."""
+    """p - q is 0 throughout: the token comes from p."""
     s = inputs(26, batch, 2, vocab, "bf16", True)
     s["draft_logits"] = s["logits"][:, :-1].clone()
     s["draft_lengths"] = None
@@ -210,6 +210,25 @@ def test_drafts_outside_the_vocabulary_where_p_is_q(ctx, batch, vocab):
     announce(f"accept outside, p = q {batch} {vocab}")
     got = check(ctx, s)
     assert (got[1] == 0).all() and (got[0][:, 0] >= 0).all()
+
+
+@pytest.mark.parametrize("batch,vocab,size", [
+    (4, 900, 1e-6), (4, 900, 2.0 ** -16), (4, 900, 2.0 ** -14), (4, 900, 1e-2),
+    (3, 60000, 2.0 ** -16), (3, 60000, 2.0 ** -14), (3, 60000, 1e-2), (40, 50000, 1e-2)])
+def test_rests_of_nearly_equal_distributions(ctx, batch, vocab, size):
+    """Many tokens in which p is nearly q, more of them above it, below it, and equal."""
+    s = inputs(31, batch, 2, vocab, "f32", True)
+    gen = torch.Generator().manual_seed(28)
+    by = torch.randn(batch, 1, vocab, generator=gen) * size
+    by[..., ::7] = 0
+    s["draft_logits"] = s["logits"][:, :-1] + by
+    s["draft_lengths"] = None
+    s["drafts"][:] = -1
+    announce(f"accept nearly equal {batch} {vocab} {size}")
+    # two exponentials and two sums, each right to 8e-13, in a running sum and in the whole: 6.4e-12
+    # of p; what is left of p is 0.4 of the size times 6/7
+    got = check(ctx, s, margin=2e-11 / size)
+    assert (got[1] == 0).all()
 
 
 def test_the_edges_of_the_random_numbers(ctx):
@@ -232,6 +251,32 @@ def test_the_edges_of_the_random_numbers(ctx):
         s["uniforms"][:] = u
         tokens, accepted, _ = ctx.sample_accept(**on_gpu(s))
         assert ((tokens >= -1) & (tokens < 4990)).all() and tokens[1, 0] >= 17
+
+
+@pytest.mark.parametrize("vocab", [3000, 300000])
+def test_many_tokens_of_no_weight_in_front(ctx, vocab):
+    """Probabilities under 2^-1000 of the largest are 0, also where hundreds of them side by side
+    would come to more: u = 0 takes the first of the others."""
+    at = vocab - 700
+    x = torch.full((4, 2, vocab), -695.0)      # e^-695 = 2^-1002.7
+    x[..., at] = 0
+    x[..., at + 1] = -690.0                    # 2^-995.5
+    y = torch.full((4, 1, vocab), -695.0)
+    y[..., at + 300] = 2.0
+    x[2:, 0, at + 300] = 0
+    for drafts in ([at, at + 300, at, at + 300], [-1] * 4, [5] * 4):
+        for draft_logits in (None, y):
+            u = torch.zeros(4, 2)
+            u[:, 0] = 1 - 2.0 ** -24
+            announce(f"accept of no weight {vocab} {drafts}")
+            tokens, accepted, _ = ctx.sample_accept(
+                x.cuda(), u.cuda(), torch.tensor(drafts, dtype=torch.int32)[:, None].cuda(),
+                draft_logits=None if draft_logits is None else draft_logits.cuda())
+            for b in range(4):
+                n, d = int(accepted[b]), drafts[b]
+                first = at if n or draft_logits is not None or d != at else at + 1
+                assert tokens[b, n] == first, (b, n, d, tokens[b].tolist())
+                assert n == 0 or d in (at, at + 300)
 
 
 def test_a_draw_at_its_border(ctx):
@@ -458,9 +503,9 @@ def test_a_certain_draft_refused_by_a_number_past_1(ctx):
 
 @pytest.mark.parametrize("name", sorted(DTYPES))
 @pytest.mark.parametrize("border", (False, True))
-def test_calls_whose_rows_are_summed_in_fp32(ctx, name, border):
-    """More than 24 M logits with draft logits: three launches, ragged, greedy and bad rows among
-    them, and drafts next to their border, which are decided again."""
+def test_many_logits(ctx, name, border):
+    """27 M logits with draft logits, ragged, greedy and bad rows among them, and drafts next to
+    their border, which are decided again."""
     s = inputs(70, 190, 4, 20003, name, True, mixed=not border)
     if border:
         s["draft_lengths"] = None
@@ -477,8 +522,8 @@ def test_calls_whose_rows_are_summed_in_fp32(ctx, name, border):
     assert all(torch.equal(a, b) for a, b in zip(got, again))
 
 
-def test_both_ways_agree(ctx):
-    """The same sequences in one large call and in small ones, whose rows are summed otherwise."""
+def test_a_large_call_and_small_ones_agree(ctx):
+    """The same sequences in one call and in small ones, whose work is split otherwise."""
     s = on_gpu(inputs(71, 26, 5, 120011, "bf16", True))
     whole = ctx.sample_accept(**s)
     for at in range(0, 26, 9):
@@ -490,7 +535,7 @@ def test_both_ways_agree(ctx):
         assert bool((off <= CHANCE * got[2]).all())
 
 
-def test_a_captured_call_of_three_launches(ctx):
+def test_a_captured_call_with_draft_logits(ctx):
     s = on_gpu(inputs(72, 190, 4, 20003, "f16", True))
     ws = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
     ctx.sample_accept(**s)
