@@ -99,7 +99,7 @@ struct AcceptParams {
     int32_t* accepted;          /* [batch]                                         */
     float* chances;             /* [batch][rows - 1] or NULL                       */
     AcceptPart* parts;          /* [batch][rows, then draft rows][ranges]          */
-    uint64_t* sums;             /* [batch][sums_apart]: of units, one or (p - q) four; doubles' bits */
+    uint64_t* sums;             /* [batch][sums_apart]: of units, one or (p - q) six; doubles' bits */
     uint64_t* totals;           /* [batch][chunks][2]: both rows' sums, with draft logits  */
     int32_t* arrived;           /* [batch][DFQ_ACCEPT_APART]: workgroups whose sums are there */
     int64_t batch_stride, row_stride, draft_batch_stride, draft_row_stride;
@@ -107,7 +107,7 @@ struct AcceptParams {
     int rows, vocab;
     int jobs;                   /* ranges of all rows                              */
     int units;                  /* 64 lanes' 16 bytes each, of a row               */
-    int sums_apart;             /* units, four times that with draft logits        */
+    int sums_apart;             /* units, six times that with draft logits         */
     Divisor all_rows, ranges;   /* rows and draft rows of a sequence; ranges a row */
     Divisor chunks;             /* workgroups of a sequence in the second kernel   */
 };

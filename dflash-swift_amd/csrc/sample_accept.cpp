@@ -64,7 +64,7 @@ AcceptPlan plan_accept(int cus, int batch, int rows, int V, dfq_dtype dtype, boo
     a.all_rows = drafted ? 2 * rows - 1 : rows;
     const int unit = 64 * (dtype == DFQ_F32 ? 4 : 8);
     a.units = (V + unit - 1) / unit;
-    a.sums_apart = drafted ? 4 * a.units : a.units;
+    a.sums_apart = drafted ? 6 * a.units : a.units;
     const int range = unit * DFQ_ACCEPT_PIECES;
     a.ranges = (V + range - 1) / range;
     /* Workgroups of a sequence: as many units a wave as leave no more than four workgroups a CU,

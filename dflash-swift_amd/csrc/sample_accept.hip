@@ -656,9 +656,9 @@ struct Accept : LogitPiece<DT> {
      * their logits have been seen; in which tokens p is larger is known before, but for those where
      * the two are within 2^-15 of each other by the fp32 sums (off by 2^-17 at most each; four or so
      * of 151936).  So a unit's part is kept as the sums of p's and of q's exponentials over the
-     * tokens where p is surely larger, and the two of a token in between, to be scaled and
-     * subtracted when the sums are known; the last workgroup weighs units with more tokens in
-     * between again.  (Two launches instead, of both rows' sums and then of their differences,
+     * tokens where p is surely larger, and over those in between with the least and the largest of
+     * their quotients, to be scaled and subtracted when the sums are known.  The last workgroup
+     * weighs a unit again whose quotients lie to both sides of the border then.  (Two launches instead, of both rows' sums and then of their differences,
      * took 24 and 21 us for 64 sequences, this 29.)  Of a product with 0 or 1 in the sums: one
      * select instead of four. */
     static __device__ __forceinline__ int from_rest(const AcceptParams& p, const Sequence& s,
@@ -694,27 +694,31 @@ struct Accept : LogitPiece<DT> {
                 q_more = fma(c, more, q_more);
             }
             double part = wave_sums(p_more, q_more);
-            double p_one = 0.0, q_one = 0.0;
+            /* of the tokens in between: their sums, and the least and largest a / c */
+            double between = 0.0, least = __builtin_inf(), most = 0.0;
             if (__ballot(close)) {
-                int n = 0;
+                double p_between = 0.0, q_between = 0.0;
 #pragma unroll 1
                 for (int j = 0; j < kN; ++j) {
-                    const float x = load_any(row, DT, min(i + j, p.vocab - 1));
-                    const float y = load_any(other, DT, min(i + j, p.vocab - 1));
-                    const double a = e(x), c = f(y);
-                    const bool is = i + j < p.vocab && is_close(a, c);
-                    const uint64_t who = __ballot(is);
-                    if (!who) continue;
-                    n += __popcll(who);
-                    p_one = __shfl(a, (int)__builtin_ctzll(who));
-                    q_one = __shfl(c, (int)__builtin_ctzll(who));
+                    const int at = min(i + j, p.vocab - 1);
+                    const double a = e(load_any(row, DT, at)), c = f(load_any(other, DT, at));
+                    if (i + j >= p.vocab || !is_close(a, c)) continue;
+                    p_between += a;
+                    q_between += c;
+                    least = fmin(least, a / c);
+                    most = fmax(most, a / c);
                 }
-                if (n > 1) part = -1.0;
+                between = wave_sums(p_between, q_between);
+                for (int d = 1; d < 64; d *= 2) {
+                    least = fmin(least, __shfl_xor(least, d));
+                    most = fmax(most, __shfl_xor(most, d));
+                }
             }
-            /* a unit's four numbers at once: p's and q's lie in the lanes' halves */
+            /* a unit's six numbers at once: p's and q's lie in the lanes' halves */
             const int half = lane / 32, k = lane % 32;
-            if (k == 1) part = half ? q_one : p_one;
-            if (k < 2) put(&sums[4 * (int64_t)unit + 2 * k + half], part);
+            if (k == 1) part = between;
+            if (k == 2) part = half ? most : least;
+            if (k < 3) put(&sums[6 * (int64_t)unit + 2 * k + half], part);
         }
         block_sums(p_sum, q_sum);
         if (threadIdx.x == 0) {
@@ -727,7 +731,7 @@ struct Accept : LogitPiece<DT> {
             p_sum += got(&totals[2 * i]);
             q_sum += got(&totals[2 * i + 1]);
         }
-        double by = 0.0, draft_by = 0.0;
+        double by = 0.0, draft_by = 0.0, border = 0.0;
         bool known = false;
         const auto scale = [&] {
             if (known) return;
@@ -735,6 +739,7 @@ struct Accept : LogitPiece<DT> {
             block_sums(p_sum, q_sum);
             by = 1.0 / p_sum;
             draft_by = 1.0 / q_sum;
+            border = p_sum / q_sum;
         };
         const auto rest = [&](double a, double c) {
             /* both rounded: a product fused with the difference leaves its rounding where p = q */
@@ -742,15 +747,18 @@ struct Accept : LogitPiece<DT> {
             return fmax(a * by - c * draft_by, 0.0);
         };
         struct Part {
-            double p, q, p_one, q_one;
+            double p, q, p_between, q_between, least, most;
         };
         const Search unit = find(p.units, [&](int i) {
-            const uint64_t* v = &sums[4 * (int64_t)i];
-            return Part{got(v), got(v + 1), got(v + 2), got(v + 3)};
+            const uint64_t* v = &sums[6 * (int64_t)i];
+            return Part{got(v), got(v + 1), got(v + 2), got(v + 3), got(v + 4), got(v + 5)};
         }, [&](int i, const Part& part) {
             scale();   /* here: units' parts are on their way meanwhile */
-            double weight = rest(part.p, part.q) + rest(part.p_one, part.q_one);
-            uint64_t close = __ballot(part.p < 0.0);
+            /* p is larger where a / c is above p's sum over q's */
+            double weight = rest(part.p, part.q);
+            const bool above = part.least > border * (1.0 + 0x1p-48);
+            if (above && part.most > 0.0) weight += rest(part.p_between, part.q_between);
+            uint64_t close = __ballot(!above && part.most > border * (1.0 - 0x1p-48));
             while (close) {
                 const int at = __shfl(i, __builtin_ctzll(close)), first = at * kUnit + lane * kN;
                 float x[kN], y[kN];

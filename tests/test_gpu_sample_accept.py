@@ -231,6 +231,28 @@ def test_rests_of_nearly_equal_distributions(ctx, batch, vocab, size):
     assert (got[1] == 0).all()
 
 
+@pytest.mark.parametrize("name", sorted(DTYPES))
+@pytest.mark.parametrize("vocab", [900, 30000])
+@pytest.mark.parametrize("banned", ["target", "draft"])
+def test_rests_of_distributions_that_differ_in_few_tokens(ctx, name, vocab, banned):
+    """The same logits, but for a few unlikely tokens that one of the two rules out: every other
+    token's p / q is the same number next to 1, a little above or below it."""
+    s = inputs(32, 3, 2, vocab, name, True)
+    s["draft_logits"] = s["logits"][:, :-1].clone()
+    s["draft_lengths"] = None
+    s["temperature"][:] = 1.0
+    s["drafts"][:] = -1
+    s["logits"][:, 0, 5::vocab // 3] = s["draft_logits"][:, 0, 5::vocab // 3] = -1.0
+    s["logits" if banned == "target" else "draft_logits"][:, 0, 5::vocab // 3] = -math.inf
+    left = [np.maximum(distribution(s["logits"][b, 0].double().numpy(), 1.0) -
+                       distribution(s["draft_logits"][b, 0].double().numpy(), 1.0), 0).sum()
+            for b in range(3)]
+    assert max(left) < 2.0 ** -9 and (vocab == 900 or max(left) < 2.0 ** -15)
+    announce(f"accept few tokens {name} {vocab} {banned}")
+    got = check(ctx, s, margin=2 * 6.4e-12 / min(left))
+    assert (got[1] == 0).all() and (got[0][:, 0] >= 0).all()
+
+
 def test_the_edges_of_the_random_numbers(ctx):
     """0 takes any draft that can be and the first token that can be; 1 - 2^-24 the last."""
     last = 1 - 2.0 ** -24
