@@ -766,7 +766,8 @@ class Context:
         [batch, rows-1] (None where rows is 1), of which draft_lengths int32 [batch] count;
         draft_logits [batch, rows-1, V] are what they were drawn from, None where each was
         certain.  uniforms fp32 [batch, rows] are the random numbers.  Temperatures are numbers or
-        fp32 [batch]; draft_temperature defaults to temperature."""
+        fp32 [batch]; draft_temperature defaults to temperature.  Where ws gives none, a
+        captured call has a workspace of its own beside its outputs."""
         import torch
         if stream is not None and self._is_other(stream):
             with self._current(stream):
@@ -808,12 +809,26 @@ class Context:
             if ds[2] != 1 and V > 1:
                 raise ValueError("a row's draft logits must be contiguous")
             p_draft = draft_logits.data_ptr() if rows > 1 else None
-        tokens = torch.empty_like(uniforms, dtype=torch.int32)
-        accepted = torch.empty(batch, dtype=torch.int32, device=logits.device)
-        chances = torch.empty((batch, 0), dtype=torch.float32, device=logits.device) \
-            if drafts is None else torch.empty_like(drafts, dtype=torch.float32)
         code = dtype_code(logits)
         stream = self._stream_of(stream)
+        if ws is None and stream and torch.cuda.is_current_stream_capturing():
+            # The graph's own workspace: graphs that were captured on one stream may run at the same
+            # time.  It is cut from one buffer with the outputs and lives as long as they do.
+            need = ctypes.c_size_t()
+            _check(self.lib.dfq_sample_accept_workspace_bytes(
+                self.handle, batch, rows, V, code, p_draft is not None, ctypes.byref(need)),
+                "dfq_sample_accept_workspace_bytes")
+            words = -(-need.value // 16) * 4
+            ws, tokens, accepted, chances = torch.empty(
+                words + 2 * batch * rows, dtype=torch.int32, device=logits.device).split(
+                (words, batch * rows, batch, batch * (rows - 1)))
+            ws, tokens = ws.view(torch.uint8), tokens.view(batch, rows)
+            chances = chances.view(torch.float32).view(batch, rows - 1)
+        else:
+            tokens = torch.empty_like(uniforms, dtype=torch.int32)
+            accepted = torch.empty(batch, dtype=torch.int32, device=logits.device)
+            chances = torch.empty((batch, 0), dtype=torch.float32, device=logits.device) \
+                if drafts is None else torch.empty_like(drafts, dtype=torch.float32)
         own_ws = ws is None
         with self._lock if own_ws else _no_lock:
             if own_ws:

@@ -410,6 +410,31 @@ def test_captured_and_replayed(ctx):
         assert all(torch.equal(a, b) for a, b in zip(got, ctx.sample_accept(**s)))
 
 
+def test_graphs_captured_on_one_stream_run_at_once(ctx):
+    """Each has a workspace of its own, apart from the eager calls' too."""
+    side, sets, graphs = torch.cuda.Stream(), [], []
+    for n in range(2):
+        s = on_gpu(inputs(73 + n, 40, 4, 20003, "bf16", True))
+        sets.append((s, ctx.sample_accept(**s)))
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = ctx.sample_accept(**s)
+        graphs.append((graph, got))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for n in range(20):
+        for (graph, got), stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                for a in got:
+                    a.fill_(7)
+                graph.replay()
+        again = ctx.sample_accept(**sets[n % 2][0])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(again, sets[n % 2][1])), n
+        for (_, got), (_, want) in zip(graphs, sets):
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), n
+
+
 def test_two_streams_at_once(ctx):
     cases = [on_gpu(inputs(30 + i, 6, 5, 40000, "bf16", True)) for i in range(2)]
     want = [ctx.sample_accept(**s) for s in cases]
