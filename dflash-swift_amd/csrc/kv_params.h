@@ -103,6 +103,7 @@ struct AcceptParams {
     uint64_t* totals;           /* [batch][chunks][2]: both rows' sums, with draft logits  */
     int32_t* arrived;           /* [batch][DFQ_ACCEPT_APART]: workgroups whose sums are there */
     int64_t batch_stride, row_stride, draft_batch_stride, draft_row_stride;
+    double near;                /* how far the fp32 sums' p / q may be off, of itself */
     float temperature, draft_temperature;
     int rows, vocab;
     int jobs;                   /* ranges of all rows                              */

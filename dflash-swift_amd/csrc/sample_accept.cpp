@@ -157,6 +157,9 @@ dfq_status dfq_sample_accept(dfq_ctx* ctx, const void* logits, int64_t batch_str
     p.row_stride = row_stride;
     p.draft_batch_stride = draft_batch_stride;
     p.draft_row_stride = draft_row_stride;
+    int bits = 0;
+    while ((V - 1) >> bits) ++bits;
+    p.near = (drafted ? 2 : 1) * (1.75 * bits + 21.0) * 0x1p-24;   /* sample_accept.hip's bound */
     p.temperature = temperature;
     p.draft_temperature = draft_temperature;
     p.rows = rows;

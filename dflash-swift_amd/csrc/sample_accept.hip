@@ -10,12 +10,12 @@
  *
  * Tokens and counts are whole numbers that a sum's last bits decide, and come out as 64-bit
  * arithmetic has them (exponentials to 8e-13): draws sum and search in 64 bits, and a draft whose
- * u q is within 2^-16 of p is decided again from 64-bit sums.  Other drafts need no more than fp32,
- * in which a logit costs 8 instructions against 20: all rows of 64 sequences of seven drafts of
- * 151936 tokens in 64 bits took 93 us for 43.  An fp32 sum is off by less than 2^-17 / 2 of itself:
- * an exponent a has three roundings, 2.5 2^-24 |a|, and the mean of |a| over a row's mass is at most
- * log2 V, which makes 34 2^-24 for 2^20 tokens and 52 for 2^30; 13 sums in a row and the
- * exponential's last bits are 20 more.
+ * u q is as near to p as fp32 sums may be wrong is decided again from 64-bit ones.  Other drafts
+ * need no more than fp32, in which a logit costs 8 instructions against 20: all rows of 64 sequences
+ * of seven drafts of 151936 tokens in 64 bits took 93 us for 43.  An fp32 sum is off by less than
+ * (7/4 log2 V + 20) 2^-24 of itself: an exponent a of 2 has three roundings, 2.5 2^-24 |a|, which
+ * change its power by that times ln 2, and the mean of |a| over a row's mass is at most log2 V; 13
+ * sums in a row and the exponential's last bits are the 20.
  *
  * The first launch reads all rows once: a wave takes a range of one row in registers, finds its
  * largest logit and the sum of e^((x - largest) / T).  In the second each workgroup joins its
@@ -477,12 +477,19 @@ struct Accept : LogitPiece<DT> {
     static __device__ __noinline__ double whole_row(const char* row, int vocab, float top,
                                                     float t) {
         const Powers e(t, top);
+        constexpr int kOnce = 4, kStep = DFQ_KV_THREADS * kN;   /* loads on their way together */
         double sum = 0.0;
-        for (int i = threadIdx.x * kN; i < vocab; i += DFQ_KV_THREADS * kN) {
-            float x[kN];
-            widen(load(row, i, vocab), x);
+        for (int from = threadIdx.x * kN; from < vocab; from += kOnce * kStep) {
+            u32x4_t v[kOnce];
 #pragma unroll
-            for (int j = 0; j < kN; ++j) sum += e(x[j]);
+            for (int k = 0; k < kOnce; ++k) v[k] = load(row, from + k * kStep, vocab);
+#pragma unroll
+            for (int k = 0; k < kOnce; ++k) {
+                float x[kN];
+                widen(v[k], x);
+#pragma unroll
+                for (int j = 0; j < kN; ++j) sum += e(x[j]);
+            }
         }
         return block_sum(sum);
     }
@@ -550,11 +557,11 @@ struct Accept : LogitPiece<DT> {
             }
             known = known && lane < s.drafts;
             const uint64_t near =
-                __ballot(known && mine > 0.0 && fabs(u * theirs - mine) < 0x1p-16 * mine);
+                __ballot(known && mine > 0.0 && fabs(u * theirs - mine) < p.near * mine);
             if (lane == 0) again = near;
         }
         __syncthreads();
-        /* drafts next to the border: fewer than one in ten thousand */
+        /* drafts next to the border: one in a hundred thousand or so */
         for (uint64_t near = again; near; near &= near - 1) {
             const int i = __builtin_ctzll(near);
             double p_sum = 0.0, q_sum = 0.0;
@@ -654,8 +661,7 @@ struct Accept : LogitPiece<DT> {
 
     /* A token drawn from max(p - q, 0), as from_row.  The rows' sums in 64 bits are known when all
      * their logits have been seen; in which tokens p is larger is known before, but for those where
-     * the two are within 2^-15 of each other by the fp32 sums (off by 2^-17 at most each; four or so
-     * of 151936).  So a unit's part is kept as the sums of p's and of q's exponentials over the
+     * the two are as near to each other as fp32 sums may be wrong (one or two of 151936).  So a unit's part is kept as the sums of p's and of q's exponentials over the
      * tokens where p is surely larger, and over those in between with the least and the largest of
      * their quotients, to be scaled and subtracted when the sums are known.  The last workgroup
      * weighs a unit again whose quotients lie to both sides of the border then.  (Two launches instead, of both rows' sums and then of their differences,
@@ -670,9 +676,9 @@ struct Accept : LogitPiece<DT> {
         const double ratio = uniform(d.q_sum / d.p_sum);
         uint64_t* sums = p.sums + (int64_t)b * p.sums_apart;
         uint64_t* totals = p.totals + 2 * (int64_t)b * p.chunks.by;
-        const auto is_more = [&](double a, double c) { return fma(a, ratio, -c) > c * 0x1p-15; };
+        const auto is_more = [&](double a, double c) { return fma(a, ratio, -c) > c * p.near; };
         const auto is_close = [&](double a, double c) {
-            return fabs(fma(a, ratio, -c)) <= c * 0x1p-15 && a > kNothing;
+            return fabs(fma(a, ratio, -c)) <= c * p.near && a > kNothing;
         };
         double p_sum = 0.0, q_sum = 0.0;
         for (int unit = chunk * kWaves + wave; unit < p.units; unit += p.chunks.by * kWaves) {

@@ -491,7 +491,7 @@ dfq_status dfq_token_logprobs(dfq_ctx* ctx, const void* logits, int64_t row_stri
  * A token is drawn as the first whose running sum of probabilities exceeds u[b][rows-1] times their
  * sum.  uniforms u [batch][rows] are in [0, 1) and the caller's, so that a call with the same
  * numbers gives the same tokens, distributed as p (counts and tokens are those of 64-bit sums, with
- * exponentials to 8e-13; chances are right to 2^-17 of themselves).  temperatures and
+ * exponentials to 8e-13; chances are right to 2^-16 of themselves).  temperatures and
  * draft_temperatures [batch] are in device memory; NULL: `temperature`, `draft_temperature` for
  * all.  T = 0 takes p = 1 for the row's argmax, as dfq_argmax_accept finds it.  A logit of -inf has
  * probability 0, as have probabilities under 2^-1000 of the row's largest.  A row with a NaN or
