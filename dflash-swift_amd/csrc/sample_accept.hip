@@ -35,7 +35,7 @@
 namespace {
 
 constexpr int kWaves = DFQ_KV_THREADS / 64;
-constexpr double kLog2e = 1.44269504088896340736;
+constexpr double kLog2e = 1.44269504088896340736, kLn2 = 0.693147180559945309417;
 constexpr int kNone = 0x7fffffff;
 
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
@@ -70,14 +70,13 @@ __device__ __forceinline__ double power(double d, double rate, double least) {
 
 /* Temperatures below the least normal number are taken for it: their reciprocal is finite, and
  * the logits' differences pass any exponent with either. */
-__device__ __forceinline__ double rate_of(float t) {
-    return kLog2e / (double)fmaxf(t, 1.17549435e-38f);
-}
+__device__ __forceinline__ double at_least(float t) { return (double)fmaxf(t, 1.17549435e-38f); }
+__device__ __forceinline__ double rate_of(float t) { return kLog2e / at_least(t); }
 /* A row's exponentials: of its logits x, 2^((x - top) rate). */
 struct Powers {
     double rate, least, top;
     __device__ __forceinline__ Powers(float t, float largest)
-        : rate(rate_of(t)), least(-1022.0 / rate), top(largest) {}
+        : rate(rate_of(t)), least(-1022.0 * kLn2 * at_least(t)), top(largest) {}
     __device__ __forceinline__ double operator()(float x) const {
         return power((double)x - top, rate, least);
     }
@@ -187,16 +186,25 @@ __device__ __forceinline__ void block_sums(double& a, double& b) {
     __syncthreads();
 }
 
-/* The sum over the threads in front of this one; `all` gets that over all. */
+__device__ __forceinline__ double of_lane(double v, int lane) {
+    const u32x2_t w = __builtin_bit_cast(u32x2_t, v);
+    return __builtin_bit_cast(double, u32x2_t{(uint32_t)__builtin_amdgcn_readlane(w[0], lane),
+                                              (uint32_t)__builtin_amdgcn_readlane(w[1], lane)});
+}
+
+/* The sum over the threads in front of this one; `all` gets that over all.  The caller has a barrier
+ * before the next call. */
 __device__ __forceinline__ double block_before(double v, double& all) {
     __shared__ double waves[kWaves];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    /* running sums within rows of 16 lanes, by DPP's shifts, then the rows in front */
     double run = v;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const double o = __shfl_up(run, d);
-        if (lane >= d) run += o;
-    }
+    run += dpp_f64<0x111>(run);
+    run += dpp_f64<0x112>(run);
+    run += dpp_f64<0x114>(run);
+    run += dpp_f64<0x118>(run);
+    const double one = of_lane(run, 15), two = one + of_lane(run, 31), three = two + of_lane(run, 47);
+    run += lane < 16 ? 0.0 : lane < 32 ? one : lane < 48 ? two : three;
     if (lane == 63) waves[wave] = run;
     __syncthreads();
     double before = 0.0;
@@ -206,7 +214,6 @@ __device__ __forceinline__ double block_before(double v, double& all) {
         if (w < wave) before += waves[w];
         all += waves[w];
     }
-    __syncthreads();
     return before + (run - v);
 }
 
@@ -288,7 +295,6 @@ __device__ __forceinline__ Search find(int n, Fetch fetch, Weight weight, double
         }
         from = s.front;
         goal = s.goal;
-        __syncthreads();
     }
 }
 
