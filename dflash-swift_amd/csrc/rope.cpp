@@ -45,6 +45,29 @@ struct RotationOps : LoadedOps {
 
 constexpr double kTurn = 6.28318530717958647692528676655900577;
 
+/* f / (2 pi) mod 1 in units of 2^-64, to the nearest: f = m 2^e, m a whole number of 53 bits, times
+ * 1 / (2 pi) in units of 2^-256, whose rounding is less than 2^-129 turns of any |f| < 2^127.  (A
+ * quotient of 64 bits, its whole turns dropped afterwards, loses as many bits as they have.) */
+uint64_t turn_of(double f) {
+    static constexpr uint64_t kOverTurn[4] = {0x7f9458eaf7aef158ull, 0x36d8a5664f10e410ull,
+                                              0x7f09d5f47d4d3770ull, 0x28be60db9391054aull};
+    int e;
+    const uint64_t m = (uint64_t)std::ldexp(std::frexp(std::fabs(f), &e), 53);
+    uint64_t product[5], carry = 0;   /* in units of 2^(e - 309) turns */
+    for (int i = 0; i < 4; ++i) {
+        const unsigned __int128 v = (unsigned __int128)m * kOverTurn[i] + carry;
+        product[i] = (uint64_t)v;
+        carry = (uint64_t)(v >> 64);
+    }
+    product[4] = carry;
+    const auto bit = [&](int at) { return at < 0 || at > 319 ? 0 : product[at / 64] >> at % 64 & 1; };
+    const int from = 245 - e;         /* the bit of 2^-64 turns */
+    uint64_t turn = 0;
+    for (int i = 63; i >= 0; --i) turn = turn << 1 | bit(from + i);
+    turn += bit(from - 1);
+    return f < 0 ? 0 - turn : turn;
+}
+
 bool good(double v) { return v > 0 && std::isfinite(v); }
 
 dfq_status check_heads(const dfq_heads* t, const char* name, dfq_dtype dtype) {
@@ -211,13 +234,9 @@ dfq_status dfq_rope_turns(const double* frequencies, int count, uint64_t* turns)
     if (!frequencies || !turns) return fail(DFQ_ERR_INVALID_ARGUMENT, "null argument");
     if (count < 1) return fail(DFQ_ERR_INVALID_ARGUMENT, "count must be >= 1");
     for (int i = 0; i < count; ++i) {
-        if (!std::isfinite(frequencies[i]))
-            return fail(DFQ_ERR_INVALID_ARGUMENT, "frequency %d is not finite", i);
-        /* a double's 53 bits over 2 pi in the 64 of a long double, its whole turns dropped */
-        const long double turn = (long double)frequencies[i] / 6.28318530717958647692528676655900577L;
-        const long double part = turn - std::floor(turn);
-        const long double scaled = std::floor(part * 18446744073709551616.0L + 0.5L);
-        turns[i] = scaled >= 18446744073709551616.0L ? 0 : (uint64_t)scaled;
+        if (!(std::fabs(frequencies[i]) < 0x1p127))
+            return fail(DFQ_ERR_INVALID_ARGUMENT, "frequency %d is not under 2^127", i);
+        turns[i] = turn_of(frequencies[i]);
     }
     return DFQ_OK;
 }

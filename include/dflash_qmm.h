@@ -384,7 +384,7 @@ dfq_status dfq_cache_attention(dfq_ctx* ctx, const dfq_kv_cache* prefix, int pre
  * (a, b) -> amplitude * (a cos - b sin, b cos + a sin).  Pair i is (i, i + rotary_dim/2) or,
  * interleaved, (2i, 2i + 1); the channels behind rotary_dim stay as they are.  `turns` (device
  * memory, 8-byte aligned) are the frequencies as fractions of a turn in units of 2^-64
- * (dfq_rope_turns), so that an angle is right to 2^-32 turns at every position.  The reference's
+ * (dfq_rope_turns), so that an angle is right to 2^-31 turns at every position.  The reference's
  * target rotates its queries and keys in the model library (mlx-swift-lm), between the projections
  * that the swap replaces (Sources/DFlashKit/SmallMQuantizedMatmul.swift:303-317). */
 typedef struct dfq_rope_table {
@@ -416,7 +416,8 @@ typedef struct dfq_rope_desc {
 /* Host only: frequencies[rotary_dim/2] in radians a position, and the amplitude (may be NULL).
  * Fields that the scaling does not use are not looked at. */
 dfq_status dfq_rope_frequencies(const dfq_rope_desc* desc, double* frequencies, float* amplitude);
-/* Host only: any finite frequencies as turns in host memory, to be copied to the device. */
+/* Host only: frequencies (of less than 2^127) as turns in host memory, each right to half of its
+ * last unit, to be copied to the device. */
 dfq_status dfq_rope_turns(const double* frequencies, int count, uint64_t* turns);
 
 /* The heads of one tensor, channels side by side: channel 0 of head h of row m of sequence b is
