@@ -81,6 +81,19 @@ struct Powers {
         return power((double)x - top, rate, least);
     }
 };
+/* The same exponents (x - top) rate in fp32.  Logits may lie further apart than fp32 reaches, which
+ * counts where a temperature is as large: there both are taken 2^-8 fold, exactly. */
+struct Exponents {
+    float fold, rate;
+    __device__ __forceinline__ Exponents(float t) {
+        const bool large = t > 0x1p100f;
+        fold = large ? 0x1p-8f : 1.0f;
+        rate = (float)(rate_of(t) * (large ? 0x1p8 : 1.0));
+    }
+    __device__ __forceinline__ float operator()(float x, float top) const {
+        return fmaf(x, fold, -(top * fold)) * rate;
+    }
+};
 __device__ __forceinline__ bool is_temperature(float t) {
     return t >= 0.0f && t < __builtin_inff();
 }
@@ -391,7 +404,7 @@ struct Accept : LogitPiece<DT> {
             top = wave_of(top, [](float a, float c) { return larger(a, c); });
             part.top = top;
             if (fabsf(top) < __builtin_inff()) {
-                const float rate = (float)rate_of(t);
+                const Exponents exponent(t);
                 float sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i) {
@@ -399,7 +412,7 @@ struct Accept : LogitPiece<DT> {
                     widen(v[i], x);
 #pragma unroll
                     for (int j = 0; j < kN; ++j)
-                        x[j] = __builtin_amdgcn_exp2f((x[j] - top) * rate);
+                        x[j] = __builtin_amdgcn_exp2f(exponent(x[j], top));
                     /* in pairs: fewer roundings in a row */
 #pragma unroll
                     for (int d = kN / 2; d; d /= 2)
@@ -419,9 +432,9 @@ struct Accept : LogitPiece<DT> {
         const int lane = threadIdx.x % 16, n = p.ranges.by;
         const int64_t first = ((int64_t)b * p.all_rows.by + r) * n;
         Row row = {-__builtin_inff(), kNone, 0.0};
-        const float rate = (float)rate_of(t);
+        const Exponents exponent(t);
         const auto factor = [&](float from, float to) -> double {
-            return __builtin_amdgcn_exp2f((from - to) * rate);
+            return __builtin_amdgcn_exp2f(exponent(from, to));
         };
         constexpr int kOnce = 4;   /* loads on their way together */
         for (int from = 0; from < n; from += 16 * kOnce) {
