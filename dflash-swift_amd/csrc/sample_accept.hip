@@ -68,30 +68,29 @@ __device__ __forceinline__ double power(double d, double rate, double least) {
     return __builtin_bit_cast(double, w);
 }
 
-/* Temperatures below the least normal number are taken for it: their reciprocal is finite, and
- * the logits' differences pass any exponent with either. */
-__device__ __forceinline__ double at_least(float t) { return (double)fmaxf(t, 1.17549435e-38f); }
-__device__ __forceinline__ double rate_of(float t) { return kLog2e / at_least(t); }
+__device__ __forceinline__ double rate_of(float t) { return kLog2e / t; }
 /* A row's exponentials: of its logits x, 2^((x - top) rate). */
 struct Powers {
     double rate, least, top;
     __device__ __forceinline__ Powers(float t, float largest)
-        : rate(rate_of(t)), least(-1022.0 * kLn2 * at_least(t)), top(largest) {}
+        : rate(rate_of(t)), least(-1022.0 * kLn2 * t), top(largest) {}
     __device__ __forceinline__ double operator()(float x) const {
         return power((double)x - top, rate, least);
     }
 };
 /* The same exponents (x - top) rate in fp32.  Logits may lie further apart than fp32 reaches, which
- * counts where a temperature is as large: there both are taken 2^-8 fold, exactly. */
+ * counts where a temperature is as large: there both are taken 2^-8 fold, exactly.  The rate of a
+ * temperature under the least normal number has no room in fp32: 2^23 of it go to the difference. */
 struct Exponents {
-    float fold, rate;
+    float fold, lift, rate;
     __device__ __forceinline__ Exponents(float t) {
-        const bool large = t > 0x1p100f;
+        const bool large = t > 0x1p100f, small = t < 0x1p-126f;
         fold = large ? 0x1p-8f : 1.0f;
-        rate = (float)(rate_of(t) * (large ? 0x1p8 : 1.0));
+        lift = small ? 0x1p23f : 1.0f;
+        rate = (float)(rate_of(t) * (large ? 0x1p8 : small ? 0x1p-23 : 1.0));
     }
     __device__ __forceinline__ float operator()(float x, float top) const {
-        return fmaf(x, fold, -(top * fold)) * rate;
+        return fmaf(x, fold, -(top * fold)) * lift * rate;
     }
 };
 __device__ __forceinline__ bool is_temperature(float t) {

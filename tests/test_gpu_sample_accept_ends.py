@@ -52,6 +52,21 @@ def test_wide_logits_over_many_ranges(ctx, name, drafted):
 
 
 @pytest.mark.parametrize("drafted", (False, True))
+@pytest.mark.parametrize("name,step,temperature", [
+    ("f32", 2.0 ** -149, 40 * 2.0 ** -149), ("f32", 2.0 ** -149, 2.0 ** -149),
+    ("f32", 2.0 ** -140, 1e-41), ("bf16", 2.0 ** -133, 30 * 2.0 ** -133),
+    ("bf16", 2.0 ** -133, 1e-38)])
+def test_logits_as_small_as_their_temperature(ctx, name, step, temperature, drafted):
+    """Temperatures and logits below the least normal number."""
+    announce(f"accept small {name} {step} {temperature} {drafted}")
+    s = inputs(82, 6, 4, 700, name, drafted)
+    spread_evenly(s, -100 * step, step, name)
+    s["temperature"] = torch.full((6,), temperature)
+    assert (s["temperature"] > 0).all() and s["logits"].float().unique().numel() > 100
+    check(ctx, s)
+
+
+@pytest.mark.parametrize("drafted", (False, True))
 @pytest.mark.parametrize("name", ("bf16", "f32"))
 @pytest.mark.parametrize("temperature", [2.0 ** -149, 1e-40, 2.0 ** -126])
 def test_large_logits_at_the_least_temperatures(ctx, name, temperature, drafted):
