@@ -199,10 +199,11 @@ __device__ __forceinline__ void rotate_heads(const RopeParams& p) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum = fmaf(x[0][i], x[0][i], fmaf(x[1][i], x[1][i], sum));
             const float scale = rsqrtf(head_sum(sum, p.lanes) / (float)p.dim + p.eps);
+            /* first the factor of the head, whose product with a weight fp32 need not hold */
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                x[0][i] *= scale * w[0][i];
-                x[1][i] *= scale * w[1][i];
+                x[0][i] = x[0][i] * scale * w[0][i];
+                x[1][i] = x[1][i] * scale * w[1][i];
             }
         }
         /* channels behind the rotated ones stay as they are, infinities and NaN among them */
