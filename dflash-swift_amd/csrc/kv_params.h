@@ -114,6 +114,7 @@ struct AcceptParams {
 };
 
 #define DFQ_ROPE_DIM 512     /* widest head */
+#define DFQ_NORM_SMALL 0x1p-100f   /* mean square and eps from which on fp32 squares serve */
 
 struct RopeTensor {
     const void* in;

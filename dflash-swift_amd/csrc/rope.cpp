@@ -21,18 +21,19 @@ namespace {
 struct RotationOps : LoadedOps {
     static constexpr OpsGroup kGroup = kRotationOps;
     hipModule_t module = nullptr;
-    hipFunction_t rotate[2][3][3] = {};  // [alone/with norms][halves/pairs/any][bf16/f16/f32]
+    /* [alone/with norms/with norms of a small eps][halves/pairs/any][bf16/f16/f32] */
+    hipFunction_t rotate[3][3][3] = {};
     dfq_status resolve() {
         static const char* kDt[3] = {"bf16", "f16", "f32"};
         static const char* kWay[3] = {"halves", "pairs", "any"};
+        static const char* kOp[3] = {"rope", "norm_rope", "norm_small_rope"};
         hipError_t e = hipModuleLoadData(&module, dfq_rope_hsaco);
         if (e != hipSuccess) return hip_error(e, "hipModuleLoadData(gfx950 rotation object)");
         char name[80];
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < 3; ++n)
             for (int w = 0; w < 3; ++w)
                 for (int t = 0; t < 3; ++t) {
-                    snprintf(name, sizeof name, "dfq_%s_%s_%s", n ? "norm_rope" : "rope", kWay[w],
-                             kDt[t]);
+                    snprintf(name, sizeof name, "dfq_%s_%s_%s", kOp[n], kWay[w], kDt[t]);
                     if ((e = hipModuleGetFunction(&rotate[n][w][t], module, name)) != hipSuccess)
                         return hip_error(e, name);
                 }
@@ -173,9 +174,10 @@ dfq_status rotate(dfq_ctx* ctx, const dfq_rope_table* rope, const dfq_heads* q, 
     if ((s = ops_of(ctx, &ops))) return s;
     DeviceScope scope(ctx);
     void* args[] = {&p};
+    const int op = !norms ? 0 : norms->eps < DFQ_NORM_SMALL ? 2 : 1;
     const hipError_t e = hipModuleLaunchKernel(
-        ops->rotate[norms != nullptr][way][(int)dtype], (unsigned)(q_groups + k_groups), 1, 1,
-        DFQ_KV_THREADS, 1, 1, 0, (hipStream_t)stream, args, nullptr);
+        ops->rotate[op][way][(int)dtype], (unsigned)(q_groups + k_groups), 1, 1, DFQ_KV_THREADS,
+        1, 1, 0, (hipStream_t)stream, args, nullptr);
     return e == hipSuccess ? DFQ_OK : hip_error(e, what);
 }
 

@@ -41,3 +41,29 @@ def test_weights_that_are_far_from_their_heads(ctx, name, dim, rotary, interleav
         for kind in (DTYPES[name], torch.float32):
             normed(ctx, (q * size).to(DTYPES[name]), (w * weight).to(kind), 0.0, rotary,
                    interleaved)
+
+
+@pytest.mark.parametrize("interleaved", (False, True))
+@pytest.mark.parametrize("dim,rotary", WIDTHS)
+@pytest.mark.parametrize("name", sorted(DTYPES))
+def test_heads_whose_squares_are_no_normal_numbers(ctx, name, dim, rotary, interleaved):
+    """Down to the type's least number with an eps of nearly nothing, beside ordinary heads."""
+    announce(f"norms small {name} {dim} {rotary} {interleaved}")
+    dt = DTYPES[name]
+    f = torch.finfo(dt)
+    least = f.smallest_normal * f.eps
+    gen = torch.Generator(device="cuda").manual_seed(32)
+    q = torch.randn(1, 6, 5, dim, device="cuda", generator=gen)
+    w = torch.randn(dim, device="cuda", generator=gen).to(dt)
+    size = torch.tensor([1.0, 1e-15, 1e-19, 1e-21, 1e-30, 0.0]).cuda()
+    if name == "f16":
+        size = torch.tensor([1.0, 1e-3, 1e-4, 1e-5, 1e-6, 0.0]).cuda()
+    q = (q * size[:, None, None]).to(dt)
+    q[:, 5] = 3 * least
+    q[:, :, 1] = 1.5          # neighbours in the same waves
+    q[:, 2, 4] = 1e4
+    # a head that rounds to zeros has no norm with an eps of 0
+    q[..., 0] = torch.where(q[..., 0] == 0, 3 * least, q[..., 0].double()).to(dt)
+    for eps in (0.0, 1e-42, 1e-38, 3e-31):
+        for weight in (w, None):
+            normed(ctx, q, weight, eps, rotary, interleaved)
