@@ -811,7 +811,7 @@ class Context:
             p_draft = draft_logits.data_ptr() if rows > 1 else None
         code = dtype_code(logits)
         stream = self._stream_of(stream)
-        if ws is None and stream and torch.cuda.is_current_stream_capturing():
+        if ws is None and stream and self._is_capturing():
             # The graph's own workspace: graphs that were captured on one stream may run at the same
             # time.  It is cut from one buffer with the outputs and lives as long as they do.
             need = ctypes.c_size_t()
@@ -859,6 +859,15 @@ class Context:
 
     def _is_other(self, stream) -> bool:
         return (_stream(stream) or 0) != _current_stream(self.device)
+
+    def _is_capturing(self) -> bool:
+        """Whether torch's current stream of this context's GPU, which need not be the current GPU,
+        is being captured."""
+        import torch
+        if torch.cuda.current_device() == self.device:
+            return torch.cuda.is_current_stream_capturing()
+        with torch.cuda.device(self.device):
+            return torch.cuda.is_current_stream_capturing()
 
     def _current(self, stream):
         """torch.cuda.stream of a launch's stream: what the call allocates is that stream's, so that
