@@ -494,10 +494,12 @@ dfq_status dfq_token_logprobs(dfq_ctx* ctx, const void* logits, int64_t row_stri
  * numbers gives the same tokens, distributed as p (counts and tokens are those of 64-bit sums, with
  * exponentials to 8e-13; chances are right to 2^-16 of themselves).  temperatures and
  * draft_temperatures [batch] are in device memory; NULL: `temperature`, `draft_temperature` for
- * all.  T = 0 takes p = 1 for the row's argmax, as dfq_argmax_accept finds it.  A logit of -inf has
- * probability 0, as have probabilities under 2^-1000 of the row's largest.  A row with a NaN or
- * +inf, with nothing above -inf, or with a temperature of its sequence that is negative or not
- * finite has no distribution: a draft judged by such a row of the target or the draft is refused
+ * all.  T = 0 takes p = 1 for the row's argmax, as dfq_argmax_accept finds it: NaN is passed over,
+ * +inf is the largest, and a row of -inf throughout gives its first token.  Draft rows are not looked
+ * at where Td is 0.  A logit of -inf has probability 0 at T > 0, as have probabilities under 2^-1000
+ * of the row's largest.  No distribution has a row of NaN throughout at T = 0; at T > 0 one with a
+ * NaN or +inf, or with nothing above -inf; and any whose sequence's temperature is negative or not
+ * finite.  A draft judged by such a row of the target or the draft is refused
  * (chance 0), and the token in its place is -1.  So is refused a draft outside 0..V-1 (the token is
  * then drawn as for q = 0 in all of p, or from p - q).  Strides are in elements, logits of a row
  * side by side; sequences or rows may share logits (a stride of 0).  Outputs and workspace overlap
