@@ -12,10 +12,15 @@
  * arithmetic has them (exponentials to 8e-13): draws sum and search in 64 bits, and a draft whose
  * u q is as near to p as fp32 sums may be wrong is decided again from 64-bit ones.  Other drafts
  * need no more than fp32, in which a logit costs 8 instructions against 20: all rows of 64 sequences
- * of seven drafts of 151936 tokens in 64 bits took 93 us for 43.  An fp32 sum is off by less than
- * (7/4 log2 V + 20) 2^-24 of itself: an exponent a of 2 has three roundings, 2.5 2^-24 |a|, which
- * change its power by that times ln 2, and the mean of |a| over a row's mass is at most log2 V; 13
- * sums in a row and the exponential's last bits are the 20.
+ * of seven drafts of 151936 tokens in 64 bits took 93 us for 43.
+ *
+ * An fp32 sum is off by less than (7/4 log2 V + 20) 2^-24 of itself.  An exponent a of 2 has three
+ * roundings (rate, difference, product) of up to 2^-24 |a| each, which change its power by
+ * 3 ln 2 |a| 2^-24, and so the sum by the mean of that over the row's mass.  The mean of |a| is largest
+ * where all tokens but the largest are alike, W((V-1)/e) / ln 2 with Lambert's W: its 3 W((V-1)/e) is
+ * below 7/4 log2 V for any V up to 2^30 (26.3 for 30.1 at 151936 tokens, 50.9 for 52.5 at the most).
+ * 13 sums in a row and the last bits of three exponentials (a token's, and the factors that join ranges)
+ * are 19 more.
  *
  * The first launch reads all rows once: a wave takes a range of one row in registers, finds its
  * largest logit and the sum of e^((x - largest) / T).  In the second each workgroup joins its
