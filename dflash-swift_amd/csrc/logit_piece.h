@@ -5,11 +5,9 @@
 #ifndef DFQ_LOGIT_PIECE_H
 #define DFQ_LOGIT_PIECE_H
 
-#include "qmm_device.h"
+#include "kv_device.h"
 
 namespace {
-
-typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
 template <int DT>
 struct LogitPiece {

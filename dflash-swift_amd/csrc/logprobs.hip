@@ -16,7 +16,6 @@
  * whose candidates are issue-bound work between the loads.  Few rows: two launches, 8 rows with 5
  * alternatives 7.3 and 4.3 us.
  */
-#include "kv_params.h"
 #include "logit_piece.h"
 
 namespace {

@@ -17,17 +17,17 @@
  * Bound by memory where there are many rows, and by the launch where there are few.  A pair's angle
  * costs 30 instructions, so that a lane turns up to 16 heads of its token by the same ones, the next
  * head's channels on their way meanwhile; outputs go past the caches.  8192 rows of 40 + 8 heads of
- * 128 in bf16, cut from fused rows (201 MB): 39.6 us (5.1 TB/s, a large copy's rate), with norms
- * 40.7.  One head a lane took 57 us, up to 8 of them with plain stores 45.  One row of 8 sequences
- * 4.0 us, 8 rows with norms 4.5, 1665 rows of 18 heads of 256 with a quarter rotated 9.7 (31 MB).
+ * 128 in bf16, cut from fused rows (201 MB): 39.5 us (5.1 TB/s, a large copy's rate), with norms
+ * 40.5.  One head a lane took 57 us, up to 8 of them with plain stores 45.  One row of 8 sequences
+ * 4.0 us, 8 rows with norms 4.6, 1665 rows of 18 heads of 256 with a quarter rotated 9.8 (31 MB).
+ *
+ * Stores past the caches have little effect on the kernels that read the outputs next.  Norms, cache
+ * append and attention over 300 to 500 tokens with plain stores, then with these: 8 rows 18.4 and 18.5
+ * us, 16 sequences of 8 rows 24.2 and 24.3, 64 of 8 rows 40.7 and 40.3, 64 of 16 rows 97.0 and 98.2.
  */
-#include "kv_params.h"
-#include "qmm_device.h"
+#include "kv_device.h"
 
 namespace {
-
-/* 16 bytes at any element's address (heads cut from a fused projection have any offset). */
-typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
 /* Two numbers to nearest even, the first in the low half. */
 template <bool F16>
@@ -77,7 +77,8 @@ __device__ __forceinline__ void turn(float& a, float& b, float sine, float cosin
     b = b * cosine + c * sine;
 }
 
-/* 8 neighbouring elements, as they lie in memory and as fp32. */
+/* 8 neighbouring elements, as they lie in memory (heads cut from a fused projection have any offset)
+ * and as fp32. */
 template <int DT>
 struct Chunk {
     static constexpr int kSize = DT == 2 ? 4 : 2, kWords = kSize / 2;
@@ -110,10 +111,6 @@ struct Chunk {
         }
     }
 };
-
-__device__ __forceinline__ int divided(int n, const Divisor& d) {
-    return (int)((n + (uint64_t)((uint64_t)(uint32_t)n * d.mul >> 32)) >> d.shift);
-}
 
 /* The sum over the `lanes` (a power of two) that hold a head. */
 __device__ __forceinline__ float head_sum(float v, int lanes) {
@@ -258,7 +255,12 @@ __device__ __forceinline__ void rotate_heads(const RopeParams& p) {
     }
 }
 
-/* Any even head and any number of pairs: a wave a head, a lane a pair at a time. */
+/* Any even head and any number of pairs: a wave a head, a lane a pair at a time.
+ *
+ * Bound by instructions: a wave finds its head's angles and addresses for itself, and its lanes take
+ * an element at a time.  8192 rows of 40 + 8 heads of 80 with 20 or 40 channels rotated take 103 us in
+ * bf16 (126 MB, 1.2 TB/s) and 109 in fp32 (twice the bytes), with norms 133 in both; heads of 96 with
+ * 24 rotated 106 and 114, with norms 135 and 138. */
 template <int DT, int NORM>
 __device__ __forceinline__ void rotate_any(const RopeParams& p) {
     const int lane = threadIdx.x % 64;

@@ -29,12 +29,12 @@
  * A draw from p - q needs no third launch either, though its terms are known only when both rows
  * have been summed: nearly all tokens' signs are, from the fp32 sums (from_rest).
  *
- * 64 sequences of seven sampled drafts of 151936 tokens in bf16: 72 us in all.  The sums take 43
- * (254 MB, 5.9 TB/s) and the draws 29, of which vector instructions are some 18 and the rest what the
- * launch's start, its decisions and its last workgroup take.  16 sequences 29.3 us, one block of
- * seven certain drafts 12.3, 33 plain draws from 50257 logits in fp32 13.9.
+ * 64 sequences of seven sampled drafts of 151936 tokens in bf16: 73 us a call where calls follow each
+ * other in a graph.  Launches traced one by one, the sums take 43.8 (254 MB, 5.8 TB/s) and the draws 31,
+ * of which vector instructions are some 18 and the rest what the launch's start, its decisions and its
+ * last workgroup take.  16 sequences 29.5 us, one block of seven certain drafts 12.5, 33 plain draws
+ * from 50257 logits in fp32 13.9.
  */
-#include "kv_params.h"
 #include "logit_piece.h"
 
 namespace {
@@ -130,10 +130,6 @@ __device__ __forceinline__ Sequence sequence_of(const AcceptParams& p, int b) {
     }
     s.drafted = p.draft_logits && s.dt != 0.0f;
     return s;
-}
-
-__device__ __forceinline__ int divided(int n, const Divisor& d) {
-    return (int)((n + (uint64_t)((uint64_t)(uint32_t)n * d.mul >> 32)) >> d.shift);
 }
 
 /* Exchanges over a wave: within rows of 16 lanes by DPP, then across. */
@@ -684,12 +680,13 @@ struct Accept : LogitPiece<DT> {
 
     /* A token drawn from max(p - q, 0), as from_row.  The rows' sums in 64 bits are known when all
      * their logits have been seen; in which tokens p is larger is known before, but for those where
-     * the two are as near to each other as fp32 sums may be wrong (one or two of 151936).  So a unit's part is kept as the sums of p's and of q's exponentials over the
-     * tokens where p is surely larger, and over those in between with the least and the largest of
-     * their quotients, to be scaled and subtracted when the sums are known.  The last workgroup
-     * weighs a unit again whose quotients lie to both sides of the border then.  (Two launches instead, of both rows' sums and then of their differences,
-     * took 24 and 21 us for 64 sequences, this 29.)  Of a product with 0 or 1 in the sums: one
-     * select instead of four. */
+     * the two are as near to each other as fp32 sums may be wrong (one or two of 151936).  So a
+     * unit's part is kept as the sums of p's and of q's exponentials over the tokens where p is
+     * surely larger, and over those in between with the least and the largest of their quotients, to
+     * be scaled and subtracted when the sums are known.  The last workgroup weighs a unit again whose
+     * quotients lie to both sides of the border then.  (Two launches instead, of both rows' sums and
+     * then of their differences, took 24 and 21 us for 64 sequences, this 29.)  Exponentials are
+     * summed by a product with 0 or 1: one select a token instead of four. */
     static __device__ __forceinline__ int from_rest(const AcceptParams& p, const Sequence& s,
                                                     const Draw& d, int b, int chunk, double u) {
         const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
