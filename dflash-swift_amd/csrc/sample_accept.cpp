@@ -68,7 +68,7 @@ AcceptPlan plan_accept(int cus, int batch, int rows, int V, dfq_dtype dtype, boo
     const int range = unit * DFQ_ACCEPT_PIECES;
     a.ranges = (V + range - 1) / range;
     /* Workgroups of a sequence: as many units a wave as leave no more than four workgroups a CU,
-     * which are there at once (115 registers), and as few workgroups as that many units take: each
+     * which are there at once (117 registers), and as few workgroups as that many units take: each
      * decides its sequence's drafts first.  With five a CU 64 sequences of seven drafts of 151936
      * tokens took 73.6 us for 71.9 and 16 32.3 for 29.9; eight took 33 rows of 50257 from 14.3 to
      * 16.2. */

@@ -435,8 +435,9 @@ typedef struct dfq_heads {
  * by the same angles.  Row m of sequence b is at position start + starts[b] + m (starts:
  * device memory, may be NULL for zeros) or at positions[b*rows + m] (device memory, as draft
  * trees need them; then start is 0 and starts NULL).  Positions may be negative.  head_dim is even
- * and at most 512, heads at most 65535 a token; bf16, fp16 or fp32, in fp32 and rounded once.
- * Asynchronous on `stream`. */
+ * and at most 512, heads at most 65535 a token, and calls past a launch's grid are refused (2^26 heads
+ * in all where head_dim is no multiple of 16 or, in pairs half apart, rotary_dim none; at 128 wide
+ * 2^31).  bf16, fp16 or fp32, in fp32 and rounded once.  Asynchronous on `stream`. */
 dfq_status dfq_rope(dfq_ctx* ctx, const dfq_rope_table* rope, const dfq_heads* q,
                     const dfq_heads* k, int head_dim, dfq_dtype dtype, int batch, int rows,
                     int start, const int32_t* starts, const int32_t* positions, int inverse,
